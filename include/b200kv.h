@@ -70,6 +70,8 @@ typedef enum b200kv_status {
 #define B200KV_STATUS_SPLIT_TIMEOUT 2u  /* the in-launch merge never saw the partial of one of its splits */
 #define B200KV_STATUS_PEER_TIMEOUT 4u   /* the cross-GPU merge never saw the partial of one of its peers */
 #define B200KV_STATUS_PIPE_TIMEOUT 8u   /* a tensor-core pipeline stage (MMA completion) never signalled */
+#define B200KV_STATUS_BAD_PAGE 16u      /* a page table named a page outside the pool (b200kv_paged_*; the page was not touched) */
+#define B200KV_STATUS_BAD_BOUND 32u     /* the sequences of a paged batch hold more than its host-side bounds say (b200kv_paged_batch) */
 
 /* KvCacheQuantMode, include/miinfer/prefill_v2/kv_cache.hpp:16-21 (same values). */
 typedef enum b200kv_quant_mode {
@@ -477,6 +479,89 @@ B200KV_API int b200kv_prefill_attn_prepared(const b200kv_view* view, const void*
                                  float* gated_output, uint32_t token_count, uint32_t base_position,
                                  uint32_t query_heads, float scale, const b200kv_prefill_state* prefill_state,
                                  void* workspace, size_t workspace_bytes, uint32_t prepared_rows, void* stream);
+
+/* ---- a paged cache: many sequences in one pool of pages, ragged batches of new tokens -------------------------------
+ *
+ * No counterpart in the reference, which keeps one session resident (tools/miinfer_cli.cpp:5663-5676); formats, quantiser, RoPE and
+ * arithmetic of a row are those of the calls above.  A pool's planes are [page][kv_head][page_size][...]; position j of a
+ * sequence lies in slot j % page_size of page page_table[sequence][j / page_size].  Sequences may share pages (a common
+ * prefix); what writes pages (store, evict) is given pages that no other sequence of the call uses.
+ *
+ * All calls take the batch as device memory, so that a captured graph replays with whatever the arrays then hold, and host-side
+ * bounds that size the launches.  A sequence that exceeds a bound never leads to an access out of range: it is cut to it, and
+ * B200KV_STATUS_BAD_BOUND set in the registered status word.  A page number outside [0, pages) is never followed: its rows read as zeros and are
+ * not written, and B200KV_STATUS_BAD_PAGE is set.  Page table entries past a sequence's length are not read. */
+typedef struct b200kv_paged_view {
+    void* key_f16;      /* [pages][kv_heads][page_size][head_dim] fp16 */
+    void* value_f16;
+    int8_t* key_q8;     /* the same of int8 */
+    void* key_scales;   /* [pages][kv_heads][page_size][head_dim / qblock] fp16 */
+    int8_t* value_q8;
+    void* value_scales;
+    uint32_t pages;
+    uint32_t page_size;  /* positions: 16, 32, 64, 128 or 256 */
+    uint32_t kv_heads;
+    uint32_t head_dim;   /* 128 or 256 */
+    uint32_t qblock;     /* 32 or head_dim */
+    uint32_t quant_mode; /* b200kv_quant_mode; planes of the other format may be NULL, the others are 16-byte aligned */
+} b200kv_paged_view;
+
+typedef struct b200kv_paged_batch {
+    const int32_t* page_table;    /* DEVICE [sequences][max_pages] */
+    const int32_t* query_starts;  /* DEVICE [sequences + 1], ascending: sequence s has the rows query_starts[s] .. query_starts[s + 1] of the
+                                     activations, its newest tokens; none for a sequence that only waits */
+    const int32_t* lengths;       /* DEVICE [sequences]: cached positions, the newest tokens among them */
+    uint32_t sequences;
+    uint32_t max_pages;
+    uint32_t total_tokens;        /* rows of the activations; rows at or past query_starts[sequences] are neither read nor written */
+    uint32_t max_tokens;          /* upper bound of the new tokens of a sequence */
+    uint32_t max_length;          /* upper bound of a length */
+    uint64_t total_length;        /* upper bound of the sum of the lengths; 0 = sequences * max_length */
+} b200kv_paged_batch;
+
+/* b200kv_append for a ragged batch: token t of sequence s goes to position lengths[s] - (its new tokens) + t.  key/value:
+ * [total_tokens][kv_heads * head_dim] of `dtype`.  rope_positions (DEVICE int32 [total_tokens], may be NULL): the position each token is
+ * rotated by where that is not its place in the cache, as after an eviction.  The same bits as b200kv_append for the same
+ * position. */
+B200KV_API int b200kv_paged_store(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* key, const void* value, int dtype,
+                       const float* k_norm_weight, int rope_mode, float theta, float epsilon, const int32_t* rope_positions, void* stream);
+/* The rows of the new tokens read back: key/value fp16 [total_tokens][kv_heads][head_dim], int8 rows as the values they stand for; either may be NULL.
+ * (With query_starts of whole sequences it takes a sequence out of its pages.) */
+B200KV_API int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_paged_batch* batch, void* key, void* value, void* stream);
+
+/* Attention of every new token over its sequence's pages, the chunk already stored.  q, gate (may be NULL), output: [total_tokens][query_heads]
+ * [head_dim], q of q_dtype, gate fp32, output of output_dtype = attention * sigmoid(gate).  A token at cache position i
+ * sees positions j <= i; with window > 0 only j > i - window and the first `sinks` ones.  (Positions are places in the cache: after an eviction the
+ * window counts the positions that are left.)  lse (may be NULL): fp32 [total_tokens][query_heads], the natural logarithm of the sum of exponentials of
+ * the scaled scores, for b200kv_paged_weights.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8.
+ * Sequences of a few query rows (tokens * query_heads / kv_heads <= 8) take a streaming kernel in which values that a token does not see never
+ * count; the others' kernel asks that all cache rows which a sequence's new tokens see are finite, as b200kv_prefill_attn does.  Rows past a length may
+ * hold anything in both.  q, output and gate 16-byte aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no
+ * consequence; one launch at a time uses it. */
+B200KV_API size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window,
+                       uint32_t sinks);
+B200KV_API int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* gate,
+                      void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Adds to weights[s][kv_head][j] the weight that position j gets from sequence s's new tokens: sum of exp(score - lse) over them and over the query
+ * heads of the kv head.  weights: fp32 [sequences][kv_heads][weights_stride], weights_stride >= max_length; entries at and past a
+ * length are left alone.  q, lse, scale, window and sinks as in the b200kv_paged_attn call that produced lse.  observe > 0: only the last `observe`
+ * new tokens of a sequence count. */
+B200KV_API int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* lse,
+                         float* weights, uint32_t weights_stride, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+                         uint32_t observe, void* stream);
+
+/* Brings every sequence of more than `keep` positions back to `keep`, each kv head for itself: the first `sinks` and the last `recent` positions stay, and of
+ * the others those with the largest weights (ties: the lowest position; a NaN counts as the least).  The rows that stay go, in order, to positions 0, 1, ...
+ * of the pages of target_table (DEVICE [sequences][target_max_pages], target_max_pages * page_size >= keep); a sequence of at most `keep` positions
+ * is copied as it is.  target_table == batch->page_table compacts in place; otherwise the target's pages and the sequences' must not overlap.
+ * kept: DEVICE int32 [sequences][kv_heads][keep], the positions that stayed, -1 behind them.  new_weights (may be NULL): fp32 [sequences][kv_heads]
+ * [keep], their weights, 0 behind them; must not overlap weights.  new_lengths: DEVICE int32 [sequences] = min(length, keep); not batch->lengths itself.
+ * sinks + recent <= keep. */
+B200KV_API int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const int32_t* target_table, uint32_t target_max_pages,
+                       const float* weights, uint32_t weights_stride, uint32_t keep, uint32_t sinks, uint32_t recent, int32_t* kept,
+                       float* new_weights, int32_t* new_lengths, void* stream);
 
 /* ---- prefix snapshot / restore ---------------------------------------------
  * Raw compact layout of AttentionLayerKvCacheStorage::download_raw/upload_raw

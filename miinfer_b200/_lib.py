@@ -26,8 +26,31 @@ class View(C.Structure):
     ]
 
 
+class PagedView(C.Structure):
+    """b200kv_paged_view (include/b200kv.h): a pool of pages of one attention layer."""
+
+    _fields_ = [
+        ("key_f16", C.c_void_p), ("value_f16", C.c_void_p),
+        ("key_q8", C.c_void_p), ("key_scales", C.c_void_p),
+        ("value_q8", C.c_void_p), ("value_scales", C.c_void_p),
+        ("pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+        ("qblock", C.c_uint32), ("quant_mode", C.c_uint32),
+    ]
+
+
+class PagedBatch(C.Structure):
+    """b200kv_paged_batch: the sequences of a call over a paged cache."""
+
+    _fields_ = [
+        ("page_table", C.c_void_p), ("query_starts", C.c_void_p), ("lengths", C.c_void_p),
+        ("sequences", C.c_uint32), ("max_pages", C.c_uint32), ("total_tokens", C.c_uint32), ("max_tokens", C.c_uint32),
+        ("max_length", C.c_uint32), ("total_length", C.c_uint64),
+    ]
+
+
 u32, u64, sz, vp, fl, i32 = C.c_uint32, C.c_uint64, C.c_size_t, C.c_void_p, C.c_float, C.c_int
 VP = C.POINTER(View)
+PV, PB = C.POINTER(PagedView), C.POINTER(PagedBatch)
 
 
 class PoolCounters(C.Structure):
@@ -93,6 +116,12 @@ SIGNATURES = {
     "b200kv_prefill_attn": (i32, [VP, vp, i32, vp, vp, u32, u32, u32, fl, vp, vp, sz, vp]),
     "b200kv_prefill_prepare": (i32, [VP, u32, u64, vp, sz, vp]),
     "b200kv_prefill_attn_prepared": (i32, [VP, vp, i32, vp, vp, u32, u32, u32, fl, vp, vp, sz, u32, vp]),
+    "b200kv_paged_store": (i32, [PV, PB, vp, vp, i32, vp, i32, fl, fl, vp, vp]),
+    "b200kv_paged_load": (i32, [PV, PB, vp, vp, vp]),
+    "b200kv_paged_attn_workspace_bytes": (sz, [PV, PB, u32, u32, u32]),
+    "b200kv_paged_attn": (i32, [PV, PB, vp, i32, vp, vp, i32, vp, u32, fl, u32, u32, vp, sz, vp]),
+    "b200kv_paged_weights": (i32, [PV, PB, vp, i32, vp, vp, u32, u32, fl, u32, u32, u32, vp]),
+    "b200kv_paged_evict": (i32, [PV, PB, vp, u32, vp, u32, u32, u32, u32, vp, vp, vp, vp]),
     "b200kv_snapshot_bytes": (sz, [VP, u64]),
     "b200kv_snapshot_save": (i32, [VP, u64, vp, vp]),
     "b200kv_snapshot_restore": (i32, [VP, u64, vp, vp]),
@@ -150,7 +179,7 @@ def load_native():
     spec = importlib.util.spec_from_file_location("_native", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.bind({"View": View, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
+    module.bind({"View": View, "PagedView": PagedView, "PagedBatch": PagedBatch, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
     return module
 
 

@@ -26,6 +26,7 @@
 // The row arithmetic is the same, operation for operation, as append_row.cuh's (used by the decode kernel's fused
 // single-token append and the query-side kernel): all three write identical bits.
 #include "append_row.cuh"
+#include "paged_common.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -51,6 +52,39 @@ struct AppendParams {
     // before the wait.  (12 launches of 8192 tokens: 205 us so, 216 behind the wait.)
     int fills_device;
 };
+
+// The store into a paged cache (b200kv_paged_store) is an instance of the kernel: the view's planes are the pool's and its capacity the page
+// size, which is then the distance between two heads' rows, and every token's row is looked up.  The bits of a row are the same.
+template <bool PAGED> struct AppendArgs : AppendParams {};
+template <> struct AppendArgs<true> : AppendParams {
+    Paged pool;
+    const int32_t* rope_positions;   // may be null: a token is rotated by its place in the cache
+};
+
+// Where a token of a ragged batch goes.
+struct TokenPlace {
+    uint32_t token, end;   // the token; where its sequence's tokens end
+    uint32_t position;     // its place in the cache
+    long long row;         // its row for kv head 0; negative where there is none
+};
+__device__ __forceinline__ TokenPlace place_of(const Paged& pool, uint32_t token) {
+    const uint32_t s = sequence_of(pool, token);
+    const Span span = span_of(pool, s);
+    const uint32_t t = token - span.first;
+    TokenPlace at{token, span.first + span.tokens, 0, -1};
+    const int j = span.base() + static_cast<int>(t);
+    if (token >= span.first && t < span.tokens && j >= 0) {
+        at.position = static_cast<uint32_t>(j);
+        at.row = row_of(pool, s, 0, at.position);
+    }
+    return at;
+}
+// The place of the token behind `at`: most lie in the same page.
+__device__ __forceinline__ TokenPlace place_behind(const Paged& pool, const TokenPlace& at) {
+    const uint32_t next = at.position + 1;
+    if (at.row < 0 || at.token + 1 >= at.end || (next & ((1u << pool.page_shift) - 1)) == 0) return place_of(pool, at.token + 1);
+    return TokenPlace{at.token + 1, at.end, next, at.row + 1};
+}
 
 constexpr int kAppendWarps = 2;
 constexpr int kUnitElems = 1024;       // 32 q8_0 blocks: one scale per lane
@@ -140,9 +174,9 @@ __device__ __forceinline__ uint32_t half_pair(Pair x) {
     const __half2 h = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int D, bool IN_F16, int CTAS>
+template <int D, bool IN_F16, int CTAS, bool PAGED = false>
 __global__ void __launch_bounds__(kAppendWarps * 32, CTAS)
-append_kernel(const __grid_constant__ AppendParams p, const uint32_t align) {
+append_kernel(const __grid_constant__ AppendArgs<PAGED> p, const uint32_t align) {
     constexpr int LPR = D / (2 * kRun);         // lanes per row
     constexpr int HB = kUnitElems / D;          // kv heads per unit: its rows
     constexpr int NB = D / 32;                  // q8_0 blocks per row
@@ -160,7 +194,7 @@ append_kernel(const __grid_constant__ AppendParams p, const uint32_t align) {
     if (p.fills_device) pdl_launch_dependents();   // the next kernel may become resident; it orders itself against this one
     // K/V inputs and the device-side position come from preceding kernels.  Where the position is known on the host, the first token's rotation is taken ahead of the
     // wait.
-    bool waited = p.prefill_state != nullptr || p.decode_state != nullptr;
+    bool waited = PAGED || p.prefill_state != nullptr || p.decode_state != nullptr;
     if (waited) pdl_wait();
 
     uint32_t base_position = p.base_position;
@@ -197,7 +231,12 @@ append_kernel(const __grid_constant__ AppendParams p, const uint32_t align) {
             if (++c.pass == passes) { c.pass = 0; ++c.token; }
         }
     };
-    auto inside = [&](const Cursor& c) { return static_cast<uint64_t>(base_position) + c.token < capacity; };   // never write outside the cache
+    [[maybe_unused]] TokenPlace here, ahead;   // PAGED: of the unit's token and of the next unit's
+    // never write outside the cache
+    auto inside = [&](const Cursor& c, [[maybe_unused]] const TokenPlace& at) {
+        if constexpr (PAGED) return at.row >= 0;
+        else return static_cast<uint64_t>(base_position) + c.token < capacity;
+    };
     auto heads = [&](const Cursor& c) { return static_cast<int>(min(static_cast<uint32_t>(HB), H - c.pass * HB)); };
     RawRun<IN_F16> raw[2][2];   // per step: elements 8l .. and D/2 + 8l .. of the unit that comes next; a row that does not exist comes as zeros and is only not stored
     auto fetch = [&](const Cursor& c) {
@@ -366,20 +405,26 @@ append_kernel(const __grid_constant__ AppendParams p, const uint32_t align) {
 
     Cursor cur{unit0 / (2 * passes), (unit0 / 2) % passes, unit0 & 1};
     if (waited) {
-        if (unit0 < unit1 && inside(cur)) fetch(cur);
+        if constexpr (PAGED) {
+            if (unit0 < unit1) here = place_of(p.pool, cur.token);
+        }
+        if (unit0 < unit1 && inside(cur, here)) fetch(cur);
         if (!p.fills_device) pdl_launch_dependents();
     }
     uint32_t rotated_token = 0xffffffffu;
     for (uint32_t unit = unit0; unit < unit1; ++unit) {
-        const uint64_t position = static_cast<uint64_t>(base_position) + cur.token;
+        uint64_t position;   // PAGED: the row
+        if constexpr (PAGED) position = static_cast<uint64_t>(here.row);
+        else position = static_cast<uint64_t>(base_position) + cur.token;
         if (cur.side == 0 && cur.token != rotated_token) {
             rotated_token = cur.token;
-            rotation(static_cast<uint32_t>(position));
+            if constexpr (PAGED) rotation(p.rope_positions != nullptr ? static_cast<uint32_t>(max(p.rope_positions[cur.token], 0)) : here.position);
+            else rotation(static_cast<uint32_t>(position));
         }
         if (!waited) {
             waited = true;
             pdl_wait();
-            if (inside(cur)) fetch(cur);
+            if (inside(cur, here)) fetch(cur);
             if (!p.fills_device) pdl_launch_dependents();
         }
         Rows a, b;
@@ -387,16 +432,50 @@ append_kernel(const __grid_constant__ AppendParams p, const uint32_t align) {
         for (int s = 0; s < 2; ++s) { widen<IN_F16>(raw[s][0], a[s]); widen<IN_F16>(raw[s][1], b[s]); }
         Cursor next = cur;
         advance(next);
-        if (unit + 1 < unit1 && inside(next)) fetch(next);   // under this unit's arithmetic
-        if (inside(cur)) {
+        if constexpr (PAGED) ahead = next.token == cur.token || unit + 1 == unit1 ? here : place_behind(p.pool, here);
+        if (unit + 1 < unit1 && inside(next, ahead)) fetch(next);   // under this unit's arithmetic
+        if (inside(cur, here)) {
             if (cur.side == 0) transform_k(a, b);
             if (!row_scale && (cur.side == 0 ? k_q8 : v_q8)) store(std::true_type{}, cur, a, b, position);
             else store(std::false_type{}, cur, a, b, position);
         }
         cur = next;
+        if constexpr (PAGED) here = ahead;
     }
     if (!waited) pdl_wait();
 }
+
+template <int D, bool PAGED>
+static int launch_append(AppendArgs<PAGED>& p, bool f16, uint64_t units, cudaStream_t s) {
+    int device = 0, sms = 0;
+    B200KV_CUDA_TRY(cudaGetDevice(&device));
+    B200KV_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    const int ctas = f16 ? pick_ctas(units, static_cast<uint32_t>(sms)) : kFewCtas;
+    const unsigned grid = static_cast<unsigned>(std::min<uint64_t>((units + kAppendWarps - 1) / kAppendWarps, static_cast<uint64_t>(sms) * ctas));
+    // 16-byte loads need aligned pointers (a lane's runs start at multiples of eight elements)
+    const auto aligned = [](auto... ptr) { return ((reinterpret_cast<uintptr_t>(ptr) | ...) & 15u) == 0; };
+    const uint32_t align = (aligned(p.key, p.value) ? kInputAligned : 0u) | (aligned(p.k_norm_weight) ? kWeightAligned : 0u);
+    const dim3 block(kAppendWarps * 32);
+    auto launch = [&](auto kernel, std::atomic<int>& slots) {   // slots: CTAs of the kernel that fit on an SM
+        int n = slots.load(std::memory_order_relaxed);
+        if (n == 0) {
+            const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kAppendWarps * 32, 0);
+            if (e != cudaSuccess) return e;
+            slots.store(n, std::memory_order_relaxed);
+        }
+        p.fills_device = grid >= static_cast<uint64_t>(sms) * n;
+        return launch_kernel(kernel, grid, block, 0, s, true, p, align);
+    };
+    static std::atomic<int> slots[3] = {};   // one set per instantiation
+    const cudaError_t err = !f16                ? launch(append_kernel<D, false, kFewCtas, PAGED>, slots[0])
+                            : ctas == kFewCtas ? launch(append_kernel<D, true, kFewCtas, PAGED>, slots[1])
+                                               : launch(append_kernel<D, true, kManyCtas, PAGED>, slots[2]);
+    B200KV_CUDA_TRY(err);
+    return B200KV_OK;
+}
+
+// Units of work of `tokens` tokens; a pass is the kv heads of one unit.
+static uint64_t append_passes(uint32_t kv_heads, uint32_t head_dim) { return (static_cast<uint64_t>(kv_heads) + kUnitElems / head_dim - 1) / (kUnitElems / head_dim); }
 
 }  // namespace b200kv
 
@@ -420,7 +499,7 @@ extern "C" int b200kv_append(const b200kv_view* view, const void* key, const voi
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
 
-    AppendParams p{};
+    AppendArgs<false> p{};
     p.view = *view;
     p.key = key;
     p.value = value;
@@ -429,7 +508,7 @@ extern "C" int b200kv_append(const b200kv_view* view, const void* key, const voi
     p.decode_state = decode_state;
     // A bound above any cache's capacity, where the count is on the device: as many tokens as the kernel's 32-bit unit numbers hold (with
     // more than eight heads of 128 dims that is 2^30, a cache of terabytes).
-    const uint64_t passes = (static_cast<uint64_t>(view->kv_heads) + kUnitElems / view->head_dim - 1) / (kUnitElems / view->head_dim);
+    const uint64_t passes = append_passes(view->kv_heads, view->head_dim);
     if (prefill_state != nullptr || decode_state != nullptr) token_count = static_cast<uint32_t>(std::min<uint64_t>(token_count, 0xffffffffu / (2 * passes)));
     p.token_count = token_count;
     p.base_position = base_position;
@@ -437,34 +516,37 @@ extern "C" int b200kv_append(const b200kv_view* view, const void* key, const voi
     p.epsilon = epsilon;
     rope_constants(rope_mode, theta, view->head_dim, p.inv_freq, &p.sectioned_step);
 
-    const uint32_t d = view->head_dim;
     const uint64_t units = 2 * token_count * passes;
     if (units >= (1ull << 32)) return B200KV_ERR_RANGE;
-    int device = 0, sms = 0;
-    B200KV_CUDA_TRY(cudaGetDevice(&device));
-    B200KV_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    const bool f16 = (dtype == B200KV_F16);
-    const int ctas = f16 ? pick_ctas(units, static_cast<uint32_t>(sms)) : kFewCtas;
-    const unsigned grid = static_cast<unsigned>(std::min<uint64_t>((units + kAppendWarps - 1) / kAppendWarps, static_cast<uint64_t>(sms) * ctas));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // 16-byte loads need aligned pointers (a lane's runs start at multiples of eight elements)
-    const auto aligned = [](auto... ptr) { return ((reinterpret_cast<uintptr_t>(ptr) | ...) & 15u) == 0; };
-    const uint32_t align = (aligned(key, value) ? kInputAligned : 0u) | (aligned(k_norm_weight) ? kWeightAligned : 0u);
-    const dim3 block(kAppendWarps * 32);
-    cudaError_t err;
-    auto launch = [&](auto kernel, std::atomic<int>& slots) {   // slots: CTAs of the kernel that fit on an SM
-        int n = slots.load(std::memory_order_relaxed);
-        if (n == 0) {
-            const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kAppendWarps * 32, 0);
-            if (e != cudaSuccess) return e;
-            slots.store(n, std::memory_order_relaxed);
-        }
-        p.fills_device = grid >= static_cast<uint64_t>(sms) * n;
-        return launch_kernel(kernel, grid, block, 0, s, true, p, align);
-    };
-    static std::atomic<int> slots[6] = {};
-    if (d == 128) err = !f16 ? launch(append_kernel<128, false, kFewCtas>, slots[0]) : ctas == kFewCtas ? launch(append_kernel<128, true, kFewCtas>, slots[1]) : launch(append_kernel<128, true, kManyCtas>, slots[2]);
-    else err = !f16 ? launch(append_kernel<256, false, kFewCtas>, slots[3]) : ctas == kFewCtas ? launch(append_kernel<256, true, kFewCtas>, slots[4]) : launch(append_kernel<256, true, kManyCtas>, slots[5]);
-    B200KV_CUDA_TRY(err);
-    return B200KV_OK;
+    return view->head_dim == 128 ? launch_append<128>(p, dtype == B200KV_F16, units, s) : launch_append<256>(p, dtype == B200KV_F16, units, s);
+}
+
+extern "C" int b200kv_paged_store(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* key, const void* value, int dtype,
+                                  const float* k_norm_weight, int rope_mode, float theta, float epsilon, const int32_t* rope_positions,
+                                  void* stream) {
+    int rc = validate_paged(view, batch);
+    if (rc != B200KV_OK) return rc;
+    if (key == nullptr || value == nullptr || (dtype != B200KV_F16 && dtype != B200KV_F32)) return B200KV_ERR_INVALID;
+    if (rope_mode < B200KV_ROPE_NONE || rope_mode > B200KV_ROPE_SECTIONED64) return B200KV_ERR_INVALID;
+    if (!std::isfinite(theta) || !std::isfinite(epsilon) || (rope_mode != B200KV_ROPE_NONE && !(theta > 0.0f))) return B200KV_ERR_INVALID;
+    if (batch->total_tokens == 0 || batch->sequences == 0) return B200KV_OK;
+    const uint64_t units = 2 * static_cast<uint64_t>(batch->total_tokens) * append_passes(view->kv_heads, view->head_dim);
+    if (units >= (1ull << 32)) return B200KV_ERR_RANGE;
+    rc = ensure_device();
+    if (rc != B200KV_OK) return rc;
+    AppendArgs<true> p{};
+    p.view = b200kv_view{view->key_f16, view->value_f16, view->key_q8, view->key_scales, view->value_q8, view->value_scales,
+                         view->page_size, view->kv_heads, view->head_dim, view->qblock, view->quant_mode};
+    p.pool = paged_of(*view, *batch);
+    p.rope_positions = rope_positions;
+    p.key = key;
+    p.value = value;
+    p.k_norm_weight = k_norm_weight;
+    p.token_count = batch->total_tokens;
+    p.rope_mode = rope_mode;
+    p.epsilon = epsilon;
+    rope_constants(rope_mode, theta, view->head_dim, p.inv_freq, &p.sectioned_step);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return view->head_dim == 128 ? launch_append<128>(p, dtype == B200KV_F16, units, s) : launch_append<256>(p, dtype == B200KV_F16, units, s);
 }

@@ -27,8 +27,8 @@ uint32_t device_sms();   // SMs of the current device (of the slice it is); behi
         }                                                            \
     } while (0)
 
-inline bool is_k_q8(uint32_t mode) { return mode == B200KV_Q8_F16 || mode == B200KV_Q8_Q8; }
-inline bool is_v_q8(uint32_t mode) { return mode == B200KV_F16_Q8 || mode == B200KV_Q8_Q8; }
+__host__ __device__ inline bool is_k_q8(uint32_t mode) { return mode == B200KV_Q8_F16 || mode == B200KV_Q8_Q8; }
+__host__ __device__ inline bool is_v_q8(uint32_t mode) { return mode == B200KV_F16_Q8 || mode == B200KV_Q8_Q8; }
 
 // Launch overlap (programmatic dependent launch): 0 = off, n > 0 = on with a guard of n trailing positions.
 uint32_t launch_overlap_tail();

@@ -28,9 +28,13 @@
 //     come once for both; their S and O fill TMEM, so Q is an A operand in shared memory.
 // Every mbarrier wait is bounded; a wait that runs out poisons the output rows with NaN, and the CTA still frees
 // its TMEM and exits.
+//
+// Chunks over a paged cache (b200kv_paged_attn) take instances of the attention kernel of their own: a CTA's rows and tiles come from a list in device
+// memory, the fp16 copy of a sequence holds the tiles of its sinks and its window only, and the mask has a lower edge as well.
 #include "decode_common.cuh"
 #include "dequant.cuh"
 #include "mbarrier_wait.cuh"
+#include "paged_plan.cuh"
 #include "reference_word.h"
 
 #include <algorithm>
@@ -66,6 +70,27 @@ struct Tc5Params {
     uint32_t rows_padded;        // query rows per kv head, rounded up to the row tile
     float* part_o;               // [split][kv_head][rows_padded][D]
     float2* part_ml;             // [split][kv_head][rows_padded] {maximum in log2 units, sum}
+};
+
+// A CTA's item is read anew where it is used: kept, its words would be registers that the tile loop needs (384 bytes of spills at head_dim 128).
+__device__ __forceinline__ ChunkItem reload(const ChunkItem* from) {
+    ChunkItem item;
+    uint32_t* to = reinterpret_cast<uint32_t*>(&item);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to[4 * i]), "=r"(to[4 * i + 1]), "=r"(to[4 * i + 2]), "=r"(to[4 * i + 3])
+                     : "l"(reinterpret_cast<const uint4*>(from) + i));
+    return item;
+}
+
+template <bool PAGED> struct KernelParams : Tc5Params {};
+template <> struct KernelParams<true> : Tc5Params {   // of the base: maps, q, gate, heads, scale and partials
+    const ChunkItem* items;
+    const ChunkPlan* plan;
+    void* typed_out;
+    int out_is_f16;
+    float* lse;                  // may be null
+    uint32_t window, sinks;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -252,9 +277,10 @@ struct RowOffsets {
     }
 };
 
-// STATE: the position comes from a device-side state (one row tile a CTA).
-template <int D, int RT, bool STATE>
-__global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel(const __grid_constant__ Tc5Params p) {
+// STATE: the position comes from a device-side state (one row tile a CTA).  PAGED: everything does (ChunkItem).
+template <int D, int RT, bool STATE, bool PAGED = false>
+__global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel(const __grid_constant__ KernelParams<PAGED> p) {
+    static_assert(!PAGED || (RT == 1 && !STATE));
     using L = Layout<D, RT>;
     constexpr int kThreads = L::kThreads;
     constexpr int kTmaWarp = L::kTmaWarp, kSWarp = L::kSWarp, kPvWarp = L::kPvWarp, kTmaVWarp = L::kTmaVWarp;
@@ -270,8 +296,20 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Row tiles from the last (the longest causal range) to the first, kv heads and KV splits of a row tile next to each
     // other: the CTAs dispatched last are the short ones, and a fresh chunk's last wave is nearly even.
-    const uint32_t split_u = blockIdx.x % p.kv_splits, tile_head = blockIdx.x / p.kv_splits;
-    const uint32_t kv_head = tile_head % p.kv_heads;
+    [[maybe_unused]] ChunkItem item;
+    [[maybe_unused]] uint32_t sink_tiles = 0;   // PAGED: the CTA's tiles from this one on lie `row_gap` rows and `position_gap` positions further
+    [[maybe_unused]] int row_gap = 0, position_gap = 0;
+    if constexpr (PAGED) {
+        pdl_wait();   // the list comes from the call's first kernel
+        if (blockIdx.x >= p.plan->items) return;   // the grid is sized by bounds
+        item = reload(p.items + blockIdx.x);
+        sink_tiles = item.sink_tiles;
+        row_gap = static_cast<int>(item.skip * kBN);
+        position_gap = static_cast<int>(item.window0 + (item.skip - item.sink_tiles) * kBN);
+    }
+    const uint32_t split_u = PAGED ? 0 : blockIdx.x % p.kv_splits, tile_head = PAGED ? 0 : blockIdx.x / p.kv_splits;
+    uint32_t kv_head = PAGED ? 0 : tile_head % p.kv_heads;
+    if constexpr (PAGED) kv_head = item.kv_head;
     const uint32_t G = p.query_heads / p.kv_heads;
     uint32_t base = p.base_position, count = p.token_count;
     if constexpr (STATE) {
@@ -279,15 +317,23 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         base = p.prefill_state->base_position;
         count = min(count, p.prefill_state->token_count);
     }
-    const uint32_t total_rows = p.token_count * G;
-    const uint32_t row0 = ((total_rows + L::kRows - 1) / L::kRows - 1 - tile_head / p.kv_heads) * L::kRows;
+    uint32_t total_rows = p.token_count * G, row0 = 0;
+    if constexpr (PAGED) {
+        total_rows = item.tokens * G;
+        row0 = item.row_tile * L::kRows;
+    } else {
+        row0 = ((total_rows + L::kRows - 1) / L::kRows - 1 - tile_head / p.kv_heads) * L::kRows;
+    }
+    // first element of the sequence's rows in q, gate and output
+    size_t own_rows = 0;
+    if constexpr (PAGED) own_rows = static_cast<size_t>(item.first) * p.query_heads * D;
     // The next kernel of the stream (the merge of the KV splits) may become resident once every CTA has got here; it
     // orders itself against this one.  This kernel's own dependency wait comes after its set-up.
     pdl_launch_dependents();
 
     // longest causal range among this CTA's rows (rows are token-major; see prefill_mma.cu)
     uint32_t kv_end = 0;
-    if (count > 0 && p.capacity > base) {
+    if (!PAGED && count > 0 && p.capacity > base) {
         const uint32_t t_first = row0 / G, t_last = (min(row0 + L::kRows, total_rows) - 1) / G;
         const uint64_t t_cap = p.capacity - base - 1;
         uint64_t t_max = t_last;
@@ -297,9 +343,48 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     }
     if (kv_end > p.scratch_rows) kv_end = p.scratch_rows;   // never read past what the pre-pass wrote
     const int ntiles_all = static_cast<int>((kv_end + kBN - 1) / kBN);
-    const int split = static_cast<int>(split_u), nsplit = static_cast<int>(p.kv_splits);
-    const int tile0 = static_cast<int>(static_cast<long long>(ntiles_all) * split / nsplit);
-    const int ntiles = static_cast<int>(static_cast<long long>(ntiles_all) * (split + 1) / nsplit) - tile0;   // tiles of this CTA
+    int split = 0, nsplit = 1, tile0, ntiles;   // tile0, ntiles: tiles of this CTA
+    if constexpr (PAGED) {
+        nsplit = item.part == kNoPart ? 1 : 2;
+        tile0 = static_cast<int>(item.tile0);
+        ntiles = static_cast<int>(item.tiles);
+    } else {
+        split = static_cast<int>(split_u);
+        nsplit = static_cast<int>(p.kv_splits);
+        tile0 = static_cast<int>(static_cast<long long>(ntiles_all) * split / nsplit);
+        ntiles = static_cast<int>(static_cast<long long>(ntiles_all) * (split + 1) / nsplit) - tile0;
+    }
+    [[maybe_unused]] int scratch_row = 0;
+    if constexpr (PAGED) scratch_row = static_cast<int>(item.scratch_row);
+    // where the CTA's tile j lies: its row in what the maps cover, and its first position
+    auto tile_row = [&](int j) -> int {
+        if constexpr (PAGED) {
+            const uint32_t u = static_cast<uint32_t>(tile0 + j);
+            return scratch_row + static_cast<int>(u) * kBN + (u < sink_tiles ? 0 : row_gap);
+        } else {
+            return (tile0 + j) * kBN;
+        }
+    };
+    auto tile_position = [&](int j) -> uint32_t {
+        if constexpr (PAGED) {
+            const uint32_t u = static_cast<uint32_t>(tile0 + j);
+            return u * kBN + (u < sink_tiles ? 0 : position_gap);
+        } else {
+            return static_cast<uint32_t>(tile0 + j) * kBN;
+        }
+    };
+    // four elements of the output at `at`
+    auto store_out = [&](size_t at, const float4& v) {
+        if constexpr (PAGED) {
+            if (p.out_is_f16) *reinterpret_cast<uint2*>(static_cast<__half*>(p.typed_out) + at) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+            else *reinterpret_cast<float4*>(static_cast<float*>(p.typed_out) + at) = v;
+        } else {
+            *reinterpret_cast<float4*>(p.out + at) = v;
+        }
+    };
+    size_t part_row0;   // first row of the CTA's partial
+    if constexpr (PAGED) part_row0 = static_cast<size_t>(item.part) * kBM;
+    else part_row0 = (static_cast<size_t>(split) * p.kv_heads + kv_head) * p.rows_padded + row0;
 
     // The layout (swizzled TMA tiles, MMA descriptors) needs the 1024-byte alignment the declaration above asks for; the
     // allocation has no slack for rounding up, so that a CTA of the neighbouring kernels fits beside this one on an SM.
@@ -308,14 +393,12 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         pdl_wait();
         const float nan = __int_as_float(0x7fc00000);
         for (uint32_t r = tid; r < static_cast<uint32_t>(L::kRows); r += kThreads)
-            if (nsplit > 1 && row0 + r < total_rows)
-                p.part_ml[(static_cast<size_t>(split) * p.kv_heads + kv_head) * p.rows_padded + row0 + r] = make_float2(0.0f, nan);
+            if (nsplit > 1 && row0 + r < total_rows) p.part_ml[part_row0 + r] = make_float2(0.0f, nan);
         if (nsplit == 1)
             for (uint32_t i = tid; i < static_cast<uint32_t>(L::kRows) * (D / 4); i += kThreads) {
                 const uint32_t gr = row0 + i / (D / 4);
                 if (gr >= total_rows) continue;
-                const size_t off = (static_cast<size_t>(gr / G) * p.query_heads + kv_head * G + gr % G) * D + (i % (D / 4)) * 4;
-                *reinterpret_cast<float4*>(p.out + off) = make_float4(nan, nan, nan, nan);
+                store_out(own_rows + (static_cast<size_t>(gr / G) * p.query_heads + kv_head * G + gr % G) * D + (i % (D / 4)) * 4, make_float4(nan, nan, nan, nan));
             }
         return;
     }
@@ -338,20 +421,20 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         for (int t = 0; t < n; ++t)
             for (int s = 0; s < L::kSlabs; ++s)
                 tma_load_3d(sbase + L::kOffK + ps * L::kPairBytes + s * (2 * kBN * 128) + t * (kBN * 128), &p.kmap, s * 64,
-                            (tile0 + 2 * i + t) * kBN, kv_head, bar(K_FULL + ps));
+                            tile_row(2 * i + t), kv_head, bar(K_FULL + ps));
     };
     // The query rows from r0 on of kv head `head` on their way to L2 (a prefetch reads nothing yet: whatever still writes them, the loads behind the wait
     // see).  A warp.
     auto prefetch_q = [&](uint32_t r0, uint32_t head) {
         const uint32_t elem = p.q_is_f16 ? 2 : 4, t_last = (min(r0 + L::kRows, total_rows) - 1) / G;
         for (uint32_t t = r0 / G + lane; t <= t_last; t += 32)
-            prefetch_l2(static_cast<const uint8_t*>(p.q) + (static_cast<size_t>(t) * p.query_heads + head * G) * D * elem, G * D * elem);
+            prefetch_l2(static_cast<const uint8_t*>(p.q) + (own_rows + (static_cast<size_t>(t) * p.query_heads + head * G) * D) * elem, G * D * elem);
     };
     constexpr int kTurns = D / 128;            // 32 columns = 64 dims per store; all loads are in flight together
     constexpr int kQWarps = RT * 8;            // two threads of a row each take half of it
     auto fetch_q = [&](const RowOffsets<D>& rows, uint4 (&q)[kTurns][8]) {
         auto fetch = [&](auto f16) {
-            const size_t base0 = (static_cast<size_t>(warp_row0 / G) * p.query_heads + kv_head * G) * D + ((warp >> 2) & 1) * (D / 2) + turn_chunk * 8;
+            const size_t base0 = own_rows + (static_cast<size_t>(warp_row0 / G) * p.query_heads + kv_head * G) * D + ((warp >> 2) & 1) * (D / 2) + turn_chunk * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -409,6 +492,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     bool failed = false;
     // The query rows of the CTA that takes this one's place, as far as the order of dispatch tells.  A warp.
     auto next_q = [&] {
+        if constexpr (PAGED) return;
         const uint32_t next = blockIdx.x + p.sms;
         if (next < gridDim.x && next % p.kv_splits == 0)
             prefetch_q(((total_rows + L::kRows - 1) / L::kRows - 1 - next / p.kv_splits / p.kv_heads) * L::kRows, next / p.kv_splits % p.kv_heads);
@@ -417,7 +501,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     auto copy_v = [&](int j, int full) {
         mbar_expect_tx(bar(full), L::kTileBytes);
         for (int s = 0; s < L::kSlabs; ++s)
-            tma_load_3d(sbase + L::kOffV + j % L::kVTiles * L::kTileBytes + s * (kBN * 128), &p.vmap, s * 64, (tile0 + j) * kBN, kv_head, bar(full));
+            tma_load_3d(sbase + L::kOffV + j % L::kVTiles * L::kTileBytes + s * (kBN * 128), &p.vmap, s * 64, tile_row(j), kv_head, bar(full));
     };
     auto load_v = [&](int j) -> bool {
         if (!mbar_wait(bar(V_EMPTY + j % L::kVTiles), static_cast<uint32_t>((j / L::kVTiles) & 1) ^ 1)) return false;
@@ -453,7 +537,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         if (p.gate != nullptr && split_u == 0) {
             const uint32_t t_last = (min(row0 + L::kRows, total_rows) - 1) / G;
             for (uint32_t t = row0 / G + lane; t <= t_last; t += 32)
-                prefetch_l2(p.gate + (static_cast<size_t>(t) * p.query_heads + kv_head * G) * D, G * D * 4);
+                prefetch_l2(p.gate + own_rows + (static_cast<size_t>(t) * p.query_heads + kv_head * G) * D, G * D * 4);
         }
         if (lane == 0) {
             for (int j = 0; ok && j < whole_tiles; ++j) {
@@ -480,7 +564,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         if (p.gate != nullptr && split_u == 0) {
             const uint32_t t_last = (min(row0 + L::kRows, total_rows) - 1) / G;
             for (uint32_t t = row0 / G + lane; t <= t_last; t += 32)
-                prefetch_l2(p.gate + (static_cast<size_t>(t) * p.query_heads + kv_head * G) * D, G * D * 4);
+                prefetch_l2(p.gate + own_rows + (static_cast<size_t>(t) * p.query_heads + kv_head * G) * D, G * D * 4);
         }
         bool ok = have_q;
         if (lane == 0)
@@ -662,9 +746,15 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         uint32_t len = 0;
         if (gr < total_rows) {
             const uint32_t token = gr / G;
-            const uint64_t l64 = static_cast<uint64_t>(base) + token + 1u;
-            len = (token < count && l64 <= p.capacity) ? static_cast<uint32_t>(l64) : 0u;
+            if constexpr (PAGED) {
+                len = static_cast<uint32_t>(max(item.base + static_cast<int>(token) + 1, 0));
+            } else {
+                const uint64_t l64 = static_cast<uint64_t>(base) + token + 1u;
+                len = (token < count && l64 <= p.capacity) ? static_cast<uint32_t>(l64) : 0u;
+            }
         }
+        uint32_t low = 0;   // PAGED: the row sees positions [low, len) and those below p.sinks
+        if constexpr (PAGED) low = p.window > 0 && len > p.window ? len - p.window : 0u;
         volatile unsigned long long* ref = reinterpret_cast<volatile unsigned long long*>(smem + L::kOffRef) + rt * kBM + r;
         auto ref_after = [&](uint32_t seq, float* value) -> bool {   // the reference as tile seq-1 left it
             // Rolled up at 256: less code in the longer of the tile loops, whose warps wait for instructions (0.7 stalls an issue; 0.3 at 128, where it makes no
@@ -706,12 +796,17 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 tc_fence_before();
                 mbar_arrive(bar(S_EMPTY + buf));   // this row of S is in registers
             }
-            const uint32_t pos0 = static_cast<uint32_t>(tile0 + t) * kBN;
+            const uint32_t pos0 = tile_position(t);
             // Raw scores stay unscaled; the softmax scale is folded into the exponent: p = 2^(s*c - m*c).  The loop's instructions count: products and
             // sums go in pairs, maxima three values at a time.  32 / 8 heads of 128, 1024 tokens over 8192: 168.0 -> 163.7 us; 24 / 4 of 256, 512 over
             // 8192: 111.6 -> 110.3.
             // Only the tiles that straddle this row's causal length need the mask.
-            if (pos0 + kBN > len) {
+            if constexpr (PAGED) {
+                if (pos0 + kBN > len || pos0 < low) {
+#pragma unroll
+                    for (int i = 0; i < kBN; ++i) s[i] = pos0 + i < len && (pos0 + i >= low || pos0 + i < p.sinks) ? s[i] : -INFINITY;
+                }
+            } else if (pos0 + kBN > len) {
 #pragma unroll
                 for (int i = 0; i < kBN; ++i) s[i] = (pos0 + i < len) ? s[i] : -INFINITY;
             }
@@ -799,11 +894,16 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         }
         // ---- epilogue: O / sum, gate, store; the columns are divided among a row's threads ----
         const bool partial = nsplit > 1, gated = !partial && p.gate != nullptr;
-        const size_t part_row0 = (static_cast<size_t>(split) * p.kv_heads + kv_head) * p.rows_padded + row0;
         constexpr int kCols = D / L::kGroups;
         const int col0 = grp * kCols;
+        if constexpr (PAGED) {
+            item = reload(p.items + blockIdx.x);
+            own_rows = static_cast<size_t>(item.first) * p.query_heads * D;
+            part_row0 = static_cast<size_t>(item.part) * kBM;
+            total_rows = item.tokens * G;
+        }
         const RowOffsets<D> rows(warp_row0, turn_row, G, p.query_heads, total_rows);   // worked out anew: no registers for it in between
-        const size_t out0 = (static_cast<size_t>(warp_row0 / G) * p.query_heads + kv_head * G) * D + col0 + 4 * turn_chunk;
+        const size_t out0 = own_rows + (static_cast<size_t>(warp_row0 / G) * p.query_heads + kv_head * G) * D + col0 + 4 * turn_chunk;
         float4 g[8];
         auto fetch_gate = [&](int i, int c0) {
             if (i < rows.valid) g[i] = *reinterpret_cast<const float4*>(p.gate + out0 + rows.rel[i] + c0);
@@ -833,9 +933,14 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
             if (partial && gr < total_rows && grp == 0)   // a poisoned or empty partial is recognised by its sum
                 p.part_ml[part_row0 + rt * kBM + r] = make_float2(m_ref, failed ? __int_as_float(0x7fc00000) : (len == 0 ? 0.0f : l_sum));
+            if constexpr (PAGED) {
+                if (!partial && p.lse != nullptr && gr < total_rows && grp == 0)
+                    p.lse[(static_cast<size_t>(item.first) + gr / G) * p.query_heads + kv_head * G + gr % G] =
+                        failed ? __int_as_float(0x7fc00000) : l_sum > 0.0f ? (m_ref + log2f(l_sum)) * 0.69314718055994531f : -INFINITY;
+            }
             // Rows leave 32 columns at a time through the same 4 KB per warp: read back four rows an instruction, 128
             // contiguous bytes each, so that the gate is fetched and the result stored in whole lines.
-            float* const dst = partial ? p.part_o + (part_row0 + (warp_row0 - row0) + turn_row) * D + col0 + 4 * turn_chunk : p.out + out0;
+            float* const dst = partial ? p.part_o + (part_row0 + (warp_row0 - row0) + turn_row) * D + col0 + 4 * turn_chunk : PAGED ? nullptr : p.out + out0;
             const bool zero = len == 0 && !partial;
             const float factor = failed ? __int_as_float(0x7fc00000) : partial ? 1.0f : inv;
 #pragma unroll 1
@@ -883,7 +988,9 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                             v.z *= 1.0f / (1.0f + __expf(-g[i].z)); v.w *= 1.0f / (1.0f + __expf(-g[i].w));
                         }
                     }
-                    if (i < rows.valid) *reinterpret_cast<float4*>(dst + (partial ? static_cast<uint32_t>(4 * i * D) : rows.rel[i]) + c0) = v;
+                    if (i >= rows.valid) continue;
+                    if (PAGED && !partial) store_out(out0 + rows.rel[i] + c0, v);
+                    else *reinterpret_cast<float4*>(dst + (partial ? static_cast<uint32_t>(4 * i * D) : rows.rel[i]) + c0) = v;
                 }
                 __syncwarp();
             }
@@ -1090,7 +1197,8 @@ int launch_tc5(const b200kv_view& view, Tc5Params& p, __half* k_scratch, __half*
     }
     const uint32_t G = p.query_heads / p.kv_heads;
     const uint32_t row_tiles = (p.token_count * G + L::kRows - 1) / L::kRows;
-    B200KV_CUDA_TRY(launch_kernel(prefill_tc5_kernel<D, RT, STATE>, dim3(row_tiles * p.kv_heads * p.kv_splits), dim3(L::kThreads), L::kAlloc, stream, true, p));
+    KernelParams<false> kp{p};
+    B200KV_CUDA_TRY(launch_kernel(prefill_tc5_kernel<D, RT, STATE>, dim3(row_tiles * p.kv_heads * p.kv_splits), dim3(L::kThreads), L::kAlloc, stream, true, kp));
     if (p.kv_splits > 1) {
         PrefillMergeParams mp{};
         mp.part_o = p.part_o;
@@ -1244,6 +1352,41 @@ int launch_prefill_tc5_prepare(const b200kv_view& view, uint32_t prepared_rows, 
     __half* v_scratch = k_scratch + static_cast<size_t>(view.kv_heads) * scratch_rows * view.head_dim;
     return view.head_dim == 128 ? launch_dequant<128>(view, k_scratch, v_scratch, prepared_rows, scratch_rows, 0, prepared_rows, Sides{true, true}, stream)
                                 : launch_dequant<256>(view, k_scratch, v_scratch, prepared_rows, scratch_rows, 0, prepared_rows, Sides{true, true}, stream);
+}
+
+// Chunks over a paged cache: the attention kernel alone, behind the call's other kernels.
+template <int D>
+static int launch_chunk_of(const KernelParams<true>& p, uint32_t max_items, cudaStream_t stream) {
+    using L = Layout<D, 1>;
+    static std::atomic<uint64_t> done{0};
+    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prefill_tc5_kernel<D, 1, false, true>), L::kAlloc, done));
+    B200KV_CUDA_TRY(launch_behind(prefill_tc5_kernel<D, 1, false, true>, dim3(max_items), dim3(L::kThreads), L::kAlloc, stream, p));
+    return B200KV_OK;
+}
+int launch_chunk(const ChunkLaunch& c, cudaStream_t stream) {
+    static_assert(kChunkRows == kBM && kChunkTile == kBN);
+    KernelParams<true> p{};
+    if (!encode_f16_plane(&p.kmap, c.k_scratch, c.head_dim, c.scratch_rows, c.scratch_rows, c.kv_heads) ||
+        !encode_f16_plane(&p.vmap, c.v_scratch, c.head_dim, c.scratch_rows, c.scratch_rows, c.kv_heads))
+        return B200KV_ERR_UNSUPPORTED;
+    p.q = c.q;
+    p.q_is_f16 = c.q_is_f16;
+    p.gate = c.gate;
+    p.query_heads = c.query_heads;
+    p.kv_heads = c.kv_heads;
+    p.scale_log2 = c.scale_log2;
+    p.kv_splits = 1;
+    p.sms = device_sms();
+    p.part_o = c.part_o;
+    p.part_ml = c.part_ml;
+    p.items = c.items;
+    p.plan = c.plan;
+    p.typed_out = c.out;
+    p.out_is_f16 = c.out_is_f16;
+    p.lse = c.lse;
+    p.window = c.window;
+    p.sinks = c.sinks;
+    return c.head_dim == 256 ? launch_chunk_of<256>(p, c.max_items, stream) : launch_chunk_of<128>(p, c.max_items, stream);
 }
 
 }  // namespace b200kv

@@ -9,11 +9,13 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <cstring>
+#include <utility>
 #include <vector>
 
 #include "b200kv.h"
@@ -27,10 +29,17 @@ struct Api {
     decltype(&b200kv_decode_step) decode_step;
     decltype(&b200kv_decode_attn_batched) decode_attn_batched;
     decltype(&b200kv_prefill_attn_prepared) prefill_attn_prepared;
+    decltype(&b200kv_paged_store) paged_store;
+    decltype(&b200kv_paged_load) paged_load;
+    decltype(&b200kv_paged_attn) paged_attn;
+    decltype(&b200kv_paged_weights) paged_weights;
+    decltype(&b200kv_paged_evict) paged_evict;
     decltype(&b200kv_pool_capture) pool_capture;
     decltype(&b200kv_pool_restore) pool_restore;
 } g_api;
 PyObject* g_view_type;   // the ctypes structure of a cache view
+PyObject* g_paged_view_type;    // ... of a paged cache's view, and of a batch over it
+PyObject* g_paged_batch_type;
 
 // One call's arguments, read left to right; the first failure sticks and leaves a Python exception set.
 class Args {
@@ -103,6 +112,50 @@ public:
         }
         return views(1, false);
     }
+    // A paged cache's view or a batch over it, likewise.
+    template <typename T>
+    const T* structure(PyObject* type, const char* what) {
+        if (!ok_) return nullptr;
+        PyObject* o = args_[i_++];
+        const int is = PyObject_IsInstance(o, type);
+        if (is <= 0) {
+            if (is == 0) PyErr_Format(PyExc_TypeError, "expected %s, got %s", what, Py_TYPE(o)->tp_name);
+            ok_ = false;
+            return nullptr;
+        }
+        if (PyObject_GetBuffer(o, &buffers_[held_], PyBUF_SIMPLE) != 0) { ok_ = false; return nullptr; }
+        const Py_buffer& b = buffers_[held_++];
+        if (static_cast<size_t>(b.len) < sizeof(T)) { fail(PyExc_ValueError, "a structure of another size"); return nullptr; }
+        return static_cast<const T*>(b.buf);
+    }
+    const b200kv_paged_view* paged_view() { return structure<b200kv_paged_view>(g_paged_view_type, "a paged cache's view"); }
+    const b200kv_paged_batch* paged_batch() { return structure<b200kv_paged_batch>(g_paged_batch_type, "a paged batch"); }
+    // A tensor of one type and at least `least` elements, or None where that is allowed.
+    template <typename T>
+    T* exactly(at::ScalarType type, const char* text, uint64_t least, bool optional = false) {
+        if (!ok_) return nullptr;
+        PyObject* o = args_[i_];
+        if (o == Py_None) {
+            if (!optional) fail(PyExc_ValueError, "a tensor is required");
+            ++i_;
+            return nullptr;
+        }
+        int64_t n = 0;
+        void* p = tensor(&n);
+        if (!ok_) return nullptr;
+        if (!here(o)) return nullptr;
+        if (THPVariable_Unpack(o).scalar_type() != type || static_cast<uint64_t>(n) < least) return static_cast<T*>(fail(PyExc_ValueError, text));
+        return static_cast<T*>(p);
+    }
+    // An activation tensor of fp16 or fp32 with at least `least` elements.
+    void* activation(int* dtype, uint64_t least, const char* text) {
+        int64_t n = 0;
+        PyObject* o = ok_ ? args_[i_] : nullptr;
+        void* p = tensor(&n, dtype);
+        if (!ok_ || !here(o)) return nullptr;
+        if (static_cast<uint64_t>(n) < least) return fail(PyExc_ValueError, text);
+        return p;
+    }
     // An array of them (the caller has built it), or None.
     const b200kv_view* views(uint32_t count, bool optional) {
         if (!ok_) return nullptr;
@@ -143,6 +196,11 @@ public:
     }
 
 private:
+    bool here(PyObject* o) {   // on the current device, whose stream the launch goes to
+        if (THPVariable_Unpack(o).get_device() == c10::cuda::current_device()) return true;
+        fail(PyExc_ValueError, "a tensor of another device than the current one");
+        return false;
+    }
     uint32_t checked(uint32_t v) {
         if (v == 0xffffffffu && PyErr_Occurred()) ok_ = false;
         return v;
@@ -293,6 +351,101 @@ PyObject* py_suffix_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- the paged cache ------------------------------------------------------------------------------------------
+
+constexpr const char* kSmall = "a tensor of another type, or with fewer elements than the batch has rows";
+
+PyObject* py_paged_store(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 10);
+    int kd = 0, vd = 0;
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const uint64_t tokens = a.ok() ? batch->total_tokens : 0, width = a.ok() ? static_cast<uint64_t>(view->kv_heads) * view->head_dim : 0;
+    const void* key = a.activation(&kd, tokens * width, kSmall);
+    const void* value = a.activation(&vd, tokens * width, kSmall);
+    if (a.ok() && kd != vd) a.fail(PyExc_ValueError, "key and value must share a dtype");
+    const float* w = a.exactly<const float>(at::kFloat, "the norm's weight: fp32 of head_dim elements", a.ok() ? view->head_dim : 0, true);
+    const int rope = a.rope();
+    const float theta = a.f32(), eps = a.f32();
+    const int32_t* positions = a.exactly<const int32_t>(at::kInt, "positions: int32 of every token", tokens, true);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.paged_store(view, batch, key, value, kd, w, rope, theta, eps, positions, s); });
+}
+
+PyObject* py_paged_load(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 5);
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const uint64_t least = a.ok() ? static_cast<uint64_t>(batch->total_tokens) * view->kv_heads * view->head_dim : 0;
+    void* key = a.exactly<void>(at::kHalf, kSmall, least, true);
+    void* value = a.exactly<void>(at::kHalf, kSmall, least, true);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.paged_load(view, batch, key, value, s); });
+}
+
+PyObject* py_paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 12);
+    int qd = 0, od = 0;
+    int64_t ws_bytes = 0;
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const uint32_t heads = a.u32();
+    const uint64_t rows = a.ok() ? static_cast<uint64_t>(batch->total_tokens) * heads : 0, dim = a.ok() ? view->head_dim : 0;
+    const void* q = a.activation(&qd, rows * dim, kSmall);
+    const float* gate = a.exactly<const float>(at::kFloat, kSmall, rows * dim, true);
+    void* out = a.activation(&od, rows * dim, kSmall);
+    float* lse = a.exactly<float>(at::kFloat, kSmall, rows, true);
+    const float scale = a.f32();
+    const uint32_t window = a.u32(), sinks = a.u32();
+    void* ws = a.exactly<void>(at::kByte, "workspace: a uint8 tensor", 0, true);
+    if (a.ok() && ws != nullptr) ws_bytes = THPVariable_Unpack(args[10]).numel();
+    void* s = a.stream();
+    return call(a, [&] {
+        return g_api.paged_attn(view, batch, q, qd, gate, out, od, lse, heads, scale, window, sinks, ws, static_cast<size_t>(ws_bytes), s);
+    });
+}
+
+PyObject* py_paged_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 11);
+    int qd = 0;
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const uint32_t heads = a.u32();
+    const uint64_t rows = a.ok() ? static_cast<uint64_t>(batch->total_tokens) * heads : 0;
+    const void* q = a.activation(&qd, rows * (a.ok() ? view->head_dim : 0), kSmall);
+    const float* lse = a.exactly<const float>(at::kFloat, kSmall, rows);
+    float* weights = a.exactly<float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]",
+                                      a.ok() ? static_cast<uint64_t>(batch->sequences) * view->kv_heads * batch->max_length : 0);
+    const uint64_t stride = a.ok() && batch->sequences > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[5]).numel()) / (static_cast<uint64_t>(batch->sequences) * view->kv_heads) : 0;
+    const float scale = a.f32();
+    const uint32_t window = a.u32(), sinks = a.u32(), observe = a.u32();
+    void* s = a.stream();
+    if (a.ok() && stride > 0xffffffffu) a.fail(PyExc_ValueError, "weights: too many positions");
+    return call(a, [&] { return g_api.paged_weights(view, batch, q, qd, lse, weights, static_cast<uint32_t>(stride), heads, scale, window, sinks, observe, s); });
+}
+
+PyObject* py_paged_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 11);
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const uint64_t sequences = a.ok() ? batch->sequences : 0, heads = a.ok() ? sequences * view->kv_heads : 0;
+    const uint32_t keep = a.u32(), sinks = a.u32(), recent = a.u32();
+    const int32_t* target = a.exactly<const int32_t>(at::kInt, "target: int32 [sequences][pages]", sequences);
+    const float* weights = a.exactly<const float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]", a.ok() ? heads * batch->max_length : 0);
+    int32_t* kept = a.exactly<int32_t>(at::kInt, "kept: int32 [sequences][kv_heads][keep]", heads * keep);
+    float* new_weights = a.exactly<float>(at::kFloat, "new_weights: fp32 [sequences][kv_heads][keep]", heads * keep, true);
+    int32_t* new_lengths = a.exactly<int32_t>(at::kInt, "new_lengths: int32 [sequences]", sequences);
+    void* s = a.stream();
+    if (!a.ok()) return nullptr;
+    const uint64_t stride = heads > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[6]).numel()) / heads : 0;
+    const uint64_t pages = sequences > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[5]).numel()) / sequences : 0;
+    if (stride > 0xffffffffu || pages > 0xffffffffu) a.fail(PyExc_ValueError, "too many positions or pages");
+    return call(a, [&] {
+        return g_api.paged_evict(view, batch, target, static_cast<uint32_t>(pages), weights, static_cast<uint32_t>(stride), keep, sinks, recent, kept, new_weights,
+                                 new_lengths, s);
+    });
+}
+
 // ---- the snapshot pool: token ids and storage objects in, one library call ------------------------------------
 
 // Anything with a length that can be iterated over, as a list or tuple.
@@ -414,11 +567,17 @@ PyObject* py_pool(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return Py_BuildValue("iI", rc, CAPTURE ? static_cast<unsigned>(captured) : matched);
 }
 
-PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and "View": the structure
+PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the structures "View", "PagedView" and "PagedBatch"
     PyObject* view = PyDict_GetItemString(arg, "View");
     if (view == nullptr || !PyType_Check(view)) return PyErr_Format(PyExc_KeyError, "View");
     Py_INCREF(view);
     Py_XSETREF(g_view_type, view);
+    for (auto [name, slot] : {std::pair{"PagedView", &g_paged_view_type}, std::pair{"PagedBatch", &g_paged_batch_type}}) {
+        PyObject* type = PyDict_GetItemString(arg, name);
+        if (type == nullptr || !PyType_Check(type)) return PyErr_Format(PyExc_KeyError, "%s", name);
+        Py_INCREF(type);
+        Py_XSETREF(*slot, type);
+    }
     struct { const char* name; void** slot; } table[] = {
         {"b200kv_append", reinterpret_cast<void**>(&g_api.append)},
         {"b200kv_q_split_norm_rope", reinterpret_cast<void**>(&g_api.q_split_norm_rope)},
@@ -426,6 +585,11 @@ PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and "View": 
         {"b200kv_decode_step", reinterpret_cast<void**>(&g_api.decode_step)},
         {"b200kv_decode_attn_batched", reinterpret_cast<void**>(&g_api.decode_attn_batched)},
         {"b200kv_prefill_attn_prepared", reinterpret_cast<void**>(&g_api.prefill_attn_prepared)},
+        {"b200kv_paged_store", reinterpret_cast<void**>(&g_api.paged_store)},
+        {"b200kv_paged_load", reinterpret_cast<void**>(&g_api.paged_load)},
+        {"b200kv_paged_attn", reinterpret_cast<void**>(&g_api.paged_attn)},
+        {"b200kv_paged_weights", reinterpret_cast<void**>(&g_api.paged_weights)},
+        {"b200kv_paged_evict", reinterpret_cast<void**>(&g_api.paged_evict)},
         {"b200kv_pool_capture", reinterpret_cast<void**>(&g_api.pool_capture)},
         {"b200kv_pool_restore", reinterpret_cast<void**>(&g_api.pool_restore)},
     };
@@ -462,6 +626,11 @@ PyMethodDef g_methods[] = {{"bind", py_bind, METH_O, nullptr},
                            ENTRY("decode_step", py_decode_step),
                            ENTRY("decode_attn_batched", py_decode_attn_batched),
                            ENTRY("suffix_attn", py_suffix_attn),
+                           ENTRY("paged_store", py_paged_store),
+                           ENTRY("paged_load", py_paged_load),
+                           ENTRY("paged_attn", py_paged_attn),
+                           ENTRY("paged_weights", py_paged_weights),
+                           ENTRY("paged_evict", py_paged_evict),
                            ENTRY("pool_capture", py_pool<true>),
                            ENTRY("pool_restore", py_pool<false>),
                            {nullptr, nullptr, 0, nullptr}};
