@@ -554,7 +554,7 @@ B200KV_API int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_
 
 /* Brings every sequence of more than `keep` positions back to `keep`, each kv head for itself: the first `sinks` and the last `recent` positions stay, and of
  * the others those with the largest weights (ties: the lowest position; a NaN counts as the least).  The rows that stay go, in order, to positions 0, 1, ...
- * of the pages of target_table (DEVICE [sequences][target_max_pages], target_max_pages * page_size >= keep); a sequence of at most `keep` positions
+ * of the pages of target_table (DEVICE [sequences][target_max_pages], target_max_pages * page_size >= min(keep, max_length)); a sequence of at most `keep` positions
  * is copied as it is.  target_table == batch->page_table compacts in place; otherwise the target's pages and the sequences' must not overlap.
  * kept: DEVICE int32 [sequences][kv_heads][keep], the positions that stayed, -1 behind them.  new_weights (may be NULL): fp32 [sequences][kv_heads]
  * [keep], their weights, 0 behind them; must not overlap weights.  new_lengths: DEVICE int32 [sequences] = min(length, keep); not batch->lengths itself.

@@ -3,11 +3,15 @@
 //   o_i = sum_j exp(s_ij - lse_i) v_j,  s_ij = scale q_i.k_j,  lse_i = log sum_j exp s_ij,  j over what token i sees: j <= i, and under a window of w positions
 //   only j > i - w and the first sinks.
 //
+// Sequences of a few query rows take the streaming kernel (paged_decode.cu), the others the chunk kernel; a call launches what its bounds allow, and the
+// kernels find their sequences.
+//
 // The host knows bounds, the device the lengths, so a call over chunks begins with a kernel that lays out the work (paged_plan_kernel: which rows and tiles
 // each CTA of the chunk kernel takes, how many of them share a row tile), goes on with the gather of the visible rows into an fp16 copy, tile by tile
 // as the chunk kernel's TMA reads them (paged_gather_kernel: int8 rows dequantised, rows past a length zero), the chunk kernel itself, and the merge
 // of what its CTAs left for shared row tiles.  Each follows the one before without a gap (programmatic launches).
 #include "dequant.cuh"
+#include "paged_decode.cuh"
 #include "paged_plan.cuh"
 
 #include <algorithm>
@@ -33,7 +37,9 @@ struct PlanParams {
     uint32_t* groups;           // first item of each shared row tile
     uint32_t max_items, max_parts, scratch_tiles;
     uint32_t group, window, sinks, sms;
+    uint32_t few_rows;          // sequences of at most so many query rows are the other kernel's
     ChunkCosts costs;
+    __device__ __forceinline__ bool mine(const Span& span) const { return span.tokens > 0 && static_cast<uint64_t>(span.tokens) * group > few_rows; }
 };
 
 struct Sums { uint32_t a, b, c; };
@@ -98,7 +104,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
         Sums v{0, 0, 0};
         if (s < S) {
             const Span span = span_of(p.pool, s);
-            if (span.tokens > 0) {
+            if (p.mine(span)) {
                 v.a = (span.tokens * p.group + kChunkRows - 1) / kChunkRows;
                 v.b = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles;
             }
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
         float work = 0.0f;
         for (uint32_t s = lane; s < S; s += 32) {
             const Span span = span_of(p.pool, s);
-            if (span.tokens == 0) continue;
+            if (!p.mine(span)) continue;
             const uint32_t tiles = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles, n = (span.tokens * p.group + kChunkRows - 1) / kChunkRows * H;
             const uint32_t pieces = max(1u, (tiles + piece - 1) / piece);
             items += n * pieces;
@@ -364,14 +370,20 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
 struct Room {
     uint64_t scratch_tiles;    // of all sequences together
     uint32_t max_items, max_parts;
-    size_t items, tile_starts, scratch_starts, groups, k, v, part_o, part_ml, bytes;   // offsets
+    bool decode, chunks;       // which kernels the call may need
+    size_t decode_parts, items, tile_starts, scratch_starts, groups, k, v, part_o, part_ml, bytes;   // offsets
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uint32_t query_heads, uint32_t window, uint32_t sinks, uint32_t sms) {
     Room r{};
-    const uint64_t group = query_heads / view.kv_heads, sequences = std::min<uint64_t>(batch.sequences, batch.total_tokens);
+    const uint64_t group = query_heads / view.kv_heads;
+    // A single sequence goes by its bound: the chunk kernel takes a token as well, and the other's launch is saved.
+    r.chunks = !decode_takes_all(batch, static_cast<uint32_t>(group));
+    r.decode = !r.chunks || batch.sequences > 1;
+    const uint64_t least = r.decode ? kDecodeRows / group + 1 : 1;   // new tokens of a sequence of the chunk kernel
+    const uint64_t sequences = std::min<uint64_t>(batch.sequences, batch.total_tokens / least);
     // a sequence's tiles: its length's, or those of its sinks and of the windows of its tokens
     uint64_t each = (static_cast<uint64_t>(batch.max_length) + kChunkTile - 1) / kChunkTile;
     if (window > 0) each = std::min<uint64_t>(each, (static_cast<uint64_t>(sinks) + kChunkTile - 1) / kChunkTile + (static_cast<uint64_t>(window) + batch.max_tokens + kChunkTile - 1) / kChunkTile + 1);
@@ -385,6 +397,11 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     size_t at = 256;                                     // the plan
     const auto take = [&](uint64_t bytes) { const size_t here = at; at += up(bytes, 1024); return here; };
     at = up(at, 1024);
+    r.decode_parts = take(r.decode ? decode_part_bytes(view, query_heads, sms) : 0);
+    if (!r.chunks) {
+        r.bytes = at + 1024;
+        return r;
+    }
     r.items = take(static_cast<uint64_t>(r.max_items) * sizeof(ChunkItem));
     r.tile_starts = take((static_cast<uint64_t>(batch.sequences) + 1) * 4);
     r.scratch_starts = take((static_cast<uint64_t>(batch.sequences) + 1) * 4);
@@ -398,8 +415,6 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     return r;
 }
 
-constexpr uint32_t kWorkspaceSms = 160;   // what the workspace is sized for, on any device
-
 }  // namespace
 
 }  // namespace b200kv
@@ -411,7 +426,7 @@ extern "C" {
 size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window, uint32_t sinks) {
     if (view == nullptr || batch == nullptr || view->kv_heads == 0 || query_heads % view->kv_heads != 0) return 0;
     settle_window(*batch, &window, &sinks);
-    return room_of(*view, *batch, query_heads, window, sinks, kWorkspaceSms).bytes;
+    return room_of(*view, *batch, query_heads, window, sinks, kMostSms).bytes;
 }
 
 int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* gate,
@@ -430,32 +445,38 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     if (workspace == nullptr || workspace_bytes < b200kv_paged_attn_workspace_bytes(view, batch, query_heads, window, sinks)) return B200KV_ERR_WORKSPACE;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    const Room room = room_of(*view, *batch, query_heads, window, sinks, kWorkspaceSms);
+    const Room room = room_of(*view, *batch, query_heads, window, sinks, kMostSms);
     if (room.scratch_tiles * kChunkTile * view->kv_heads > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;
     uint8_t* ws = reinterpret_cast<uint8_t*>(up(reinterpret_cast<uintptr_t>(workspace), 1024));
     const Paged pool = paged_of(*view, *batch);
-    const uint32_t group = query_heads / view->kv_heads, sms = std::min(device_sms(), kWorkspaceSms);
+    const uint32_t group = query_heads / view->kv_heads, sms = std::min(device_sms(), kMostSms);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
-    PlanParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.tile_starts),
-                  reinterpret_cast<uint32_t*>(ws + room.scratch_starts), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items, room.max_parts,
-                  static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms,
-                  view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.3f, 0.017f}};
-    B200KV_CUDA_TRY(launch_kernel(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, pp));
-    GatherParams gp{pool, pp.plan, pp.scratch_starts, {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)},
-                    static_cast<uint32_t>(room.scratch_tiles * kChunkTile), window, sinks};
-    const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
-    B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_gather_kernel<128>, dim3(blocks), dim3(kGatherThreads), 0, s, gp)
-                                          : launch_behind(paged_gather_kernel<256>, dim3(blocks), dim3(kGatherThreads), 0, s, gp));
-    const ChunkLaunch cl{pp.items, pp.plan, room.max_items, gp.out[0], gp.out[1], gp.scratch_rows, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse,
-                         query_heads, view->kv_heads, view->head_dim, window, sinks, scale * 1.4426950408889634f, reinterpret_cast<float*>(ws + room.part_o),
-                         reinterpret_cast<float2*>(ws + room.part_ml)};
-    rc = launch_chunk(cl, s);
-    if (rc != B200KV_OK) return rc;
-    const MergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
-    const dim3 merge_grid(std::min(room.max_parts / 2, 2 * sms), view->head_dim / 32);
-    B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, merge_grid, dim3(256), 0, s, mp)
-                                          : launch_behind(paged_merge_kernel<256>, merge_grid, dim3(256), 0, s, mp));
+    if (room.chunks) {
+        PlanParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.tile_starts),
+                      reinterpret_cast<uint32_t*>(ws + room.scratch_starts), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items, room.max_parts,
+                      static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, room.decode ? kDecodeRows : 0,
+                      view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.3f, 0.017f}};
+        B200KV_CUDA_TRY(launch_kernel(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, pp));
+        GatherParams gp{pool, pp.plan, pp.scratch_starts, {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)},
+                        static_cast<uint32_t>(room.scratch_tiles * kChunkTile), window, sinks};
+        const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
+        B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_gather_kernel<128>, dim3(blocks), dim3(kGatherThreads), 0, s, gp)
+                                              : launch_behind(paged_gather_kernel<256>, dim3(blocks), dim3(kGatherThreads), 0, s, gp));
+        const ChunkLaunch cl{pp.items, pp.plan, room.max_items, gp.out[0], gp.out[1], gp.scratch_rows, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse,
+                             query_heads, view->kv_heads, view->head_dim, window, sinks, scale * 1.4426950408889634f, reinterpret_cast<float*>(ws + room.part_o),
+                             reinterpret_cast<float2*>(ws + room.part_ml)};
+        rc = launch_chunk(cl, s);
+        if (rc != B200KV_OK) return rc;
+        const MergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
+        const dim3 merge_grid(std::min(room.max_parts / 2, 2 * sms), view->head_dim / 32);
+        B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, merge_grid, dim3(256), 0, s, mp)
+                                              : launch_behind(paged_merge_kernel<256>, merge_grid, dim3(256), 0, s, mp));
+    }
+    if (room.decode) {
+        PagedDecode dp{pool, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse, query_heads, window, sinks, scale * 1.4426950408889634f};
+        return launch_paged_decode(dp, ws + room.decode_parts, s, room.chunks);
+    }
     return B200KV_OK;
 }
 

@@ -1,0 +1,950 @@
+// Attention of a few query rows per sequence over a paged cache: a decode step of many sequences, one new token or a few each.
+//
+// Bound by HBM: every visible row of K and V is read once for all query rows of its kv head, and the kernel's work is to keep copies under way on every SM.
+//
+//  * The tiles of 128 positions of all (sequence, kv head) pairs form one list, and every CTA of a grid that fits the device at once takes an equal piece
+//    of it, whatever the lengths are (sequences of 512 to 16384 positions in one launch end together).  A piece crosses from one pair to the next with its
+//    copies running on; a pair that lies in several pieces leaves partials, two a CTA at most, for paged_decode_merge_kernel.  Nothing waits for another CTA.
+//  * K and V come as units of 128 rows through tensor maps over the whole pool, a box a page (pages of less than 128 positions: several), each into a ring
+//    of its own, the block scales beside them as bulk copies.  (One ring K0 V0 K1 V1 ... of an odd number of units would show an issuer, which reads one of
+//    the two, every second phase of a slot only, and a parity does not tell those apart.)  The bytes are operands as they land:
+//      S^T = K Q^T        M = 128 positions (a thread each), N = 16 columns
+//      O^T = V^T P        M = 128 dims (a thread each, per half of 256), K = positions
+//    int8 sides on kind::i8 -- the sums of a block of 32 dims are exact, so its scale multiplies the sum -- and fp16 sides on kind::f16.
+//  * Against int8 keys a query is a whole number in two int8 planes (16 bits; 8 rows) or three (24 bits; up to 4 rows: they fit the 16 columns all the
+//    same); against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
+//    position's value scale, in two uint8 planes; for fp16 values two fp16 terms.  Sums of a tile are folded into fp32 registers.
+//  * A softmax thread has four query rows of a position; with five to eight rows a second group of 128 threads has the others.
+//  * Positions that no row sees weigh nothing and their values are cleared in shared memory where they are fp16 (0 x NaN is NaN), tiles that nobody sees
+//    (between the sinks and the window) are not in the list.
+// Every wait is bounded: one that runs out poisons the CTA's results with NaN, sets a status bit, and the CTA ends in the normal way.
+#include "paged_decode.cuh"
+#include "decode_common.cuh"
+#include "mbarrier_wait.cuh"
+
+#include <algorithm>
+
+namespace b200kv {
+
+namespace {
+
+enum Fmt { F16 = 0, ROW = 1, BLOCK = 2 };   // a side's storage: fp16, int8 with one scale per row, int8 with a scale per 32 dims
+
+template <int D, int KF, int VF, int RG>   // RG: groups of four query rows
+struct Layout {
+    static constexpr int kTile = kDecodeTile;
+    static constexpr int kHalves = D / 128;
+    static constexpr int kSoftmax = RG * 128;
+    static constexpr int kProducerWarp = RG * 4, kSWarp = kProducerWarp + 1, kPvWarp = kSWarp + 1, kQWarp = kPvWarp + 1;
+    static constexpr int kThreads = kSoftmax + 128;
+    static constexpr int kCtas = D == 128 && KF != F16 && VF != F16 && RG == 1 ? 2 : 1;   // per SM
+    static constexpr int kKData = kTile * D * (KF == F16 ? 2 : 1), kVData = kTile * D * (VF == F16 ? 2 : 1);
+    static constexpr int kKScales = KF == F16 ? 0 : kTile * 2 * (KF == BLOCK ? D / 32 : 1), kVScales = VF == F16 ? 0 : kTile * 2 * (VF == BLOCK ? D / 32 : 1);
+    // weights of a row group: rows of 32 bytes per position, one set per half of the dims where the halves' scales differ
+    static constexpr int kPSets = VF == BLOCK ? kHalves : 1;
+    static constexpr int kPBytes = kPSets * kTile * 32;
+    [[maybe_unused]] static constexpr int kPlanes = KF == F16 || RG == 2 ? 2 : 3;                          // of a query row
+    static constexpr int kQBytes = 16 * D * (KF == F16 ? 2 : 1);
+    static constexpr int kSCols = KF == BLOCK ? D / 32 * 16 : 16;                         // TMEM columns of a score buffer
+    static constexpr int kOCols = RG * kHalves * 32;                                      // of a buffer of sums
+    static constexpr uint32_t kTmemCols = 2 * (kSCols + kOCols) <= 128 ? 128 : 2 * (kSCols + kOCols) <= 256 ? 256 : 512;
+    static constexpr uint32_t kColS = 0, kColO = 2 * kSCols;
+    static constexpr int kXchWords = 16;                                                  // 4 maxima of scores, up to 8 of value scales
+    static constexpr int kMiscBytes = RG * 2 * 4 * kXchWords * 4 + RG * 64 + 2 * 8 * 4 + 12 * 16 + 24 * 8 + 64;
+    static constexpr int kMostUnits = 6;
+    static constexpr int kBudget = (kCtas == 2 ? 115712 : 232448) - 1024;                 // the base is brought to a multiple of 1024
+    static constexpr int kFixed = 2 * RG * kPBytes + 2 * kQBytes + kMiscBytes;
+    static constexpr int kKUnit = kKData + kKScales, kVUnit = kVData + kVScales, kRoom = kBudget - kFixed;
+    // a V unit is held for longer, until its weights are there, so V has the odd one
+    static constexpr int units(bool v) {
+        int k = 1, n = 1;
+        while (true) {
+            if (n < kMostUnits && n <= k && k * kKUnit + (n + 1) * kVUnit <= kRoom) ++n;
+            else if (k < kMostUnits && (k + 1) * kKUnit + n * kVUnit <= kRoom) ++k;
+            else if (n < kMostUnits && k * kKUnit + (n + 1) * kVUnit <= kRoom) ++n;
+            else return v ? n : k;
+        }
+    }
+    static constexpr int kKUnits = units(false), kVUnits = units(true);
+    static constexpr int kOffV = kKUnits * kKData;
+    static constexpr int kOffP = kOffV + kVUnits * kVData;                                // [buffer][group]
+    static constexpr int kOffQ = kOffP + 2 * RG * kPBytes;                                // [buffer]
+    static constexpr int kOffKScales = kOffQ + 2 * kQBytes, kOffVScales = kOffKScales + kKUnits * kKScales;
+    static constexpr int kOffXch = kOffVScales + kVUnits * kVScales;                      // [group][parity][warp][words]
+    static constexpr int kOffSum = kOffXch + RG * 2 * 4 * kXchWords * 4;                  // [group][warp][4]
+    static constexpr int kOffQmul = kOffSum + RG * 64;                                    // [buffer][8]
+    static constexpr int kOffBar = kOffQmul + 2 * 8 * 4;
+    static constexpr int K_FULL = 0, V_FULL = K_FULL + kKUnits, K_EMPTY = V_FULL + kVUnits, V_EMPTY = K_EMPTY + kKUnits, LANDED = V_EMPTY + kVUnits, S_FULL = LANDED + 1, S_EMPTY = S_FULL + 2, P_FULL = S_EMPTY + 2, P_EMPTY = P_FULL + 2 * RG,
+                         Q_FULL = P_EMPTY + 2 * RG, Q_EMPTY = Q_FULL + 2, kNumBars = Q_EMPTY + 2;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8;                               // tmem slot, fail flag, the piece
+    static constexpr int kTotal = (kOffMisc + 32 + 15) / 16 * 16;
+    static constexpr int kAlloc = kTotal + 1024;
+    static_assert(kTotal <= kBudget);
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// Shared-memory matrix descriptor (sm_100 format); `layout`: 2 = 128-byte swizzle, 6 = 32-byte swizzle.  K-major: rows of 128 bytes, groups of eight `sbo` apart.
+// MN-major: one swizzle span contiguous along M or N, consecutive k a span apart, groups of eight k `sbo`, further spans `lbo` apart.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes, uint32_t layout) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(layout) << 61;
+    return d;
+}
+// Instruction descriptors: kind::i8 with int32 sums (formats: 1 = signed), kind::f16 with fp16 operands and fp32 sums.
+__host__ __device__ constexpr uint32_t idesc_i8(uint32_t m, uint32_t n, uint32_t a_signed, uint32_t b_signed, uint32_t a_mn, uint32_t b_mn) {
+    return (2u << 4) | (a_signed << 7) | (b_signed << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, uint32_t a_mn, uint32_t b_mn) {
+    return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }"
+                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, int (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, int (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
+// The sum of a value's two terms.  Where the first is infinite or NaN it is the result: the second is 0 x infinity, or what was left of infinity.
+__device__ __forceinline__ float terms(float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// ---- the list of tiles -------------------------------------------------------------------------------------------------------------
+
+// A sequence's tiles, the same for each of its kv heads: those of the sinks, if the window leaves a gap behind them, then those from tile `first` on.
+struct Tiles { uint32_t n, sink, first; };
+__device__ __forceinline__ Tiles tiles_of(const PagedDecode& p, const Span& span) {
+    const uint32_t group = p.query_heads / p.pool.view.kv_heads;
+    if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * group > kDecodeRows) return {0, 0, 0};
+    const uint32_t all = (span.length + kDecodeTile - 1) / kDecodeTile;
+    Tiles t{max(all, 1u), 0, 0};   // one tile where there is no position: the rows that see nothing come out as zeros
+    if (p.window == 0) return t;
+    const long long lowest = static_cast<long long>(span.base()) + 1 - p.window;
+    const uint32_t first = lowest > 0 ? static_cast<uint32_t>(lowest) / kDecodeTile : 0, sink = (p.sinks + kDecodeTile - 1) / kDecodeTile;
+    if (first <= sink || first >= all) return t;
+    return {sink + all - first, sink, first};
+}
+
+// Tiles of all pairs before sequence s (up to S: of all), of which a warp adds up 32 sequences at a time.
+__device__ uint64_t tiles_before(const PagedDecode& p, uint32_t s, int lane) {
+    uint64_t sum = 0;
+    for (uint32_t i = lane; i < s; i += 32) sum += tiles_of(p, span_of(p.pool, i)).n;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum * p.pool.view.kv_heads;
+}
+
+// CTAs that have a piece, and where piece c begins.
+__device__ __forceinline__ uint32_t pieces_of(const PagedDecode& p, uint64_t all) {
+    return static_cast<uint32_t>(min(static_cast<uint64_t>(p.ctas), max(static_cast<uint64_t>(1), all / p.least_tiles)));
+}
+__device__ __forceinline__ uint64_t piece_begin(uint64_t all, uint32_t c, uint32_t pieces) {
+    const uint64_t each = all / pieces, more = all % pieces;
+    return c * each + min(static_cast<uint64_t>(c), more);
+}
+
+// A place in the list, and how much of the piece is left from there.
+struct Cursor {
+    uint32_t s, head, tile;
+    uint64_t left;
+    Span span;
+    Tiles t;
+    __device__ __forceinline__ void settle(const PagedDecode& p) {   // the pair's sequence
+        span = span_of(p.pool, s);
+        t = tiles_of(p, span);
+    }
+    __device__ __forceinline__ uint32_t take() const { return static_cast<uint32_t>(min(left, static_cast<uint64_t>(t.n - tile))); }   // tiles of this pair
+    __device__ __forceinline__ void advance(const PagedDecode& p) {  // to the next pair that has tiles
+        left -= take();
+        tile = 0;
+        if (left == 0 || ++head < p.pool.view.kv_heads) return;
+        head = 0;
+        do {
+            ++s;
+            settle(p);
+        } while (t.n == 0 && s + 1 < p.pool.batch.sequences);
+    }
+    __device__ __forceinline__ uint32_t position(uint32_t j) const {   // first position of the pair's tile j
+        return (j < t.sink ? j : t.first + (j - t.sink)) * kDecodeTile;
+    }
+};
+
+template <int D, int KF, int VF, int RG>
+__global__ void __launch_bounds__(Layout<D, KF, VF, RG>::kThreads, Layout<D, KF, VF, RG>::kCtas)
+paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using L = Layout<D, KF, VF, RG>;
+    constexpr int kHalves = L::kHalves;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::kOffBar;
+    auto bar = [&](int i) { return bar0 + i * 8; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+    volatile uint32_t* fail_flag = tmem_slot + 1;
+    uint32_t* start = tmem_slot + 2;   // the piece: sequence, head, tile, and how many tiles (two words)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H;
+
+    // ---- set-up ---------------------------------------------------------------------------------------------
+    pdl_launch_dependents();
+    if (warp == L::kProducerWarp && lane == 0) {
+        for (int i = 0; i < L::kNumBars; ++i) {
+            uint32_t count = 1;
+            if (i >= L::K_EMPTY && i < L::LANDED) count = 1 + RG * 4;                     // the MMAs that read it, and a lane of every softmax warp
+            else if (i >= L::S_EMPTY && i < L::P_FULL) count = RG * 128;
+            else if (i >= L::P_FULL && i < L::P_EMPTY) count = 128;
+            else if (i >= L::Q_EMPTY) count = 1 + RG * 4;
+            mbar_init(bar(i), count);
+        }
+        *fail_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    } else if (warp == L::kSWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();   // lengths, queries and cache rows come from preceding kernels
+    if (warp == L::kPvWarp) {   // this CTA's piece of the list
+        const uint32_t S = p.pool.batch.sequences;
+        const uint64_t all = tiles_before(p, S, lane);
+        const uint32_t pieces = pieces_of(p, all);
+        uint64_t begin = 0, count = 0;
+        if (all > 0 && blockIdx.x < pieces) {
+            begin = piece_begin(all, blockIdx.x, pieces);
+            count = piece_begin(all, blockIdx.x + 1, pieces) - begin;
+        }
+        if (count > 0) {
+            uint64_t before = 0;   // the sequence in which it begins, 32 at a time
+            for (uint32_t s0 = 0; s0 < S; s0 += 32) {
+                const uint32_t s = s0 + lane;
+                const uint32_t n = s < S ? tiles_of(p, span_of(p.pool, s)).n : 0;
+                uint64_t inc = static_cast<uint64_t>(n) * H;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += u;
+                }
+                const uint64_t mine = before + inc - static_cast<uint64_t>(n) * H;
+                if (n > 0 && begin >= mine && begin < before + inc) {
+                    start[0] = s;
+                    start[1] = static_cast<uint32_t>((begin - mine) / n);
+                    start[2] = static_cast<uint32_t>((begin - mine) % n);
+                }
+                before += __shfl_sync(0xffffffffu, inc, 31);
+                if (begin < before) break;
+            }
+        }
+        if (lane == 0) {
+            start[3] = static_cast<uint32_t>(count);
+            start[4] = static_cast<uint32_t>(count >> 32);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    Cursor c;
+    c.s = start[0];
+    c.head = start[1];
+    c.tile = start[2];
+    c.left = start[3] | static_cast<uint64_t>(start[4]) << 32;
+    if (c.left > 0) c.settle(p);
+    bool failed = false;
+
+    if (warp == L::kProducerWarp) {
+        // =============================== copies: K and V units, a page's rows each lane ===============================
+        const uint32_t seg = min(p.pool.view.page_size, kDecodeTile), segs = kDecodeTile / seg;   // rows of a box; boxes of a tile
+        uint32_t i = 0, fixes = 0;
+        for (; c.left > 0 && !failed; c.advance(p)) {
+            const int32_t* pages = pages_of(p.pool, c.s);
+            const int lowest = p.window > 0 ? c.span.base() + 1 - static_cast<int>(p.window) : 0;
+            const uint32_t low = lowest > 0 ? static_cast<uint32_t>(lowest) : 0;   // positions below it that are not sinks are seen by nobody
+            const uint32_t n = c.take();
+            for (uint32_t j = 0; j < n && !failed; ++j, ++i) {
+                const uint32_t pos0 = c.position(c.tile + j), mine = pos0 + lane * seg;
+                const bool there = static_cast<uint32_t>(lane) < segs && mine < c.span.length;
+                long long row = -1;
+                if (there) {
+                    row = page_row(p.pool, pages[mine >> p.pool.page_shift], c.head);
+                    if (row >= 0) row += mine & ((1u << p.pool.page_shift) - 1);
+                }
+                const uint32_t found = __popc(__ballot_sync(0xffffffffu, row >= 0));
+                const uint32_t missing = __ballot_sync(0xffffffffu, there && row < 0);       // boxes of no page: zeros
+                const bool edge = pos0 + kDecodeTile > c.span.length || (pos0 < low && pos0 + kDecodeTile > p.sinks);
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                    const int fmt = side == 0 ? KF : VF;
+                    const int data = fmt == F16 ? 2 * D : D, slabs = data / 128, scale = fmt == F16 ? 0 : fmt == BLOCK ? D / 16 : 2;   // bytes of a row
+                    const uint32_t units = side == 0 ? L::kKUnits : L::kVUnits, slot = i % units;
+                    if (i >= units && !wait_warp(bar((side == 0 ? L::K_EMPTY : L::V_EMPTY) + slot), ((i / units) & 1) ^ 1)) { failed = true; break; }
+                    const uint32_t off = side == 0 ? slot * L::kKData : L::kOffV + slot * L::kVData;
+                    const uint32_t scale_off = side == 0 ? L::kOffKScales + slot * L::kKScales : L::kOffVScales + slot * L::kVScales;
+                    const uint32_t dst = sbase + off, sdst = sbase + scale_off, full = bar((side == 0 ? L::K_FULL : L::V_FULL) + slot);
+                    const bool fix = missing != 0 || (side == 1 && VF == F16 && edge);
+                    const uint32_t to = fix ? bar(L::LANDED) : full;
+                    const uint32_t bytes = found * seg * (data + scale);
+                    if (lane == 0) {
+                        if (bytes > 0) mbar_expect_tx(to, bytes);
+                        else if (!fix) mbar_arrive(to);
+                    }
+                    __syncwarp();
+                    if (row >= 0) {
+                        for (int x = 0; x < slabs; ++x)   // 128 bytes of every row
+                            tma_load_2d(dst + x * (kDecodeTile * 128) + lane * seg * 128, side == 0 ? &kmap : &vmap, x * (fmt == F16 ? 64 : 128), static_cast<int>(row), to);
+                        if (fmt != F16)
+                            bulk_load(sdst + lane * seg * scale, static_cast<const uint8_t*>(side == 0 ? p.pool.view.key_scales : p.pool.view.value_scales) + static_cast<size_t>(row) * scale,
+                                      seg * scale, to);
+                    }
+                    if (fix) {   // what is not seen, or of no page, is cleared before anybody reads the unit
+                        if (bytes > 0) {
+                            if (!wait_warp(to, fixes & 1)) { failed = true; break; }
+                            ++fixes;
+                        }
+                        for (uint32_t r = 0; r < kDecodeTile; ++r) {
+                            const uint32_t pos = pos0 + r;
+                            const bool unseen = side == 1 && VF == F16 && (pos >= c.span.length || (pos < low && pos >= p.sinks));
+                            if (!unseen && !((missing >> (r / seg)) & 1)) continue;
+                            if (lane < slabs * 8) *reinterpret_cast<uint4*>(smem + off + (lane >> 3) * (kDecodeTile * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            if (fmt != F16 && lane < scale / 2) *reinterpret_cast<uint16_t*>(smem + scale_off + r * scale + lane * 2) = 0;
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full);
+                    }
+                }
+            }
+        }
+    } else if (warp == L::kQWarp) {
+        // =============================== the query rows of a pair, as the operand of its score MMAs ===============================
+        // 16 rows of the operand: row 4 plane + r (three planes of four query rows) or 8 plane + r (two of eight); rows of 128-byte slabs, 128-byte swizzle.
+        constexpr int E = D / 32;   // consecutive elements a lane has
+        for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
+            const uint32_t buf = k & 1;
+            const uint32_t rows = c.span.tokens * G;
+            float x[RG * 4][E];
+#pragma unroll
+            for (int r = 0; r < RG * 4; ++r) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[r][e] = 0.0f;
+                if (static_cast<uint32_t>(r) >= rows) continue;
+                const size_t at = ((static_cast<size_t>(c.span.first) + r / G) * p.query_heads + c.head * G + r % G) * D + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    if (p.q_is_f16) {
+                        const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + at + e);
+                        const float2 a = unpack2(raw.x), b = unpack2(raw.y);
+                        x[r][e] = a.x; x[r][e + 1] = a.y; x[r][e + 2] = b.x; x[r][e + 3] = b.y;
+                    } else {
+                        const float4 raw = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + e);
+                        x[r][e] = raw.x; x[r][e + 1] = raw.y; x[r][e + 2] = raw.z; x[r][e + 3] = raw.w;
+                    }
+                }
+            }
+            if (k >= 2 && !wait_warp(bar(L::Q_EMPTY + buf), ((k >> 1) & 1) ^ 1)) break;
+            uint8_t* q = smem + L::kOffQ + buf * L::kQBytes;
+#pragma unroll
+            for (int r = 0; r < RG * 4; ++r) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[r][e]));
+                amax = warp_max(amax);
+                if constexpr (KF == F16) {
+                    // scaled by a power of two, the largest element to [2^13, 2^14), and split into two fp16 terms
+                    const int exponent = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+                    const int up = amax > 0.0f ? max(-100, min(100, 13 - exponent)) : 0;
+                    const float mult = exp2i(up);
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const int dim = lane * E + e, chunk = (dim % 64) / 8;
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a = x[r][e + 2 * i] * mult, b = x[r][e + 2 * i + 1] * mult;
+                            hi[i] = pack2(a, b);
+                            const float2 h = unpack2(hi[i]);
+                            lo[i] = pack2(a - h.x, b - h.y);
+                        }
+                        auto at = [&](int row) { return q + (dim / 64) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4) + (dim % 8) * 2; };
+                        *reinterpret_cast<uint2*>(at(r)) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(at(8 + r)) = make_uint2(lo[0], lo[1]);
+                    }
+                    if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = p.scale_log2 * exp2i(-up);
+                } else {
+                    constexpr float kMost = L::kPlanes == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
+                    const float inv = amax > 0.0f ? kMost / amax : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const int dim = lane * E + e, chunk = (dim % 128) / 16;
+                        uint32_t w[3] = {0, 0, 0};   // the planes from the lowest digit: signed bytes
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            int v = __float2int_rn(x[r][e + i] * inv);
+#pragma unroll
+                            for (int d = 0; d < L::kPlanes; ++d) {
+                                const int digit = d + 1 < L::kPlanes ? ((v + 128) & 255) - 128 : v;
+                                w[d] |= static_cast<uint32_t>(digit & 0xff) << (8 * i);
+                                v = (v - digit) >> 8;
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < L::kPlanes; ++d) {
+                            const int row = (L::kPlanes - 1 - d) * (L::kPlanes == 3 ? 4 : 8) + r;
+                            *reinterpret_cast<uint32_t*>(q + (dim / 128) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4) + (dim % 16)) = w[d];
+                        }
+                    }
+                    if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = amax / kMost * p.scale_log2;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read it through the async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::Q_FULL + buf));
+        }
+    } else if (warp == L::kSWarp) {
+        // =============================== issuer of S^T = K Q^T ===============================
+        const uint64_t k_desc = umma_desc(sbase, 16, 1024, 2), q_desc = umma_desc(sbase + L::kOffQ, 16, 1024, 2);
+        uint32_t i = 0;
+        bool ok = true;
+        for (uint32_t k = 0; c.left > 0 && ok; c.advance(p), ++k) {
+            const uint32_t n = c.take();
+            ok = wait_warp(bar(L::Q_FULL + (k & 1)), (k >> 1) & 1);
+            const uint64_t qd = q_desc + (((k & 1) * L::kQBytes) >> 4);
+            for (uint32_t j = 0; j < n && ok; ++j, ++i) {
+                const uint32_t buf = i & 1, slot = i % L::kKUnits;
+                ok = mbar_wait_both(bar(L::S_EMPTY + buf), ((i >> 1) & 1) ^ 1, bar(L::K_FULL + slot), (i / L::kKUnits) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t kd = k_desc + ((slot * L::kKData) >> 4);
+                const uint32_t d = tmem_base + L::kColS + buf * L::kSCols;
+                if (elect_one()) {
+                    if constexpr (KF == F16) {
+                        constexpr uint32_t idesc = idesc_f16(128, 16, 0, 0);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            umma_f16(d, kd + (((kk >> 2) * (kDecodeTile * 128) + (kk & 3) * 32) >> 4), qd + (((kk >> 2) * 2048 + (kk & 3) * 32) >> 4), idesc, kk > 0);
+                    } else {
+                        constexpr uint32_t idesc = idesc_i8(128, 16, 1, 1, 0, 0);
+#pragma unroll
+                        for (int b = 0; b < D / 32; ++b)   // 32 dims each: a block's sums in columns of their own, or all in the same
+                            umma_i8(d + (KF == BLOCK ? b * 16 : 0), kd + (((b >> 2) * (kDecodeTile * 128) + (b & 3) * 32) >> 4), qd + (((b >> 2) * 2048 + (b & 3) * 32) >> 4), idesc,
+                                    KF == ROW && b > 0);
+                    }
+                    umma_commit(bar(L::S_FULL + buf));
+                    umma_commit(bar(L::K_EMPTY + slot));
+                    if (j + 1 == n) umma_commit(bar(L::Q_EMPTY + (k & 1)));
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == L::kPvWarp) {
+        // =============================== issuer of O^T = V^T P ===============================
+        const uint64_t v_desc = umma_desc(sbase + L::kOffV, kDecodeTile * 128, 1024, 2);
+        const uint64_t p_desc = umma_desc(sbase + L::kOffP, 32, 256, 6);
+        bool ok = true;
+        for (uint64_t i64 = 0; i64 < c.left && ok; ++i64) {
+            const uint32_t i = static_cast<uint32_t>(i64), buf = i & 1, slot = i % L::kVUnits;
+#pragma unroll
+            for (int g = 0; g < RG; ++g) {
+                const int pb = buf * RG + g;
+                ok = mbar_wait_both(bar(L::P_FULL + pb), (i >> 1) & 1, bar(L::V_FULL + slot), (i / L::kVUnits) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t vd = v_desc + ((slot * L::kVData) >> 4), pd = p_desc + ((pb * L::kPBytes) >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        const uint32_t d = tmem_base + L::kColO + buf * L::kOCols + (g * kHalves + half) * 32;
+                        const uint64_t ph = pd + ((VF == BLOCK ? half * (kDecodeTile * 32) : 0) >> 4);
+                        if constexpr (VF == F16) {
+                            constexpr uint32_t idesc = idesc_f16(128, 16, 1, 1);
+#pragma unroll
+                            for (int kk = 0; kk < kDecodeTile / 16; ++kk)   // 16 positions; 128 dims are two slabs
+                                umma_f16(d, vd + ((half * 2 * (kDecodeTile * 128) + kk * (16 * 128)) >> 4), ph + ((kk * (16 * 32)) >> 4), idesc, kk > 0);
+                        } else {
+                            constexpr uint32_t idesc = idesc_i8(128, 32, 1, 0, 1, 1);
+#pragma unroll
+                            for (int kk = 0; kk < kDecodeTile / 32; ++kk)   // 32 positions
+                                umma_i8(d, vd + ((half * (kDecodeTile * 128) + kk * (32 * 128)) >> 4), ph + ((kk * (32 * 32)) >> 4), idesc, kk > 0);
+                        }
+                    }
+                    umma_commit(bar(L::P_EMPTY + pb));
+                    if (g + 1 == RG) umma_commit(bar(L::V_EMPTY + slot));
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // =============================== softmax: a thread has a position and four query rows ===============================
+        const int g = warp >> 2, w4 = warp & 3, t128 = tid & 127;
+        const uint32_t lane_addr = static_cast<uint32_t>(w4 * 32) << 16;
+        const uint32_t p_flip = static_cast<uint32_t>((t128 >> 2) & 1) << 4;   // 32-byte swizzle: chunk c of row r at 32 r + ((c ^ ((r >> 2) & 1)) << 4)
+        int* xch = reinterpret_cast<int*>(smem + L::kOffXch) + g * (2 * 4 * L::kXchWords);
+        float* sums = reinterpret_cast<float*>(smem + L::kOffSum) + g * 16;
+        auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); };
+        auto wait = [&](uint32_t b, uint32_t parity) { if (!failed && !mbar_wait(b, parity)) failed = true; };
+        constexpr int NB = VF == BLOCK ? D / 32 : 1;     // value scales of a position
+        uint32_t i = 0;
+        for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
+            const uint32_t n = c.take(), rows = c.span.tokens * G;
+            wait(bar(L::Q_FULL + (k & 1)), (k >> 1) & 1);
+            float qmul[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) qmul[r] = reinterpret_cast<const volatile float*>(smem + L::kOffQmul)[(k & 1) * 8 + g * 4 + r];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::Q_EMPTY + (k & 1)));
+            uint32_t upto[4], low[4];                    // a row sees positions [low, upto) and the sinks below upto
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t row = g * 4 + r;
+                const int at = row < rows ? c.span.base() + static_cast<int>(row / G) + 1 : 0;
+                upto[r] = static_cast<uint32_t>(max(at, 0));
+                low[r] = p.window > 0 && upto[r] > p.window ? upto[r] - p.window : 0;
+            }
+            const uint32_t first_upto = static_cast<uint32_t>(max(c.span.base() + 1, 0));                             // what every row sees: [.., first_upto)
+            const uint32_t last_low = p.window > 0 && c.span.length > p.window ? c.span.length - p.window : 0;        // from here on
+            float acc[kHalves][4], m_run[4], l_run[4], pend[2][kHalves][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                m_run[r] = -INFINITY;
+                l_run[r] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) acc[h][r] = pend[0][h][r] = pend[1][h][r] = 0.0f;
+            }
+            auto fold = [&](auto buf_c) {                // the sums of a tile into the accumulators of this thread's dims
+                constexpr int buf = decltype(buf_c)::value;
+                int o[kHalves][8];
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) tmem_ld8(tmem_base + lane_addr + L::kColO + buf * L::kOCols + (g * kHalves + h) * 32 + (VF == F16 ? 0 : w4 * 8), o[h]);
+                tmem_ld_wait();
+                tc_fence_before();
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = VF == F16 ? terms(__int_as_float(o[h][r]), __int_as_float(o[h][4 + r])) : static_cast<float>(o[h][r] * 256 + o[h][4 + r]);
+                        acc[h][r] = fmaf(v, pend[buf][h][r], acc[h][r]);
+                    }
+            };
+            auto step = [&](auto buf_c, uint32_t j) {
+                constexpr int buf = decltype(buf_c)::value;
+                const uint32_t slot = i % L::kKUnits, vslot = i % L::kVUnits;
+                const uint32_t pos = c.position(c.tile + j) + t128;
+                if (!failed && !mbar_wait_both_lane(bar(L::K_FULL + slot), (i / L::kKUnits) & 1, bar(L::S_FULL + buf), (i >> 1) & 1)) failed = true;
+                __syncwarp();
+                tc_fence_after();
+                // ---- scores, in base-2 units ----
+                float s[4];
+                [[maybe_unused]] const uint8_t* kst = smem + L::kOffKScales + slot * L::kKScales;
+                const uint32_t s_at = tmem_base + lane_addr + L::kColS + buf * L::kSCols;
+                if constexpr (KF == F16) {
+                    int hi[4], lo[4];
+                    tmem_ld4(s_at + 4 * g, hi);
+                    tmem_ld4(s_at + 8 + 4 * g, lo);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[r] = terms(__int_as_float(hi[r]), __int_as_float(lo[r]));
+                } else {
+                    constexpr int B = KF == BLOCK ? D / 32 : 1;
+                    int v[B][L::kPlanes][4];
+#pragma unroll
+                    for (int b = 0; b < B; ++b)
+#pragma unroll
+                        for (int d = 0; d < L::kPlanes; ++d) tmem_ld4(s_at + b * 16 + (L::kPlanes == 3 ? 4 * d : 8 * d + 4 * g), v[b][d]);
+                    float ks[B];
+                    if constexpr (KF == BLOCK) {
+                        uint32_t raw[B / 2];
+                        if constexpr (B == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(kst + t128 * 16);
+                        else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(kst + t128 * 8);
+#pragma unroll
+                        for (int b = 0; b < B; b += 2) { const float2 f = unpack2(raw[b / 2]); ks[b] = f.x; ks[b + 1] = f.y; }
+                    } else {
+                        ks[0] = __half2float(*reinterpret_cast<const __half*>(kst + t128 * 2));
+                    }
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float a = 0.0f;
+#pragma unroll
+                        for (int b = 0; b < B; ++b) {
+                            float x;
+                            if constexpr (L::kPlanes == 3) x = fmaf(static_cast<float>(v[b][0][r]), 65536.0f, static_cast<float>(v[b][1][r] * 256 + v[b][2][r]));
+                            else x = static_cast<float>(v[b][0][r] * 256 + v[b][1][r]);
+                            a = fmaf(x, ks[b], a);
+                        }
+                        s[r] = a;
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(bar(L::S_EMPTY + buf));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::K_EMPTY + slot));      // the scales are read
+                const uint32_t pos0 = pos - t128;
+                bool any = true;
+                if (pos0 + kDecodeTile <= first_upto && pos0 >= last_low) {   // every row sees all of the tile
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[r] *= qmul[r];
+                } else {
+                    any = false;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool seen = pos < upto[r] && (pos >= low[r] || pos < p.sinks);
+                        s[r] = seen ? s[r] * qmul[r] : -INFINITY;
+                        any |= seen;
+                    }
+                }
+                // ---- the value scales, and the tile's maxima: inside the warp, then across the four ----
+                wait(bar(L::V_FULL + vslot), (i / L::kVUnits) & 1);
+                __syncwarp();
+                [[maybe_unused]] uint32_t vs_bits[NB];
+                if constexpr (VF != F16) {
+                    const uint8_t* vst = smem + L::kOffVScales + vslot * L::kVScales;
+                    if constexpr (VF == ROW) {
+                        vs_bits[0] = *reinterpret_cast<const uint16_t*>(vst + t128 * 2);
+                    } else {
+                        uint32_t raw[NB / 2];
+                        if constexpr (NB == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(vst + t128 * 16);
+                        else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(vst + t128 * 8);
+#pragma unroll
+                        for (int b = 0; b < NB; b += 2) { vs_bits[b] = raw[b / 2] & 0xffffu; vs_bits[b + 1] = raw[b / 2] >> 16; }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::V_EMPTY + vslot));
+                float m_tile[4];
+                [[maybe_unused]] float vs_max[NB];
+                {
+                    float mx[4];
+                    [[maybe_unused]] uint32_t vmx[NB];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx[r] = warp_max_redux(s[r]);
+                    if constexpr (VF != F16) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) vmx[b] = __reduce_max_sync(0xffffffffu, any ? vs_bits[b] : 0u);   // positive fp16 order like integers
+                    }
+                    int* dst = xch + (buf * 4 + w4) * L::kXchWords;
+                    if (lane == 0) {
+                        *reinterpret_cast<float4*>(dst) = make_float4(mx[0], mx[1], mx[2], mx[3]);
+                        if constexpr (VF != F16) {
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) dst[4 + b] = static_cast<int>(vmx[b]);
+                        }
+                    }
+                    group_sync();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m_tile[r] = -INFINITY;
+                    [[maybe_unused]] uint32_t vall[NB] = {};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int* src = xch + (buf * 4 + x) * L::kXchWords;
+                        const float4 a = *reinterpret_cast<const float4*>(src);
+                        m_tile[0] = fmaxf(m_tile[0], a.x); m_tile[1] = fmaxf(m_tile[1], a.y); m_tile[2] = fmaxf(m_tile[2], a.z); m_tile[3] = fmaxf(m_tile[3], a.w);
+                        if constexpr (VF != F16) {
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) vall[b] = max(vall[b], static_cast<uint32_t>(src[4 + b]));
+                        }
+                    }
+                    if constexpr (VF != F16) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) vs_max[b] = __half2float(__ushort_as_half(static_cast<uint16_t>(vall[b])));
+                    }
+                }
+                // ---- the running maxima; the branch is the group's ----
+                if (m_tile[0] > m_run[0] || m_tile[1] > m_run[1] || m_tile[2] > m_run[2] || m_tile[3] > m_run[3]) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float m_new = fmaxf(m_run[r], m_tile[r]);
+                        const float alpha = m_run[r] == -INFINITY ? 0.0f : ex2(m_run[r] - m_new);
+                        l_run[r] *= alpha;
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) { acc[h][r] *= alpha; pend[0][h][r] *= alpha; pend[1][h][r] *= alpha; }
+                        m_run[r] = m_new;
+                    }
+                }
+                // ---- weights ----
+                uint32_t words[L::kPSets][8];            // this position's 32 bytes
+                float scale_now[kHalves][4];             // what the tile's sums count for, relative to the running maxima
+                if constexpr (VF == F16) {
+                    float w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        w[r] = s[r] == -INFINITY ? 0.0f : ex2(s[r] - m_run[r]);
+                        l_run[r] += w[r];
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) scale_now[h][r] = 1.0f;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        words[0][x] = pack2(w[2 * x], w[2 * x + 1]);
+                        const float2 h = unpack2(words[0][x]);
+                        words[0][2 + x] = pack2(w[2 * x] - h.x, w[2 * x + 1] - h.y);
+                    }
+                } else {
+                    float wn[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w = s[r] == -INFINITY ? 0.0f : ex2(s[r] - m_run[r]);
+                        l_run[r] += w;
+                        const float wmax = m_tile[r] == -INFINITY ? 0.0f : ex2(m_tile[r] - m_run[r]);
+                        wn[r] = s[r] == -INFINITY || !(wmax > 0.0f) ? 0.0f : ex2(s[r] - m_tile[r]);   // relative to the tile's largest
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+                            float own = vs_max[0];       // the largest value scale of this thread's block
+                            if constexpr (VF == BLOCK) own = w4 == 0 ? vs_max[4 * h] : w4 == 1 ? vs_max[4 * h + 1] : w4 == 2 ? vs_max[4 * h + 2] : vs_max[4 * h + 3];
+                            scale_now[h][r] = wmax * own * (1.0f / 65535.0f);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const float wv = any && vs_max[b] > 0.0f ? __half2float(__ushort_as_half(static_cast<uint16_t>(vs_bits[b]))) * __fdividef(65535.0f, vs_max[b]) : 0.0f;
+                        uint32_t pq[4];                  // beside 2^23 the products come rounded to whole numbers in the low 16 bits
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) pq[r] = __float_as_uint(__fmaf_rn(wn[r], wv, 8388608.0f));
+                        const uint32_t p01 = __byte_perm(pq[0], pq[1], 0x5410), p23 = __byte_perm(pq[2], pq[3], 0x5410);
+                        const uint32_t hi = __byte_perm(p01, p23, 0x7531), lo = __byte_perm(p01, p23, 0x6420);
+                        if constexpr (VF == BLOCK) {
+                            words[b >> 2][2 * (b & 3)] = hi;
+                            words[b >> 2][2 * (b & 3) + 1] = lo;
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) { words[0][2 * x] = hi; words[0][2 * x + 1] = lo; }
+                        }
+                    }
+                }
+                // ---- the buffers were last used by the tile before the last: fold its sums, then hand the weights over ----
+                if (j >= 2) {
+                    wait(bar(L::P_EMPTY + buf * RG + g), ((i >> 1) & 1) ^ 1);
+                    __syncwarp();
+                    fold(buf_c);
+                }
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) pend[buf][h][r] = scale_now[h][r];
+                const uint32_t pt = sbase + L::kOffP + (buf * RG + g) * L::kPBytes + t128 * 32;
+#pragma unroll
+                for (int x = 0; x < L::kPSets; ++x) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(pt + x * (kDecodeTile * 32) + p_flip), "r"(words[x][0]), "r"(words[x][1]), "r"(words[x][2]), "r"(words[x][3]) : "memory");
+                    if constexpr (VF != F16)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(pt + x * (kDecodeTile * 32) + (p_flip ^ 16u)), "r"(words[x][4]), "r"(words[x][5]), "r"(words[x][6]), "r"(words[x][7]) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar(L::P_FULL + buf * RG + g));
+                ++i;
+            };
+            using Buf0 = std::integral_constant<int, 0>;
+            using Buf1 = std::integral_constant<int, 1>;
+            for (uint32_t j = 0; j < n; ++j) {
+                if ((i & 1) == 0) step(Buf0{}, j);
+                else step(Buf1{}, j);
+            }
+            // ---- the pair's end: row sums, the last two tiles' sums ----
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l_run[r] = warp_sum(l_run[r]);
+            if (lane == 0) *reinterpret_cast<float4*>(sums + w4 * 4) = make_float4(l_run[0], l_run[1], l_run[2], l_run[3]);
+            for (uint32_t back = min(n, 2u); back > 0; --back) {
+                const uint32_t x = i - back;
+                wait(bar(L::P_EMPTY + (x & 1) * RG + g), (x >> 1) & 1);
+                __syncwarp();
+                if ((x & 1) == 0) fold(Buf0{});
+                else fold(Buf1{});
+            }
+            if (failed) *fail_flag = 1;
+            group_sync();
+            float lt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float4 a = *reinterpret_cast<const float4*>(sums + x * 4);
+                lt[0] += a.x; lt[1] += a.y; lt[2] += a.z; lt[3] += a.w;
+            }
+            const bool poisoned = *fail_flag != 0;
+            group_sync();                                // the sums are read: the next pair may write its own
+            if (poisoned && t128 == 0) report(p.pool, B200KV_STATUS_PIPE_TIMEOUT);
+            const float nan = __int_as_float(0x7fc00000);
+            const bool whole = c.tile == 0 && n == c.t.n;
+            const size_t part = (2 * static_cast<size_t>(blockIdx.x) + (c.tile > 0 ? 0 : 1)) * kDecodeRows;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t row = g * 4 + r;
+                if (row >= rows) break;
+                const size_t head_row = (static_cast<size_t>(c.span.first) + row / G) * p.query_heads + c.head * G + row % G;
+                if (!whole) {
+                    if (t128 == 0) p.part_ml[part + row] = make_float2(m_run[r], poisoned ? nan : lt[r]);
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) p.part_o[(part + row) * D + h * 128 + t128] = acc[h][r];
+                    continue;
+                }
+                if (p.lse != nullptr && t128 == 0)
+                    p.lse[head_row] = poisoned ? nan : m_run[r] == -INFINITY ? (lt[r] != lt[r] ? nan : -INFINITY) : (m_run[r] + log2f(lt[r])) * 0.69314718055994531f;
+                const float f = poisoned || lt[r] != lt[r] ? nan : lt[r] > 0.0f ? 1.0f / lt[r] : 0.0f;
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) {
+                    const size_t at = head_row * D + h * 128 + t128;
+                    float v = acc[h][r] * f;
+                    if (lt[r] == 0.0f) v = 0.0f;
+                    if (p.gate != nullptr) v *= 1.0f / (1.0f + __expf(-p.gate[at]));
+                    if (p.out_is_f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+                    else static_cast<float*>(p.out)[at] = v;
+                }
+            }
+        }
+    }
+
+    // ---- teardown: every role arrives here, with or without a timeout; TMEM is always released ----
+    tc_fence_before();
+    __syncthreads();
+    if (warp == L::kSWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+    }
+}
+
+// out = sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M), times sigmoid(gate), over the CTAs whose pieces hold tiles of a pair.  A block: a query row of a pair, a
+// thread a dim.  Pairs of one piece have been written by their CTA.
+template <int D>
+__global__ void __launch_bounds__(D) paged_decode_merge_kernel(const __grid_constant__ PagedDecode p) {
+    __shared__ uint64_t range[2];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t s = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
+    const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H;
+    const Span span = span_of(p.pool, s);
+    const Tiles t = tiles_of(p, span);
+    if (t.n == 0 || row >= span.tokens * G) return;
+    if (tid < 32) {
+        const uint64_t all = tiles_before(p, p.pool.batch.sequences, tid), before = tiles_before(p, s, tid);
+        if (tid == 0) { range[0] = all; range[1] = before; }
+    }
+    __syncthreads();
+    const uint64_t all = range[0], begin = range[1] + static_cast<uint64_t>(head) * t.n, end = begin + t.n;
+    const uint32_t pieces = pieces_of(p, all);
+    auto piece_of = [&](uint64_t w) {   // the piece that holds tile w: the first all % pieces of them have a tile more
+        const uint64_t each = all / pieces, more = all % pieces, bound = more * (each + 1);
+        return static_cast<uint32_t>(w < bound ? w / (each + 1) : more + (w - bound) / each);
+    };
+    const uint32_t c0 = piece_of(begin), c1 = piece_of(end - 1);
+    if (c0 == c1) return;
+    // a CTA's first partial is of a pair that began before its piece
+    auto part_of = [&](uint32_t c) { return (2 * static_cast<size_t>(c) + (piece_begin(all, c, pieces) > begin ? 0 : 1)) * kDecodeRows + row; };
+    float m = -INFINITY;
+    bool poisoned = false;
+    for (uint32_t c = c0; c <= c1; ++c) {
+        const float2 ml = p.part_ml[part_of(c)];
+        poisoned |= ml.y != ml.y;
+        if (ml.y > 0.0f) m = fmaxf(m, ml.x);
+    }
+    float l = 0.0f, acc = 0.0f;
+#pragma unroll 8
+    for (uint32_t c = c0; c <= c1; ++c) {
+        const size_t part = part_of(c);
+        const float2 ml = p.part_ml[part];
+        const float o = p.part_o[part * D + tid];
+        const float w = ml.y > 0.0f ? exp2f(ml.x - m) : 0.0f;
+        l = fmaf(w, ml.y, l);
+        acc = w > 0.0f ? fmaf(w, o, acc) : acc;
+    }
+    const float nan = __int_as_float(0x7fc00000);
+    const size_t head_row = (static_cast<size_t>(span.first) + row / G) * p.query_heads + head * G + row % G, at = head_row * D + tid;
+    if (p.lse != nullptr && tid == 0) p.lse[head_row] = poisoned ? nan : l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    float v = poisoned ? nan : l > 0.0f ? acc / l : 0.0f;
+    if (p.gate != nullptr) v *= 1.0f / (1.0f + __expf(-p.gate[at]));
+    if (p.out_is_f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+    else static_cast<float*>(p.out)[at] = v;
+}
+
+template <int D, int KF, int VF, int RG>
+int launch_of(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+    using L = Layout<D, KF, VF, RG>;
+    const auto kernel = paged_decode_kernel<D, KF, VF, RG>;
+    static std::atomic<uint64_t> done{0};
+    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, done));
+    if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, p, kmap, vmap));
+    else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap, vmap));
+    return B200KV_OK;
+}
+template <int D, int RG>
+int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+    const bool blocks = p.pool.view.qblock != D;
+    switch (p.pool.view.quant_mode) {
+        case B200KV_F16_F16: return launch_of<D, F16, F16, RG>(p, kmap, vmap, stream, behind);
+        case B200KV_Q8_F16: return blocks ? launch_of<D, BLOCK, F16, RG>(p, kmap, vmap, stream, behind) : launch_of<D, ROW, F16, RG>(p, kmap, vmap, stream, behind);
+        case B200KV_F16_Q8: return blocks ? launch_of<D, F16, BLOCK, RG>(p, kmap, vmap, stream, behind) : launch_of<D, F16, ROW, RG>(p, kmap, vmap, stream, behind);
+        default: return blocks ? launch_of<D, BLOCK, BLOCK, RG>(p, kmap, vmap, stream, behind) : launch_of<D, ROW, ROW, RG>(p, kmap, vmap, stream, behind);
+    }
+}
+
+bool four_rows(const b200kv_paged_batch& b, uint32_t group) { return static_cast<uint64_t>(b.max_tokens) * group <= 4; }
+
+}  // namespace
+
+uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t, uint32_t sms) {
+    return sms * (view.head_dim == 128 && view.quant_mode == B200KV_Q8_Q8 ? 2 : 1);
+}
+size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms) {
+    return 2ull * decode_ctas(view, query_heads, sms) * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2));
+}
+
+int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind) {
+    const b200kv_paged_view& v = p.pool.view;
+    const b200kv_paged_batch& b = p.pool.batch;
+    const uint64_t rows = static_cast<uint64_t>(v.pages) * v.kv_heads * v.page_size;
+    if (rows > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
+    const uint32_t box = std::min(v.page_size, kDecodeTile), group = p.query_heads / v.kv_heads;
+    CUtensorMap kmap, vmap;
+    if (!encode_pool_map(&kmap, is_k_q8(v.quant_mode) ? static_cast<const void*>(v.key_q8) : v.key_f16, !is_k_q8(v.quant_mode), rows, v.head_dim, box) ||
+        !encode_pool_map(&vmap, is_v_q8(v.quant_mode) ? static_cast<const void*>(v.value_q8) : v.value_f16, !is_v_q8(v.quant_mode), rows, v.head_dim, box))
+        return B200KV_ERR_UNSUPPORTED;
+    const bool few = four_rows(b, group);
+    const uint32_t sms = std::min(device_sms(), kMostSms), most = decode_ctas(v, p.query_heads, sms);
+    p.ctas = few ? most : sms;
+    p.least_tiles = 2;
+    p.part_o = static_cast<float*>(parts);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ull * most * kDecodeRows * v.head_dim);
+    const int rc = v.head_dim == 128 ? (few ? launch_modes<128, 1>(p, kmap, vmap, stream, behind) : launch_modes<128, 2>(p, kmap, vmap, stream, behind))
+                                     : (few ? launch_modes<256, 1>(p, kmap, vmap, stream, behind) : launch_modes<256, 2>(p, kmap, vmap, stream, behind));
+    if (rc != B200KV_OK) return rc;
+    // one tile a pair: no pair lies in two pieces
+    if (b.max_length <= kDecodeTile) return B200KV_OK;
+    const uint32_t most_rows = static_cast<uint32_t>(std::min<uint64_t>(kDecodeRows, static_cast<uint64_t>(b.max_tokens) * group));
+    const dim3 grid(most_rows, v.kv_heads, b.sequences);
+    B200KV_CUDA_TRY(v.head_dim == 128 ? launch_behind(paged_decode_merge_kernel<128>, grid, dim3(128), 0, stream, p)
+                                      : launch_behind(paged_decode_merge_kernel<256>, grid, dim3(256), 0, stream, p));
+    return B200KV_OK;
+}
+
+}  // namespace b200kv

@@ -1,0 +1,39 @@
+// The tokens-a-few attention over a paged cache (paged_decode.cu) as the entry point launches it.
+#pragma once
+
+#include "paged_common.cuh"
+
+#include <cuda.h>
+
+namespace b200kv {
+
+constexpr uint32_t kDecodeRows = 8;        // query rows (tokens x heads of a kv head) of a sequence that this kernel takes
+constexpr uint32_t kDecodeTile = 128;      // positions of a tile
+constexpr uint32_t kMostSms = 160;         // what workspaces are sized for, on any device; launches use no more
+
+struct PagedDecode {
+    Paged pool;
+    const void* q;             // [total_tokens][query_heads][head_dim]
+    int q_is_f16;
+    const float* gate;         // may be null
+    void* out;
+    int out_is_f16;
+    float* lse;                // may be null
+    uint32_t query_heads, window, sinks;
+    float scale_log2;
+    uint32_t ctas;             // of the launch: the tiles of all sequences are dealt to them in equal pieces
+    uint32_t least_tiles;      // fewest tiles of a piece
+    float* part_o;             // [2 ctas][kDecodeRows][head_dim]: a CTA's piece begins and ends inside a kv head's tiles at most once each
+    float2* part_ml;           // [2 ctas][kDecodeRows] {maximum in log2 units, sum}
+};
+
+// Whether the sequences of a batch can all be of this kernel, and whether any can be.
+inline bool decode_takes_all(const b200kv_paged_batch& b, uint32_t group) { return static_cast<uint64_t>(b.max_tokens) * group <= kDecodeRows; }
+uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);     // at most
+size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);
+int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind);
+
+// A tensor map over a pool's plane as rows of head_dim: boxes of 128 bytes by `box_rows` rows, 128-byte swizzle.
+bool encode_pool_map(CUtensorMap* map, const void* plane, bool f16, uint64_t rows, uint32_t head_dim, uint32_t box_rows);
+
+}  // namespace b200kv

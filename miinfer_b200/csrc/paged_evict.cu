@@ -300,7 +300,7 @@ extern "C" int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_pa
     if (!word(target_table) || !word(weights) || !word(kept) || !word(new_lengths) || (new_weights != nullptr && !word(new_weights))) return B200KV_ERR_INVALID;
     if (keep == 0 || static_cast<uint64_t>(sinks) + recent > keep || new_lengths == batch->lengths) return B200KV_ERR_INVALID;
     if (weights_stride < batch->max_length) return B200KV_ERR_INVALID;
-    if (keep > 0x7fffffffu / 40 || static_cast<uint64_t>(target_max_pages) * view->page_size < keep) return B200KV_ERR_RANGE;   // 33 pieces of a row at most
+    if (keep > 0x7fffffffu / 40 || static_cast<uint64_t>(target_max_pages) * view->page_size < std::min(keep, batch->max_length)) return B200KV_ERR_RANGE;   // 33 pieces of a row at most
     if (view->kv_heads > 32767u) return B200KV_ERR_UNSUPPORTED;                                                                 // two grid rows a head
     const uint64_t heads = static_cast<uint64_t>(batch->sequences) * view->kv_heads;
     const uintptr_t w0 = reinterpret_cast<uintptr_t>(weights), w1 = w0 + heads * weights_stride * 4, n0 = reinterpret_cast<uintptr_t>(new_weights);

@@ -1150,6 +1150,21 @@ bool encode_f16_plane(CUtensorMap* map, const void* base, uint32_t d, uint64_t r
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+}  // namespace
+
+// (paged_decode.cuh)
+bool encode_pool_map(CUtensorMap* map, const void* plane, bool f16, uint64_t rows, uint32_t head_dim, uint32_t box_rows) {
+    EncodeFn fn = tc5_encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {head_dim, rows};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim) * (f16 ? 2 : 1)};
+    const cuuint32_t box[2] = {f16 ? 64u : 128u, box_rows}, elem[2] = {1, 1};
+    return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(plane), dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
 // An fp16 side of the cache is read where it lies; only int8 sides go through the scratch.  (The map ends at the rows the launch may see, so the last tile's
 // other rows come as zeros, as in the scratch; with a device-side state that is the capacity, and the kernel clears what lies past the visible rows.)  24 / 4 heads of
 // 256, us a layer: 67 over 4826 30.8 -> 24.0.  Where the caller has converted rows ahead

@@ -46,6 +46,13 @@ class Pool:
         sc = scales[pages, h].reshape(-1, self.d // self.qblock)[:n].astype(np.float64)
         return (x.reshape(n, self.d // self.qblock, self.qblock) * sc[:, :, None]).reshape(n, self.d)
 
+    def whole_values(self, s, h, length):
+        """|int8 values| of a sequence's kv head times the largest scale of their block of dims, float64 [length][d]."""
+        pages = self.table[s, :-(-length // self.page)]
+        q = np.abs(self.v[pages, h].reshape(-1, self.d)[:length].astype(np.float64))
+        most = self.vs[pages, h].reshape(-1, self.d // self.qblock)[:length].astype(np.float64).max(0)
+        return q * np.repeat(most, self.qblock)
+
     def place(self, s, j):
         return self.table[s, j // self.page], j % self.page
 
@@ -112,6 +119,10 @@ def attention(pool, q, starts, scale, window=0, sinks=0, gate=None):
                     # rounded weights divides
                     away = (np.abs(k[m]) @ np.abs(q[row, e])).max() * scale * (u_k + u_q + 2.0 ** -20)
                     b = (p @ np.abs(v[m])) * (np.expm1(2 * away) + 2 * HALF_STEP + u_v + 2.0 ** -18)
+                    # int8 values: a weight times its value scale may be a whole number of 65535ths of the largest weight times the largest scale of the block
+                    # (of a tile: no more than of all), each off by half of one, and multiplies a whole number of at most 128
+                    if u_v:
+                        b = b + 2.0 ** -17 * (1 + 2.0 ** -10) * p.max() * pool.whole_values(s, h, length)[m].sum(0)
                     if gate is not None:
                         f = 1 / (1 + np.exp(-gate[row, e].astype(np.float64)))
                         o, b = o * f, b * f + np.abs(o) * 2.0 ** -20

@@ -204,6 +204,21 @@ def test_attention_of_long_single_tokens_splits_and_merges(cuda, status, d, head
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("d,heads,hq,mode,qblock", [(128, 8, 32, 3, 32), (128, 8, 32, 0, 32), (256, 4, 24, 3, 32), (256, 4, 16, 0, 32), (256, 4, 24, 3, 256), (128, 8, 64, 1, 32)])
+def test_attention_of_many_sequences_whose_pieces_cross_from_one_to_the_next(cuda, status, d, heads, hq, mode, qblock):
+    """Pieces of a dozen tiles and more, most of them with the ends of two or three kv heads."""
+    rng = np.random.default_rng(d + mode)
+    lengths = [int(x) for x in rng.integers(1, 3500, 36)]
+    pool = po.Pool(rng, lengths, d=d, heads=heads, page=64, mode=mode, qblock=qblock)
+    tokens = [1] * 36
+    tokens[7] = tokens[20] = 0
+    run_attention(rng, pool, tokens, hq=hq, stale=False)
+    if hq == 32:
+        tokens[5] = 2       # eight rows: the other kernel for all
+        run_attention(rng, pool, tokens, hq=hq, stale=False)
+    assert int(status) == 0
+
+
 def test_attention_where_scores_reach_far(cuda):
     """Scores of several hundred, the largest last or first."""
     rng = np.random.default_rng(3)
