@@ -19,16 +19,13 @@
 //    (between the sinks and the window) are not in the list.
 // Every wait is bounded: one that runs out poisons the CTA's results with NaN, sets a status bit, and the CTA ends in the normal way.
 #include "paged_decode.cuh"
-#include "decode_common.cuh"
-#include "mbarrier_wait.cuh"
+#include "paged_unit.cuh"
 
 #include <algorithm>
 
 namespace b200kv {
 
 namespace {
-
-enum Fmt { F16 = 0, ROW = 1, BLOCK = 2 };   // a side's storage: fp16, int8 with one scale per row, int8 with a scale per 32 dims
 
 template <int D, int KF, int VF, int RG>   // RG: groups of four query rows
 struct Layout {
@@ -38,12 +35,12 @@ struct Layout {
     static constexpr int kProducerWarp = RG * 4, kSWarp = kProducerWarp + 1, kPvWarp = kSWarp + 1, kQWarp = kPvWarp + 1;
     static constexpr int kThreads = kSoftmax + 128;
     static constexpr int kCtas = D == 128 && KF != F16 && VF != F16 && RG == 1 ? 2 : 1;   // per SM
-    static constexpr int kKData = kTile * D * (KF == F16 ? 2 : 1), kVData = kTile * D * (VF == F16 ? 2 : 1);
-    static constexpr int kKScales = KF == F16 ? 0 : kTile * 2 * (KF == BLOCK ? D / 32 : 1), kVScales = VF == F16 ? 0 : kTile * 2 * (VF == BLOCK ? D / 32 : 1);
+    static constexpr int kKData = Unit<D, KF>::kData, kVData = Unit<D, VF>::kData, kKScales = Unit<D, KF>::kScales, kVScales = Unit<D, VF>::kScales;
     // weights of a row group: rows of 32 bytes per position, one set per half of the dims where the halves' scales differ
     static constexpr int kPSets = VF == BLOCK ? kHalves : 1;
     static constexpr int kPBytes = kPSets * kTile * 32;
-    [[maybe_unused]] static constexpr int kPlanes = KF == F16 || RG == 2 ? 2 : 3;                          // of a query row
+    static constexpr int kPlanes = KF == F16 || RG == 2 ? 2 : 3;                          // of a query row: int8 planes, or fp16 terms
+    static_assert(kPlanes * RG * 4 <= 16, "the 16 columns of a score MMA");
     static constexpr int kQBytes = 16 * D * (KF == F16 ? 2 : 1);
     static constexpr int kSCols = KF == BLOCK ? D / 32 * 16 : 16;                         // TMEM columns of a score buffer
     static constexpr int kOCols = RG * kHalves * 32;                                      // of a buffer of sums
@@ -82,130 +79,6 @@ struct Layout {
     static_assert(kTotal <= kBudget);
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-// Shared-memory matrix descriptor (sm_100 format); `layout`: 2 = 128-byte swizzle, 6 = 32-byte swizzle.  K-major: rows of 128 bytes, groups of eight `sbo` apart.
-// MN-major: one swizzle span contiguous along M or N, consecutive k a span apart, groups of eight k `sbo`, further spans `lbo` apart.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes, uint32_t layout) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(layout) << 61;
-    return d;
-}
-// Instruction descriptors: kind::i8 with int32 sums (formats: 1 = signed), kind::f16 with fp16 operands and fp32 sums.
-__host__ __device__ constexpr uint32_t idesc_i8(uint32_t m, uint32_t n, uint32_t a_signed, uint32_t b_signed, uint32_t a_mn, uint32_t b_mn) {
-    return (2u << 4) | (a_signed << 7) | (b_signed << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, uint32_t a_mn, uint32_t b_mn) {
-    return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }"
-                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld4(uint32_t taddr, int (&r)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, int (&r)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
-// The sum of a value's two terms.  Where the first is infinite or NaN it is the result: the second is 0 x infinity, or what was left of infinity.
-__device__ __forceinline__ float terms(float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; }
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-
-// ---- the list of tiles -------------------------------------------------------------------------------------------------------------
-
-// A sequence's tiles, the same for each of its kv heads: those of the sinks, if the window leaves a gap behind them, then those from tile `first` on.
-struct Tiles { uint32_t n, sink, first; };
-__device__ __forceinline__ Tiles tiles_of(const PagedDecode& p, const Span& span) {
-    const uint32_t group = p.query_heads / p.pool.view.kv_heads;
-    if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * group > kDecodeRows) return {0, 0, 0};
-    const uint32_t all = (span.length + kDecodeTile - 1) / kDecodeTile;
-    Tiles t{max(all, 1u), 0, 0};   // one tile where there is no position: the rows that see nothing come out as zeros
-    if (p.window == 0) return t;
-    const long long lowest = static_cast<long long>(span.base()) + 1 - p.window;
-    const uint32_t first = lowest > 0 ? static_cast<uint32_t>(lowest) / kDecodeTile : 0, sink = (p.sinks + kDecodeTile - 1) / kDecodeTile;
-    if (first <= sink || first >= all) return t;
-    return {sink + all - first, sink, first};
-}
-
-// Tiles of all pairs before sequence s (up to S: of all), of which a warp adds up 32 sequences at a time.
-__device__ uint64_t tiles_before(const PagedDecode& p, uint32_t s, int lane) {
-    uint64_t sum = 0;
-    for (uint32_t i = lane; i < s; i += 32) sum += tiles_of(p, span_of(p.pool, i)).n;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum * p.pool.view.kv_heads;
-}
-
-// CTAs that have a piece, and where piece c begins.
-__device__ __forceinline__ uint32_t pieces_of(const PagedDecode& p, uint64_t all) {
-    return static_cast<uint32_t>(min(static_cast<uint64_t>(p.ctas), max(static_cast<uint64_t>(1), all / p.least_tiles)));
-}
-__device__ __forceinline__ uint64_t piece_begin(uint64_t all, uint32_t c, uint32_t pieces) {
-    const uint64_t each = all / pieces, more = all % pieces;
-    return c * each + min(static_cast<uint64_t>(c), more);
-}
-
-// A place in the list, and how much of the piece is left from there.
-struct Cursor {
-    uint32_t s, head, tile;
-    uint64_t left;
-    Span span;
-    Tiles t;
-    __device__ __forceinline__ void settle(const PagedDecode& p) {   // the pair's sequence
-        span = span_of(p.pool, s);
-        t = tiles_of(p, span);
-    }
-    __device__ __forceinline__ uint32_t take() const { return static_cast<uint32_t>(min(left, static_cast<uint64_t>(t.n - tile))); }   // tiles of this pair
-    __device__ __forceinline__ void advance(const PagedDecode& p) {  // to the next pair that has tiles
-        left -= take();
-        tile = 0;
-        if (left == 0 || ++head < p.pool.view.kv_heads) return;
-        head = 0;
-        do {
-            ++s;
-            settle(p);
-        } while (t.n == 0 && s + 1 < p.pool.batch.sequences);
-    }
-    __device__ __forceinline__ uint32_t position(uint32_t j) const {   // first position of the pair's tile j
-        return (j < t.sink ? j : t.first + (j - t.sink)) * kDecodeTile;
-    }
-};
-
 template <int D, int KF, int VF, int RG>
 __global__ void __launch_bounds__(Layout<D, KF, VF, RG>::kThreads, Layout<D, KF, VF, RG>::kCtas)
 paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -240,196 +113,51 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();   // lengths, queries and cache rows come from preceding kernels
-    if (warp == L::kPvWarp) {   // this CTA's piece of the list
-        const uint32_t S = p.pool.batch.sequences;
-        const uint64_t all = tiles_before(p, S, lane);
-        const uint32_t pieces = pieces_of(p, all);
-        uint64_t begin = 0, count = 0;
-        if (all > 0 && blockIdx.x < pieces) {
-            begin = piece_begin(all, blockIdx.x, pieces);
-            count = piece_begin(all, blockIdx.x + 1, pieces) - begin;
-        }
-        if (count > 0) {
-            uint64_t before = 0;   // the sequence in which it begins, 32 at a time
-            for (uint32_t s0 = 0; s0 < S; s0 += 32) {
-                const uint32_t s = s0 + lane;
-                const uint32_t n = s < S ? tiles_of(p, span_of(p.pool, s)).n : 0;
-                uint64_t inc = static_cast<uint64_t>(n) * H;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += u;
-                }
-                const uint64_t mine = before + inc - static_cast<uint64_t>(n) * H;
-                if (n > 0 && begin >= mine && begin < before + inc) {
-                    start[0] = s;
-                    start[1] = static_cast<uint32_t>((begin - mine) / n);
-                    start[2] = static_cast<uint32_t>((begin - mine) % n);
-                }
-                before += __shfl_sync(0xffffffffu, inc, 31);
-                if (begin < before) break;
-            }
-        }
-        if (lane == 0) {
-            start[3] = static_cast<uint32_t>(count);
-            start[4] = static_cast<uint32_t>(count >> 32);
-        }
-    }
+    if (warp == L::kPvWarp) find_piece(p, blockIdx.x, lane, start);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    Cursor c;
-    c.s = start[0];
-    c.head = start[1];
-    c.tile = start[2];
-    c.left = start[3] | static_cast<uint64_t>(start[4]) << 32;
-    if (c.left > 0) c.settle(p);
+    Cursor c(p, start);
     bool failed = false;
 
     if (warp == L::kProducerWarp) {
         // =============================== copies: K and V units, a page's rows each lane ===============================
-        const uint32_t seg = min(p.pool.view.page_size, kDecodeTile), segs = kDecodeTile / seg;   // rows of a box; boxes of a tile
         uint32_t i = 0, fixes = 0;
         for (; c.left > 0 && !failed; c.advance(p)) {
             const int32_t* pages = pages_of(p.pool, c.s);
             const int lowest = p.window > 0 ? c.span.base() + 1 - static_cast<int>(p.window) : 0;
             const uint32_t low = lowest > 0 ? static_cast<uint32_t>(lowest) : 0;   // positions below it that are not sinks are seen by nobody
-            const uint32_t n = c.take();
+            const uint32_t n = c.take(), length = c.span.length;
             for (uint32_t j = 0; j < n && !failed; ++j, ++i) {
-                const uint32_t pos0 = c.position(c.tile + j), mine = pos0 + lane * seg;
-                const bool there = static_cast<uint32_t>(lane) < segs && mine < c.span.length;
-                long long row = -1;
-                if (there) {
-                    row = page_row(p.pool, pages[mine >> p.pool.page_shift], c.head);
-                    if (row >= 0) row += mine & ((1u << p.pool.page_shift) - 1);
-                }
-                const uint32_t found = __popc(__ballot_sync(0xffffffffu, row >= 0));
-                const uint32_t missing = __ballot_sync(0xffffffffu, there && row < 0);       // boxes of no page: zeros
-                const bool edge = pos0 + kDecodeTile > c.span.length || (pos0 < low && pos0 + kDecodeTile > p.sinks);
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    const int fmt = side == 0 ? KF : VF;
-                    const int data = fmt == F16 ? 2 * D : D, slabs = data / 128, scale = fmt == F16 ? 0 : fmt == BLOCK ? D / 16 : 2;   // bytes of a row
-                    const uint32_t units = side == 0 ? L::kKUnits : L::kVUnits, slot = i % units;
-                    if (i >= units && !wait_warp(bar((side == 0 ? L::K_EMPTY : L::V_EMPTY) + slot), ((i / units) & 1) ^ 1)) { failed = true; break; }
-                    const uint32_t off = side == 0 ? slot * L::kKData : L::kOffV + slot * L::kVData;
-                    const uint32_t scale_off = side == 0 ? L::kOffKScales + slot * L::kKScales : L::kOffVScales + slot * L::kVScales;
-                    const uint32_t dst = sbase + off, sdst = sbase + scale_off, full = bar((side == 0 ? L::K_FULL : L::V_FULL) + slot);
-                    const bool fix = missing != 0 || (side == 1 && VF == F16 && edge);
-                    const uint32_t to = fix ? bar(L::LANDED) : full;
-                    const uint32_t bytes = found * seg * (data + scale);
-                    if (lane == 0) {
-                        if (bytes > 0) mbar_expect_tx(to, bytes);
-                        else if (!fix) mbar_arrive(to);
-                    }
-                    __syncwarp();
-                    if (row >= 0) {
-                        for (int x = 0; x < slabs; ++x)   // 128 bytes of every row
-                            tma_load_2d(dst + x * (kDecodeTile * 128) + lane * seg * 128, side == 0 ? &kmap : &vmap, x * (fmt == F16 ? 64 : 128), static_cast<int>(row), to);
-                        if (fmt != F16)
-                            bulk_load(sdst + lane * seg * scale, static_cast<const uint8_t*>(side == 0 ? p.pool.view.key_scales : p.pool.view.value_scales) + static_cast<size_t>(row) * scale,
-                                      seg * scale, to);
-                    }
-                    if (fix) {   // what is not seen, or of no page, is cleared before anybody reads the unit
-                        if (bytes > 0) {
-                            if (!wait_warp(to, fixes & 1)) { failed = true; break; }
-                            ++fixes;
-                        }
-                        for (uint32_t r = 0; r < kDecodeTile; ++r) {
-                            const uint32_t pos = pos0 + r;
-                            const bool unseen = side == 1 && VF == F16 && (pos >= c.span.length || (pos < low && pos >= p.sinks));
-                            if (!unseen && !((missing >> (r / seg)) & 1)) continue;
-                            if (lane < slabs * 8) *reinterpret_cast<uint4*>(smem + off + (lane >> 3) * (kDecodeTile * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            if (fmt != F16 && lane < scale / 2) *reinterpret_cast<uint16_t*>(smem + scale_off + r * scale + lane * 2) = 0;
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(full);
-                    }
-                }
+                const uint32_t pos0 = c.t.position(c.tile + j), ks = i % L::kKUnits, vs = i % L::kVUnits;
+                const Boxes boxes = boxes_of(p.pool, pages, c.head, pos0, length, lane);
+                const bool edge = pos0 + kDecodeTile > length || (pos0 < low && pos0 + kDecodeTile > p.sinks);
+                const auto unseen = [&](uint32_t r) { return pos0 + r >= length || (pos0 + r < low && pos0 + r >= p.sinks); };
+                failed = i >= L::kKUnits && !wait_warp(bar(L::K_EMPTY + ks), ((i / L::kKUnits) & 1) ^ 1);
+                failed = failed || !bring_unit<D, KF>(smem, ks * L::kKData, L::kOffKScales + ks * L::kKScales, &kmap, p.pool.view.key_scales, boxes, bar(L::K_FULL + ks), bar(L::LANDED),
+                                                      &fixes, false, unseen, lane);
+                failed = failed || (i >= L::kVUnits && !wait_warp(bar(L::V_EMPTY + vs), ((i / L::kVUnits) & 1) ^ 1));
+                // fp16 values that nobody sees are cleared; int8 ones are finite whatever they are
+                failed = failed || !bring_unit<D, VF>(smem, L::kOffV + vs * L::kVData, L::kOffVScales + vs * L::kVScales, &vmap, p.pool.view.value_scales, boxes, bar(L::V_FULL + vs),
+                                                      bar(L::LANDED), &fixes, VF == F16 && edge, unseen, lane);
             }
         }
     } else if (warp == L::kQWarp) {
         // =============================== the query rows of a pair, as the operand of its score MMAs ===============================
-        // 16 rows of the operand: row 4 plane + r (three planes of four query rows) or 8 plane + r (two of eight); rows of 128-byte slabs, 128-byte swizzle.
-        constexpr int E = D / 32;   // consecutive elements a lane has
+        // 16 rows of the operand: row 4 plane + r (three planes of four query rows) or 8 plane + r (two of eight).
         for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
             const uint32_t buf = k & 1;
-            const uint32_t rows = c.span.tokens * G;
-            float x[RG * 4][E];
-#pragma unroll
-            for (int r = 0; r < RG * 4; ++r) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[r][e] = 0.0f;
-                if (static_cast<uint32_t>(r) >= rows) continue;
-                const size_t at = ((static_cast<size_t>(c.span.first) + r / G) * p.query_heads + c.head * G + r % G) * D + lane * E;
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    if (p.q_is_f16) {
-                        const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + at + e);
-                        const float2 a = unpack2(raw.x), b = unpack2(raw.y);
-                        x[r][e] = a.x; x[r][e + 1] = a.y; x[r][e + 2] = b.x; x[r][e + 3] = b.y;
-                    } else {
-                        const float4 raw = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + e);
-                        x[r][e] = raw.x; x[r][e + 1] = raw.y; x[r][e + 2] = raw.z; x[r][e + 3] = raw.w;
-                    }
-                }
-            }
+            float x[RG * 4][D / 32];
+            load_query<D, RG * 4>(x, p.q, p.q_is_f16, p.query_heads, c.span.first, c.head, G, c.span.tokens * G, lane);
             if (k >= 2 && !wait_warp(bar(L::Q_EMPTY + buf), ((k >> 1) & 1) ^ 1)) break;
             uint8_t* q = smem + L::kOffQ + buf * L::kQBytes;
 #pragma unroll
             for (int r = 0; r < RG * 4; ++r) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[r][e]));
-                amax = warp_max(amax);
-                if constexpr (KF == F16) {
-                    // scaled by a power of two, the largest element to [2^13, 2^14), and split into two fp16 terms
-                    const int exponent = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-                    const int up = amax > 0.0f ? max(-100, min(100, 13 - exponent)) : 0;
-                    const float mult = exp2i(up);
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        const int dim = lane * E + e, chunk = (dim % 64) / 8;
-                        uint32_t hi[2], lo[2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float a = x[r][e + 2 * i] * mult, b = x[r][e + 2 * i + 1] * mult;
-                            hi[i] = pack2(a, b);
-                            const float2 h = unpack2(hi[i]);
-                            lo[i] = pack2(a - h.x, b - h.y);
-                        }
-                        auto at = [&](int row) { return q + (dim / 64) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4) + (dim % 8) * 2; };
-                        *reinterpret_cast<uint2*>(at(r)) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(at(8 + r)) = make_uint2(lo[0], lo[1]);
-                    }
-                    if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = p.scale_log2 * exp2i(-up);
-                } else {
-                    constexpr float kMost = L::kPlanes == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
-                    const float inv = amax > 0.0f ? kMost / amax : 0.0f;
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        const int dim = lane * E + e, chunk = (dim % 128) / 16;
-                        uint32_t w[3] = {0, 0, 0};   // the planes from the lowest digit: signed bytes
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            int v = __float2int_rn(x[r][e + i] * inv);
-#pragma unroll
-                            for (int d = 0; d < L::kPlanes; ++d) {
-                                const int digit = d + 1 < L::kPlanes ? ((v + 128) & 255) - 128 : v;
-                                w[d] |= static_cast<uint32_t>(digit & 0xff) << (8 * i);
-                                v = (v - digit) >> 8;
-                            }
-                        }
-#pragma unroll
-                        for (int d = 0; d < L::kPlanes; ++d) {
-                            const int row = (L::kPlanes - 1 - d) * (L::kPlanes == 3 ? 4 : 8) + r;
-                            *reinterpret_cast<uint32_t*>(q + (dim / 128) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4) + (dim % 16)) = w[d];
-                        }
-                    }
-                    if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = amax / kMost * p.scale_log2;
-                }
+                float unit;
+                if constexpr (KF == F16) unit = store_terms<D, 8>(q, 2048, r, x[r], lane);
+                else unit = store_planes<D, L::kPlanes, L::kPlanes == 3 ? 4 : 8>(q, 2048, r, x[r], lane);
+                if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = unit * p.scale_log2;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read it through the async proxy
             __syncwarp();
@@ -564,7 +292,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
             auto step = [&](auto buf_c, uint32_t j) {
                 constexpr int buf = decltype(buf_c)::value;
                 const uint32_t slot = i % L::kKUnits, vslot = i % L::kVUnits;
-                const uint32_t pos = c.position(c.tile + j) + t128;
+                const uint32_t pos = c.t.position(c.tile + j) + t128;
                 if (!failed && !mbar_wait_both_lane(bar(L::K_FULL + slot), (i / L::kKUnits) & 1, bar(L::S_FULL + buf), (i >> 1) & 1)) failed = true;
                 __syncwarp();
                 tc_fence_after();
@@ -844,7 +572,7 @@ __global__ void __launch_bounds__(D) paged_decode_merge_kernel(const __grid_cons
     const uint32_t s = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
     const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H;
     const Span span = span_of(p.pool, s);
-    const Tiles t = tiles_of(p, span);
+    const Tiles t = p.tiles_of(span);
     if (t.n == 0 || row >= span.tokens * G) return;
     if (tid < 32) {
         const uint64_t all = tiles_before(p, p.pool.batch.sequences, tid), before = tiles_before(p, s, tid);

@@ -1,15 +1,13 @@
 // The tokens-a-few attention over a paged cache (paged_decode.cu) as the entry point launches it.
 #pragma once
 
-#include "paged_common.cuh"
+#include "paged_tiles.cuh"
 
 #include <cuda.h>
 
 namespace b200kv {
 
 constexpr uint32_t kDecodeRows = 8;        // query rows (tokens x heads of a kv head) of a sequence that this kernel takes
-constexpr uint32_t kDecodeTile = 128;      // positions of a tile
-constexpr uint32_t kMostSms = 160;         // what workspaces are sized for, on any device; launches use no more
 
 struct PagedDecode {
     Paged pool;
@@ -25,6 +23,12 @@ struct PagedDecode {
     uint32_t least_tiles;      // fewest tiles of a piece
     float* part_o;             // [2 ctas][kDecodeRows][head_dim]: a CTA's piece begins and ends inside a kv head's tiles at most once each
     float2* part_ml;           // [2 ctas][kDecodeRows] {maximum in log2 units, sum}
+    __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
+        if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * (query_heads / pool.view.kv_heads) > kDecodeRows) return {0, 0, 0};
+        Tiles t = tiles_seen(span.base(), span.length, window, sinks);
+        t.n = max(t.n, 1u);    // one tile where there is no position: the rows that see nothing come out as zeros
+        return t;
+    }
 };
 
 // Whether the sequences of a batch can all be of this kernel, and whether any can be.
@@ -35,5 +39,7 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
 
 // A tensor map over a pool's plane as rows of head_dim: boxes of 128 bytes by `box_rows` rows, 128-byte swizzle.
 bool encode_pool_map(CUtensorMap* map, const void* plane, bool f16, uint64_t rows, uint32_t head_dim, uint32_t box_rows);
+// One over fp16 activations [tokens][heads][head_dim]: boxes of 64 dims of `box_heads` heads of `box_tokens` tokens, 128-byte swizzle.
+bool encode_rows_map(CUtensorMap* map, const void* rows, uint32_t head_dim, uint32_t heads, uint32_t tokens, uint32_t box_heads, uint32_t box_tokens);
 
 }  // namespace b200kv

@@ -1,7 +1,23 @@
 // The weight that every cached position of a paged cache gets from a batch's new tokens, summed over tokens and query heads of the kv head:
 // A[j] += sum over (token, head) of exp(scale q.k_j - lse), with the statistics lse that the attention call left.
-#include "paged_common.cuh"
+//
+// With the statistics known a weight needs nothing but its own score, so there is no running maximum and nothing to rescale: S^T = K Q^T with positions as
+// rows of the tensor core's result and a thread for each of them that adds up its row.  A position belongs to one CTA, whose threads add to the
+// account alone: no atomics, the same sums on every run.  The scores are those of fp32: against them weights are held to 1e-5.
+//
+// Both kernels take equal pieces of one list of tiles (paged_tiles.cuh); a sequence is of one or the other by its observed query rows.
+//
+//  * few_kernel, up to 8 rows: bound by HBM, the first half of the attention kernel (paged_decode.cu).  int8 keys go straight into kind::i8 MMAs, the
+//    queries are whole numbers of 24 bits in three int8 planes; fp16 keys meet two fp16 terms of the queries.
+//  * many_kernel, any number: K of a tile becomes the A operand in TMEM, as fp16: fp16 as it is, int8 with one scale a row as whole numbers (the scale
+//    multiplies the score), int8 with a scale a block of 32 as two fp16 terms of the product, 22 bits.  The query rows that see any of the tile stream past it, 64 at a
+//    time: fp16 ones by TMA, whole tokens' heads of the kv head as boxes of a map over the activations; fp32 ones split into two terms by two warps.  Eight warps
+//    convert K and take the exponentials.  A from TMEM halves what an MMA reads from shared memory (K in shared memory: 78 clocks an MMA of 32).
+//    Bound by the MMAs where K has two terms (two for every product), by the exponentials otherwise.
+#include "paged_decode.cuh"
+#include "paged_unit.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace b200kv {
@@ -15,90 +31,636 @@ struct WeightsParams {
     const float* lse;          // [total_tokens][query_heads]
     float* weights;            // [sequences][kv_heads][stride]
     uint32_t stride, query_heads, window, sinks, observe;
+    uint32_t from_rows, to_rows;   // this launch's sequences: from .. to observed query rows
+    uint32_t ctas, least_tiles;
     float scale_log2;
+    __device__ __forceinline__ uint32_t observed(const Span& span) const { return observe > 0 ? min(observe, span.tokens) : span.tokens; }
+    __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
+        const uint32_t n = observed(span);
+        const uint64_t rows = static_cast<uint64_t>(n) * (query_heads / pool.view.kv_heads);
+        if (rows < from_rows || rows > to_rows) return {0, 0, 0};
+        return tiles_seen(static_cast<long long>(span.length) - n, span.length, window, sinks);
+    }
+    __device__ __forceinline__ const float* lse_of(const Span& span, uint32_t token) const { return lse + (static_cast<size_t>(span.first) + token) * query_heads; }
 };
 
-constexpr int kPositions = 64, kRows = 8;
+// ---- up to 8 rows ------------------------------------------------------------------------------------------------------------------------
 
-// A CTA takes 64 positions of a (sequence, kv head) and walks the observed rows, eight at a time; four threads share a position's dot products.
-template <int D>
-__global__ void __launch_bounds__(256) paged_weights_kernel(const __grid_constant__ WeightsParams p) {
-    constexpr int KS = D + 4;
-    extern __shared__ float smem[];
-    float* k_s = smem;                       // [64][KS]
-    float* q_s = smem + kPositions * KS;     // [8][D]
-    __shared__ float lse_s[kRows];
-    __shared__ int at_s[kRows];
+template <int D, int KF, int ROWS>   // ROWS: 4 or 8
+struct FewLayout {
+    using U = Unit<D, KF>;
+    static constexpr int kPlanes = KF == F16 ? 2 : 3;
+    static constexpr int kCols = kPlanes * ROWS <= 16 ? 16 : 32;                              // columns of an MMA
+    static constexpr int kSCols = KF == BLOCK ? D / 32 * kCols : kCols;                        // of a score buffer
+    static constexpr uint32_t kTmemCols = 2 * kSCols <= 32 ? 32 : 2 * kSCols <= 64 ? 64 : 2 * kSCols <= 128 ? 128 : 2 * kSCols <= 256 ? 256 : 512;
+    static constexpr int kCtas = D == 128 && KF != F16 ? 2 : 1;                                // per SM
+    static constexpr int kProducerWarp = 4, kSWarp = 5, kQWarp = 6, kThreads = 256;
+    static constexpr int kQSlab = kCols * 128, kQBytes = kCols * D * (KF == F16 ? 2 : 1);
+    static constexpr int kMisc = 1024;
+    static constexpr int kFit = ((kCtas == 2 ? 115712 : 232448) - 1024 - kMisc - 2 * kQBytes) / (U::kData + U::kScales);
+    static constexpr int kUnits = kFit > 8 ? 8 : kFit;
+    static_assert(kUnits >= 2);
+    static constexpr int kOffQ = kUnits * U::kData, kOffScales = kOffQ + 2 * kQBytes, kOffRows = kOffScales + kUnits * U::kScales;   // rows: [buffer][8] {factor, statistics}
+    static constexpr int kOffBar = kOffRows + 2 * 8 * 8;
+    static constexpr int FULL = 0, EMPTY = kUnits, LANDED = 2 * kUnits, S_FULL = LANDED + 1, S_EMPTY = S_FULL + 2, Q_FULL = S_EMPTY + 2, Q_EMPTY = Q_FULL + 2, kNumBars = Q_EMPTY + 2;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 32 + 1024;
+    static_assert(kOffMisc + 32 - kOffRows <= kMisc);
+};
+
+template <int D, int KF, int ROWS>
+__global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUtensorMap kmap) {
+    using L = FewLayout<D, KF, ROWS>;
+    using U = Unit<D, KF>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::kOffBar;
+    auto bar = [&](int i) { return bar0 + i * 8; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+    uint32_t* start = tmem_slot + 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H;
     pdl_launch_dependents();
+    if (warp == L::kProducerWarp && lane == 0) {
+        for (int i = 0; i < L::kNumBars; ++i) mbar_init(bar(i), i >= L::EMPTY && i < L::LANDED ? 1 + 4 : i >= L::S_EMPTY && i < L::Q_FULL ? 128 : i >= L::Q_EMPTY ? 1 + 4 : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    } else if (warp == L::kSWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     pdl_wait();
-    const Paged& pool = p.pool;
-    const uint32_t s = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
-    const Span span = span_of(pool, s);
-    const uint32_t pos0 = blockIdx.x * kPositions, G = p.query_heads / pool.view.kv_heads;
-    const uint32_t observed = p.observe > 0 ? min(p.observe, span.tokens) : span.tokens;
-    if (pos0 >= span.length || observed == 0) return;
-    const uint32_t t0 = span.tokens - observed;
-    const bool q8 = is_k_q8(pool.view.quant_mode);
-    for (uint32_t i = tid; i < kPositions * (D / 8); i += 256) {
-        const uint32_t r = i / (D / 8), c = i % (D / 8);
-        float v[8] = {};
-        const long long row = pos0 + r < span.length ? row_of(pool, s, head, pos0 + r) : -1;
-        if (row >= 0) {
-            const size_t at = static_cast<size_t>(row) * D + c * 8;
-            if (q8) {
-                const uint32_t blocks = D / pool.view.qblock;
-                const float scale = __half2float(static_cast<const __half*>(pool.view.key_scales)[static_cast<size_t>(row) * blocks + (blocks == 1 ? 0 : c / 4)]);
-                for (int e = 0; e < 8; ++e) v[e] = scale * static_cast<float>(pool.view.key_q8[at + e]);
-            } else {
-                for (int e = 0; e < 8; ++e) v[e] = __half2float(static_cast<const __half*>(pool.view.key_f16)[at + e]);
+    if (warp == L::kQWarp) find_piece(p, blockIdx.x, lane, start);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    Cursor c(p, start);
+
+    if (warp == L::kProducerWarp) {
+        uint32_t i = 0, fixes = 0;
+        bool ok = true;
+        for (; c.left > 0 && ok; c.advance(p)) {
+            const int32_t* pages = pages_of(p.pool, c.s);
+            const uint32_t n = c.take();
+            for (uint32_t j = 0; j < n && ok; ++j, ++i) {
+                const uint32_t slot = i % L::kUnits;
+                const Boxes boxes = boxes_of(p.pool, pages, c.head, c.t.position(c.tile + j), c.span.length, lane);
+                ok = i < L::kUnits || wait_warp(bar(L::EMPTY + slot), ((i / L::kUnits) & 1) ^ 1);
+                ok = ok && bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes,
+                                             false, [](uint32_t) { return false; }, lane);
             }
         }
-        for (int e = 0; e < 8; ++e) k_s[r * KS + c * 8 + e] = v[e];
-    }
-    const uint32_t mine = tid / 4, part = tid % 4, j = pos0 + mine;
-    float sum = 0.0f;
-    for (uint32_t row0 = 0; row0 < observed * G; row0 += kRows) {
-        __syncthreads();
-        for (uint32_t i = tid; i < kRows * D; i += 256) {
-            const uint32_t r = row0 + i / D;
-            const size_t row = static_cast<size_t>(span.first + t0 + r / G) * p.query_heads + head * G + r % G;
-            if (r >= observed * G) q_s[i] = 0.0f;
-            else q_s[i] = p.q_is_f16 ? __half2float(static_cast<const __half*>(p.q)[row * D + i % D]) : static_cast<const float*>(p.q)[row * D + i % D];
+    } else if (warp == L::kQWarp) {
+        for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
+            const uint32_t buf = k & 1, tokens = p.observed(c.span), t0 = c.span.tokens - tokens;
+            float x[ROWS][D / 32];
+            load_query<D, ROWS>(x, p.q, p.q_is_f16, p.query_heads, c.span.first + t0, c.head, G, tokens * G, lane);
+            float lse = INFINITY;      // lane r: of row r; a row that does not exist, or sees nothing, has no weights
+            if (lane < ROWS && static_cast<uint32_t>(lane) < tokens * G) {
+                lse = p.lse_of(c.span, t0 + lane / G)[c.head * G + lane % G];
+                lse = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+            }
+            if (k >= 2 && !wait_warp(bar(L::Q_EMPTY + buf), ((k >> 1) & 1) ^ 1)) break;
+            uint8_t* q = smem + L::kOffQ + buf * L::kQBytes;
+            float2* rows = reinterpret_cast<float2*>(smem + L::kOffRows) + buf * 8;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                float unit;
+                if constexpr (KF == F16) unit = store_terms<D, ROWS>(q, L::kQSlab, r, x[r], lane);
+                else unit = store_planes<D, 3, ROWS>(q, L::kQSlab, r, x[r], lane);
+                if (lane == r) rows[r] = make_float2(unit * p.scale_log2, lse);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::Q_FULL + buf));
         }
-        if (tid < kRows) {
-            const uint32_t r = row0 + tid;
-            const bool in = r < observed * G;
-            at_s[tid] = in ? span.base() + static_cast<int>(t0 + r / G) : -1;
-            lse_s[tid] = in ? p.lse[static_cast<size_t>(span.first + t0 + r / G) * p.query_heads + head * G + r % G] : 0.0f;
-        }
-        __syncthreads();
-        float dot[kRows] = {};
-        for (int c = part; c < D / 4; c += 4) {
-            const float4 k = *reinterpret_cast<const float4*>(k_s + mine * KS + 4 * c);
-            for (int r = 0; r < kRows; ++r) {
-                const float4 q = *reinterpret_cast<const float4*>(q_s + r * D + 4 * c);
-                dot[r] += k.x * q.x + k.y * q.y + k.z * q.z + k.w * q.w;
+    } else if (warp == L::kSWarp) {
+        const uint64_t k_desc = umma_desc(sbase, 16, 1024, 2), q_desc = umma_desc(sbase + L::kOffQ, 16, 1024, 2);
+        uint32_t i = 0;
+        bool ok = true;
+        for (uint32_t k = 0; c.left > 0 && ok; c.advance(p), ++k) {
+            const uint32_t n = c.take();
+            ok = wait_warp(bar(L::Q_FULL + (k & 1)), (k >> 1) & 1);
+            const uint64_t qd = q_desc + (((k & 1) * L::kQBytes) >> 4);
+            for (uint32_t j = 0; j < n && ok; ++j, ++i) {
+                const uint32_t buf = i & 1, slot = i % L::kUnits;
+                ok = mbar_wait_both(bar(L::S_EMPTY + buf), ((i >> 1) & 1) ^ 1, bar(L::FULL + slot), (i / L::kUnits) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t kd = k_desc + ((slot * U::kData) >> 4);
+                const uint32_t d = tmem_base + buf * L::kSCols;
+                if (elect_one()) {
+                    if constexpr (KF == F16) {
+                        constexpr uint32_t idesc = idesc_f16(128, L::kCols, 0, 0);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            umma_f16(d, kd + (((kk >> 2) * (kDecodeTile * 128) + (kk & 3) * 32) >> 4), qd + (((kk >> 2) * L::kQSlab + (kk & 3) * 32) >> 4), idesc, kk > 0);
+                    } else {
+                        constexpr uint32_t idesc = idesc_i8(128, L::kCols, 1, 1, 0, 0);
+#pragma unroll
+                        for (int b = 0; b < D / 32; ++b)
+                            umma_i8(d + (KF == BLOCK ? b * L::kCols : 0), kd + (((b >> 2) * (kDecodeTile * 128) + (b & 3) * 32) >> 4), qd + (((b >> 2) * L::kQSlab + (b & 3) * 32) >> 4), idesc,
+                                    KF == ROW && b > 0);
+                    }
+                    umma_commit(bar(L::S_FULL + buf));
+                    umma_commit(bar(L::EMPTY + slot));
+                    if (j + 1 == n) umma_commit(bar(L::Q_EMPTY + (k & 1)));
+                }
+                __syncwarp();
             }
         }
-        for (int r = 0; r < kRows; ++r) {
-            dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 1);
-            dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 2);
-            const int at = at_s[r];
-            const bool seen = static_cast<int>(j) <= at && (p.window == 0 || j + p.window > static_cast<uint32_t>(at) || j < p.sinks);
-            if (seen && lse_s[r] != -INFINITY) sum += exp2f(dot[r] * p.scale_log2 - lse_s[r] * 1.4426950408889634f);
+    } else if (warp < 4) {
+        // =============================== a thread a position ===============================
+        const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+        uint32_t i = 0;
+        bool failed = false;
+        auto wait = [&](uint32_t b, uint32_t parity) { if (!failed && !mbar_wait(b, parity)) failed = true; };
+        for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
+            const uint32_t n = c.take(), tokens = p.observed(c.span);
+            wait(bar(L::Q_FULL + (k & 1)), (k >> 1) & 1);
+            float2 row[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) row[r] = reinterpret_cast<const float2*>(smem + L::kOffRows)[(k & 1) * 8 + r];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::Q_EMPTY + (k & 1)));
+            const int first = static_cast<int>(c.span.length) - static_cast<int>(tokens);   // place of the first observed token
+            float* account = p.weights + (static_cast<size_t>(c.s) * H + c.head) * p.stride;
+            for (uint32_t j = 0; j < n; ++j, ++i) {
+                const uint32_t buf = i & 1, slot = i % L::kUnits, pos0 = c.t.position(c.tile + j), pos = pos0 + tid;
+                const float before = pos < c.span.length ? account[pos] : 0.0f;
+                if (!failed && !mbar_wait_both_lane(bar(L::FULL + slot), (i / L::kUnits) & 1, bar(L::S_FULL + buf), (i >> 1) & 1)) failed = true;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t s_at = tmem_base + lane_addr + buf * L::kSCols;
+                const uint8_t* scales = smem + L::kOffScales + slot * U::kScales + tid * U::kScale;
+                float s[ROWS];
+                if constexpr (KF == F16) {
+                    int v[2][ROWS];
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int r = 0; r < ROWS; r += 4) tmem_ld4(s_at + d * ROWS + r, reinterpret_cast<int(&)[4]>(v[d][r]));
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) s[r] = terms(__int_as_float(v[0][r]), __int_as_float(v[1][r]));
+                } else {
+                    constexpr int B = KF == BLOCK ? D / 32 : 1;
+                    float ks[B];
+                    if constexpr (KF == BLOCK) {
+                        uint32_t raw[B / 2];
+                        if constexpr (B == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(scales);
+                        else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(scales);
+#pragma unroll
+                        for (int b = 0; b < B; b += 2) { const float2 f = unpack2(raw[b / 2]); ks[b] = f.x; ks[b + 1] = f.y; }
+                    } else {
+                        ks[0] = __half2float(*reinterpret_cast<const __half*>(scales));
+                    }
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) s[r] = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < B; b += 2) {   // two blocks' sums at a time
+                        int v[2][3][ROWS];
+#pragma unroll
+                        for (int x = 0; x < 2 && b + x < B; ++x)
+#pragma unroll
+                            for (int d = 0; d < 3; ++d)
+#pragma unroll
+                                for (int r = 0; r < ROWS; r += 4) tmem_ld4(s_at + (b + x) * L::kCols + d * ROWS + r, reinterpret_cast<int(&)[4]>(v[x][d][r]));
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 2 && b + x < B; ++x)
+#pragma unroll
+                            for (int r = 0; r < ROWS; ++r)
+                                s[r] = fmaf(fmaf(static_cast<float>(v[x][0][r]), 65536.0f, static_cast<float>(v[x][1][r] * 256 + v[x][2][r])), ks[b + x], s[r]);
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(bar(L::S_EMPTY + buf));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::EMPTY + slot));
+                float sum = 0.0f;
+                if (static_cast<int>(pos0) + static_cast<int>(kDecodeTile) <= first + 1 && (p.window == 0 || static_cast<long long>(pos0) + p.window >= c.span.length)) {   // all rows see all positions
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) sum += ex2(fmaf(s[r], row[r].x, -row[r].y));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const int at = first + static_cast<int>(r / G);
+                        const bool seen = static_cast<uint32_t>(r) < tokens * G && static_cast<int>(pos) <= at && (p.window == 0 || static_cast<long long>(pos) + p.window > at || pos < p.sinks);
+                        const float w = ex2(fmaf(s[r], row[r].x, -row[r].y));
+                        sum += seen ? w : 0.0f;
+                    }
+                }
+                if (pos < c.span.length) account[pos] = before + (failed ? __int_as_float(0x7fc00000) : sum);
+            }
         }
+        if (failed && lane == 0) report(p.pool, B200KV_STATUS_PIPE_TIMEOUT);
     }
-    if (part == 0 && j < span.length) p.weights[(static_cast<size_t>(s) * pool.view.kv_heads + head) * p.stride + j] += sum;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == L::kSWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+    }
 }
 
-template <int D>
-int launch_weights(const WeightsParams& p, cudaStream_t stream) {
-    constexpr int kSmem = (kPositions * (D + 4) + kRows * D) * 4;
+// ---- any number of rows ----------------------------------------------------------------------------------------------------------------
+
+constexpr int kTile = kDecodeTile;
+constexpr int kGroup = 64;           // query rows of an MMA: as many whole tokens as fit
+constexpr int kWorkers = 256, kProducerWarp = 8, kQWarp = 9, kMmaWarp = 11, kThreads = 384;   // warps 9 and 10 bring the queries
+
+template <int D, int KF, bool Q32>
+struct ManyLayout {
+    using U = Unit<D, KF>;
+    static constexpr int kKTerms = KF == BLOCK ? 2 : 1, kQTerms = Q32 ? 2 : 1;
+    static constexpr int kCtas = D == 128 ? 2 : 1;                                             // per SM
+    static constexpr int kSBufs = D == 128 ? 2 : 4;
+    static constexpr uint32_t kColK = 0, kColS = kKTerms * D / 2, kTmemCols = kColS + kSBufs * kGroup <= 256 ? 256 : 512;   // K: two fp16 a column
+    static_assert(kColS + kSBufs * kGroup <= 512 && (kCtas == 1 || kTmemCols == 256));
+    static constexpr int kQTerm = kGroup * D * 2;
+    static constexpr int kRaw = 2;                                                             // units of K on their way
+    static constexpr int kMisc = 5120;
+    static constexpr int kFit = ((kCtas == 2 ? 115712 : 232448) - 1024 - kMisc - kRaw * (U::kData + U::kScales)) / (kQTerms * kQTerm);
+    static constexpr int kQBufs = kFit > 4 ? 4 : kFit;
+    static_assert(kQBufs >= 1 && !(Q32 && kQBufs == 3), "two warps that take the groups in turn see every phase of their buffers only if those are even in number");
+    static constexpr int kOffQ = kRaw * U::kData, kOffScales = kOffQ + kQBufs * kQTerms * kQTerm;
+    static constexpr int kOffRows = kOffScales + kRaw * U::kScales;                           // [buffer][64] {statistics in log2 units, place of the token}
+    static constexpr int kOffSum = kOffRows + kQBufs * kGroup * 8;                            // [parity][128]
+    static constexpr int kOffBar = kOffSum + 2 * kTile * 4;
+    static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + kRaw, LANDED = RAW_EMPTY + kRaw, K_FULL = LANDED + 1, Q_FULL = K_FULL + 1, Q_EMPTY = Q_FULL + kQBufs,
+                         S_FULL = Q_EMPTY + kQBufs, S_EMPTY = S_FULL + kSBufs, kNumBars = S_EMPTY + kSBufs;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 32 + 1024;
+    static_assert(kOffMisc + 32 - kOffRows <= kMisc);
+};
+
+// eight fp16 of a row as one 16-byte chunk of a K-major operand: slabs of 64 dims, kGroup rows of 128 bytes each, 128-byte swizzle
+__device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t chunk) { return (chunk >> 3) * (kGroup * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
+__device__ __forceinline__ void umma_f16_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// A tile's first position, and the tokens [t0, t1) that see any of it.  The tiles of a pair come from both ends in turn: the first are seen by the most tokens
+// of a chunk, the last by the fewest, and a piece is a few tiles.
+struct Share { uint32_t pos0, t0, t1; };
+__device__ __forceinline__ Share share_of(const WeightsParams& p, const Cursor& c, uint32_t j) {
+    const uint32_t x = c.tile + j, turned = (x & 1) ? c.t.n - 1 - (x >> 1) : x >> 1;
+    Share s{c.t.position(turned), c.span.tokens - p.observed(c.span), c.span.tokens};
+    const long long base = c.span.base(), first = static_cast<long long>(s.pos0) - base;
+    if (first > s.t0) s.t0 = static_cast<uint32_t>(min(first, static_cast<long long>(s.t1)));
+    if (p.window > 0 && s.pos0 >= p.sinks) {
+        const long long end = static_cast<long long>(s.pos0) + kTile - 1 + p.window - base;   // the first token whose window lies behind the tile
+        s.t1 = end <= 0 ? 0 : static_cast<uint32_t>(min(static_cast<long long>(s.t1), end));
+    }
+    if (s.t1 < s.t0) s.t1 = s.t0;
+    return s;
+}
+
+template <int D, int KF, bool Q32>
+__global__ void __launch_bounds__(kThreads, ManyLayout<D, KF, Q32>::kCtas)
+many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
+    using L = ManyLayout<D, KF, Q32>;
+    using U = Unit<D, KF>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::kOffBar;
+    auto bar = [&](int i) { return bar0 + i * 8; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+    uint32_t* start = tmem_slot + 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H, group_tokens = kGroup / G, group_rows = group_tokens * G;
+    pdl_launch_dependents();
+    if (warp == kProducerWarp && lane == 0) {
+        for (int i = 0; i < L::kNumBars; ++i) {
+            uint32_t count = 1;
+            if (i >= L::RAW_EMPTY && i < L::LANDED) count = kWorkers / 32;
+            else if (i == L::K_FULL) count = kWorkers;
+            else if (i >= L::Q_FULL && i < L::Q_EMPTY) count = Q32 ? 32 : 33;                  // the statistics' warp, and the copies
+            else if (i >= L::Q_EMPTY && i < L::S_FULL) count = 1 + kWorkers / 32;
+            else if (i >= L::S_EMPTY) count = kWorkers / 32;
+            mbar_init(bar(i), count);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    } else if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp < kProducerWarp) {   // rows of a group that no token's head takes: zeros once, no copy reaches them
+        const uint32_t spare = (kGroup - group_rows) * 8;
+        for (uint32_t i = tid; i < L::kQBufs * L::kQTerms * (D / 64) * spare; i += kWorkers)
+            *reinterpret_cast<uint4*>(smem + L::kOffQ + i / spare * (kGroup * 128) + group_rows * 128 + i % spare * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    pdl_wait();
+    if (warp == kQWarp) find_piece(p, blockIdx.x, lane, start);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    Cursor c(p, start);
+    // the tiles of the piece that some token sees, in order: f(share) until it says false
+    auto each_tile = [&](auto f) {
+        for (; c.left > 0; c.advance(p)) {
+            const uint32_t n = c.take();
+            for (uint32_t j = 0; j < n; ++j) {
+                const Share s = share_of(p, c, j);
+                if (s.t0 < s.t1 && !f(s)) return;
+            }
+        }
+    };
+
+    if (warp < kProducerWarp) {
+        // =============================== K into TMEM, then the exponentials ===============================
+        const int wg = warp >> 2, col0 = wg * (kGroup / 2), t128 = tid & 127;   // half of a row's dims, then half of a group's rows
+        const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        uint32_t i = 0, k = 0;   // tiles and groups so far
+        bool failed = false;
+        auto wait = [&](uint32_t b, uint32_t parity) { if (!failed && !mbar_wait(b, parity)) failed = true; };
+        each_tile([&](const Share& sh) {
+            const uint32_t raw = i % L::kRaw, mine = sh.pos0 + t128;
+            float* account = p.weights + (static_cast<size_t>(c.s) * H + c.head) * p.stride + mine;
+            const bool writes = wg == 0 && mine < c.span.length;
+            const float before = writes ? *account : 0.0f;
+            wait(bar(L::RAW_FULL + raw), (i / L::kRaw) & 1);
+            __syncwarp();
+            // (the tile before has been multiplied through: its last scores have been seen)
+            const uint8_t* scales = smem + L::kOffScales + raw * U::kScales + t128 * U::kScale;
+            const uint8_t* src = smem + raw * U::kData + t128 * 128;
+            constexpr int kChunks = U::kRow / 32;                            // 16-byte chunks of half a row
+#pragma unroll
+            for (int x = 0; x < kChunks; x += KF == F16 ? 2 : 1) {
+                const int chunk = wg * kChunks + x;
+                auto piece = [&](int n) { return *reinterpret_cast<const uint4*>(src + (n >> 3) * (kTile * 128) + (((n & 7) ^ (t128 & 7)) << 4)); };
+                const uint32_t col = tmem_base + lane_addr + L::kColK + chunk * (KF == F16 ? 4 : 8);   // 8 or 16 dims
+                const uint4 a = piece(chunk);
+                if constexpr (KF == F16) {
+                    const uint4 b = piece(chunk + 1);
+                    const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    tmem_st8(col, v);
+                } else {
+                    // int8 as exact fp16: 1024 + 128 + q beside the exponent of 1024, less 1152
+                    const uint32_t w[4] = {a.x ^ 0x80808080u, a.y ^ 0x80808080u, a.z ^ 0x80808080u, a.w ^ 0x80808080u};
+                    uint32_t hi[8];
+                    [[maybe_unused]] uint32_t lo[8];
+                    [[maybe_unused]] float sc = 1.0f;
+                    if constexpr (KF == BLOCK) sc = __half2float(reinterpret_cast<const __half*>(scales)[chunk >> 1]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t pair = __byte_perm(w[e >> 1], 0x64646464u, e & 1 ? 0x4342 : 0x4140);
+                        const __half2 q2 = __hadd2(*reinterpret_cast<const __half2*>(&pair), __float2half2_rn(-1152.0f));
+                        if constexpr (KF == ROW) {
+                            hi[e] = *reinterpret_cast<const uint32_t*>(&q2);
+                        } else {   // the product as two terms; q x scale is exact in fp32
+                            const float2 f = __half22float2(q2);
+                            const float u = f.x * sc, v = f.y * sc;
+                            hi[e] = pack2(u, v);
+                            const float2 h = unpack2(hi[e]);
+                            lo[e] = pack2(u - h.x, v - h.y);
+                        }
+                    }
+                    tmem_st8(col, hi);
+                    if constexpr (KF == BLOCK) tmem_st8(col + D / 2, lo);
+                }
+            }
+            float factor = p.scale_log2;
+            if constexpr (KF == ROW) factor *= __half2float(*reinterpret_cast<const __half*>(scales));
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            mbar_arrive(bar(L::K_FULL));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::RAW_EMPTY + raw));
+            const int base = c.span.base();
+            const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
+            float sum[2] = {0.0f, 0.0f};
+            for (uint32_t g = 0; g < groups; ++g, ++k) {
+                const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
+                if (!failed && !mbar_wait_both_lane(bar(L::Q_FULL + qb), (k / L::kQBufs) & 1, bar(L::S_FULL + sb), (k / L::kSBufs) & 1)) failed = true;
+                __syncwarp();
+                tc_fence_after();
+                int x[kGroup / 2];
+#pragma unroll
+                for (int e = 0; e < kGroup / 2; e += 8) tmem_ld8(tmem_base + lane_addr + L::kColS + sb * kGroup + col0 + e, reinterpret_cast<int(&)[8]>(x[e]));
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::S_EMPTY + sb));
+                const float2* info = reinterpret_cast<const float2*>(smem + L::kOffRows) + qb * kGroup;   // rows that do not exist have infinite statistics
+                const uint32_t first = sh.t0 + g * group_tokens, last = first + group_tokens - 1;
+                const bool whole = last < sh.t1 && static_cast<int>(sh.pos0) + kTile - 1 <= base + static_cast<int>(first) &&
+                                   (p.window == 0 || static_cast<long long>(sh.pos0) + p.window > static_cast<long long>(base) + last);   // all rows see all positions
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < kGroup / 2; e += 2) {
+                        const float4 two = *reinterpret_cast<const float4*>(info + col0 + e);
+                        sum[0] += ex2(fmaf(__int_as_float(x[e]), factor, -two.x));
+                        sum[1] += ex2(fmaf(__int_as_float(x[e + 1]), factor, -two.z));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kGroup / 2; ++e) {
+                        const float2 one = info[col0 + e];
+                        const int at = __float_as_int(one.y);
+                        const bool seen = static_cast<int>(mine) <= at && (p.window == 0 || static_cast<long long>(mine) + p.window > at || mine < p.sinks);
+                        const float w = ex2(fmaf(__int_as_float(x[e]), factor, -one.x));
+                        sum[e & 1] += seen ? w : 0.0f;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::Q_EMPTY + qb));
+            }
+            float* other = reinterpret_cast<float*>(smem + L::kOffSum) + (i & 1) * kTile;
+            const float total = failed ? __int_as_float(0x7fc00000) : sum[0] + sum[1];
+            if (wg == 1) other[t128] = total;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (writes) *account = before + (total + other[t128]);
+            ++i;
+            return true;
+        });
+        if (failed && lane == 0) report(p.pool, B200KV_STATUS_PIPE_TIMEOUT);
+    } else if (warp == kProducerWarp) {
+        // =============================== K as it lies in the pages ===============================
+        uint32_t i = 0, fixes = 0;
+        each_tile([&](const Share& sh) {
+            const uint32_t raw = i % L::kRaw;
+            const Boxes boxes = boxes_of(p.pool, pages_of(p.pool, c.s), c.head, sh.pos0, c.span.length, lane);
+            if (i >= L::kRaw && !wait_warp(bar(L::RAW_EMPTY + raw), ((i / L::kRaw) & 1) ^ 1)) return false;
+            ++i;
+            return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, false,
+                                     [](uint32_t) { return false; }, lane);
+        });
+    } else if (warp < kMmaWarp) {
+        // =============================== the query rows, 64 at a time ===============================
+        const uint32_t w = warp - kQWarp;
+        uint32_t k = 0;
+        each_tile([&](const Share& sh) {
+            const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
+            // statistics and places of a group's rows, by a warp
+            auto bring_info = [&](uint32_t t0, uint32_t qb) {
+                for (uint32_t x = lane; x < kGroup; x += 32) {
+                    const uint32_t token = t0 + x / G;
+                    float2 info = make_float2(INFINITY, __int_as_float(-1));
+                    if (x < group_rows && token < sh.t1) {
+                        const float lse = p.lse_of(c.span, token)[c.head * G + x % G];
+                        info.x = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;   // a row that sees nothing has no weights
+                        info.y = __int_as_float(c.span.base() + static_cast<int>(token));
+                    }
+                    reinterpret_cast<float2*>(smem + L::kOffRows)[qb * kGroup + x] = info;
+                }
+            };
+            for (uint32_t g = 0; g < groups; ++g, ++k) {
+                const uint32_t qb = k % L::kQBufs, t0 = sh.t0 + g * group_tokens;
+                if (Q32 && L::kQBufs > 1 && (k & 1) != w) continue;   // fp32: the warps take the groups in turn; with one buffer the first takes them all
+                if (Q32 && L::kQBufs == 1 && w != 0) continue;
+                if (k >= L::kQBufs && !wait_warp(bar(L::Q_EMPTY + qb), ((k / L::kQBufs) & 1) ^ 1)) return false;
+                if constexpr (!Q32) {
+                    if (w == 1) {
+                        bring_info(t0, qb);
+                        mbar_arrive(bar(L::Q_FULL + qb));
+                    } else if (lane == 0) {
+                        mbar_expect_tx(bar(L::Q_FULL + qb), group_rows * D * 2);   // rows past the last token's, or of no tensor, come along: they are masked
+#pragma unroll
+                        for (int x = 0; x < D / 64; ++x)
+                            tma_load_3d(sbase + L::kOffQ + qb * L::kQTerm + x * (kGroup * 128), &qmap, x * 64, static_cast<int>(c.head * G), static_cast<int>(c.span.first + t0), bar(L::Q_FULL + qb));
+                    }
+                } else {
+                    constexpr uint32_t CPR = D / 8, kStep = 32 / CPR;   // 16-byte pieces of a row of the operand; rows of a step
+                    uint8_t* dst = smem + L::kOffQ + qb * L::kQTerms * L::kQTerm;
+                    const uint32_t piece = lane % CPR;
+                    uint32_t token = t0, in_group = 0;                  // of the step's first row
+#pragma unroll 4
+                    for (uint32_t r0 = 0; r0 < group_rows; r0 += kStep) {
+                        const uint32_t r = r0 + lane / CPR;
+                        uint32_t tk = token, h = in_group + lane / CPR;
+                        while (h >= G) { h -= G; ++tk; }
+                        float4 a = make_float4(0, 0, 0, 0), b = a;
+                        if (r < group_rows && tk < sh.t1) {
+                            const float* src = static_cast<const float*>(p.q) + ((static_cast<size_t>(c.span.first) + tk) * p.query_heads + c.head * G + h) * D + piece * 8;
+                            a = *reinterpret_cast<const float4*>(src);
+                            b = *reinterpret_cast<const float4*>(src + 4);
+                        }
+                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            hi[x] = pack2(v[2 * x], v[2 * x + 1]);
+                            const float2 f = unpack2(hi[x]);
+                            lo[x] = pack2(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+                        }
+                        if (r < group_rows) {
+                            *reinterpret_cast<uint4*>(dst + chunk_at(r, piece)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(dst + L::kQTerm + chunk_at(r, piece)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                        in_group += kStep;
+                        while (in_group >= G) { in_group -= G; ++token; }
+                    }
+                    bring_info(t0, qb);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(bar(L::Q_FULL + qb));
+                }
+            }
+            return true;
+        });
+    } else {
+        // =============================== issuer of S^T = K Q^T ===============================
+        constexpr uint32_t idesc = idesc_f16(kTile, kGroup, 0, 0);
+        const uint64_t q_desc = umma_desc(sbase + L::kOffQ, 16, 1024, 2);
+        uint32_t i = 0, k = 0;
+        each_tile([&](const Share& sh) {
+            const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
+            if (!wait_warp(bar(L::K_FULL), i & 1)) return false;
+            ++i;
+            for (uint32_t g = 0; g < groups; ++g, ++k) {
+                const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
+                if (!mbar_wait_both(bar(L::Q_FULL + qb), (k / L::kQBufs) & 1, bar(L::S_EMPTY + sb), ((k / L::kSBufs) & 1) ^ 1)) return false;
+                tc_fence_after();
+                const uint32_t d = tmem_base + L::kColS + sb * kGroup;
+                const uint64_t qd = q_desc + ((qb * L::kQTerms * L::kQTerm) >> 4);
+                if (elect_one()) {
+                    auto product = [&](uint32_t a, uint64_t b, bool first) {
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            umma_f16_a_tmem(d, a + kk * 8, b + (((kk >> 2) * (kGroup * 128) + (kk & 3) * 32) >> 4), idesc, !first || kk > 0);
+                    };
+                    const uint32_t a = tmem_base + L::kColK;
+                    // the small terms first: what they add is not lost beside the large sums
+                    if constexpr (L::kKTerms == 2) product(a + D / 2, qd, true);
+                    if constexpr (L::kQTerms == 2) product(a, qd + (L::kQTerm >> 4), L::kKTerms == 1);
+                    product(a, qd, L::kKTerms == 1 && L::kQTerms == 1);
+                    umma_commit(bar(L::S_FULL + sb));
+                    umma_commit(bar(L::Q_EMPTY + qb));
+                }
+                __syncwarp();
+            }
+            return true;
+        });
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------------------------------
+
+bool key_map(CUtensorMap* map, const b200kv_paged_view& v) {
+    const bool q8 = is_k_q8(v.quant_mode);
+    return encode_pool_map(map, q8 ? static_cast<const void*>(v.key_q8) : v.key_f16, !q8, static_cast<uint64_t>(v.pages) * v.kv_heads * v.page_size, v.head_dim,
+                           std::min(v.page_size, kDecodeTile));
+}
+
+template <int D, int KF, int ROWS>
+int launch_few(WeightsParams p, cudaStream_t stream) {
+    using L = FewLayout<D, KF, ROWS>;
     static std::atomic<uint64_t> done{0};
-    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(paged_weights_kernel<D>), kSmem, done));
-    const dim3 grid((p.pool.batch.max_length + kPositions - 1) / kPositions, p.pool.view.kv_heads, p.pool.batch.sequences);
-    B200KV_CUDA_TRY(launch_kernel(paged_weights_kernel<D>, grid, dim3(256), kSmem, stream, true, p));
+    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(few_kernel<D, KF, ROWS>), L::kAlloc, done));
+    CUtensorMap kmap;
+    if (!key_map(&kmap, p.pool.view)) return B200KV_ERR_UNSUPPORTED;
+    p.ctas = std::min(device_sms(), kMostSms) * L::kCtas;
+    p.least_tiles = 1;
+    B200KV_CUDA_TRY(launch_kernel(few_kernel<D, KF, ROWS>, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap));
     return B200KV_OK;
+}
+template <int D, int KF, bool Q32>
+int launch_many(WeightsParams p, bool behind, cudaStream_t stream) {
+    using L = ManyLayout<D, KF, Q32>;
+    static std::atomic<uint64_t> done{0};
+    const auto kernel = many_kernel<D, KF, Q32>;
+    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, done));
+    const uint32_t G = p.query_heads / p.pool.view.kv_heads;
+    CUtensorMap kmap, qmap{};
+    if (!key_map(&kmap, p.pool.view) || (!Q32 && !encode_rows_map(&qmap, p.q, D, p.query_heads, p.pool.batch.total_tokens, G, kGroup / G))) return B200KV_ERR_UNSUPPORTED;
+    p.ctas = std::min(device_sms(), kMostSms) * L::kCtas;
+    p.least_tiles = 1;
+    if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(kThreads), L::kAlloc, stream, p, kmap, qmap));
+    else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kThreads), L::kAlloc, stream, true, p, kmap, qmap));
+    return B200KV_OK;
+}
+template <int D, int KF>
+int launch_both(WeightsParams p, uint64_t most_rows, uint32_t sequences, cudaStream_t stream) {
+    // what the bounds allow; a single sequence goes by its bound
+    const bool many = most_rows > kDecodeRows, few = !many || sequences > 1;
+    if (few) {
+        p.from_rows = 1;
+        p.to_rows = kDecodeRows;
+        const int rc = most_rows <= 4 ? launch_few<D, KF, 4>(p, stream) : launch_few<D, KF, 8>(p, stream);
+        if (rc != B200KV_OK || !many) return rc;
+    }
+    p.from_rows = few ? kDecodeRows + 1 : 1;
+    p.to_rows = 0xffffffffu;
+    return p.q_is_f16 ? launch_many<D, KF, false>(p, few, stream) : launch_many<D, KF, true>(p, few, stream);
+}
+template <int D>
+int launch_formats(const WeightsParams& p, uint64_t most_rows, uint32_t sequences, cudaStream_t stream) {
+    const b200kv_paged_view& v = p.pool.view;
+    if (!is_k_q8(v.quant_mode)) return launch_both<D, F16>(p, most_rows, sequences, stream);
+    return v.qblock == D ? launch_both<D, ROW>(p, most_rows, sequences, stream) : launch_both<D, BLOCK>(p, most_rows, sequences, stream);
 }
 
 }  // namespace
@@ -116,12 +678,14 @@ extern "C" int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_
     if ((reinterpret_cast<uintptr_t>(q) & 15u) != 0 || ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(weights)) & 3u) != 0) return B200KV_ERR_INVALID;
     if (query_heads == 0 || query_heads % view->kv_heads != 0 || !std::isfinite(scale) || !(scale > 0.0f)) return B200KV_ERR_INVALID;
     if (query_heads / view->kv_heads > 8) return B200KV_ERR_UNSUPPORTED;
-    if (batch->sequences == 0 || batch->total_tokens == 0 || batch->max_length == 0) return B200KV_OK;
+    if (static_cast<uint64_t>(view->pages) * view->kv_heads * view->page_size > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
+    if (batch->sequences == 0 || batch->total_tokens == 0 || batch->max_tokens == 0 || batch->max_length == 0) return B200KV_OK;
     if (weights_stride < batch->max_length) return B200KV_ERR_INVALID;
     settle_window(*batch, &window, &sinks);
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    const WeightsParams p{paged_of(*view, *batch), q, q_dtype == B200KV_F16, lse, weights, weights_stride, query_heads, window, sinks, observe,
-                          scale * 1.4426950408889634f};
-    return view->head_dim == 128 ? launch_weights<128>(p, static_cast<cudaStream_t>(stream)) : launch_weights<256>(p, static_cast<cudaStream_t>(stream));
+    const WeightsParams p{paged_of(*view, *batch), q, q_dtype == B200KV_F16, lse, weights, weights_stride, query_heads, window, sinks, observe, 0, 0, 0, 0, scale * 1.4426950408889634f};
+    const uint64_t most_rows = static_cast<uint64_t>(observe > 0 ? std::min(observe, batch->max_tokens) : batch->max_tokens) * (query_heads / view->kv_heads);
+    return view->head_dim == 128 ? launch_formats<128>(p, most_rows, batch->sequences, static_cast<cudaStream_t>(stream))
+                                 : launch_formats<256>(p, most_rows, batch->sequences, static_cast<cudaStream_t>(stream));
 }

@@ -34,6 +34,7 @@
 #include "decode_common.cuh"
 #include "dequant.cuh"
 #include "mbarrier_wait.cuh"
+#include "paged_decode.cuh"
 #include "paged_plan.cuh"
 #include "reference_word.h"
 
@@ -1161,6 +1162,16 @@ bool encode_pool_map(CUtensorMap* map, const void* plane, bool f16, uint64_t row
     const cuuint32_t box[2] = {f16 ? 64u : 128u, box_rows}, elem[2] = {1, 1};
     return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(plane), dims, strides, box, elem,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_rows_map(CUtensorMap* map, const void* rows, uint32_t head_dim, uint32_t heads, uint32_t tokens, uint32_t box_heads, uint32_t box_tokens) {
+    EncodeFn fn = tc5_encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {head_dim, heads, tokens};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2, static_cast<cuuint64_t>(heads) * head_dim * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_tokens}, elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(rows), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 namespace {
