@@ -511,7 +511,7 @@ typedef struct b200kv_paged_batch {
     const int32_t* query_starts;  /* DEVICE [sequences + 1], ascending: sequence s has the rows query_starts[s] .. query_starts[s + 1] of the
                                      activations, its newest tokens; none for a sequence that only waits */
     const int32_t* lengths;       /* DEVICE [sequences]: cached positions, the newest tokens among them */
-    uint32_t sequences;
+    uint32_t sequences;           /* up to 8192 */
     uint32_t max_pages;
     uint32_t total_tokens;        /* rows of the activations; rows at or past query_starts[sequences] are neither read nor written */
     uint32_t max_tokens;          /* upper bound of the new tokens of a sequence */

@@ -6,10 +6,12 @@
 // Sequences of a few query rows take the streaming kernel (paged_decode.cu), the others the chunk kernel; a call launches what its bounds allow, and the
 // kernels find their sequences.
 //
-// The host knows bounds, the device the lengths, so a call over chunks begins with a kernel that lays out the work (paged_plan_kernel: which rows and tiles
-// each CTA of the chunk kernel takes, how many of them share a row tile), goes on with the gather of the visible rows into an fp16 copy, tile by tile
-// as the chunk kernel's TMA reads them (paged_gather_kernel: int8 rows dequantised, rows past a length zero), the chunk kernel itself, and the merge
-// of what its CTAs left for shared row tiles.  Each follows the one before without a gap (programmatic launches).
+// The host knows bounds, the device the lengths, so a call over chunks begins with paged_prepare_kernel: one block lays out the work (which rows and tiles each
+// CTA of the chunk kernel takes, how many of them share a row tile) while the others gather the visible rows into an fp16 copy, tile by tile
+// as the chunk kernel's TMA reads them (int8 rows dequantised, rows that nobody sees zero).  (As a kernel of its own ahead of the gather the layout was 12 us of
+// a call: a chain of latencies.)  The chunk kernel follows, and the merge of what its CTAs left for shared row tiles, each launched while the one before
+// still runs.
+#include "decode_common.cuh"
 #include "dequant.cuh"
 #include "paged_decode.cuh"
 #include "paged_plan.cuh"
@@ -21,31 +23,31 @@ namespace b200kv {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
 constexpr uint32_t kMostParts = 16;        // of a row tile
-constexpr int kGatherThreads = 256;
+constexpr int kPrepareThreads = 256;
 
 // Estimated costs of the chunk kernel, us, as the single-sequence launch's (pick_kv_splits): a tile, a CTA's set-up and output, a merge, a partial.
 struct ChunkCosts { float tile, cta, merge, part; };
 
-struct PlanParams {
+struct PrepareParams {
     Paged pool;
     ChunkPlan* plan;
     ChunkItem* items;
-    uint32_t* tile_starts;      // [sequences + 1]: row tiles before a sequence's
-    uint32_t* scratch_starts;   // [sequences + 1]: scratch tiles before a sequence's
     uint32_t* groups;           // first item of each shared row tile
     uint32_t max_items, max_parts, scratch_tiles;
     uint32_t group, window, sinks, sms;
     uint32_t few_rows;          // sequences of at most so many query rows are the other kernel's
     ChunkCosts costs;
+    __half* out[2];             // the copy, K and V: [kv_head][scratch_tiles * kChunkTile][D]
     __device__ __forceinline__ bool mine(const Span& span) const { return span.tokens > 0 && static_cast<uint64_t>(span.tokens) * group > few_rows; }
+    __device__ __forceinline__ uint32_t row_tiles(const Span& span) const { return (span.tokens * group + kChunkRows - 1) / kChunkRows; }
 };
 
 struct Sums { uint32_t a, b, c; };
 __device__ __forceinline__ Sums add(const Sums& x, const Sums& y) { return {x.a + y.a, x.b + y.b, x.c + y.c}; }
 // Exclusive sums over the block's threads in order, and the total.
-__device__ Sums scan(Sums v, Sums* total, Sums* scratch) {
+__device__ __forceinline__ Sums scan(Sums v, Sums* total, Sums* scratch) {
+    constexpr int kWarps = kPrepareThreads / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums inc = v;
 #pragma unroll
@@ -57,17 +59,28 @@ __device__ Sums scan(Sums v, Sums* total, Sums* scratch) {
     if (lane == 31) scratch[warp] = inc;
     __syncthreads();
     Sums before{0, 0, 0}, all{0, 0, 0};
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before = add(before, scratch[w]);
         all = add(all, scratch[w]);
     }
     *total = all;
     return {before.a + inc.a - v.a, before.b + inc.b - v.b, before.c + inc.c - v.c};
 }
+// The last s < sequences with starts[s] <= x.
+__device__ __forceinline__ uint32_t last_from(const uint32_t* starts, uint32_t sequences, uint32_t x) {
+    uint32_t lo = 0, hi = sequences;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (starts[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
 
 // The tiles that row tile `r` of a sequence walks, and how many behind the sinks' it skips.
 struct Walk { uint32_t tiles, skip; };
-__device__ __forceinline__ Walk walk_of(const PlanParams& p, const Span& span, const ChunkTiles& t, uint32_t r) {
+__device__ __forceinline__ Walk walk_of(const PrepareParams& p, const Span& span, const ChunkTiles& t, uint32_t r) {
     const uint32_t t_first = r * kChunkRows / p.group, t_last = min((r + 1) * kChunkRows - 1, span.tokens * p.group - 1) / p.group;
     const int last = span.base() + static_cast<int>(t_last);
     if (last < 0) return {0, 0};
@@ -79,7 +92,7 @@ __device__ __forceinline__ Walk walk_of(const PlanParams& p, const Span& span, c
         first = lowest > 0 ? static_cast<uint32_t>(lowest) / kChunkTile : 0;
     }
     const uint32_t own0 = t.window0 / kChunkTile;   // the sequence's first tile behind its sinks' (0 without a gap)
-    if (t.sink_tiles == 0 && own0 == 0) {           // the copy is the cache: the sinks' tiles come with the others
+    if (own0 == 0) {                                // the copy is the cache: the sinks' tiles come with the others
         const uint32_t sink = p.window > 0 ? (p.sinks + kChunkTile - 1) / kChunkTile : 0;
         if (first <= sink) return {upto, 0};
         return {sink + (upto > first ? upto - first : 0), first - sink};
@@ -89,116 +102,74 @@ __device__ __forceinline__ Walk walk_of(const PlanParams& p, const Span& span, c
     return w;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_constant__ PlanParams p) {
-    __shared__ Sums scratch[kPlanThreads / 32];
-    __shared__ float cost_s[32];
-    __shared__ uint32_t chosen;
-    pdl_launch_dependents();
-    pdl_wait();   // lengths and starts come from preceding kernels
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.pool.batch.sequences, H = p.pool.view.kv_heads;
+struct PlanScratch {
+    Sums scan[kPrepareThreads / 32];
+    uint32_t items[kMostParts], parts[kMostParts], longest, piece;
+    float work;
+};
 
-    // ---- row tiles and scratch tiles of every sequence, and where they begin
-    uint32_t row_tiles = 0, scratch_tiles = 0, longest = 0;
-    for (uint32_t s0 = 0; s0 < S; s0 += kPlanThreads) {
-        const uint32_t s = s0 + tid;
-        Sums v{0, 0, 0};
-        if (s < S) {
-            const Span span = span_of(p.pool, s);
-            if (p.mine(span)) {
-                v.a = (span.tokens * p.group + kChunkRows - 1) / kChunkRows;
-                v.b = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles;
-            }
-        }
-        Sums total;
-        const Sums before = scan(v, &total, scratch);
-        uint32_t end = scratch_tiles + before.b + v.b;
-        if (s < S) {
-            if (end > p.scratch_tiles) report(p.pool, B200KV_STATUS_BAD_BOUND);   // no room: the walks below are cut
-            p.tile_starts[s] = row_tiles + before.a;
-            p.scratch_starts[s] = min(scratch_tiles + before.b, p.scratch_tiles);
-        }
-        row_tiles += total.a;
-        scratch_tiles += total.b;
-        longest = max(longest, v.b);
-    }
-    if (tid == 0) {
-        p.tile_starts[S] = row_tiles;
-        p.scratch_starts[S] = min(scratch_tiles, p.scratch_tiles);
-        p.plan->scratch_tiles = min(scratch_tiles, p.scratch_tiles);
-    }
+// The list of the chunk kernel's CTAs; one block.
+__device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* tile_starts, const uint32_t* scratch_starts, PlanScratch& sh) {
+    const uint32_t tid = threadIdx.x, S = p.pool.batch.sequences, H = p.pool.view.kv_heads, row_tiles = tile_starts[S];
+    if (tid == 0) p.plan->items = p.plan->groups = 0;
     if (static_cast<uint64_t>(row_tiles) * H > p.max_items) {   // starts that do not ascend: nothing of this is laid out
-        if (tid == 0) {
-            report(p.pool, B200KV_STATUS_BAD_BOUND);
-            p.plan->items = p.plan->groups = 0;
-        }
+        if (tid == 0) report(p.pool, B200KV_STATUS_BAD_BOUND);
         return;
     }
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    __syncthreads();
-    if (lane == 0) scratch[warp].a = longest;
-    __syncthreads();
-    for (int w = 0; w < kPlanThreads / 32; ++w) longest = max(longest, scratch[w].a);
-    __syncthreads();
-
-    // ---- how far to split: warp c tries pieces of at most longest / (c + 1) tiles.  CTAs take one another's place as they end, so the time is about the
+    // ---- how far to split: candidate c has pieces of at most longest / (c + 1) tiles.  CTAs take one another's place as they end, so the time is about the
     // work over the SMs and half a piece more, and no less than a piece.
-    if (warp < kMostParts) {
-        const uint32_t piece = max(3u, (longest + warp) / (warp + 1));
-        uint32_t items = 0, parts = 0;
-        float work = 0.0f;
-        for (uint32_t s = lane; s < S; s += 32) {
-            const Span span = span_of(p.pool, s);
-            if (!p.mine(span)) continue;
-            const uint32_t tiles = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles, n = (span.tokens * p.group + kChunkRows - 1) / kChunkRows * H;
-            const uint32_t pieces = max(1u, (tiles + piece - 1) / piece);
-            items += n * pieces;
-            if (pieces > 1) parts += n * pieces;
-            const float average = static_cast<float>(tiles) - 0.5f * min(tiles * static_cast<float>(kChunkTile), static_cast<float>(span.tokens)) / kChunkTile;
-            work += static_cast<float>(n) * average;
-        }
-        items = __reduce_add_sync(0xffffffffu, items);
-        parts = __reduce_add_sync(0xffffffffu, parts);
-        work = warp_sum(work);
-        if (lane == 0) {
-            const float one = piece * p.costs.tile + p.costs.cta, all = (work * p.costs.tile + items * p.costs.cta) / p.sms;
-            const float us = max(one, all + 0.5f * one) + (parts > 0 ? p.costs.merge + p.costs.part * parts : 0.0f);
-            cost_s[warp] = (warp > 0 && (items > p.max_items || parts > p.max_parts)) ? INFINITY : us;
+    if (tid < kMostParts) sh.items[tid] = sh.parts[tid] = 0;
+    if (tid == 0) { sh.longest = 0; sh.work = 0.0f; }
+    __syncthreads();
+    for (uint32_t s = tid; s < S; s += kPrepareThreads)
+        if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
+    __syncthreads();
+    const uint32_t longest = sh.longest;
+    const auto piece_of = [&](uint32_t c) { return max(3u, (longest + c) / (c + 1)); };
+    for (uint32_t s = tid; s < S; s += kPrepareThreads) {
+        const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
+        if (n == 0) continue;
+        // (tokens of a chunk see on average half of it)
+        atomicAdd(&sh.work, static_cast<float>(n) * (static_cast<float>(tiles) - 0.5f * min(static_cast<float>(tiles), static_cast<float>(span_of(p.pool, s).tokens) / kChunkTile)));
+        for (uint32_t c = 0; c < kMostParts; ++c) {
+            const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
+            atomicAdd(&sh.items[c], n * pieces);
+            if (pieces > 1) atomicAdd(&sh.parts[c], n * pieces);
         }
     }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t best = 0;
-        for (uint32_t c = 1; c < kMostParts; ++c)
-            if (cost_s[c] < cost_s[best]) best = c;
-        chosen = best == 0 ? 0x7fffffffu : max(3u, (longest + best) / (best + 1));
+    if (tid < 32) {
+        float us = INFINITY;
+        if (tid < kMostParts && (tid == 0 || (sh.items[tid] <= p.max_items && sh.parts[tid] <= p.max_parts))) {
+            const float one = piece_of(tid) * p.costs.tile + p.costs.cta, all = (sh.work * p.costs.tile + sh.items[tid] * p.costs.cta) / p.sms;
+            us = max(one, all + 0.5f * one) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
+        }
+        const float best = -warp_max_redux(-us);
+        const uint32_t which = __ffs(__ballot_sync(0xffffffffu, us == best)) - 1;
+        if (tid == 0) sh.piece = which == 0 ? 0x7fffffffu : piece_of(which);
     }
     __syncthreads();
-    const uint32_t piece = chosen;
+    const uint32_t piece = sh.piece;
 
     // ---- the list: a thread lays out a row tile, the longest of a sequence first
     uint32_t items = 0, parts = 0, groups = 0;
-    for (uint32_t i0 = 0; i0 < row_tiles; i0 += kPlanThreads) {
+    for (uint32_t i0 = 0; i0 < row_tiles; i0 += kPrepareThreads) {
         const uint32_t i = i0 + tid;
         Sums v{0, 0, 0};
         ChunkItem item{};
         Walk walk{0, 0};
         uint32_t n = 1;
         if (i < row_tiles) {
-            uint32_t lo = 0, hi = S;   // the sequence: the last whose row tiles begin at or before i
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (p.tile_starts[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            const Span span = span_of(p.pool, lo);
+            const uint32_t s = last_from(tile_starts, S, i);
+            const Span span = span_of(p.pool, s);
             const ChunkTiles t = chunk_tiles(span.base(), span.length, p.window, p.sinks);
             item.first = span.first;
             item.tokens = span.tokens;
             item.base = span.base();
-            item.row_tile = p.tile_starts[lo + 1] - 1 - i;
+            item.row_tile = tile_starts[s + 1] - 1 - i;
             walk = walk_of(p, span, t, item.row_tile);
-            if (p.scratch_starts[lo] + t.tiles > p.scratch_tiles) walk.tiles = 0;
-            item.scratch_row = p.scratch_starts[lo] * kChunkTile;
+            if (scratch_starts[s] + t.tiles > p.scratch_tiles) walk.tiles = 0;   // no room for the copy
+            item.scratch_row = scratch_starts[s] * kChunkTile;
             const uint32_t sink = p.window > 0 ? (p.sinks + kChunkTile - 1) / kChunkTile : 0;
             item.sink_tiles = t.window0 == 0 ? min(sink, walk.tiles) : t.sink_tiles;
             item.window0 = t.window0 == 0 ? item.sink_tiles * kChunkTile : t.window0;
@@ -207,7 +178,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
             v = {H * n, n > 1 ? H * n : 0, n > 1 ? H : 0};
         }
         Sums total;
-        const Sums before = scan(v, &total, scratch);
+        const Sums before = scan(v, &total, sh.scan);
         if (i < row_tiles) {
             uint32_t at = items + before.a, part = parts + before.b, group = groups + before.c;
             for (uint32_t h = 0; h < H; ++h) {
@@ -232,67 +203,93 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
     }
 }
 
-struct GatherParams {
-    Paged pool;
-    const ChunkPlan* plan;
-    const uint32_t* scratch_starts;
-    __half* out[2];            // K, V: [kv_head][scratch_rows][D]
-    uint32_t scratch_rows, window, sinks;
-};
-
-// A unit: a tile of 64 positions of one side of one kv head.  CTAs take units in turn.
+// A unit of the gather: a tile of 64 positions of one side of one kv head.
 template <int D>
-__global__ void __launch_bounds__(kGatherThreads) paged_gather_kernel(const __grid_constant__ GatherParams p) {
-    constexpr uint32_t CPR = D / 8, kEach = kChunkTile * CPR / kGatherThreads;   // 16-byte pieces of a row of the copy; a thread's of a tile
-    pdl_launch_dependents();
-    pdl_wait();
+__device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32_t* scratch_starts, uint32_t unit) {
+    constexpr uint32_t CPR = D / 8, kEach = kChunkTile * CPR / kPrepareThreads;   // 16-byte pieces of a row of the copy; a thread's of a tile
     const Paged& pool = p.pool;
-    const uint32_t H = pool.view.kv_heads, units = p.plan->scratch_tiles * H * 2, c = threadIdx.x % CPR;
-    for (uint32_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const uint32_t side = unit & 1, head = (unit >> 1) % H, tile = (unit >> 1) / H;
-        uint32_t lo = 0, hi = pool.batch.sequences;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (p.scratch_starts[mid] <= tile) lo = mid;
-            else hi = mid;
-        }
-        const Span span = span_of(pool, lo);
-        const ChunkTiles t = chunk_tiles(span.base(), span.length, p.window, p.sinks);
-        const uint32_t u = tile - p.scratch_starts[lo];
-        const uint32_t pos0 = u < t.sink_tiles ? u * kChunkTile : t.window0 + (u - t.sink_tiles) * kChunkTile;
-        const bool q8 = side == 0 ? is_k_q8(pool.view.quant_mode) : is_v_q8(pool.view.quant_mode);
-        const int8_t* q = side == 0 ? pool.view.key_q8 : pool.view.value_q8;
-        const __half* scales = static_cast<const __half*>(side == 0 ? pool.view.key_scales : pool.view.value_scales);
-        const __half* f16 = static_cast<const __half*>(side == 0 ? pool.view.key_f16 : pool.view.value_f16);
-        const uint32_t blocks = D / pool.view.qblock;
-        __half* out = p.out[side] + (static_cast<size_t>(head) * p.scratch_rows + static_cast<size_t>(tile) * kChunkTile) * D + c * 8;
-        uint4 v[kEach];
-        __half scale[kEach];
+    const uint32_t H = pool.view.kv_heads, c = threadIdx.x % CPR;
+    const uint32_t side = unit & 1, head = (unit >> 1) % H, tile = (unit >> 1) / H;
+    const uint32_t s = last_from(scratch_starts, pool.batch.sequences, tile);
+    const Span span = span_of(pool, s);
+    const ChunkTiles t = chunk_tiles(span.base(), span.length, p.window, p.sinks);
+    const uint32_t u = tile - scratch_starts[s];
+    const uint32_t pos0 = u < t.sink_tiles ? u * kChunkTile : t.window0 + (u - t.sink_tiles) * kChunkTile;
+    const bool q8 = side == 0 ? is_k_q8(pool.view.quant_mode) : is_v_q8(pool.view.quant_mode);
+    const int8_t* q = side == 0 ? pool.view.key_q8 : pool.view.value_q8;
+    const __half* scales = static_cast<const __half*>(side == 0 ? pool.view.key_scales : pool.view.value_scales);
+    const __half* f16 = static_cast<const __half*>(side == 0 ? pool.view.key_f16 : pool.view.value_f16);
+    const uint32_t blocks = D / pool.view.qblock;
+    __half* out = p.out[side] + (static_cast<size_t>(head) * p.scratch_tiles + tile) * kChunkTile * D + c * 8;
+    uint4 v[kEach];
+    __half scale[kEach];
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t j = pos0 + threadIdx.x / CPR + i * (kGatherThreads / CPR);
-            v[i] = make_uint4(0, 0, 0, 0);
-            scale[i] = __ushort_as_half(0);
-            const bool seen = j < span.length && (p.window == 0 || j < p.sinks || static_cast<int>(j + p.window) > span.base());   // by any of the tokens
-            const long long row = seen ? row_of(pool, lo, head, j) : -1;
-            if (row < 0) continue;   // zeros (a weight of 0 times what lies there would still be NaN where that is)
-            const size_t at = static_cast<size_t>(row) * D + c * 8;
-            if (q8) {
-                const uint2 raw = *reinterpret_cast<const uint2*>(q + at);
-                v[i].x = raw.x; v[i].y = raw.y;
-                scale[i] = scales[static_cast<size_t>(row) * blocks + (blocks == 1 ? 0 : c / 4)];
-            } else {
-                v[i] = *reinterpret_cast<const uint4*>(f16 + at);
-            }
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t j = pos0 + threadIdx.x / CPR + i * (kPrepareThreads / CPR);
+        v[i] = make_uint4(0, 0, 0, 0);
+        scale[i] = __ushort_as_half(0);
+        const bool seen = j < span.length && (p.window == 0 || j < p.sinks || static_cast<int>(j + p.window) > span.base());   // by any of the tokens
+        const long long row = seen ? row_of(pool, s, head, j) : -1;
+        if (row < 0) continue;   // zeros (a weight of 0 times what lies there would still be NaN where that is)
+        const size_t at = static_cast<size_t>(row) * D + c * 8;
+        if (q8) {
+            const uint2 raw = *reinterpret_cast<const uint2*>(q + at);
+            v[i].x = raw.x; v[i].y = raw.y;
+            scale[i] = scales[static_cast<size_t>(row) * blocks + (blocks == 1 ? 0 : c / 4)];
+        } else {
+            v[i] = *reinterpret_cast<const uint4*>(f16 + at);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i)
-            *reinterpret_cast<uint4*>(out + static_cast<size_t>(threadIdx.x / CPR + i * (kGatherThreads / CPR)) * D) =
-                q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
     }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i)
+        *reinterpret_cast<uint4*>(out + static_cast<size_t>(threadIdx.x / CPR + i * (kPrepareThreads / CPR)) * D) =
+            q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
 }
 
-struct MergeParams {
+template <int D>
+__global__ void __launch_bounds__(kPrepareThreads) paged_prepare_kernel(const __grid_constant__ PrepareParams p) {
+    extern __shared__ uint32_t starts[];   // row tiles, then tiles of the copy, before every sequence
+    __shared__ PlanScratch sh;
+    pdl_launch_dependents();
+    pdl_wait();   // lengths, starts and cache rows come from preceding kernels
+    const uint32_t S = p.pool.batch.sequences;
+    uint32_t* tile_starts = starts;
+    uint32_t* scratch_starts = starts + S + 1;
+    uint32_t row_tiles = 0, scratch_tiles = 0;
+    for (uint32_t s0 = 0; s0 < S; s0 += kPrepareThreads) {
+        const uint32_t s = s0 + threadIdx.x;
+        Sums v{0, 0, 0};
+        if (s < S) {
+            const Span span = span_of(p.pool, s);
+            if (p.mine(span)) {
+                v.a = p.row_tiles(span);
+                v.b = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles;
+            }
+        }
+        Sums total;
+        const Sums before = scan(v, &total, sh.scan);
+        if (s < S) {
+            tile_starts[s] = row_tiles + before.a;
+            scratch_starts[s] = min(scratch_tiles + before.b, p.scratch_tiles);
+        }
+        row_tiles += total.a;
+        scratch_tiles += total.b;
+    }
+    if (threadIdx.x == 0) {
+        if (blockIdx.x == 0 && scratch_tiles > p.scratch_tiles) report(p.pool, B200KV_STATUS_BAD_BOUND);
+        tile_starts[S] = row_tiles;
+        scratch_starts[S] = min(scratch_tiles, p.scratch_tiles);
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        lay_out(p, tile_starts, scratch_starts, sh);
+        return;
+    }
+    const uint32_t units = scratch_starts[S] * p.pool.view.kv_heads * 2;
+    for (uint32_t unit = blockIdx.x - 1; unit < units; unit += gridDim.x - 1) gather_unit<D>(p, scratch_starts, unit);
+}
+
+struct ChunkMergeParams {
     const ChunkPlan* plan;
     const ChunkItem* items;
     const uint32_t* groups;
@@ -305,62 +302,70 @@ struct MergeParams {
     uint32_t query_heads, kv_heads;
 };
 
-// out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), times sigmoid(gate).  A thread: four dims of a row of a shared row tile.
+// out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), times sigmoid(gate).  A thread: four dims of a row of a shared row tile, four partials' loads under way
+// together; blocks take a quarter or an eighth of a kilorow at a time in turn.  (All 16 partials' loads in flight took 108 registers: two blocks an SM, and a
+// block's four pieces one behind the other: 34 us for 96 row tiles of three partials of 256 dims.)
 template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ MergeParams p) {
-    constexpr uint32_t VPR = D / 4;
+__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ ChunkMergeParams p) {
+    constexpr uint32_t VPR = D / 4, kBlocks = kChunkRows * VPR / 256;   // a row tile's
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t G = p.query_heads / p.kv_heads, groups = p.plan->groups;
-    for (uint32_t g = blockIdx.x; g < groups; g += gridDim.x) {
-        const ChunkItem item = p.items[p.groups[g]];
-        const uint32_t rows = min(kChunkRows, item.tokens * G - item.row_tile * kChunkRows);
-        for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < rows * VPR; i += gridDim.y * 256) {
-            const uint32_t r = i / VPR, c = i % VPR * 4, gr = item.row_tile * kChunkRows + r;
-            const size_t head_row = (static_cast<size_t>(item.first) + gr / G) * p.query_heads + item.kv_head * G + gr % G;
-            float2 ml[kMostParts];
-            float4 o[kMostParts];
+    const uint32_t G = p.query_heads / p.kv_heads, units = p.plan->groups * kBlocks;
+    for (uint32_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const ChunkItem item = p.items[p.groups[unit / kBlocks]];
+        const uint32_t i = unit % kBlocks * 256 + threadIdx.x, r = i / VPR, c = i % VPR * 4, gr = item.row_tile * kChunkRows + r;
+        if (gr >= item.tokens * G) continue;
+        const size_t head_row = (static_cast<size_t>(item.first) + gr / G) * p.query_heads + item.kv_head * G + gr % G, at = head_row * D + c;
+        float4 g4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p.gate != nullptr) g4 = *reinterpret_cast<const float4*>(p.gate + at);
+        const float2* ml = p.part_ml + static_cast<size_t>(item.part) * kChunkRows + r;
+        const float* part = p.part_o + (static_cast<size_t>(item.part) * kChunkRows + r) * D + c;
+        float m = -INFINITY, l = 0.0f;
+        bool poisoned = false;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t s0 = 0; s0 < item.parts; s0 += 4) {
+            float2 x[4];
+            float4 o[4];
 #pragma unroll
-            for (uint32_t s = 0; s < kMostParts; ++s) {
-                ml[s] = make_float2(-INFINITY, 0.0f);
+            for (uint32_t s = 0; s < 4; ++s) {
+                x[s] = make_float2(-INFINITY, 0.0f);
                 o[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (s >= item.parts) continue;
-                const size_t row = static_cast<size_t>(item.part + s) * kChunkRows + r;
-                ml[s] = p.part_ml[row];
-                o[s] = *reinterpret_cast<const float4*>(p.part_o + row * D + c);
+                if (s0 + s >= item.parts) continue;
+                x[s] = ml[(s0 + s) * kChunkRows];
+                o[s] = *reinterpret_cast<const float4*>(part + static_cast<size_t>(s0 + s) * kChunkRows * D);
             }
-            float m = -INFINITY;
-            bool poisoned = false;
+            float m_new = m;
 #pragma unroll
-            for (uint32_t s = 0; s < kMostParts; ++s) {
-                if (ml[s].y != ml[s].y) poisoned = true;
-                if (ml[s].y > 0.0f) m = fmaxf(m, ml[s].x);
+            for (uint32_t s = 0; s < 4; ++s) {
+                if (x[s].y != x[s].y) poisoned = true;
+                if (x[s].y > 0.0f) m_new = fmaxf(m_new, x[s].x);
             }
-            float l = 0.0f;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (m_new > m) {
+                const float f = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+                l *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+                m = m_new;
+            }
 #pragma unroll
-            for (uint32_t s = 0; s < kMostParts; ++s) {
-                if (!(ml[s].y > 0.0f)) continue;
-                const float w = exp2f(ml[s].x - m);
-                l += w * ml[s].y;
+            for (uint32_t s = 0; s < 4; ++s) {
+                if (!(x[s].y > 0.0f)) continue;
+                const float w = exp2f(x[s].x - m);
+                l += w * x[s].y;
                 acc.x += w * o[s].x; acc.y += w * o[s].y; acc.z += w * o[s].z; acc.w += w * o[s].w;
             }
-            float f = l > 0.0f ? 1.0f / l : 0.0f;
-            if (poisoned) f = __int_as_float(0x7fc00000);
-            if (p.lse != nullptr && c == 0) p.lse[head_row] = poisoned ? f : l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
-            acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-            const size_t at = head_row * D + c;
-            if (p.gate != nullptr) {
-                const float4 g4 = *reinterpret_cast<const float4*>(p.gate + at);
-                acc.x *= 1.0f / (1.0f + __expf(-g4.x)); acc.y *= 1.0f / (1.0f + __expf(-g4.y));
-                acc.z *= 1.0f / (1.0f + __expf(-g4.z)); acc.w *= 1.0f / (1.0f + __expf(-g4.w));
-            }
-            if (p.out_is_f16) {
-                const __half2 a = __floats2half2_rn(acc.x, acc.y), b = __floats2half2_rn(acc.z, acc.w);
-                *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-            } else {
-                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = acc;
-            }
+        }
+        float f = l > 0.0f ? 1.0f / l : 0.0f;
+        if (poisoned) f = __int_as_float(0x7fc00000);
+        if (p.lse != nullptr && c == 0) p.lse[head_row] = poisoned ? f : l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        if (p.gate != nullptr) {
+            acc.x *= 1.0f / (1.0f + __expf(-g4.x)); acc.y *= 1.0f / (1.0f + __expf(-g4.y));
+            acc.z *= 1.0f / (1.0f + __expf(-g4.z)); acc.w *= 1.0f / (1.0f + __expf(-g4.w));
+        }
+        if (p.out_is_f16) {
+            const __half2 a = __floats2half2_rn(acc.x, acc.y), b = __floats2half2_rn(acc.z, acc.w);
+            *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = acc;
         }
     }
 }
@@ -371,7 +376,7 @@ struct Room {
     uint64_t scratch_tiles;    // of all sequences together
     uint32_t max_items, max_parts;
     bool decode, chunks;       // which kernels the call may need
-    size_t decode_parts, items, tile_starts, scratch_starts, groups, k, v, part_o, part_ml, bytes;   // offsets
+    size_t decode_parts, items, groups, k, v, part_o, part_ml, bytes;   // offsets
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
@@ -382,7 +387,7 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     // A single sequence goes by its bound: the chunk kernel takes a token as well, and the other's launch is saved.
     r.chunks = !decode_takes_all(batch, static_cast<uint32_t>(group));
     r.decode = !r.chunks || batch.sequences > 1;
-    const uint64_t least = r.decode ? kDecodeRows / group + 1 : 1;   // new tokens of a sequence of the chunk kernel
+    const uint64_t least = r.decode ? decode_rows(batch, static_cast<uint32_t>(group)) / group + 1 : 1;   // new tokens of a sequence of the chunk kernel
     const uint64_t sequences = std::min<uint64_t>(batch.sequences, batch.total_tokens / least);
     // a sequence's tiles: its length's, or those of its sinks and of the windows of its tokens
     uint64_t each = (static_cast<uint64_t>(batch.max_length) + kChunkTile - 1) / kChunkTile;
@@ -403,8 +408,6 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
         return r;
     }
     r.items = take(static_cast<uint64_t>(r.max_items) * sizeof(ChunkItem));
-    r.tile_starts = take((static_cast<uint64_t>(batch.sequences) + 1) * 4);
-    r.scratch_starts = take((static_cast<uint64_t>(batch.sequences) + 1) * 4);
     r.groups = take(parts * 4);
     const uint64_t plane = r.scratch_tiles * kChunkTile * view.kv_heads * view.head_dim * sizeof(__half);
     r.k = take(plane);
@@ -453,28 +456,28 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
     if (room.chunks) {
-        PlanParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.tile_starts),
-                      reinterpret_cast<uint32_t*>(ws + room.scratch_starts), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items, room.max_parts,
-                      static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, room.decode ? kDecodeRows : 0,
-                      view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.3f, 0.017f}};
-        B200KV_CUDA_TRY(launch_kernel(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, pp));
-        GatherParams gp{pool, pp.plan, pp.scratch_starts, {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)},
-                        static_cast<uint32_t>(room.scratch_tiles * kChunkTile), window, sinks};
-        const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
-        B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_gather_kernel<128>, dim3(blocks), dim3(kGatherThreads), 0, s, gp)
-                                              : launch_behind(paged_gather_kernel<256>, dim3(blocks), dim3(kGatherThreads), 0, s, gp));
-        const ChunkLaunch cl{pp.items, pp.plan, room.max_items, gp.out[0], gp.out[1], gp.scratch_rows, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse,
-                             query_heads, view->kv_heads, view->head_dim, window, sinks, scale * 1.4426950408889634f, reinterpret_cast<float*>(ws + room.part_o),
-                             reinterpret_cast<float2*>(ws + room.part_ml)};
+        const uint32_t few_rows = room.decode ? decode_rows(*batch, group) : 0;
+        const PrepareParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items,
+                               room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
+                               view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.3f, 0.017f},
+                               {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}};
+        const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
+        const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;
+        static std::atomic<uint64_t> done[2];
+        const auto prepare = view->head_dim == 128 ? paged_prepare_kernel<128> : paged_prepare_kernel<256>;
+        if (smem > 32 * 1024) B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prepare), 2 * (kMostSequences + 1) * 4, done[view->head_dim == 256]));
+        B200KV_CUDA_TRY(launch_kernel(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, true, pp));
+        const ChunkLaunch cl{pp.items, pp.plan, room.max_items, pp.out[0], pp.out[1], static_cast<uint32_t>(room.scratch_tiles * kChunkTile), q, q_dtype == B200KV_F16, gate, output,
+                             output_dtype == B200KV_F16, lse, query_heads, view->kv_heads, view->head_dim, window, sinks, scale * 1.4426950408889634f,
+                             reinterpret_cast<float*>(ws + room.part_o), reinterpret_cast<float2*>(ws + room.part_ml)};
         rc = launch_chunk(cl, s);
         if (rc != B200KV_OK) return rc;
-        const MergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
-        const dim3 merge_grid(std::min(room.max_parts / 2, 2 * sms), view->head_dim / 32);
-        B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, merge_grid, dim3(256), 0, s, mp)
-                                              : launch_behind(paged_merge_kernel<256>, merge_grid, dim3(256), 0, s, mp));
+        const ChunkMergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
+        B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, dim3(5 * sms), dim3(256), 0, s, mp)
+                                              : launch_behind(paged_merge_kernel<256>, dim3(5 * sms), dim3(256), 0, s, mp));
     }
     if (room.decode) {
-        PagedDecode dp{pool, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse, query_heads, window, sinks, scale * 1.4426950408889634f};
+        PagedDecode dp{pool, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse, query_heads, window, sinks, 0, scale * 1.4426950408889634f};
         return launch_paged_decode(dp, ws + room.decode_parts, s, room.chunks);
     }
     return B200KV_OK;

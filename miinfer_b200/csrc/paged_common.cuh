@@ -8,6 +8,8 @@ namespace b200kv {
 
 uint32_t* current_status_word();
 
+constexpr uint32_t kMostSequences = 8192;   // of a batch
+
 // Checks geometry, pointers and bounds.
 int validate_paged(const b200kv_paged_view* view, const b200kv_paged_batch* batch);
 

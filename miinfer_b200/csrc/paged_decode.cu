@@ -636,8 +636,6 @@ int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMa
     }
 }
 
-bool four_rows(const b200kv_paged_batch& b, uint32_t group) { return static_cast<uint64_t>(b.max_tokens) * group <= 4; }
-
 }  // namespace
 
 uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t, uint32_t sms) {
@@ -657,7 +655,8 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     if (!encode_pool_map(&kmap, is_k_q8(v.quant_mode) ? static_cast<const void*>(v.key_q8) : v.key_f16, !is_k_q8(v.quant_mode), rows, v.head_dim, box) ||
         !encode_pool_map(&vmap, is_v_q8(v.quant_mode) ? static_cast<const void*>(v.value_q8) : v.value_f16, !is_v_q8(v.quant_mode), rows, v.head_dim, box))
         return B200KV_ERR_UNSUPPORTED;
-    const bool few = four_rows(b, group);
+    p.rows = decode_rows(b, group);
+    const bool few = p.rows == 4;
     const uint32_t sms = std::min(device_sms(), kMostSms), most = decode_ctas(v, p.query_heads, sms);
     p.ctas = few ? most : sms;
     p.least_tiles = 2;
@@ -668,7 +667,7 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     if (rc != B200KV_OK) return rc;
     // one tile a pair: no pair lies in two pieces
     if (b.max_length <= kDecodeTile) return B200KV_OK;
-    const uint32_t most_rows = static_cast<uint32_t>(std::min<uint64_t>(kDecodeRows, static_cast<uint64_t>(b.max_tokens) * group));
+    const uint32_t most_rows = static_cast<uint32_t>(std::min<uint64_t>(p.rows, static_cast<uint64_t>(b.max_tokens) * group));
     const dim3 grid(most_rows, v.kv_heads, b.sequences);
     B200KV_CUDA_TRY(v.head_dim == 128 ? launch_behind(paged_decode_merge_kernel<128>, grid, dim3(128), 0, stream, p)
                                       : launch_behind(paged_decode_merge_kernel<256>, grid, dim3(256), 0, stream, p));

@@ -18,13 +18,14 @@ struct PagedDecode {
     int out_is_f16;
     float* lse;                // may be null
     uint32_t query_heads, window, sinks;
+    uint32_t rows;             // sequences of at most so many query rows are this launch's: 4 or 8
     float scale_log2;
     uint32_t ctas;             // of the launch: the tiles of all sequences are dealt to them in equal pieces
     uint32_t least_tiles;      // fewest tiles of a piece
     float* part_o;             // [2 ctas][kDecodeRows][head_dim]: a CTA's piece begins and ends inside a kv head's tiles at most once each
     float2* part_ml;           // [2 ctas][kDecodeRows] {maximum in log2 units, sum}
     __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
-        if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * (query_heads / pool.view.kv_heads) > kDecodeRows) return {0, 0, 0};
+        if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * (query_heads / pool.view.kv_heads) > rows) return {0, 0, 0};
         Tiles t = tiles_seen(span.base(), span.length, window, sinks);
         t.n = max(t.n, 1u);    // one tile where there is no position: the rows that see nothing come out as zeros
         return t;
@@ -33,6 +34,8 @@ struct PagedDecode {
 
 // Whether the sequences of a batch can all be of this kernel, and whether any can be.
 inline bool decode_takes_all(const b200kv_paged_batch& b, uint32_t group) { return static_cast<uint64_t>(b.max_tokens) * group <= kDecodeRows; }
+// The rows of the launch: four where they are enough for all sequences, or, beside the chunk kernel, for a token (four rows leave room for two CTAs an SM).
+inline uint32_t decode_rows(const b200kv_paged_batch& b, uint32_t group) { return group <= 4 && (b.max_tokens * static_cast<uint64_t>(group) <= 4 || !decode_takes_all(b, group)) ? 4 : kDecodeRows; }
 uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);     // at most
 size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);
 int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind);

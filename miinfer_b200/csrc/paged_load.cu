@@ -20,7 +20,7 @@ int validate_paged(const b200kv_paged_view* v, const b200kv_paged_batch* b) {
     if (b->sequences == 0) return B200KV_OK;
     const auto word = [](const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
     if (!word(b->page_table) || !word(b->query_starts) || !word(b->lengths) || b->max_pages == 0) return B200KV_ERR_INVALID;
-    if (b->sequences > 65535u) return B200KV_ERR_UNSUPPORTED;                             // a dimension of a grid
+    if (b->sequences > kMostSequences) return B200KV_ERR_UNSUPPORTED;
     if (b->total_tokens > 0x7fffffffu || b->max_length > 0x7fffffffu || b->max_tokens > b->total_tokens) return B200KV_ERR_INVALID;
     if (b->max_length > static_cast<uint64_t>(b->max_pages) * v->page_size) return B200KV_ERR_RANGE;
     return B200KV_OK;

@@ -803,9 +803,11 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // 8192: 111.6 -> 110.3.
             // Only the tiles that straddle this row's causal length need the mask.
             if constexpr (PAGED) {
-                if (pos0 + kBN > len || pos0 < low) {
+                if (pos0 + kBN > len || pos0 < low) {   // 64 bits, one a position: below len, and from low on or among the sinks
+                    const auto below = [&](uint32_t n) -> uint64_t { return n <= pos0 ? 0ull : n - pos0 >= kBN ? ~0ull : (1ull << (n - pos0)) - 1; };
+                    const uint64_t seen = below(len) & (~below(low) | below(p.sinks));
 #pragma unroll
-                    for (int i = 0; i < kBN; ++i) s[i] = pos0 + i < len && (pos0 + i >= low || pos0 + i < p.sinks) ? s[i] : -INFINITY;
+                    for (int i = 0; i < kBN; ++i) s[i] = (seen >> i) & 1 ? s[i] : -INFINITY;
                 }
             } else if (pos0 + kBN > len) {
 #pragma unroll
