@@ -27,7 +27,7 @@ constexpr uint32_t kMostParts = 16;        // of a row tile
 constexpr int kPrepareThreads = 256;
 
 // Estimated costs of the chunk kernel, us, as the single-sequence launch's (pick_kv_splits): a tile, a CTA's set-up and output, a merge, a partial.
-struct ChunkCosts { float tile, cta, merge, part; };
+struct ChunkCosts { float tile, cta, last_wave, merge, part; };   // last_wave: of a wave, where it is not full
 
 struct PrepareParams {
     Paged pool;
@@ -116,8 +116,9 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         if (tid == 0) report(p.pool, B200KV_STATUS_BAD_BOUND);
         return;
     }
-    // ---- how far to split: candidate c has pieces of at most longest / (c + 1) tiles.  CTAs take one another's place as they end, so the time is about the
-    // work over the SMs and half a piece more, and no less than a piece.
+    // ---- how far to split: candidate c has pieces of at most longest / (c + 1) tiles.  The time is no less than a piece, than the work over the SMs and half a
+    // piece more (CTAs take one another's place as they end), and than as many waves of average pieces as there are (152 pieces of one size on 148 SMs
+    // take twice as long as 148: 77 us for two chunks of 333 tokens over 5000).
     if (tid < kMostParts) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0.0f; }
     __syncthreads();
@@ -142,7 +143,9 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         float us = INFINITY;
         if (tid < kMostParts && (tid == 0 || (sh.items[tid] <= p.max_items && sh.parts[tid] <= p.max_parts))) {
             const float one = piece_of(tid) * p.costs.tile + p.costs.cta, all = (sh.work * p.costs.tile + sh.items[tid] * p.costs.cta) / p.sms;
-            us = max(one, all + 0.5f * one) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
+            const uint32_t n = sh.items[tid], full = n / p.sms, rest = n % p.sms;
+            const float waves = full + (rest == 0 ? 0.0f : full == 0 ? 1.0f : p.costs.last_wave + (1.0f - p.costs.last_wave) * rest / p.sms);
+            us = max(max(one, all + 0.5f * one), waves * (sh.work / n * p.costs.tile + p.costs.cta)) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
         }
         const float best = -warp_max_redux(-us);
         const uint32_t which = __ffs(__ballot_sync(0xffffffffu, us == best)) - 1;
@@ -396,8 +399,9 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     if (batch.total_length > 0) r.scratch_tiles = std::min(r.scratch_tiles, batch.total_length / kChunkTile + sequences);
     // every sequence's last row tile may be a partial one
     const uint64_t row_tiles = std::min<uint64_t>(batch.total_tokens * group / kChunkRows + sequences, sequences * ((batch.max_tokens * group + kChunkRows - 1) / kChunkRows));
+    // (CTAs of the grid that turn out to have nothing to do cost a launch microseconds: row tiles are split where there are fewer of them than this)
     const uint64_t units = row_tiles * view.kv_heads, parts = 4ull * sms;
-    r.max_items = static_cast<uint32_t>(std::min<uint64_t>(units + parts, 0x7fffffffu));
+    r.max_items = static_cast<uint32_t>(std::min<uint64_t>(std::max(units, parts), 0x7fffffffu));
     r.max_parts = static_cast<uint32_t>(parts);
     size_t at = 256;                                     // the plan
     const auto take = [&](uint64_t bytes) { const size_t here = at; at += up(bytes, 1024); return here; };
@@ -459,7 +463,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const uint32_t few_rows = room.decode ? decode_rows(*batch, group) : 0;
         const PrepareParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items,
                                room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
-                               view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.3f, 0.017f},
+                               view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.0f, 1.3f, 0.017f},
                                {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}};
         const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
         const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;

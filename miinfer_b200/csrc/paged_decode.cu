@@ -4,7 +4,8 @@
 //
 //  * The tiles of 128 positions of all (sequence, kv head) pairs form one list, and every CTA of a grid that fits the device at once takes an equal piece
 //    of it, whatever the lengths are (sequences of 512 to 16384 positions in one launch end together).  A piece crosses from one pair to the next with its
-//    copies running on; a pair that lies in several pieces leaves partials, two a CTA at most, for paged_decode_merge_kernel.  Nothing waits for another CTA.
+//    copies running on; a pair that lies in several pieces leaves partials, two a CTA at most, and the CTA in whose piece it begins, of which there is one
+//    such pair at most, leaves word of it for paged_decode_merge_kernel.  Nothing waits for another CTA.
 //  * K and V come as units of 128 rows through tensor maps over the whole pool, a box a page (pages of less than 128 positions: several), each into a ring
 //    of its own, the block scales beside them as bulk copies.  (One ring K0 V0 K1 V1 ... of an odd number of units would show an issuer, which reads one of
 //    the two, every second phase of a slot only, and a parity does not tell those apart.)  The bytes are operands as they land:
@@ -47,7 +48,7 @@ struct Layout {
     static constexpr uint32_t kTmemCols = 2 * (kSCols + kOCols) <= 128 ? 128 : 2 * (kSCols + kOCols) <= 256 ? 256 : 512;
     static constexpr uint32_t kColS = 0, kColO = 2 * kSCols;
     static constexpr int kXchWords = 16;                                                  // 4 maxima of scores, up to 8 of value scales
-    static constexpr int kMiscBytes = RG * 2 * 4 * kXchWords * 4 + RG * 64 + 2 * 8 * 4 + 12 * 16 + 24 * 8 + 64;
+    static constexpr int kMiscBytes = RG * 2 * 4 * kXchWords * 4 + RG * 64 + 2 * 8 * 4 + 12 * 16 + 24 * 8 + 80;
     static constexpr int kMostUnits = 6;
     static constexpr int kBudget = (kCtas == 2 ? 115712 : 232448) - 1024;                 // the base is brought to a multiple of 1024
     static constexpr int kFixed = 2 * RG * kPBytes + 2 * kQBytes + kMiscBytes;
@@ -74,7 +75,7 @@ struct Layout {
     static constexpr int K_FULL = 0, V_FULL = K_FULL + kKUnits, K_EMPTY = V_FULL + kVUnits, V_EMPTY = K_EMPTY + kKUnits, LANDED = V_EMPTY + kVUnits, S_FULL = LANDED + 1, S_EMPTY = S_FULL + 2, P_FULL = S_EMPTY + 2, P_EMPTY = P_FULL + 2 * RG,
                          Q_FULL = P_EMPTY + 2 * RG, Q_EMPTY = Q_FULL + 2, kNumBars = Q_EMPTY + 2;
     static constexpr int kOffMisc = kOffBar + kNumBars * 8;                               // tmem slot, fail flag, the piece
-    static constexpr int kTotal = (kOffMisc + 32 + 15) / 16 * 16;
+    static constexpr int kTotal = (kOffMisc + 48 + 15) / 16 * 16;
     static constexpr int kAlloc = kTotal + 1024;
     static_assert(kTotal <= kBudget);
 };
@@ -119,6 +120,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     Cursor c(p, start);
+    if (c.left == 0 && tid == 0) p.shared[blockIdx.x] = make_uint4(0, 0, 0, 0);
     bool failed = false;
 
     if (warp == L::kProducerWarp) {
@@ -520,6 +522,16 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 const float4 a = *reinterpret_cast<const float4*>(sums + x * 4);
                 lt[0] += a.x; lt[1] += a.y; lt[2] += a.z; lt[3] += a.w;
             }
+            if (tid == 0 && c.left == n) {               // the piece's last pair
+                uint4 word = make_uint4(c.s, c.head, 0, 0);
+                if (c.tile == 0 && n < c.t.n) {
+                    const uint64_t all = start[5] | static_cast<uint64_t>(start[6]) << 32;
+                    const uint32_t pieces = pieces_of(p, all);
+                    word.z = piece_with(all, piece_begin(all, blockIdx.x + 1, pieces) - n + c.t.n - 1, pieces);
+                    word.w = 1;
+                }
+                p.shared[blockIdx.x] = word;
+            }
             const bool poisoned = *fail_flag != 0;
             group_sync();                                // the sums are read: the next pair may write its own
             if (poisoned && t128 == 0) report(p.pool, B200KV_STATUS_PIPE_TIMEOUT);
@@ -562,52 +574,51 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
     }
 }
 
-// out = sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M), times sigmoid(gate), over the CTAs whose pieces hold tiles of a pair.  A block: a query row of a pair, a
-// thread a dim.  Pairs of one piece have been written by their CTA.
+// out = sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M), times sigmoid(gate), over the CTAs whose pieces hold tiles of a pair.  A block: a query row of the pair that
+// begins in piece blockIdx.y and ends in a later one, a thread a dim.  All other pairs have been written by their CTA.
 template <int D>
 __global__ void __launch_bounds__(D) paged_decode_merge_kernel(const __grid_constant__ PagedDecode p) {
-    __shared__ uint64_t range[2];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t s = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
-    const uint32_t H = p.pool.view.kv_heads, G = p.query_heads / H;
-    const Span span = span_of(p.pool, s);
-    const Tiles t = p.tiles_of(span);
-    if (t.n == 0 || row >= span.tokens * G) return;
-    if (tid < 32) {
-        const uint64_t all = tiles_before(p, p.pool.batch.sequences, tid), before = tiles_before(p, s, tid);
-        if (tid == 0) { range[0] = all; range[1] = before; }
-    }
-    __syncthreads();
-    const uint64_t all = range[0], begin = range[1] + static_cast<uint64_t>(head) * t.n, end = begin + t.n;
-    const uint32_t pieces = pieces_of(p, all);
-    auto piece_of = [&](uint64_t w) {   // the piece that holds tile w: the first all % pieces of them have a tile more
-        const uint64_t each = all / pieces, more = all % pieces, bound = more * (each + 1);
-        return static_cast<uint32_t>(w < bound ? w / (each + 1) : more + (w - bound) / each);
-    };
-    const uint32_t c0 = piece_of(begin), c1 = piece_of(end - 1);
-    if (c0 == c1) return;
-    // a CTA's first partial is of a pair that began before its piece
-    auto part_of = [&](uint32_t c) { return (2 * static_cast<size_t>(c) + (piece_begin(all, c, pieces) > begin ? 0 : 1)) * kDecodeRows + row; };
-    float m = -INFINITY;
+    const uint32_t c0 = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, G = p.query_heads / p.pool.view.kv_heads;
+    const uint4 word = p.shared[c0];
+    if (word.w == 0) return;
+    const Span span = span_of(p.pool, word.x);
+    if (row >= span.tokens * G) return;
+    auto part_of = [&](uint32_t c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * kDecodeRows + row; };   // a later CTA's first partial
+    float m = -INFINITY, l = 0.0f, acc = 0.0f;
     bool poisoned = false;
-    for (uint32_t c = c0; c <= c1; ++c) {
-        const float2 ml = p.part_ml[part_of(c)];
-        poisoned |= ml.y != ml.y;
-        if (ml.y > 0.0f) m = fmaxf(m, ml.x);
-    }
-    float l = 0.0f, acc = 0.0f;
-#pragma unroll 8
-    for (uint32_t c = c0; c <= c1; ++c) {
-        const size_t part = part_of(c);
-        const float2 ml = p.part_ml[part];
-        const float o = p.part_o[part * D + tid];
-        const float w = ml.y > 0.0f ? exp2f(ml.x - m) : 0.0f;
-        l = fmaf(w, ml.y, l);
-        acc = w > 0.0f ? fmaf(w, o, acc) : acc;
+    for (uint32_t c = c0; c <= word.z; c += 8) {   // eight partials' loads under way together
+        float2 ml[8];
+        float o[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            o[i] = 0.0f;
+            if (c + i > word.z) continue;
+            ml[i] = p.part_ml[part_of(c + i)];
+            o[i] = p.part_o[part_of(c + i) * D + tid];
+        }
+        float m_new = m;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            poisoned |= ml[i].y != ml[i].y;
+            if (ml[i].y > 0.0f) m_new = fmaxf(m_new, ml[i].x);
+        }
+        const float f = m_new > m && m > -INFINITY ? ex2(m - m_new) : m_new > m ? 0.0f : 1.0f;
+        l *= f;
+        acc *= f;
+        m = m_new;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (!(ml[i].y > 0.0f)) continue;
+            const float w = ex2(ml[i].x - m);
+            l = fmaf(w, ml[i].y, l);
+            if (w > 0.0f) acc = fmaf(w, o[i], acc);
+        }
     }
     const float nan = __int_as_float(0x7fc00000);
-    const size_t head_row = (static_cast<size_t>(span.first) + row / G) * p.query_heads + head * G + row % G, at = head_row * D + tid;
+    const size_t head_row = (static_cast<size_t>(span.first) + row / G) * p.query_heads + word.y * G + row % G, at = head_row * D + tid;
     if (p.lse != nullptr && tid == 0) p.lse[head_row] = poisoned ? nan : l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
     float v = poisoned ? nan : l > 0.0f ? acc / l : 0.0f;
     if (p.gate != nullptr) v *= 1.0f / (1.0f + __expf(-p.gate[at]));
@@ -642,7 +653,7 @@ uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t, uint32_t sms) {
     return sms * (view.head_dim == 128 && view.quant_mode == B200KV_Q8_Q8 ? 2 : 1);
 }
 size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms) {
-    return 2ull * decode_ctas(view, query_heads, sms) * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2));
+    return decode_ctas(view, query_heads, sms) * (2ull * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2)) + sizeof(uint4));
 }
 
 int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind) {
@@ -662,13 +673,14 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     p.least_tiles = 2;
     p.part_o = static_cast<float*>(parts);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ull * most * kDecodeRows * v.head_dim);
+    p.shared = reinterpret_cast<uint4*>(p.part_ml + 2ull * most * kDecodeRows);
     const int rc = v.head_dim == 128 ? (few ? launch_modes<128, 1>(p, kmap, vmap, stream, behind) : launch_modes<128, 2>(p, kmap, vmap, stream, behind))
                                      : (few ? launch_modes<256, 1>(p, kmap, vmap, stream, behind) : launch_modes<256, 2>(p, kmap, vmap, stream, behind));
     if (rc != B200KV_OK) return rc;
     // one tile a pair: no pair lies in two pieces
     if (b.max_length <= kDecodeTile) return B200KV_OK;
     const uint32_t most_rows = static_cast<uint32_t>(std::min<uint64_t>(p.rows, static_cast<uint64_t>(b.max_tokens) * group));
-    const dim3 grid(most_rows, v.kv_heads, b.sequences);
+    const dim3 grid(most_rows, p.ctas);
     B200KV_CUDA_TRY(v.head_dim == 128 ? launch_behind(paged_decode_merge_kernel<128>, grid, dim3(128), 0, stream, p)
                                       : launch_behind(paged_decode_merge_kernel<256>, grid, dim3(256), 0, stream, p));
     return B200KV_OK;

@@ -24,6 +24,7 @@ struct PagedDecode {
     uint32_t least_tiles;      // fewest tiles of a piece
     float* part_o;             // [2 ctas][kDecodeRows][head_dim]: a CTA's piece begins and ends inside a kv head's tiles at most once each
     float2* part_ml;           // [2 ctas][kDecodeRows] {maximum in log2 units, sum}
+    uint4* shared;             // [ctas]: the pair that begins in a CTA's piece and ends in another's: sequence, kv head, the other CTA, 1 (0: there is none)
     __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
         if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * (query_heads / pool.view.kv_heads) > rows) return {0, 0, 0};
         Tiles t = tiles_seen(span.base(), span.length, window, sinks);

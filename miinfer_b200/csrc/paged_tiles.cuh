@@ -48,7 +48,13 @@ __device__ __forceinline__ uint64_t piece_begin(uint64_t all, uint32_t c, uint32
     return c * each + min(static_cast<uint64_t>(c), more);
 }
 
-// CTA c's piece, by a warp: start = {sequence, kv head, tile, tiles of the piece (two words)}.
+// The piece that holds tile w.
+__device__ __forceinline__ uint32_t piece_with(uint64_t all, uint64_t w, uint32_t pieces) {
+    const uint64_t each = all / pieces, more = all % pieces, bound = more * (each + 1);
+    return static_cast<uint32_t>(w < bound ? w / (each + 1) : more + (w - bound) / each);
+}
+
+// CTA c's piece, by a warp: start = {sequence, kv head, tile, tiles of the piece (two words), tiles of the list (two words)}.
 template <class P>
 __device__ __forceinline__ void find_piece(const P& p, uint32_t c, int lane, uint32_t* start) {
     const uint32_t S = p.pool.batch.sequences, H = p.pool.view.kv_heads;
@@ -83,6 +89,8 @@ __device__ __forceinline__ void find_piece(const P& p, uint32_t c, int lane, uin
     if (lane == 0) {
         start[3] = static_cast<uint32_t>(count);
         start[4] = static_cast<uint32_t>(count >> 32);
+        start[5] = static_cast<uint32_t>(all);
+        start[6] = static_cast<uint32_t>(all >> 32);
     }
 }
 

@@ -63,8 +63,8 @@ struct FewLayout {
     static constexpr int kOffQ = kUnits * U::kData, kOffScales = kOffQ + 2 * kQBytes, kOffRows = kOffScales + kUnits * U::kScales;   // rows: [buffer][8] {factor, statistics}
     static constexpr int kOffBar = kOffRows + 2 * 8 * 8;
     static constexpr int FULL = 0, EMPTY = kUnits, LANDED = 2 * kUnits, S_FULL = LANDED + 1, S_EMPTY = S_FULL + 2, Q_FULL = S_EMPTY + 2, Q_EMPTY = Q_FULL + 2, kNumBars = Q_EMPTY + 2;
-    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 32 + 1024;
-    static_assert(kOffMisc + 32 - kOffRows <= kMisc);
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 48 + 1024;
+    static_assert(kOffMisc + 48 - kOffRows <= kMisc);
 };
 
 template <int D, int KF, int ROWS>
@@ -290,8 +290,8 @@ struct ManyLayout {
     static constexpr int kOffBar = kOffSum + 2 * kTile * 4;
     static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + kRaw, LANDED = RAW_EMPTY + kRaw, K_FULL = LANDED + 1, Q_FULL = K_FULL + 1, Q_EMPTY = Q_FULL + kQBufs,
                          S_FULL = Q_EMPTY + kQBufs, S_EMPTY = S_FULL + kSBufs, kNumBars = S_EMPTY + kSBufs;
-    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 32 + 1024;
-    static_assert(kOffMisc + 32 - kOffRows <= kMisc);
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 48 + 1024;
+    static_assert(kOffMisc + 48 - kOffRows <= kMisc);
 };
 
 // eight fp16 of a row as one 16-byte chunk of a K-major operand: slabs of 64 dims, kGroup rows of 128 bytes each, 128-byte swizzle

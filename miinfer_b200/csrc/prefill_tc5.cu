@@ -302,8 +302,8 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     [[maybe_unused]] int row_gap = 0, position_gap = 0;
     if constexpr (PAGED) {
         pdl_wait();   // the list comes from the call's first kernel
+        item = reload(p.items + blockIdx.x);       // (beside the count, not behind it; the list has room for every CTA)
         if (blockIdx.x >= p.plan->items) return;   // the grid is sized by bounds
-        item = reload(p.items + blockIdx.x);
         sink_tiles = item.sink_tiles;
         row_gap = static_cast<int>(item.skip * kBN);
         position_gap = static_cast<int>(item.window0 + (item.skip - item.sink_tiles) * kBN);
