@@ -23,7 +23,7 @@ namespace b200kv {
 
 namespace {
 
-constexpr uint32_t kMostParts = 16;        // of a row tile
+constexpr uint32_t kCandidates = 31;       // sizes of a piece that the layout chooses from: the smallest a sixteenth of a row tile
 constexpr int kPrepareThreads = 256;
 
 // Estimated costs of the chunk kernel, us, as the single-sequence launch's (pick_kv_splits): a tile, a CTA's set-up and output, a merge, a partial.
@@ -104,7 +104,7 @@ __device__ __forceinline__ Walk walk_of(const PrepareParams& p, const Span& span
 
 struct PlanScratch {
     Sums scan[kPrepareThreads / 32];
-    uint32_t items[kMostParts], parts[kMostParts], longest, piece;
+    uint32_t items[kCandidates], parts[kCandidates], longest, piece;
     float work;
 };
 
@@ -116,23 +116,22 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         if (tid == 0) report(p.pool, B200KV_STATUS_BAD_BOUND);
         return;
     }
-    // ---- how far to split: candidate c has pieces of at most longest / (c + 1) tiles.  The time is no less than a piece, than the work over the SMs and half a
-    // piece more (CTAs take one another's place as they end), and than as many waves of average pieces as there are (152 pieces of one size on 148 SMs
-    // take twice as long as 148: 77 us for two chunks of 333 tokens over 5000).
-    if (tid < kMostParts) sh.items[tid] = sh.parts[tid] = 0;
+    // ---- how far to split: candidate c has pieces of at most 2 longest / (c + 2) tiles.  The time is no less than a piece's, and about as many waves of average
+    // pieces as there are: 152 pieces of one size on 148 SMs take twice as long as 148 (77 us for two chunks of 333 tokens over 5000).
+    if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0.0f; }
     __syncthreads();
     for (uint32_t s = tid; s < S; s += kPrepareThreads)
         if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
     __syncthreads();
     const uint32_t longest = sh.longest;
-    const auto piece_of = [&](uint32_t c) { return max(3u, (longest + c) / (c + 1)); };
+    const auto piece_of = [&](uint32_t c) { return max(3u, (2 * longest + c + 1) / (c + 2)); };
     for (uint32_t s = tid; s < S; s += kPrepareThreads) {
         const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
         if (n == 0) continue;
         // (tokens of a chunk see on average half of it)
         atomicAdd(&sh.work, static_cast<float>(n) * (static_cast<float>(tiles) - 0.5f * min(static_cast<float>(tiles), static_cast<float>(span_of(p.pool, s).tokens) / kChunkTile)));
-        for (uint32_t c = 0; c < kMostParts; ++c) {
+        for (uint32_t c = 0; c < kCandidates; ++c) {
             const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
             atomicAdd(&sh.items[c], n * pieces);
             if (pieces > 1) atomicAdd(&sh.parts[c], n * pieces);
@@ -141,11 +140,11 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     __syncthreads();
     if (tid < 32) {
         float us = INFINITY;
-        if (tid < kMostParts && (tid == 0 || (sh.items[tid] <= p.max_items && sh.parts[tid] <= p.max_parts))) {
-            const float one = piece_of(tid) * p.costs.tile + p.costs.cta, all = (sh.work * p.costs.tile + sh.items[tid] * p.costs.cta) / p.sms;
+        if (tid < kCandidates && (tid == 0 || (sh.items[tid] <= p.max_items && sh.parts[tid] <= p.max_parts))) {
+            const float one = piece_of(tid) * p.costs.tile + p.costs.cta;
             const uint32_t n = sh.items[tid], full = n / p.sms, rest = n % p.sms;
             const float waves = full + (rest == 0 ? 0.0f : full == 0 ? 1.0f : p.costs.last_wave + (1.0f - p.costs.last_wave) * rest / p.sms);
-            us = max(max(one, all + 0.5f * one), waves * (sh.work / n * p.costs.tile + p.costs.cta)) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
+            us = max(one, waves * (sh.work / n * p.costs.tile + p.costs.cta)) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
         }
         const float best = -warp_max_redux(-us);
         const uint32_t which = __ffs(__ballot_sync(0xffffffffu, us == best)) - 1;
