@@ -23,7 +23,7 @@ namespace b200kv {
 
 namespace {
 
-constexpr uint32_t kCandidates = 31;       // sizes of a piece that the layout chooses from: the smallest a sixteenth of a row tile
+constexpr uint32_t kCandidates = 31;       // sizes of a piece that the layout chooses from: the smallest an eleventh of a row tile
 constexpr int kPrepareThreads = 256;
 
 // Estimated costs of the chunk kernel, us, as the single-sequence launch's (pick_kv_splits): a tile, a CTA's set-up and output, a merge, a partial.
@@ -116,7 +116,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         if (tid == 0) report(p.pool, B200KV_STATUS_BAD_BOUND);
         return;
     }
-    // ---- how far to split: candidate c has pieces of at most 2 longest / (c + 2) tiles.  The time is no less than a piece's, and about as many waves of average
+    // ---- how far to split: candidate c has pieces of at most 3 longest / (c + 3) tiles.  The time is no less than a piece's, and about as many waves of average
     // pieces as there are: 152 pieces of one size on 148 SMs take twice as long as 148 (77 us for two chunks of 333 tokens over 5000).
     if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0.0f; }
@@ -125,7 +125,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
     __syncthreads();
     const uint32_t longest = sh.longest;
-    const auto piece_of = [&](uint32_t c) { return max(3u, (2 * longest + c + 1) / (c + 2)); };
+    const auto piece_of = [&](uint32_t c) { return max(3u, (3 * longest + c + 2) / (c + 3)); };
     for (uint32_t s = tid; s < S; s += kPrepareThreads) {
         const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
         if (n == 0) continue;
@@ -462,7 +462,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const uint32_t few_rows = room.decode ? decode_rows(*batch, group) : 0;
         const PrepareParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items,
                                room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
-                               view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.43f, 1.95f, 1.0f, 1.3f, 0.017f},
+                               view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.5f, 7.0f, 1.0f, 2.0f, 0.02f},
                                {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}};
         const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
         const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;

@@ -131,9 +131,11 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
             const int lowest = p.window > 0 ? c.span.base() + 1 - static_cast<int>(p.window) : 0;
             const uint32_t low = lowest > 0 ? static_cast<uint32_t>(lowest) : 0;   // positions below it that are not sinks are seen by nobody
             const uint32_t n = c.take(), length = c.span.length;
+            int page = box_page(p.pool, pages, c.t.position(c.tile), length, lane);
             for (uint32_t j = 0; j < n && !failed; ++j, ++i) {
                 const uint32_t pos0 = c.t.position(c.tile + j), ks = i % L::kKUnits, vs = i % L::kVUnits;
-                const Boxes boxes = boxes_of(p.pool, pages, c.head, pos0, length, lane);
+                const Boxes boxes = boxes_of(p.pool, page, c.head, pos0, length, lane);
+                if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), length, lane);
                 const bool edge = pos0 + kDecodeTile > length || (pos0 < low && pos0 + kDecodeTile > p.sinks);
                 const auto unseen = [&](uint32_t r) { return pos0 + r >= length || (pos0 + r < low && pos0 + r >= p.sinks); };
                 failed = i >= L::kKUnits && !wait_warp(bar(L::K_EMPTY + ks), ((i / L::kKUnits) & 1) ^ 1);
@@ -670,7 +672,7 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     const bool few = p.rows == 4;
     const uint32_t sms = std::min(device_sms(), kMostSms), most = decode_ctas(v, p.query_heads, sms);
     p.ctas = few ? most : sms;
-    p.least_tiles = 2;
+    p.least_tiles = 1;
     p.part_o = static_cast<float*>(parts);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ull * most * kDecodeRows * v.head_dim);
     p.shared = reinterpret_cast<uint4*>(p.part_ml + 2ull * most * kDecodeRows);

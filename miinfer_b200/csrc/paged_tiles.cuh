@@ -58,7 +58,24 @@ __device__ __forceinline__ uint32_t piece_with(uint64_t all, uint64_t w, uint32_
 template <class P>
 __device__ __forceinline__ void find_piece(const P& p, uint32_t c, int lane, uint32_t* start) {
     const uint32_t S = p.pool.batch.sequences, H = p.pool.view.kv_heads;
-    const uint64_t all = tiles_before(p, S, lane);
+    constexpr uint32_t kOnce = 4;   // up to 128 sequences are looked up once, their loads together
+    uint32_t mine_n[kOnce];
+    uint64_t all = 0;
+    if (S <= 32 * kOnce) {
+        Span spans[kOnce];
+#pragma unroll
+        for (uint32_t x = 0; x < kOnce; ++x) spans[x] = span_of(p.pool, min(32 * x + lane, S - 1));
+#pragma unroll
+        for (uint32_t x = 0; x < kOnce; ++x) {
+            mine_n[x] = 32 * x + lane < S ? p.tiles_of(spans[x]).n : 0;
+            all += mine_n[x];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        all *= H;
+    } else {
+        all = tiles_before(p, S, lane);
+    }
     const uint32_t pieces = pieces_of(p, all);
     uint64_t begin = 0, count = 0;
     if (all > 0 && c < pieces) {
@@ -69,7 +86,14 @@ __device__ __forceinline__ void find_piece(const P& p, uint32_t c, int lane, uin
         uint64_t before = 0;   // the sequence in which it begins, 32 at a time
         for (uint32_t s0 = 0; s0 < S; s0 += 32) {
             const uint32_t s = s0 + lane;
-            const uint32_t n = s < S ? p.tiles_of(span_of(p.pool, s)).n : 0;
+            uint32_t n = 0;
+            if (S <= 32 * kOnce) {
+#pragma unroll
+                for (uint32_t x = 0; x < kOnce; ++x)
+                    if (s0 == 32 * x) n = mine_n[x];
+            } else if (s < S) {
+                n = p.tiles_of(span_of(p.pool, s)).n;
+            }
             uint64_t inc = static_cast<uint64_t>(n) * H;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {

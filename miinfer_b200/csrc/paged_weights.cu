@@ -102,9 +102,11 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
         for (; c.left > 0 && ok; c.advance(p)) {
             const int32_t* pages = pages_of(p.pool, c.s);
             const uint32_t n = c.take();
+            int page = box_page(p.pool, pages, c.t.position(c.tile), c.span.length, lane);
             for (uint32_t j = 0; j < n && ok; ++j, ++i) {
                 const uint32_t slot = i % L::kUnits;
-                const Boxes boxes = boxes_of(p.pool, pages, c.head, c.t.position(c.tile + j), c.span.length, lane);
+                const Boxes boxes = boxes_of(p.pool, page, c.head, c.t.position(c.tile + j), c.span.length, lane);
+                if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), c.span.length, lane);
                 ok = i < L::kUnits || wait_warp(bar(L::EMPTY + slot), ((i / L::kUnits) & 1) ^ 1);
                 ok = ok && bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes,
                                              false, [](uint32_t) { return false; }, lane);
@@ -487,7 +489,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
         uint32_t i = 0, fixes = 0;
         each_tile([&](const Share& sh) {
             const uint32_t raw = i % L::kRaw;
-            const Boxes boxes = boxes_of(p.pool, pages_of(p.pool, c.s), c.head, sh.pos0, c.span.length, lane);
+            const Boxes boxes = boxes_of(p.pool, box_page(p.pool, pages_of(p.pool, c.s), sh.pos0, c.span.length, lane), c.head, sh.pos0, c.span.length, lane);
             if (i >= L::kRaw && !wait_warp(bar(L::RAW_EMPTY + raw), ((i / L::kRaw) & 1) ^ 1)) return false;
             ++i;
             return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, false,
