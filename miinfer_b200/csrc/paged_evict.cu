@@ -3,16 +3,19 @@
 // Of L > keep positions the first `sinks` and the last `recent` stay, and of the middle the k = keep - sinks - recent with the largest weights; each kv
 // head chooses for itself.  Two kernels:
 //
-//  * paged_choose_kernel, a cluster of CTAs for a (sequence, kv head).  The k-th largest weight of the middle is found digit by digit (radix
-//    selection): a weight becomes a 32-bit key that orders as the weights do, and four passes count the keys under the digits found so far by their next
-//    eight bits, in shared memory, every CTA over its own stretch of positions, all counts together through distributed shared memory.  What is left is
-//    the key T of the k-th largest and how many of the positions that share it stay, the lowest ones; a position's place among those that stay is
-//    then a count over the ones before it (a scan over warps, CTAs, and the lanes' ballots).
-//  * paged_move_kernel copies the rows.  With a table of its own for the target nothing can collide, and rows are spread over the device.  In place, row r
-//    comes from a position >= r, so a cluster takes a (sequence, kv head, side) and moves the rows in rounds of what its threads hold in registers: all
-//    of a round is read before any of it is written (a cluster barrier), and what a round writes no later round reads.
+//  * paged_choose_kernel, a CTA for a (sequence, kv head) of up to 16384 positions, a cluster of up to eight for more; a thread keeps its keys in registers
+//    (beyond 131072 positions it makes them again).  The k-th largest weight of the middle is found digit by digit (radix selection): a weight becomes a 32-bit
+//    key that orders as the weights do, and three passes count the keys under the digits found so far by their next eleven bits, in shared memory, every CTA
+//    over its own stretch of positions, a cluster's counts together through distributed shared memory.  (Four passes of eight bits: weights share sign and
+//    exponent, so a first digit without any of the mantissa has most of them wait for a handful of words; 8000 weights 12 us, 70000 21.)  What is left is the key T of the k-th largest and how many
+//    of the positions that share it stay, the lowest ones; a position's place among those that stay is then a count over the ones before it (a
+//    scan over warps, CTAs, and the lanes' ballots).
+//  * paged_move_kernel copies the rows, a warp a few at a time: its lanes look up a row each, source and target, then all of the rows' pieces are under way
+//    together.  With a table of its own for the target nothing can collide, and rows are spread over the device.  In place, row r comes from a
+//    position >= r, so a cluster takes a (sequence, kv head, side) and moves the rows in rounds: all of a round is read before any of it is written (a
+//    cluster barrier), and what a round writes no later round reads.
 //
-// The choice is bound by its chain of passes (the weights come from HBM once and from L2 or L1 after that), the copy by HBM.
+// The choice is bound by its chain of passes, the copy by HBM and the chain of its lookups.
 #include "paged_common.cuh"
 
 #include <cooperative_groups.h>
@@ -25,8 +28,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32;
+constexpr int kChooseThreads = 1024, kChooseWarps = kChooseThreads / 32;
 constexpr uint32_t kMaxCluster = 8;
+constexpr int kKept = 16;            // keys of a thread in registers
+constexpr uint32_t kDigits = 2048;   // of a pass
 
 struct EvictParams {
     Paged pool;
@@ -46,9 +51,11 @@ __device__ __forceinline__ uint32_t key_of(float w) {
     return magnitude == 0 || u == magnitude ? magnitude | 0x80000000u : ~u;   // minus infinity: 0x007fffff
 }
 
+// CACHED: a thread has no more than kKept keys.
+template <bool CACHED>
 __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const __grid_constant__ EvictParams p) {
-    __shared__ uint32_t counts[2][256];      // of a pass, two in turn: a CTA may still be read while its next pass counts
-    __shared__ uint32_t sums[256];
+    __shared__ uint32_t counts[2][kDigits];  // of a pass, two in turn: a CTA may still be read while its next pass counts
+    __shared__ uint32_t warp_sums[kChooseWarps];
     __shared__ uint32_t warp_above[kChooseWarps], warp_equal[kChooseWarps];
     __shared__ uint32_t totals[2];           // of this CTA's stretch: positions above the threshold, and at it
     __shared__ uint32_t found[2];            // a pass's digit, and how many of the chosen lie at or below it
@@ -73,119 +80,149 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const __gr
     }
     const uint32_t mid0 = p.sinks, mid1 = L - p.recent;
     uint32_t wanted = keep - p.sinks - p.recent;
+    // this CTA's stretch of the middle, and this warp's piece of it, 32 positions at a time
+    const uint32_t share = ((mid1 - mid0 + ctas - 1) / ctas + 31) / 32 * 32;
+    const uint32_t a = min(mid0 + rank * share, mid1), b = min(a + share, mid1);
+    const uint32_t piece = ((b - a + kChooseWarps - 1) / kChooseWarps + 31) / 32 * 32;
+    const uint32_t w0 = min(a + warp * piece, b), w1 = min(w0 + piece, b);
+    uint32_t mine[CACHED ? kKept : 1];
+    if constexpr (CACHED) {
+        float w[kKept];
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) w[i] = w0 + 32 * i + lane < w1 ? weights[w0 + 32 * i + lane] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) mine[i] = key_of(w[i]);
+    }
+    // f(position, key, whether there is one) for this lane's positions, in order; the whole warp
+    auto each = [&](auto f) {
+        if constexpr (CACHED) {
+#pragma unroll
+            for (int i = 0; i < kKept; ++i) {
+                const uint32_t j = w0 + 32 * i;
+                if (j < w1) f(j + lane, mine[i], j + lane < w1);
+            }
+        } else {
+#pragma unroll 4
+            for (uint32_t j = w0; j < w1; j += 32) f(j + lane, j + lane < w1 ? key_of(weights[j + lane]) : 0u, j + lane < w1);
+        }
+    };
     for (uint32_t r = me; r < p.sinks + p.recent; r += step) {   // what stays in any case
         const uint32_t j = r < p.sinks ? r : L - p.recent + (r - p.sinks), to = r < p.sinks ? r : keep - p.recent + (r - p.sinks);
         kept[to] = static_cast<int32_t>(j);
         if (new_weights != nullptr) new_weights[to] = weights[j];
     }
     if (wanted == 0) return;
-    // this CTA's stretch of the middle, in whole warps
-    const uint32_t share = ((mid1 - mid0 + ctas - 1) / ctas + 31) / 32 * 32;
-    const uint32_t a = min(mid0 + rank * share, mid1), b = min(a + share, mid1);
 
     uint32_t prefix = 0;
 #pragma unroll 1
-    for (int pass = 0; pass < 4; ++pass) {
-        const int shift = 24 - 8 * pass;
-        uint32_t* mine = counts[pass & 1];
-        if (tid < 256) mine[tid] = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above_bits = pass == 0 ? 0 : pass == 1 ? 21 : 10;   // 11, 11 and 10 bits
+        uint32_t* own = counts[pass & 1];
+        for (uint32_t i = tid; i < kDigits / 4; i += kChooseThreads) reinterpret_cast<uint4*>(own)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (uint32_t j = a + tid; j < b; j += kChooseThreads) {
-            const uint32_t key = key_of(weights[j]);
-            if (pass == 0 || (key >> (shift + 8)) == prefix) atomicAdd(&mine[(key >> shift) & 255u], 1u);
+        const uint32_t mask = pass == 2 ? 1023u : 2047u;
+        if (pass == 0) {
+            each([&](uint32_t, uint32_t key, bool there) {
+                if (there) atomicAdd(&own[key >> 21], 1u);
+            });
+        } else {
+            each([&](uint32_t, uint32_t key, bool there) {
+                if (there && (key >> above_bits) == prefix) atomicAdd(&own[(key >> shift) & mask], 1u);
+            });
         }
-        cluster.sync();
-        if (tid < 256) {
-            uint32_t n = 0;
-            for (uint32_t c = 0; c < ctas; ++c) n += cluster.map_shared_rank(mine, c)[tid];
-            sums[tid] = n;
-        }
-        __syncthreads();
-        if (warp == 0) {   // lane l: digits 8l .. 8l + 7; the digit at which the count from the top reaches `wanted`
-            uint32_t own = 0;
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
+        // a thread's two digits, from the top: how many keys have them, and how many a higher one
+        const uint32_t top = kDigits - 2 - 2 * tid;
+        uint2 n = make_uint2(0, 0);
+        if (ctas > 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) own += sums[8 * lane + i];
-            uint32_t above = own;
+            for (uint32_t c = 0; c < kMaxCluster; ++c) {
+                if (c >= ctas) break;
+                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(own, c) + top);
+                n.x += v.x;
+                n.y += v.y;
+            }
+        } else {
+            n = *reinterpret_cast<const uint2*>(own + top);
+        }
+        uint32_t inc = n.x + n.y;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_down_sync(0xffffffffu, above, o);
-                if (lane + o < 32) above += v;
-            }
-            above -= own;      // keys in higher lanes' digits
-            if (above < wanted && above + own >= wanted) {
-                for (int i = 7; i >= 0; --i) {
-                    const uint32_t n = sums[8 * lane + i];
-                    if (above + n >= wanted) { found[0] = 8 * lane + i; found[1] = wanted - above; break; }
-                    above += n;
-                }
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
+        __syncthreads();
+        const uint32_t higher = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0u) + inc - n.x - n.y;
+        if (higher < wanted && higher + n.x + n.y >= wanted) {
+            const bool upper = higher + n.y >= wanted;
+            found[0] = top + (upper ? 1 : 0);
+            found[1] = wanted - higher - (upper ? 0 : n.y);
         }
         __syncthreads();
-        prefix = (prefix << 8) | found[0];
+        prefix = pass == 0 ? found[0] : pass == 1 ? prefix << 11 | found[0] : prefix << 10 | found[0];
         wanted = found[1];
     }
     // `prefix` is the key of the last that stays, `wanted` how many positions with that key do.
 
-    // Places: a warp's positions lie in one piece, 32 at a time in order.
-    const uint32_t piece = ((b - a + kChooseWarps - 1) / kChooseWarps + 31) / 32 * 32;
-    const uint32_t w0 = min(a + warp * piece, b), w1 = min(w0 + piece, b);
     uint32_t above = 0, equal = 0;
-    for (uint32_t j0 = w0; j0 < w1; j0 += 32) {
-        const uint32_t key = j0 + lane < w1 ? key_of(weights[j0 + lane]) : 0;
-        above += __popc(__ballot_sync(0xffffffffu, j0 + lane < w1 && key > prefix));
-        equal += __popc(__ballot_sync(0xffffffffu, j0 + lane < w1 && key == prefix));
-    }
+    each([&](uint32_t, uint32_t key, bool there) {
+        above += __popc(__ballot_sync(0xffffffffu, there && key > prefix));
+        equal += __popc(__ballot_sync(0xffffffffu, there && key == prefix));
+    });
     if (lane == 0) { warp_above[warp] = above; warp_equal[warp] = equal; }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t ta = 0, te = 0;
-        for (int w = 0; w < kChooseWarps; ++w) { ta += warp_above[w]; te += warp_equal[w]; }
-        totals[0] = ta; totals[1] = te;
+    // what lies before this warp's piece: in the CTA's other pieces, and in the stretches of the CTAs before
+    uint32_t x = warp_above[lane], y = warp_equal[lane];
+    static_assert(kChooseWarps == 32);
+    if (ctas > 1 && warp == 0) {
+        const uint32_t tx = __reduce_add_sync(0xffffffffu, x), ty = __reduce_add_sync(0xffffffffu, y);
+        if (lane == 0) { totals[0] = tx; totals[1] = ty; }
     }
-    cluster.sync();
-    uint32_t before_above = 0, before_equal = 0;
-    for (uint32_t c = 0; c < rank; ++c) {
-        const uint32_t* t = cluster.map_shared_rank(totals, c);
-        before_above += t[0];
-        before_equal += t[1];
+    uint32_t before_above = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0), before_equal = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
+    if (ctas > 1) {
+        cluster.sync();
+        for (uint32_t c = 0; c < rank; ++c) {
+            const uint32_t* t = cluster.map_shared_rank(totals, c);
+            before_above += t[0];
+            before_equal += t[1];
+        }
     }
-    for (uint32_t w = 0; w < warp; ++w) { before_above += warp_above[w]; before_equal += warp_equal[w]; }
     const uint32_t lower = (1u << lane) - 1;
-    for (uint32_t j0 = w0; j0 < w1; j0 += 32) {
-        const bool in = j0 + lane < w1;
-        const float w = in ? weights[j0 + lane] : 0.0f;
-        const uint32_t key = key_of(w);
-        const uint32_t is_above = __ballot_sync(0xffffffffu, in && key > prefix), is_equal = __ballot_sync(0xffffffffu, in && key == prefix);
+    each([&](uint32_t j, uint32_t key, bool there) {
+        const uint32_t is_above = __ballot_sync(0xffffffffu, there && key > prefix), is_equal = __ballot_sync(0xffffffffu, there && key == prefix);
         const uint32_t rank_above = before_above + __popc(is_above & lower), rank_equal = before_equal + __popc(is_equal & lower);
-        if (in && (key > prefix || (key == prefix && rank_equal < wanted))) {
+        if (there && (key > prefix || (key == prefix && rank_equal < wanted))) {
             const uint32_t to = p.sinks + rank_above + min(rank_equal, wanted);
-            kept[to] = static_cast<int32_t>(j0 + lane);
-            if (new_weights != nullptr) new_weights[to] = w;
+            kept[to] = static_cast<int32_t>(j);
+            if (new_weights != nullptr) new_weights[to] = weights[j];
         }
         before_above += __popc(is_above);
         before_equal += __popc(is_equal);
-    }
-    cluster.sync();   // no CTA leaves while another may read its counts
+    });
+    if (ctas > 1) cluster.sync();   // no CTA leaves while another may read its counts
 }
 
 // ---- the rows -----------------------------------------------------------------------------------------------------------
 
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
 constexpr int kHeld = 8;   // 16-byte pieces a thread has in flight
 
-// One side's rows: pieces of 16 bytes of data, and the row's scales as one piece of 2, 8 or 16 bytes.
+// One side's rows: 16-byte pieces of data, and the row's scales of 2, 8 or 16 bytes.
 struct Side {
     uint8_t* data;
     uint8_t* scales;             // null for fp16
-    uint32_t pieces;             // 16-byte pieces of a row
+    uint32_t pieces;             // 16-byte pieces of a row: 8, 16 or 32
     uint32_t scale_bytes;
 };
+__host__ __device__ inline uint32_t pieces_of_side(const b200kv_paged_view& v, uint32_t side) { return v.head_dim * ((side == 0 ? is_k_q8(v.quant_mode) : is_v_q8(v.quant_mode)) ? 1 : 2) / 16; }
 __device__ __forceinline__ Side side_of(const b200kv_paged_view& v, uint32_t side) {
     const bool q8 = side == 0 ? is_k_q8(v.quant_mode) : is_v_q8(v.quant_mode);
     Side x;
     x.data = q8 ? reinterpret_cast<uint8_t*>(side == 0 ? v.key_q8 : v.value_q8) : static_cast<uint8_t*>(side == 0 ? v.key_f16 : v.value_f16);
     x.scales = q8 ? static_cast<uint8_t*>(side == 0 ? v.key_scales : v.value_scales) : nullptr;
-    x.pieces = v.head_dim * (q8 ? 1 : 2) / 16;
+    x.pieces = pieces_of_side(v, side);
     x.scale_bytes = q8 ? v.head_dim / v.qblock * 2 : 0;
     return x;
 }
@@ -205,65 +242,56 @@ template <bool IN_PLACE>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ EvictParams p) {
     pdl_wait();   // the choice comes from the kernel just before
     pdl_launch_dependents();   // behind the wait: this kernel writes cache rows
-    const uint32_t s = blockIdx.y, H = p.pool.view.kv_heads, head = blockIdx.z >> 1, side = blockIdx.z & 1;
+    const uint32_t s = blockIdx.y, H = p.pool.view.kv_heads, head = blockIdx.z >> 1, side = blockIdx.z & 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Span span = span_of(p.pool, s);
     const uint32_t rows = min(span.length, p.keep);
     if (IN_PLACE && span.length <= p.keep) return;   // the whole cluster: every row is where it goes
     const Side x = side_of(p.pool.view, side);
     const int32_t* kept = p.kept + (static_cast<size_t>(s) * H + head) * p.keep;
+    const int32_t* source = pages_of(p.pool, s);
     const int32_t* target = p.target_table + static_cast<size_t>(s) * p.target_max_pages;
-    const uint32_t slot_mask = (1u << p.pool.page_shift) - 1;
-    const uint32_t per_row = x.pieces + (x.scales != nullptr ? 1 : 0);   // the last piece of a row: its scales
-    const uint32_t row_bytes = x.pieces * 16;
-    // a thread's piece number n: row n / per_row, piece n % per_row
-    uint4 v[kHeld];
-    uint32_t to[kHeld], piece[kHeld];     // target row of the sequence; 0xffffffff where there is nothing to move
-    auto fetch = [&](uint32_t first, uint32_t stride, uint32_t end) {
+    const uint32_t slot_mask = (1u << p.pool.page_shift) - 1, row_bytes = x.pieces * 16;
+    const uint32_t batch = 32 * kHeld / x.pieces, per_step = 32 / x.pieces == 0 ? 1 : 32 / x.pieces;   // rows of a warp at a time; of one of its steps
+    const uint32_t sub = lane / x.pieces, piece = lane % x.pieces;
+    // lane l < batch: row r0 + l, where it comes from (-1: of no page, zeros) and where it goes (-1: nowhere)
+    long long from = -1, to = -1;
+    uint4 v[kHeld], sc = make_uint4(0, 0, 0, 0);
+    auto fetch = [&](uint32_t r0) {
+        from = to = -1;
+        const uint32_t r = r0 + lane;
+        if (lane < batch && r < rows) {
+            const int j = kept[r];
+            const int there = target[r >> p.pool.page_shift];
+            if (j >= 0 && static_cast<uint32_t>(j) < span.length && !(IN_PLACE && static_cast<uint32_t>(j) == r)) {
+                from = page_row(p.pool, source[static_cast<uint32_t>(j) >> p.pool.page_shift], head);
+                if (from >= 0) from += static_cast<uint32_t>(j) & slot_mask;
+                to = page_row(p.pool, there, head);
+                if (to >= 0) to += r & slot_mask;
+            }
+        }
+        sc = make_uint4(0, 0, 0, 0);
+        if (x.scales != nullptr && from >= 0) sc = load_scales(x.scales + static_cast<size_t>(from) * x.scale_bytes, x.scale_bytes);
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
-            const uint32_t n = first + i * stride;
-            to[i] = 0xffffffffu;
-            if (n >= end) continue;
-            const uint32_t r = n / per_row;
-            const int j = kept[r];
-            if (j < 0 || static_cast<uint32_t>(j) >= span.length || (IN_PLACE && static_cast<uint32_t>(j) == r)) continue;
-            const long long row = row_of(p.pool, s, head, static_cast<uint32_t>(j));
-            to[i] = r;
-            piece[i] = n % per_row;
+            const long long row = __shfl_sync(0xffffffffu, from, i * per_step + sub);
             v[i] = make_uint4(0, 0, 0, 0);
-            if (row < 0) continue;        // a page outside the pool reads as zeros
-            if (piece[i] < x.pieces) v[i] = *reinterpret_cast<const uint4*>(x.data + static_cast<size_t>(row) * row_bytes + piece[i] * 16);
-            else v[i] = load_scales(x.scales + static_cast<size_t>(row) * x.scale_bytes, x.scale_bytes);
+            if (row >= 0) v[i] = *reinterpret_cast<const uint4*>(x.data + static_cast<size_t>(row) * row_bytes + piece * 16);
         }
     };
     auto store = [&] {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
-            if (to[i] == 0xffffffffu) continue;
-            const long long page = page_row(p.pool, target[to[i] >> p.pool.page_shift], head);
-            if (page < 0) continue;
-            const size_t row = static_cast<size_t>(page) + (to[i] & slot_mask);
-            if (piece[i] < x.pieces) *reinterpret_cast<uint4*>(x.data + row * row_bytes + piece[i] * 16) = v[i];
-            else store_scales(x.scales + row * x.scale_bytes, x.scale_bytes, v[i]);
+            const long long row = __shfl_sync(0xffffffffu, to, i * per_step + sub);
+            if (row >= 0) *reinterpret_cast<uint4*>(x.data + static_cast<size_t>(row) * row_bytes + piece * 16) = v[i];
         }
+        if (x.scales != nullptr && to >= 0) store_scales(x.scales + static_cast<size_t>(to) * x.scale_bytes, x.scale_bytes, sc);
     };
-    const uint64_t all = static_cast<uint64_t>(rows) * per_row;
-    const uint64_t round = static_cast<uint64_t>(gridDim.x) * kMoveThreads * kHeld;
-    if constexpr (IN_PLACE) {
-        // Whole rows a round: a row that a later round still reads must not be written in this one.
-        cg::cluster_group cluster = cg::this_cluster();
-        const uint32_t rows_a_round = static_cast<uint32_t>(round / per_row);
-        for (uint32_t r0 = 0; r0 < rows; r0 += rows_a_round) {
-            const uint32_t end = min(r0 + rows_a_round, rows) * per_row;
-            fetch(r0 * per_row + blockIdx.x * kMoveThreads + threadIdx.x, gridDim.x * kMoveThreads, end);
-            cluster.sync();
-            store();
-        }
-    } else {
-        for (uint64_t n0 = static_cast<uint64_t>(blockIdx.x) * kMoveThreads * kHeld; n0 < all; n0 += round) {
-            fetch(static_cast<uint32_t>(n0) + threadIdx.x, kMoveThreads, static_cast<uint32_t>(min(all, n0 + kMoveThreads * kHeld)));
-            store();
-        }
+    const uint32_t round = gridDim.x * kMoveWarps * batch, first = (blockIdx.x * kMoveWarps + warp) * batch;
+    for (uint64_t r0 = 0; r0 < rows; r0 += round) {
+        const uint64_t mine = r0 + first;
+        fetch(static_cast<uint32_t>(min(mine, static_cast<uint64_t>(rows))));
+        if constexpr (IN_PLACE) cg::this_cluster().sync();   // a row that this round still reads must not be written yet
+        store();
     }
 }
 
@@ -300,7 +328,7 @@ extern "C" int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_pa
     if (!word(target_table) || !word(weights) || !word(kept) || !word(new_lengths) || (new_weights != nullptr && !word(new_weights))) return B200KV_ERR_INVALID;
     if (keep == 0 || static_cast<uint64_t>(sinks) + recent > keep || new_lengths == batch->lengths) return B200KV_ERR_INVALID;
     if (weights_stride < batch->max_length) return B200KV_ERR_INVALID;
-    if (keep > 0x7fffffffu / 40 || static_cast<uint64_t>(target_max_pages) * view->page_size < std::min(keep, batch->max_length)) return B200KV_ERR_RANGE;   // 33 pieces of a row at most
+    if (keep > 0x7fffffffu / 40 || static_cast<uint64_t>(target_max_pages) * view->page_size < std::min(keep, batch->max_length)) return B200KV_ERR_RANGE;
     if (view->kv_heads > 32767u) return B200KV_ERR_UNSUPPORTED;                                                                 // two grid rows a head
     const uint64_t heads = static_cast<uint64_t>(batch->sequences) * view->kv_heads;
     const uintptr_t w0 = reinterpret_cast<uintptr_t>(weights), w1 = w0 + heads * weights_stride * 4, n0 = reinterpret_cast<uintptr_t>(new_weights);
@@ -311,17 +339,20 @@ extern "C" int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_pa
     const EvictParams p{paged_of(*view, *batch), target_table, target_max_pages, weights, weights_stride, keep, sinks, recent, kept, new_weights, new_lengths};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint32_t cluster = 1;
-    while (cluster < kMaxCluster && static_cast<uint64_t>(batch->max_length) > static_cast<uint64_t>(cluster) * 4 * kChooseThreads) cluster *= 2;
-    B200KV_CUDA_TRY(launch_cluster(paged_choose_kernel, dim3(cluster, batch->sequences, view->kv_heads), kChooseThreads, cluster, false, s, p));
-    const uint64_t pieces = static_cast<uint64_t>(std::min(keep, batch->max_length)) * (view->head_dim / 8 + 1);
-    const uint64_t blocks = std::max<uint64_t>(1, (pieces + kMoveThreads * kHeld - 1) / (kMoveThreads * kHeld));
+    constexpr uint64_t kOfCta = static_cast<uint64_t>(kChooseThreads) * kKept;
+    while (cluster < kMaxCluster && batch->max_length > cluster * kOfCta) cluster *= 2;
+    // (a stretch is rounded up to whole warps, so a little less than all registers hold)
+    const bool cached = batch->max_length <= cluster * (kOfCta - kChooseThreads);
+    B200KV_CUDA_TRY(launch_cluster(cached ? paged_choose_kernel<true> : paged_choose_kernel<false>, dim3(cluster, batch->sequences, view->kv_heads), kChooseThreads, cluster, false, s, p));
+    const uint32_t rows = std::min(keep, batch->max_length), batch_rows = 32 * kHeld / std::max(pieces_of_side(*view, 0), pieces_of_side(*view, 1));
+    const uint32_t blocks = std::max<uint32_t>(1, (rows + kMoveWarps * batch_rows - 1) / (kMoveWarps * batch_rows));
     if (target_table == batch->page_table) {
         uint32_t wide = 1;
         while (wide < kMaxCluster && wide < blocks) wide *= 2;
         B200KV_CUDA_TRY(launch_cluster(paged_move_kernel<true>, dim3(wide, batch->sequences, 2 * view->kv_heads), kMoveThreads, wide, true, s, p));
     } else {
         const uint64_t most = std::max<uint64_t>(1, 16ull * device_sms() / (2 * heads));
-        B200KV_CUDA_TRY(launch_behind(paged_move_kernel<false>, dim3(static_cast<uint32_t>(std::min(blocks, most)), batch->sequences, 2 * view->kv_heads),
+        B200KV_CUDA_TRY(launch_behind(paged_move_kernel<false>, dim3(static_cast<uint32_t>(std::min<uint64_t>(blocks, most)), batch->sequences, 2 * view->kv_heads),
                                       dim3(kMoveThreads), 0, s, p));
     }
     return B200KV_OK;

@@ -43,35 +43,64 @@ struct LoadParams {
     Paged pool;
     __half* key;
     __half* value;
+    uint32_t tokens;   // of a warp: 1 or 4
 };
 
-// One thread, 16 bytes of output: eight elements of a row of one side.  A block takes 256 of them of one token, its rows of all kv heads lying one behind the
-// other in the output, and the token is looked up once.  Bound by latency for few tokens, by HBM for many.
+// A warp takes a token of one side, or four where there are many: its first lanes look up where they lie, then all of it brings the rows of all kv heads, 16 bytes of output a lane and
+// step, eight steps' loads under way together.  Bound by latency for few tokens, by HBM for many.
+constexpr int kLoadThreads = 128, kLoadSteps = 8;
 template <int D>
-__global__ void __launch_bounds__(256) paged_load_kernel(const __grid_constant__ LoadParams p) {
+__global__ void __launch_bounds__(kLoadThreads) paged_load_kernel(const __grid_constant__ LoadParams p) {
     constexpr uint32_t CPR = D / 8;   // chunks of a row
     pdl_launch_dependents();
     pdl_wait();                       // the rows come from the store kernel just before
     const Paged& pool = p.pool;
-    const uint32_t token = blockIdx.x, c = threadIdx.x % CPR, head = blockIdx.y * (256 / CPR) + threadIdx.x / CPR;
-    const bool is_k = (blockIdx.z == 0) == (p.key != nullptr) || p.value == nullptr;
-    const uint32_t s = sequence_of(pool, token);
-    const Span span = span_of(pool, s);
-    const int j = span.base() + static_cast<int>(token - span.first);
-    if (token < span.first || token - span.first >= span.tokens || head >= pool.view.kv_heads) return;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    const long long row = j < 0 ? -1 : row_of(pool, s, head, static_cast<uint32_t>(j));
-    if (row >= 0) {
-        const size_t at = static_cast<size_t>(row) * D + c * 8;
-        if (is_k ? is_k_q8(pool.view.quant_mode) : is_v_q8(pool.view.quant_mode)) {
-            const uint32_t blocks = D / pool.view.qblock;
-            const __half scale = static_cast<const __half*>(is_k ? pool.view.key_scales : pool.view.value_scales)[static_cast<size_t>(row) * blocks + (blocks == 1 ? 0 : c / 4)];
-            v = dequant8(*reinterpret_cast<const uint2*>((is_k ? pool.view.key_q8 : pool.view.value_q8) + at), scale);
-        } else {
-            v = *reinterpret_cast<const uint4*>(static_cast<const __half*>(is_k ? pool.view.key_f16 : pool.view.value_f16) + at);
+    const uint32_t lane = threadIdx.x & 31, token0 = (blockIdx.x * (kLoadThreads / 32) + threadIdx.x / 32) * p.tokens, H = pool.view.kv_heads;
+    const bool is_k = (blockIdx.y == 0) == (p.key != nullptr) || p.value == nullptr;
+    // lane l < p.tokens: token token0 + l.  -2: not of any sequence; -1: of no page, zeros; else its row for kv head 0
+    long long place = -2;
+    if (lane < p.tokens && token0 + lane < pool.batch.total_tokens) {
+        const uint32_t token = token0 + lane, s = sequence_of(pool, token);
+        const Span span = span_of(pool, s);
+        if (token >= span.first && token - span.first < span.tokens) {
+            const int j = span.base() + static_cast<int>(token - span.first);
+            place = j < 0 ? -1 : row_of(pool, s, 0, static_cast<uint32_t>(j));
         }
     }
-    *reinterpret_cast<uint4*>((is_k ? p.key : p.value) + (static_cast<size_t>(token) * pool.view.kv_heads + head) * D + c * 8) = v;
+    const bool q8 = is_k ? is_k_q8(pool.view.quant_mode) : is_v_q8(pool.view.quant_mode);
+    const int8_t* q = is_k ? pool.view.key_q8 : pool.view.value_q8;
+    const __half* scales = static_cast<const __half*>(is_k ? pool.view.key_scales : pool.view.value_scales);
+    const __half* f16 = static_cast<const __half*>(is_k ? pool.view.key_f16 : pool.view.value_f16);
+    __half* out = (is_k ? p.key : p.value) + static_cast<size_t>(token0) * H * D;
+    const uint32_t blocks = D / pool.view.qblock, chunks = H * CPR;   // of a token
+    for (uint32_t t = 0; t < p.tokens; ++t) {
+        const long long at = __shfl_sync(0xffffffffu, place, t);
+        if (at == -2) continue;
+        for (uint32_t c0 = 0; c0 < chunks; c0 += 32 * kLoadSteps) {
+            uint4 v[kLoadSteps];
+            __half scale[kLoadSteps];
+#pragma unroll
+            for (int i = 0; i < kLoadSteps; ++i) {
+                const uint32_t n = c0 + 32 * i + lane, head = n / CPR, c = n % CPR;
+                v[i] = make_uint4(0, 0, 0, 0);
+                scale[i] = __ushort_as_half(0);
+                if (n >= chunks || at < 0) continue;
+                const size_t row = static_cast<size_t>(at) + (static_cast<size_t>(head) << pool.page_shift);
+                if (q8) {
+                    const uint2 raw = *reinterpret_cast<const uint2*>(q + row * D + c * 8);
+                    v[i].x = raw.x; v[i].y = raw.y;
+                    scale[i] = scales[row * blocks + (blocks == 1 ? 0 : c / 4)];
+                } else {
+                    v[i] = *reinterpret_cast<const uint4*>(f16 + row * D + c * 8);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kLoadSteps; ++i) {
+                const uint32_t n = c0 + 32 * i + lane;
+                if (n < chunks) *reinterpret_cast<uint4*>(out + (static_cast<size_t>(t) * chunks + n) * 8) = q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -87,11 +116,12 @@ extern "C" int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
     if (batch->total_tokens == 0 || batch->sequences == 0) return B200KV_OK;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    const LoadParams p{paged_of(*view, *batch), static_cast<__half*>(key), static_cast<__half*>(value)};
-    const uint32_t heads_per_block = 256 / (view->head_dim / 8);
-    const dim3 grid(batch->total_tokens, (view->kv_heads + heads_per_block - 1) / heads_per_block, key != nullptr && value != nullptr ? 2 : 1);
+    // four where every SM has sixteen warps with work all the same
+    const uint32_t tokens = batch->total_tokens >= 4 * 16 * device_sms() / 2 ? 4 : 1, of_block = kLoadThreads / 32 * tokens;
+    const LoadParams p{paged_of(*view, *batch), static_cast<__half*>(key), static_cast<__half*>(value), tokens};
+    const dim3 grid((batch->total_tokens + of_block - 1) / of_block, key != nullptr && value != nullptr ? 2 : 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    B200KV_CUDA_TRY(view->head_dim == 128 ? launch_kernel(paged_load_kernel<128>, grid, dim3(256), 0, s, true, p)
-                                          : launch_kernel(paged_load_kernel<256>, grid, dim3(256), 0, s, true, p));
+    B200KV_CUDA_TRY(view->head_dim == 128 ? launch_kernel(paged_load_kernel<128>, grid, dim3(kLoadThreads), 0, s, true, p)
+                                          : launch_kernel(paged_load_kernel<256>, grid, dim3(kLoadThreads), 0, s, true, p));
     return B200KV_OK;
 }
