@@ -29,6 +29,8 @@ class View(C.Structure):
 class PagedView(C.Structure):
     """b200kv_paged_view (include/b200kv.h): a pool of pages of one attention layer."""
 
+    device_index = -1      # where it was built over tensors: of their device, which a launch compares with the current one
+
     _fields_ = [
         ("key_f16", C.c_void_p), ("value_f16", C.c_void_p),
         ("key_q8", C.c_void_p), ("key_scales", C.c_void_p),
@@ -40,6 +42,8 @@ class PagedView(C.Structure):
 
 class PagedBatch(C.Structure):
     """b200kv_paged_batch: the sequences of a call over a paged cache."""
+
+    device_index = -1      # likewise
 
     _fields_ = [
         ("page_table", C.c_void_p), ("query_starts", C.c_void_p), ("lengths", C.c_void_p),

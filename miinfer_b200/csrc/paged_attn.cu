@@ -430,7 +430,7 @@ using namespace b200kv;
 extern "C" {
 
 size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window, uint32_t sinks) {
-    if (view == nullptr || batch == nullptr || view->kv_heads == 0 || query_heads % view->kv_heads != 0) return 0;
+    if (view == nullptr || batch == nullptr || view->kv_heads == 0 || query_heads == 0 || query_heads % view->kv_heads != 0) return 0;
     settle_window(*batch, &window, &sinks);
     return room_of(*view, *batch, query_heads, window, sinks, kMostSms).bytes;
 }

@@ -40,6 +40,7 @@ struct Api {
 PyObject* g_view_type;   // the ctypes structure of a cache view
 PyObject* g_paged_view_type;    // ... of a paged cache's view, and of a batch over it
 PyObject* g_paged_batch_type;
+PyObject* g_device_index;       // the name of their attribute
 
 // One call's arguments, read left to right; the first failure sticks and leaves a Python exception set.
 class Args {
@@ -126,6 +127,11 @@ public:
         if (PyObject_GetBuffer(o, &buffers_[held_], PyBUF_SIMPLE) != 0) { ok_ = false; return nullptr; }
         const Py_buffer& b = buffers_[held_++];
         if (static_cast<size_t>(b.len) < sizeof(T)) { fail(PyExc_ValueError, "a structure of another size"); return nullptr; }
+        PyObject* device = PyObject_GetAttr(o, g_device_index);   // of the tensors it was built over; -1: it was not
+        const long index = device == nullptr ? -1 : PyLong_AsLong(device);
+        Py_XDECREF(device);
+        if (PyErr_Occurred()) { ok_ = false; return nullptr; }
+        if (index >= 0 && index != c10::cuda::current_device()) { fail(PyExc_ValueError, "a paged cache of another device than the current one"); return nullptr; }
         return static_cast<const T*>(b.buf);
     }
     const b200kv_paged_view* paged_view() { return structure<b200kv_paged_view>(g_paged_view_type, "a paged cache's view"); }
@@ -645,5 +651,6 @@ PyMODINIT_FUNC PyInit__native(void) {
         g_names[i] = PyUnicode_InternFromString(names[i]);
         if (g_names[i] == nullptr) return nullptr;
     }
+    if ((g_device_index = PyUnicode_InternFromString("device_index")) == nullptr) return nullptr;
     return PyModule_Create(&g_module);
 }

@@ -53,7 +53,7 @@ class PagedView(_lib.PagedView):
         ptr = lambda t, want: t.data_ptr() if want else None
         view = PagedView(ptr(key, not q8[0]), ptr(value, not q8[1]), ptr(key, q8[0]), ptr(key_scales, q8[0]), ptr(value, q8[1]), ptr(value_scales, q8[1]),
                          pages, page_size, heads, dim, blocks.pop() if blocks else dim, int(mode))
-        view.planes = (key, key_scales, value, value_scales)
+        view.planes, view.device_index = (key, key_scales, value, value_scales), key.device.index
         return view
 
 
@@ -76,7 +76,7 @@ class PagedBatch(_lib.PagedBatch):
                 raise ValueError(f"{name} out of range")
         super().__init__(page_table.data_ptr(), query_starts.data_ptr(), lengths.data_ptr(), sequences, page_table.shape[1], int(total_tokens),
                          int(max_tokens), int(max_length), int(total_length))
-        self.tensors = (page_table, query_starts, lengths)
+        self.tensors, self.device_index = (page_table, query_starts, lengths), page_table.device.index
 
 
 class PagedKvCache:
