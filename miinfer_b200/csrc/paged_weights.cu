@@ -12,7 +12,9 @@
 //  * many_kernel, any number: K of a tile becomes the A operand in TMEM, as fp16: fp16 as it is, int8 with one scale a row as whole numbers (the scale
 //    multiplies the score), int8 with a scale a block of 32 as two fp16 terms of the product, 22 bits.  The query rows that see any of the tile stream past it, 64 at a
 //    time: fp16 ones by TMA, whole tokens' heads of the kv head as boxes of a map over the activations; fp32 ones split into two terms by two warps.  Eight warps
-//    convert K and take the exponentials.  A from TMEM halves what an MMA reads from shared memory (K in shared memory: 78 clocks an MMA of 32).
+//    convert K; four of them take the exponentials of the even groups, the others those of the odd ones, so that one set's are under way while the other waits for
+//    its scores (all eight on every group: 56 us, 45 so, for the last 64 tokens
+//    of 300 over 7000 to 12000 positions, 24 / 4 heads of 256, q8_0, two sequences; either with one warp that issues: 56 to 59).  A from TMEM halves what an MMA reads from shared memory (K in shared memory: 78 clocks an MMA of 32).
 //    Bound by the MMAs where K has two terms (two for every product), by the exponentials otherwise.
 #include "paged_decode.cuh"
 #include "paged_unit.cuh"
@@ -268,9 +270,13 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
 
 // ---- any number of rows ----------------------------------------------------------------------------------------------------------------
 
+// Two fp32 values in one instruction.
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b) { Pair r; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 constexpr int kTile = kDecodeTile;
 constexpr int kGroup = 64;           // query rows of an MMA: as many whole tokens as fit
-constexpr int kWorkers = 256, kProducerWarp = 8, kQWarp = 9, kMmaWarp = 11, kThreads = 384;   // warps 9 and 10 bring the queries
+constexpr int kWorkers = 256, kProducerWarp = 8, kQWarp = 9, kMmaWarp = 11;   // warps 9 and 10 bring the queries
 
 template <int D, int KF, bool Q32>
 struct ManyLayout {
@@ -281,16 +287,18 @@ struct ManyLayout {
     static constexpr uint32_t kColK = 0, kColS = kKTerms * D / 2, kTmemCols = kColS + kSBufs * kGroup <= 256 ? 256 : 512;   // K: two fp16 a column
     static_assert(kColS + kSBufs * kGroup <= 512 && (kCtas == 1 || kTmemCols == 256));
     static constexpr int kQTerm = kGroup * D * 2;
-    static constexpr int kRaw = 2;                                                             // units of K on their way
+    static constexpr int kRaw = Q32 && KF == F16 ? 1 : 2;                                   // units of K on their way
     static constexpr int kMisc = 5120;
     static constexpr int kFit = ((kCtas == 2 ? 115712 : 232448) - 1024 - kMisc - kRaw * (U::kData + U::kScales)) / (kQTerms * kQTerm);
-    static constexpr int kQBufs = kFit > 4 ? 4 : kFit;
-    static_assert(kQBufs >= 1 && !(Q32 && kQBufs == 3), "two warps that take the groups in turn see every phase of their buffers only if those are even in number");
+    static constexpr int kQBufs = kFit >= 4 ? 4 : 2;
+    // An MMA of 64 columns takes the tensor core 32 clocks and a warp 60 to issue, so where an SM has one CTA two warps take the groups in turn.
+    static constexpr int kIssuers = kCtas == 1 ? 2 : 1, kThreads = (kMmaWarp + kIssuers) * 32;
+    static_assert(kFit >= 2 && kSBufs % 2 == 0, "warps that take the groups in turn see every phase of their buffers only if those are even in number");
     static constexpr int kOffQ = kRaw * U::kData, kOffScales = kOffQ + kQBufs * kQTerms * kQTerm;
-    static constexpr int kOffRows = kOffScales + kRaw * U::kScales;                           // [buffer][64] {statistics in log2 units, place of the token}
+    static constexpr int kOffRows = kOffScales + kRaw * U::kScales;                           // [buffer] statistics in log2 units [64], places of the tokens [64]
     static constexpr int kOffSum = kOffRows + kQBufs * kGroup * 8;                            // [parity][128]
     static constexpr int kOffBar = kOffSum + 2 * kTile * 4;
-    static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + kRaw, LANDED = RAW_EMPTY + kRaw, K_FULL = LANDED + 1, Q_FULL = K_FULL + 1, Q_EMPTY = Q_FULL + kQBufs,
+    static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + kRaw, LANDED = RAW_EMPTY + kRaw, K_FULL = LANDED + 1, Q_FULL = K_FULL + 2, Q_EMPTY = Q_FULL + kQBufs,
                          S_FULL = Q_EMPTY + kQBufs, S_EMPTY = S_FULL + kSBufs, kNumBars = S_EMPTY + kSBufs;
     static constexpr int kOffMisc = kOffBar + kNumBars * 8, kAlloc = kOffMisc + 48 + 1024;
     static_assert(kOffMisc + 48 - kOffRows <= kMisc);
@@ -324,7 +332,7 @@ __device__ __forceinline__ Share share_of(const WeightsParams& p, const Cursor& 
 }
 
 template <int D, int KF, bool Q32>
-__global__ void __launch_bounds__(kThreads, ManyLayout<D, KF, Q32>::kCtas)
+__global__ void __launch_bounds__(ManyLayout<D, KF, Q32>::kThreads, ManyLayout<D, KF, Q32>::kCtas)
 many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
     using L = ManyLayout<D, KF, Q32>;
     using U = Unit<D, KF>;
@@ -341,10 +349,10 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
         for (int i = 0; i < L::kNumBars; ++i) {
             uint32_t count = 1;
             if (i >= L::RAW_EMPTY && i < L::LANDED) count = kWorkers / 32;
-            else if (i == L::K_FULL) count = kWorkers;
+            else if (i >= L::K_FULL && i < L::Q_FULL) count = kWorkers;
             else if (i >= L::Q_FULL && i < L::Q_EMPTY) count = Q32 ? 32 : 33;                  // the statistics' warp, and the copies
-            else if (i >= L::Q_EMPTY && i < L::S_FULL) count = 1 + kWorkers / 32;
-            else if (i >= L::S_EMPTY) count = kWorkers / 32;
+            else if (i >= L::Q_EMPTY && i < L::S_FULL) count = 1 + kWorkers / 64;          // the MMAs, and the set of warps that takes the group
+            else if (i >= L::S_EMPTY) count = kWorkers / 64;
             mbar_init(bar(i), count);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -378,7 +386,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
 
     if (warp < kProducerWarp) {
         // =============================== K into TMEM, then the exponentials ===============================
-        const int wg = warp >> 2, col0 = wg * (kGroup / 2), t128 = tid & 127;   // half of a row's dims, then half of a group's rows
+        const int wg = warp >> 2, t128 = tid & 127;   // half of a row's dims, then every second group
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
         uint32_t i = 0, k = 0;   // tiles and groups so far
         bool failed = false;
@@ -390,7 +398,6 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             const float before = writes ? *account : 0.0f;
             wait(bar(L::RAW_FULL + raw), (i / L::kRaw) & 1);
             __syncwarp();
-            // (the tile before has been multiplied through: its last scores have been seen)
             const uint8_t* scales = smem + L::kOffScales + raw * U::kScales + t128 * U::kScale;
             const uint8_t* src = smem + raw * U::kData + t128 * 128;
             constexpr int kChunks = U::kRow / 32;                            // 16-byte chunks of half a row
@@ -409,20 +416,18 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                     const uint32_t w[4] = {a.x ^ 0x80808080u, a.y ^ 0x80808080u, a.z ^ 0x80808080u, a.w ^ 0x80808080u};
                     uint32_t hi[8];
                     [[maybe_unused]] uint32_t lo[8];
-                    [[maybe_unused]] float sc = 1.0f;
-                    if constexpr (KF == BLOCK) sc = __half2float(reinterpret_cast<const __half*>(scales)[chunk >> 1]);
+                    [[maybe_unused]] __half2 sc;
+                    if constexpr (KF == BLOCK) sc = __half2half2(reinterpret_cast<const __half*>(scales)[chunk >> 1]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t pair = __byte_perm(w[e >> 1], 0x64646464u, e & 1 ? 0x4342 : 0x4140);
                         const __half2 q2 = __hadd2(*reinterpret_cast<const __half2*>(&pair), __float2half2_rn(-1152.0f));
                         if constexpr (KF == ROW) {
                             hi[e] = *reinterpret_cast<const uint32_t*>(&q2);
-                        } else {   // the product as two terms; q x scale is exact in fp32
-                            const float2 f = __half22float2(q2);
-                            const float u = f.x * sc, v = f.y * sc;
-                            hi[e] = pack2(u, v);
-                            const float2 h = unpack2(hi[e]);
-                            lo[e] = pack2(u - h.x, v - h.y);
+                        } else {   // the product as two terms: rounded, and what the rounding left, which a fused multiply-add finds exactly
+                            const __half2 product = __hmul2(q2, sc), rest = __hfma2(q2, sc, __hneg2(product));
+                            hi[e] = *reinterpret_cast<const uint32_t*>(&product);
+                            lo[e] = *reinterpret_cast<const uint32_t*>(&rest);
                         }
                     }
                     tmem_st8(col, hi);
@@ -433,52 +438,72 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             if constexpr (KF == ROW) factor *= __half2float(*reinterpret_cast<const __half*>(scales));
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
-            mbar_arrive(bar(L::K_FULL));
+            mbar_arrive(bar(L::K_FULL + (i & 1)));
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::RAW_EMPTY + raw));
             const int base = c.span.base();
             const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
-            float sum[2] = {0.0f, 0.0f};
+            Pair sum[2] = {0, 0};
+            const Pair factor2 = pack_pair(factor, factor);
             for (uint32_t g = 0; g < groups; ++g, ++k) {
+                if ((k & 1) != static_cast<uint32_t>(wg)) continue;
                 const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
                 if (!failed && !mbar_wait_both_lane(bar(L::Q_FULL + qb), (k / L::kQBufs) & 1, bar(L::S_FULL + sb), (k / L::kSBufs) & 1)) failed = true;
                 __syncwarp();
                 tc_fence_after();
-                int x[kGroup / 2];
-#pragma unroll
-                for (int e = 0; e < kGroup / 2; e += 8) tmem_ld8(tmem_base + lane_addr + L::kColS + sb * kGroup + col0 + e, reinterpret_cast<int(&)[8]>(x[e]));
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(L::S_EMPTY + sb));
-                const float2* info = reinterpret_cast<const float2*>(smem + L::kOffRows) + qb * kGroup;   // rows that do not exist have infinite statistics
+                const float* stats = reinterpret_cast<const float*>(smem + L::kOffRows) + qb * 2 * kGroup;   // of the rows, negated; then their places
+                const int* places = reinterpret_cast<const int*>(stats + kGroup);
                 const uint32_t first = sh.t0 + g * group_tokens, last = first + group_tokens - 1;
                 const bool whole = last < sh.t1 && static_cast<int>(sh.pos0) + kTile - 1 <= base + static_cast<int>(first) &&
                                    (p.window == 0 || static_cast<long long>(sh.pos0) + p.window > static_cast<long long>(base) + last);   // all rows see all positions
-                if (whole) {
 #pragma unroll
-                    for (int e = 0; e < kGroup / 2; e += 2) {
-                        const float4 two = *reinterpret_cast<const float4*>(info + col0 + e);
-                        sum[0] += ex2(fmaf(__int_as_float(x[e]), factor, -two.x));
-                        sum[1] += ex2(fmaf(__int_as_float(x[e + 1]), factor, -two.z));
+                for (int col0 = 0; col0 < kGroup; col0 += 32) {
+                    int x[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) tmem_ld8(tmem_base + lane_addr + L::kColS + sb * kGroup + col0 + e, reinterpret_cast<int(&)[8]>(x[e]));
+                    tmem_ld_wait();
+                    if (col0 + 32 == kGroup) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(L::S_EMPTY + sb));
                     }
-                } else {
+                    if (whole) {
 #pragma unroll
-                    for (int e = 0; e < kGroup / 2; ++e) {
-                        const float2 one = info[col0 + e];
-                        const int at = __float_as_int(one.y);
-                        const bool seen = static_cast<int>(mine) <= at && (p.window == 0 || static_cast<long long>(mine) + p.window > at || mine < p.sinks);
-                        const float w = ex2(fmaf(__int_as_float(x[e]), factor, -one.x));
-                        sum[e & 1] += seen ? w : 0.0f;
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 four = *reinterpret_cast<const float4*>(stats + col0 + e);
+                            const float2 a = unpack_pair(fma_pair(pack_pair(__int_as_float(x[e]), __int_as_float(x[e + 1])), factor2, pack_pair(four.x, four.y)));
+                            const float2 b = unpack_pair(fma_pair(pack_pair(__int_as_float(x[e + 2]), __int_as_float(x[e + 3])), factor2, pack_pair(four.z, four.w)));
+                            sum[0] = add_pair(sum[0], pack_pair(ex2(a.x), ex2(a.y)));
+                            sum[1] = add_pair(sum[1], pack_pair(ex2(b.x), ex2(b.y)));
+                        }
+                    } else {
+                        const auto add_seen = [&](auto sees) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 stat = *reinterpret_cast<const float4*>(stats + col0 + e);
+                                const int4 at = *reinterpret_cast<const int4*>(places + col0 + e);   // -1: no row, which sees nothing
+                                const auto weight = [&](int y, float of, int place) {
+                                    const float w = ex2(fmaf(__int_as_float(x[e + y]), factor, of));
+                                    return sees(place) ? w : 0.0f;
+                                };
+                                sum[0] = add_pair(sum[0], pack_pair(weight(0, stat.x, at.x), weight(1, stat.y, at.y)));
+                                sum[1] = add_pair(sum[1], pack_pair(weight(2, stat.z, at.z), weight(3, stat.w, at.w)));
+                            }
+                        };
+                        if (p.window == 0) add_seen([&](int at) { return static_cast<int>(mine) <= at; });
+                        else add_seen([&](int at) { return static_cast<int>(mine) <= at && (static_cast<long long>(mine) + p.window > at || mine < p.sinks); });
                     }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(L::Q_EMPTY + qb));
             }
             float* other = reinterpret_cast<float*>(smem + L::kOffSum) + (i & 1) * kTile;
-            const float total = failed ? __int_as_float(0x7fc00000) : sum[0] + sum[1];
+            const float2 halves = unpack_pair(add_pair(sum[0], sum[1]));
+            const float total = failed ? __int_as_float(0x7fc00000) : halves.x + halves.y;
             if (wg == 1) other[t128] = total;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;" ::: "memory");   // and the tile is multiplied through: all its groups' scores have been seen
+            tc_fence_after();
             if (writes) *account = before + (total + other[t128]);
             ++i;
             return true;
@@ -505,19 +530,20 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             auto bring_info = [&](uint32_t t0, uint32_t qb) {
                 for (uint32_t x = lane; x < kGroup; x += 32) {
                     const uint32_t token = t0 + x / G;
-                    float2 info = make_float2(INFINITY, __int_as_float(-1));
+                    float stat = -INFINITY;
+                    int place = -1;
                     if (x < group_rows && token < sh.t1) {
                         const float lse = p.lse_of(c.span, token)[c.head * G + x % G];
-                        info.x = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;   // a row that sees nothing has no weights
-                        info.y = __int_as_float(c.span.base() + static_cast<int>(token));
+                        stat = lse == -INFINITY ? -INFINITY : lse * -1.4426950408889634f;   // a row that sees nothing has no weights
+                        place = c.span.base() + static_cast<int>(token);
                     }
-                    reinterpret_cast<float2*>(smem + L::kOffRows)[qb * kGroup + x] = info;
+                    reinterpret_cast<float*>(smem + L::kOffRows)[qb * 2 * kGroup + x] = stat;
+                    reinterpret_cast<int*>(smem + L::kOffRows)[(qb * 2 + 1) * kGroup + x] = place;
                 }
             };
             for (uint32_t g = 0; g < groups; ++g, ++k) {
                 const uint32_t qb = k % L::kQBufs, t0 = sh.t0 + g * group_tokens;
-                if (Q32 && L::kQBufs > 1 && (k & 1) != w) continue;   // fp32: the warps take the groups in turn; with one buffer the first takes them all
-                if (Q32 && L::kQBufs == 1 && w != 0) continue;
+                if (Q32 && (k & 1) != w) continue;   // fp32: the warps take the groups in turn
                 if (k >= L::kQBufs && !wait_warp(bar(L::Q_EMPTY + qb), ((k / L::kQBufs) & 1) ^ 1)) return false;
                 if constexpr (!Q32) {
                     if (w == 1) {
@@ -574,9 +600,11 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
         uint32_t i = 0, k = 0;
         each_tile([&](const Share& sh) {
             const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
-            if (!wait_warp(bar(L::K_FULL), i & 1)) return false;
+            // (two barriers in turn: a tile may be through before the warp that has no group of it looks)
+            if (!wait_warp(bar(L::K_FULL + (i & 1)), (i >> 1) & 1)) return false;
             ++i;
             for (uint32_t g = 0; g < groups; ++g, ++k) {
+                if (L::kIssuers == 2 && (k & 1) != static_cast<uint32_t>(warp - kMmaWarp)) continue;
                 const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
                 if (!mbar_wait_both(bar(L::Q_FULL + qb), (k / L::kQBufs) & 1, bar(L::S_EMPTY + sb), ((k / L::kSBufs) & 1) ^ 1)) return false;
                 tc_fence_after();
@@ -640,8 +668,8 @@ int launch_many(WeightsParams p, bool behind, cudaStream_t stream) {
     if (!key_map(&kmap, p.pool.view) || (!Q32 && !encode_rows_map(&qmap, p.q, D, p.query_heads, p.pool.batch.total_tokens, G, kGroup / G))) return B200KV_ERR_UNSUPPORTED;
     p.ctas = std::min(device_sms(), kMostSms) * L::kCtas;
     p.least_tiles = 1;
-    if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(kThreads), L::kAlloc, stream, p, kmap, qmap));
-    else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kThreads), L::kAlloc, stream, true, p, kmap, qmap));
+    if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, p, kmap, qmap));
+    else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap, qmap));
     return B200KV_OK;
 }
 template <int D, int KF>
