@@ -11,11 +11,14 @@
 //    queries are whole numbers of 24 bits in three int8 planes; fp16 keys meet two fp16 terms of the queries.
 //  * many_kernel, any number: K of a tile becomes the A operand in TMEM, as fp16: fp16 as it is, int8 with one scale a row as whole numbers (the scale
 //    multiplies the score), int8 with a scale a block of 32 as two fp16 terms of the product, 22 bits.  The query rows that see any of the tile stream past it, 64 at a
-//    time: fp16 ones by TMA, whole tokens' heads of the kv head as boxes of a map over the activations; fp32 ones split into two terms by two warps.  Eight warps
-//    convert K; four of them take the exponentials of the even groups, the others those of the odd ones, so that one set's are under way while the other waits for
-//    its scores (all eight on every group: 56 us, 45 so, for the last 64 tokens
-//    of 300 over 7000 to 12000 positions, 24 / 4 heads of 256, q8_0, two sequences; either with one warp that issues: 56 to 59).  A from TMEM halves what an MMA reads from shared memory (K in shared memory: 78 clocks an MMA of 32).
-//    Bound by the MMAs where K has two terms (two for every product), by the exponentials otherwise.
+//    time: fp16 ones by TMA, whole tokens' heads of the kv head as boxes of a map over the activations; fp32 ones split into two terms by nine warps.  Eight warps
+//    convert K; four of them take the exponentials of the even groups, the others those of the odd ones, so that one set's are under way while the other
+//    waits for its scores.  A from TMEM halves what an MMA reads from shared memory (K in shared memory: 78 clocks an MMA of 32).
+//    The last 64 tokens of 300 over 7000 to 12000 positions, two sequences, 24 / 4 heads of 256, q8_0: 39.5 us (all eight on every group 56; the groups in
+//    turn, but one warp that issues, 59).  Four sequences of 64 to 300 tokens over 5000 to 11000, all of them observed, 32 / 8 heads of 128, q8_0: 144 us; with fp32 queries
+//    368 (two warps that split them 990, five with a division a row 590).
+//    A group of 64 rows takes a CTA 0.6 us, of it 0.55 the MMAs of a K of two terms and 0.3 the exponentials; a tile 2.5 us more, K on its way and converted,
+//    which nothing of the CTA covers (TMEM holds one tile's K and the scores).  fp32 queries are bound by their loads, L2's latency and the nine warps.
 #include "paged_decode.cuh"
 #include "paged_unit.cuh"
 
@@ -276,18 +279,19 @@ __device__ __forceinline__ Pair add_pair(Pair a, Pair b) { Pair r; asm("add.rn.f
 
 constexpr int kTile = kDecodeTile;
 constexpr int kGroup = 64;           // query rows of an MMA: as many whole tokens as fit
-constexpr int kWorkers = 256, kProducerWarp = 8, kQWarp = 9, kMmaWarp = 11;   // warps 9 and 10 bring the queries
+constexpr int kWorkers = 256, kProducerWarp = 8, kQWarp = 9;
 
 template <int D, int KF, bool Q32>
 struct ManyLayout {
     using U = Unit<D, KF>;
     static constexpr int kKTerms = KF == BLOCK ? 2 : 1, kQTerms = Q32 ? 2 : 1;
-    static constexpr int kCtas = D == 128 ? 2 : 1;                                             // per SM
-    static constexpr int kSBufs = D == 128 ? 2 : 4;
+    static constexpr int kCtas = D == 128 && !Q32 ? 2 : 1;                                     // per SM
+    static constexpr int kLoaders = Q32 ? 9 : 2, kMmaWarp = kQWarp + kLoaders;                 // warps that bring the queries, from kQWarp on
+    static constexpr int kSBufs = kCtas == 2 ? 2 : 4;
     static constexpr uint32_t kColK = 0, kColS = kKTerms * D / 2, kTmemCols = kColS + kSBufs * kGroup <= 256 ? 256 : 512;   // K: two fp16 a column
     static_assert(kColS + kSBufs * kGroup <= 512 && (kCtas == 1 || kTmemCols == 256));
     static constexpr int kQTerm = kGroup * D * 2;
-    static constexpr int kRaw = Q32 && KF == F16 ? 1 : 2;                                   // units of K on their way
+    static constexpr int kRaw = Q32 && D == 256 && KF == F16 ? 1 : 2;                                 // units of K on their way
     static constexpr int kMisc = 5120;
     static constexpr int kFit = ((kCtas == 2 ? 115712 : 232448) - 1024 - kMisc - kRaw * (U::kData + U::kScales)) / (kQTerms * kQTerm);
     static constexpr int kQBufs = kFit >= 4 ? 4 : 2;
@@ -350,14 +354,14 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             uint32_t count = 1;
             if (i >= L::RAW_EMPTY && i < L::LANDED) count = kWorkers / 32;
             else if (i >= L::K_FULL && i < L::Q_FULL) count = kWorkers;
-            else if (i >= L::Q_FULL && i < L::Q_EMPTY) count = Q32 ? 32 : 33;                  // the statistics' warp, and the copies
+            else if (i >= L::Q_FULL && i < L::Q_EMPTY) count = Q32 ? L::kLoaders * 32 : 33;    // the warps that bring the rows; the statistics' warp and the copies
             else if (i >= L::Q_EMPTY && i < L::S_FULL) count = 1 + kWorkers / 64;          // the MMAs, and the set of warps that takes the group
             else if (i >= L::S_EMPTY) count = kWorkers / 64;
             mbar_init(bar(i), count);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    } else if (warp == kMmaWarp) {
+    } else if (warp == L::kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp < kProducerWarp) {   // rows of a group that no token's head takes: zeros once, no copy reaches them
@@ -456,20 +460,21 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                 const uint32_t first = sh.t0 + g * group_tokens, last = first + group_tokens - 1;
                 const bool whole = last < sh.t1 && static_cast<int>(sh.pos0) + kTile - 1 <= base + static_cast<int>(first) &&
                                    (p.window == 0 || static_cast<long long>(sh.pos0) + p.window > static_cast<long long>(base) + last);   // all rows see all positions
+                constexpr int kStep = 16;
 #pragma unroll
-                for (int col0 = 0; col0 < kGroup; col0 += 32) {
-                    int x[32];
+                for (int col0 = 0; col0 < kGroup; col0 += kStep) {
+                    int x[kStep];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) tmem_ld8(tmem_base + lane_addr + L::kColS + sb * kGroup + col0 + e, reinterpret_cast<int(&)[8]>(x[e]));
+                    for (int e = 0; e < kStep; e += 8) tmem_ld8(tmem_base + lane_addr + L::kColS + sb * kGroup + col0 + e, reinterpret_cast<int(&)[8]>(x[e]));
                     tmem_ld_wait();
-                    if (col0 + 32 == kGroup) {
+                    if (col0 + kStep == kGroup) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar(L::S_EMPTY + sb));
                     }
                     if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
+                        for (int e = 0; e < kStep; e += 4) {
                             const float4 four = *reinterpret_cast<const float4*>(stats + col0 + e);
                             const float2 a = unpack_pair(fma_pair(pack_pair(__int_as_float(x[e]), __int_as_float(x[e + 1])), factor2, pack_pair(four.x, four.y)));
                             const float2 b = unpack_pair(fma_pair(pack_pair(__int_as_float(x[e + 2]), __int_as_float(x[e + 3])), factor2, pack_pair(four.z, four.w)));
@@ -479,7 +484,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                     } else {
                         const auto add_seen = [&](auto sees) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
+                            for (int e = 0; e < kStep; e += 4) {
                                 const float4 stat = *reinterpret_cast<const float4*>(stats + col0 + e);
                                 const int4 at = *reinterpret_cast<const int4*>(places + col0 + e);   // -1: no row, which sees nothing
                                 const auto weight = [&](int y, float of, int place) {
@@ -520,34 +525,50 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, false,
                                      [](uint32_t) { return false; }, lane);
         });
-    } else if (warp < kMmaWarp) {
+    } else if (warp < L::kMmaWarp) {
         // =============================== the query rows, 64 at a time ===============================
         const uint32_t w = warp - kQWarp;
         uint32_t k = 0;
+        // fp32: a lane's rows of a group, row r of it for every kStep x kLoaders-th r, and their elements from the group's first token and head on
+        constexpr uint32_t kPieces = D / 8, kStep = 32 / kPieces, kSteps = (kGroup / kStep + L::kLoaders - 1) / L::kLoaders;   // 16-byte pieces of a row of the operand
+        const uint32_t piece = lane % kPieces, row0 = w * kStep + lane / kPieces;
+        [[maybe_unused]] uint32_t rel[kSteps];
+        if constexpr (Q32) {
+#pragma unroll
+            for (uint32_t y = 0; y < kSteps; ++y) {
+                const uint32_t r = row0 + y * (L::kLoaders * kStep);
+                rel[y] = (r / G * p.query_heads + r % G) * D + piece * 8;
+            }
+        }
         each_tile([&](const Share& sh) {
             const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
-            // statistics and places of a group's rows, by a warp
-            auto bring_info = [&](uint32_t t0, uint32_t qb) {
-                for (uint32_t x = lane; x < kGroup; x += 32) {
-                    const uint32_t token = t0 + x / G;
-                    float stat = -INFINITY;
-                    int place = -1;
-                    if (x < group_rows && token < sh.t1) {
-                        const float lse = p.lse_of(c.span, token)[c.head * G + x % G];
-                        stat = lse == -INFINITY ? -INFINITY : lse * -1.4426950408889634f;   // a row that sees nothing has no weights
-                        place = c.span.base() + static_cast<int>(token);
-                    }
-                    reinterpret_cast<float*>(smem + L::kOffRows)[qb * 2 * kGroup + x] = stat;
-                    reinterpret_cast<int*>(smem + L::kOffRows)[(qb * 2 + 1) * kGroup + x] = place;
+            // statistics and places of a group's rows, by a warp: a lane's two rows
+            static_assert(kGroup == 64);
+            auto has_row = [&](uint32_t t0, uint32_t x) { return x < group_rows && t0 + x / G < sh.t1; };
+            auto load_stats = [&](uint32_t t0, float (&lse)[2]) {
+#pragma unroll
+                for (uint32_t y = 0; y < 2; ++y) {
+                    const uint32_t x = 32 * y + lane;
+                    lse[y] = has_row(t0, x) ? p.lse_of(c.span, t0 + x / G)[c.head * G + x % G] : -INFINITY;
+                }
+            };
+            auto store_stats = [&](uint32_t t0, uint32_t qb, const float (&lse)[2]) {
+#pragma unroll
+                for (uint32_t y = 0; y < 2; ++y) {
+                    const uint32_t x = 32 * y + lane;
+                    reinterpret_cast<float*>(smem + L::kOffRows)[qb * 2 * kGroup + x] = lse[y] == -INFINITY ? -INFINITY : lse[y] * -1.4426950408889634f;   // a row that sees nothing has no weights
+                    reinterpret_cast<int*>(smem + L::kOffRows)[(qb * 2 + 1) * kGroup + x] = has_row(t0, x) ? c.span.base() + static_cast<int>(t0 + x / G) : -1;
                 }
             };
             for (uint32_t g = 0; g < groups; ++g, ++k) {
                 const uint32_t qb = k % L::kQBufs, t0 = sh.t0 + g * group_tokens;
-                if (Q32 && (k & 1) != w) continue;   // fp32: the warps take the groups in turn
-                if (k >= L::kQBufs && !wait_warp(bar(L::Q_EMPTY + qb), ((k / L::kQBufs) & 1) ^ 1)) return false;
+                const auto free = [&] { return k < L::kQBufs || wait_warp(bar(L::Q_EMPTY + qb), ((k / L::kQBufs) & 1) ^ 1); };
                 if constexpr (!Q32) {
+                    float lse[2];
+                    if (w == 1) load_stats(t0, lse);
+                    if (!free()) return false;
                     if (w == 1) {
-                        bring_info(t0, qb);
+                        store_stats(t0, qb, lse);
                         mbar_arrive(bar(L::Q_FULL + qb));
                     } else if (lane == 0) {
                         mbar_expect_tx(bar(L::Q_FULL + qb), group_rows * D * 2);   // rows past the last token's, or of no tensor, come along: they are masked
@@ -556,37 +577,43 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                             tma_load_3d(sbase + L::kOffQ + qb * L::kQTerm + x * (kGroup * 128), &qmap, x * 64, static_cast<int>(c.head * G), static_cast<int>(c.span.first + t0), bar(L::Q_FULL + qb));
                     }
                 } else {
-                    constexpr uint32_t CPR = D / 8, kStep = 32 / CPR;   // 16-byte pieces of a row of the operand; rows of a step
+                    constexpr uint32_t kHeld = 4;   // steps' loads under way together
                     uint8_t* dst = smem + L::kOffQ + qb * L::kQTerms * L::kQTerm;
-                    const uint32_t piece = lane % CPR;
-                    uint32_t token = t0, in_group = 0;                  // of the step's first row
-#pragma unroll 4
-                    for (uint32_t r0 = 0; r0 < group_rows; r0 += kStep) {
-                        const uint32_t r = r0 + lane / CPR;
-                        uint32_t tk = token, h = in_group + lane / CPR;
-                        while (h >= G) { h -= G; ++tk; }
-                        float4 a = make_float4(0, 0, 0, 0), b = a;
-                        if (r < group_rows && tk < sh.t1) {
-                            const float* src = static_cast<const float*>(p.q) + ((static_cast<size_t>(c.span.first) + tk) * p.query_heads + c.head * G + h) * D + piece * 8;
-                            a = *reinterpret_cast<const float4*>(src);
-                            b = *reinterpret_cast<const float4*>(src + 4);
-                        }
-                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                        uint32_t hi[4], lo[4];
+                    const float* src = static_cast<const float*>(p.q) + ((static_cast<size_t>(c.span.first) + t0) * p.query_heads + c.head * G) * D;
+                    const uint32_t rows = min(group_rows, (sh.t1 - t0) * G);
+                    float lse[2];
+                    if (w == 0) load_stats(t0, lse);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            hi[x] = pack2(v[2 * x], v[2 * x + 1]);
-                            const float2 f = unpack2(hi[x]);
-                            lo[x] = pack2(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+                    for (uint32_t y0 = 0; y0 < kSteps; y0 += kHeld) {
+                        float4 a[kHeld], b[kHeld];
+#pragma unroll
+                        for (uint32_t y = y0; y < y0 + kHeld && y < kSteps; ++y) {
+                            a[y - y0] = b[y - y0] = make_float4(0, 0, 0, 0);
+                            if (row0 + y * (L::kLoaders * kStep) < rows) {
+                                a[y - y0] = *reinterpret_cast<const float4*>(src + rel[y]);
+                                b[y - y0] = *reinterpret_cast<const float4*>(src + rel[y] + 4);
+                            }
                         }
-                        if (r < group_rows) {
-                            *reinterpret_cast<uint4*>(dst + chunk_at(r, piece)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4*>(dst + L::kQTerm + chunk_at(r, piece)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        if (y0 == 0 && !free()) return false;   // the first loads are under way while the buffer is still in use
+#pragma unroll
+                        for (uint32_t y = y0; y < y0 + kHeld && y < kSteps; ++y) {
+                            const uint32_t r = row0 + y * (L::kLoaders * kStep);
+                            const float4 &f0 = a[y - y0], &f1 = b[y - y0];
+                            const float v[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                hi[x] = pack2(v[2 * x], v[2 * x + 1]);
+                                const float2 f = unpack2(hi[x]);
+                                lo[x] = pack2(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+                            }
+                            if (r < group_rows) {
+                                *reinterpret_cast<uint4*>(dst + chunk_at(r, piece)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                                *reinterpret_cast<uint4*>(dst + L::kQTerm + chunk_at(r, piece)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            }
                         }
-                        in_group += kStep;
-                        while (in_group >= G) { in_group -= G; ++token; }
                     }
-                    bring_info(t0, qb);
+                    if (w == 0) store_stats(t0, qb, lse);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_arrive(bar(L::Q_FULL + qb));
                 }
@@ -604,7 +631,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             if (!wait_warp(bar(L::K_FULL + (i & 1)), (i >> 1) & 1)) return false;
             ++i;
             for (uint32_t g = 0; g < groups; ++g, ++k) {
-                if (L::kIssuers == 2 && (k & 1) != static_cast<uint32_t>(warp - kMmaWarp)) continue;
+                if (L::kIssuers == 2 && (k & 1) != static_cast<uint32_t>(warp - L::kMmaWarp)) continue;
                 const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
                 if (!mbar_wait_both(bar(L::Q_FULL + qb), (k / L::kQBufs) & 1, bar(L::S_EMPTY + sb), ((k / L::kSBufs) & 1) ^ 1)) return false;
                 tc_fence_after();
@@ -631,7 +658,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == L::kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
     }
