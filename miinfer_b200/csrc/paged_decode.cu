@@ -128,23 +128,18 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
         uint32_t i = 0, fixes = 0;
         for (; c.left > 0 && !failed; c.advance(p)) {
             const int32_t* pages = pages_of(p.pool, c.s);
-            const int lowest = p.window > 0 ? c.span.base() + 1 - static_cast<int>(p.window) : 0;
-            const uint32_t low = lowest > 0 ? static_cast<uint32_t>(lowest) : 0;   // positions below it that are not sinks are seen by nobody
             const uint32_t n = c.take(), length = c.span.length;
             int page = box_page(p.pool, pages, c.t.position(c.tile), length, lane);
             for (uint32_t j = 0; j < n && !failed; ++j, ++i) {
                 const uint32_t pos0 = c.t.position(c.tile + j), ks = i % L::kKUnits, vs = i % L::kVUnits;
                 const Boxes boxes = boxes_of(p.pool, page, c.head, pos0, length, lane);
                 if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), length, lane);
-                const bool edge = pos0 + kDecodeTile > length || (pos0 < low && pos0 + kDecodeTile > p.sinks);
-                const auto unseen = [&](uint32_t r) { return pos0 + r >= length || (pos0 + r < low && pos0 + r >= p.sinks); };
                 failed = i >= L::kKUnits && !wait_warp(bar(L::K_EMPTY + ks), ((i / L::kKUnits) & 1) ^ 1);
                 failed = failed || !bring_unit<D, KF>(smem, ks * L::kKData, L::kOffKScales + ks * L::kKScales, &kmap, p.pool.view.key_scales, boxes, bar(L::K_FULL + ks), bar(L::LANDED),
-                                                      &fixes, false, unseen, lane);
+                                                      &fixes, lane);
                 failed = failed || (i >= L::kVUnits && !wait_warp(bar(L::V_EMPTY + vs), ((i / L::kVUnits) & 1) ^ 1));
-                // fp16 values that nobody sees are cleared; int8 ones are finite whatever they are
                 failed = failed || !bring_unit<D, VF>(smem, L::kOffV + vs * L::kVData, L::kOffVScales + vs * L::kVScales, &vmap, p.pool.view.value_scales, boxes, bar(L::V_FULL + vs),
-                                                      bar(L::LANDED), &fixes, VF == F16 && edge, unseen, lane);
+                                                      bar(L::LANDED), &fixes, lane);
             }
         }
     } else if (warp == L::kQWarp) {
@@ -268,6 +263,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 low[r] = p.window > 0 && upto[r] > p.window ? upto[r] - p.window : 0;
             }
             const uint32_t first_upto = static_cast<uint32_t>(max(c.span.base() + 1, 0));                             // what every row sees: [.., first_upto)
+            [[maybe_unused]] const uint32_t first_low = p.window > 0 && first_upto > p.window ? first_upto - p.window : 0;   // seen by nobody: below it, but for the sinks
             const uint32_t last_low = p.window > 0 && c.span.length > p.window ? c.span.length - p.window : 0;        // from here on
             float acc[kHalves][4], m_run[4], l_run[4], pend[2][kHalves][4];
 #pragma unroll
@@ -363,6 +359,16 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 // ---- the value scales, and the tile's maxima: inside the warp, then across the four ----
                 wait(bar(L::V_FULL + vslot), (i / L::kVUnits) & 1);
                 __syncwarp();
+                if constexpr (VF == F16) {   // an fp16 value that none of the rows sees is cleared (int8 ones are finite whatever they are)
+                    if (g == 0 && (pos >= c.span.length || (pos < first_low && pos >= p.sinks))) {
+                        uint8_t* row = smem + L::kOffV + vslot * L::kVData + t128 * 128;
+#pragma unroll 1
+                        for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+                            for (int y = 0; y < 8; ++y)   // lanes at different chunks: different banks
+                                *reinterpret_cast<uint4*>(row + x * (kDecodeTile * 128) + ((y + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
                 [[maybe_unused]] uint32_t vs_bits[NB];
                 if constexpr (VF != F16) {
                     const uint8_t* vst = smem + L::kOffVScales + vslot * L::kVScales;

@@ -39,14 +39,14 @@ __device__ __forceinline__ Boxes boxes_of(const Paged& pool, int page, uint32_t 
     return b;
 }
 
-// One unit, by a warp: its copies complete on `full` -- or, where rows have to be cleared first (`edge`: those for which unseen(r) says so; boxes of no page), on
-// `landed`, and the warp clears them and completes `full` itself.  *fixes counts the uses of `landed`.  False if a wait ran out.
-template <int D, int FMT, class Unseen>
+// One unit, by a warp: its copies complete on `full` -- or, where a box has no page, on `landed`, and the warp clears its rows and completes `full` itself.
+// *fixes counts the uses of `landed`.  False if a wait ran out.
+template <int D, int FMT>
 __device__ __forceinline__ bool bring_unit(uint8_t* smem, uint32_t off, uint32_t scale_off, const CUtensorMap* map, const void* scales, const Boxes& b, uint32_t full, uint32_t landed,
-                                           uint32_t* fixes, bool edge, Unseen unseen, int lane) {
+                                           uint32_t* fixes, int lane) {
     using U = Unit<D, FMT>;
     const uint32_t sbase = smem_u32(smem);
-    const bool fix = b.missing != 0 || edge;
+    const bool fix = b.missing != 0;
     const uint32_t to = fix ? landed : full, bytes = b.found * b.seg * (U::kRow + U::kScale);
     if (lane == 0) {
         if (bytes > 0) mbar_expect_tx(to, bytes);
@@ -66,7 +66,7 @@ __device__ __forceinline__ bool bring_unit(uint8_t* smem, uint32_t off, uint32_t
         ++*fixes;
     }
     for (uint32_t r = 0; r < kDecodeTile; ++r) {
-        if (!(edge && unseen(r)) && !((b.missing >> (r / b.seg)) & 1)) continue;
+        if (!((b.missing >> (r / b.seg)) & 1)) continue;
         for (int i = lane; i < U::kSlabs * 8; i += 32) *reinterpret_cast<uint4*>(smem + off + (i >> 3) * (kDecodeTile * 128) + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         if (FMT != F16 && lane < U::kScale / 2) *reinterpret_cast<uint16_t*>(smem + scale_off + r * U::kScale + lane * 2) = 0;
     }

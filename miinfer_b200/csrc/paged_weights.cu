@@ -113,8 +113,7 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
                 const Boxes boxes = boxes_of(p.pool, page, c.head, c.t.position(c.tile + j), c.span.length, lane);
                 if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), c.span.length, lane);
                 ok = i < L::kUnits || wait_warp(bar(L::EMPTY + slot), ((i / L::kUnits) & 1) ^ 1);
-                ok = ok && bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes,
-                                             false, [](uint32_t) { return false; }, lane);
+                ok = ok && bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes, lane);
             }
         }
     } else if (warp == L::kQWarp) {
@@ -522,8 +521,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             const Boxes boxes = boxes_of(p.pool, box_page(p.pool, pages_of(p.pool, c.s), sh.pos0, c.span.length, lane), c.head, sh.pos0, c.span.length, lane);
             if (i >= L::kRaw && !wait_warp(bar(L::RAW_EMPTY + raw), ((i / L::kRaw) & 1) ^ 1)) return false;
             ++i;
-            return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, false,
-                                     [](uint32_t) { return false; }, lane);
+            return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, lane);
         });
     } else if (warp < L::kMmaWarp) {
         // =============================== the query rows, 64 at a time ===============================
