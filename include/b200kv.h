@@ -533,10 +533,11 @@ B200KV_API int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
  * [head_dim], q of q_dtype, gate fp32, output of output_dtype = attention * sigmoid(gate).  A token at cache position i
  * sees positions j <= i; with window > 0 only j > i - window and the first `sinks` ones.  (Positions are places in the cache: after an eviction the
  * window counts the positions that are left.)  lse (may be NULL): fp32 [total_tokens][query_heads], the natural logarithm of the sum of exponentials of
- * the scaled scores, for b200kv_paged_weights.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8.
- * Sequences of a few query rows (tokens * query_heads / kv_heads <= 8) take a streaming kernel in which values that a token does not see never
- * count; the others' kernel asks that all cache rows which a sequence's new tokens see are finite, as b200kv_prefill_attn does.  Rows past a length may
- * hold anything in both.  q, output and gate 16-byte aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no
+ * the scaled scores, for b200kv_paged_weights.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8; scale > 0.
+ * Cache rows that any of a sequence's new tokens sees are finite, as b200kv_prefill_attn asks as well; those that none of them sees (past the length,
+ * between the sinks and the window) may hold anything.  A sequence of up to 4 query rows (new tokens times query_heads / kv_heads; 8 where max_tokens allows no
+ * more, or that quotient is above 4) is computed on the cache as it is stored, a longer one on a copy in fp16, where an int8 row's value of more than 65504 is
+ * infinite; a batch of one sequence goes by max_tokens.  q, output and gate 16-byte aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no
  * consequence; one launch at a time uses it. */
 B200KV_API size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window,
                        uint32_t sinks);

@@ -446,6 +446,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         return B200KV_ERR_INVALID;
     if (query_heads == 0 || query_heads % view->kv_heads != 0 || !std::isfinite(scale) || !(scale > 0.0f)) return B200KV_ERR_INVALID;
     if (query_heads / view->kv_heads > 8) return B200KV_ERR_UNSUPPORTED;
+    if (static_cast<uint64_t>(view->pages) * view->kv_heads * view->page_size > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
     if (batch->sequences == 0 || batch->total_tokens == 0 || batch->max_tokens == 0) return B200KV_OK;
     settle_window(*batch, &window, &sinks);
     if (workspace == nullptr || workspace_bytes < b200kv_paged_attn_workspace_bytes(view, batch, query_heads, window, sinks)) return B200KV_ERR_WORKSPACE;

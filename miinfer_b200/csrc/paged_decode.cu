@@ -668,7 +668,6 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     const b200kv_paged_view& v = p.pool.view;
     const b200kv_paged_batch& b = p.pool.batch;
     const uint64_t rows = static_cast<uint64_t>(v.pages) * v.kv_heads * v.page_size;
-    if (rows > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
     const uint32_t box = std::min(v.page_size, kDecodeTile), group = p.query_heads / v.kv_heads;
     CUtensorMap kmap, vmap;
     if (!encode_pool_map(&kmap, is_k_q8(v.quant_mode) ? static_cast<const void*>(v.key_q8) : v.key_f16, !is_k_q8(v.quant_mode), rows, v.head_dim, box) ||

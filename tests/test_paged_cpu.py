@@ -67,6 +67,11 @@ def test_views_that_no_call_takes(call, status, change):
     assert call(view_of(**change), batch_of()) == status
 
 
+@pytest.mark.parametrize("call", [attend, weigh])
+def test_pools_of_more_rows_than_a_coordinate_counts(call):
+    assert call(view_of(pages=1 << 26), batch_of()) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("call", CALLS)
 @pytest.mark.parametrize("status,change", [
     (INVALID, dict(page_table=None)), (INVALID, dict(query_starts=None)), (INVALID, dict(lengths=None)), (INVALID, dict(page_table=4098)), (INVALID, dict(lengths=12289)),
