@@ -11,6 +11,10 @@
 // as the chunk kernel's TMA reads them (int8 rows dequantised, rows that nobody sees zero).  (As a kernel of its own ahead of the gather the layout was 12 us of
 // a call: a chain of latencies.)  The chunk kernel follows, and the merge of what its CTAs left for shared row tiles, each launched while the one before
 // still runs.
+//
+// Measured, us, prepare / chunk kernel / merge: 512 new tokens over 8192, 24 / 4 heads of 256, q8_0: 131 in all (9 / 115 / 6); two chunks of 333 over up to 5000 beside
+// 14 single tokens, 32 / 8 heads of 128, q8_0: 132 (10 / 77 / 6, the tokens' kernel 35); 2048 over 6001 under a window of 1024, fp16: 82 (a CTA has 18 tiles of
+// 0.5 and 7 of set-up, Q and output).
 #include "decode_common.cuh"
 #include "dequant.cuh"
 #include "paged_decode.cuh"
@@ -372,13 +376,51 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
     }
 }
 
+// The chunk kernel multiplies queries rounded to fp16, which moves the statistics of fp32 ones by up to a few 1e-4 of a score's spread: more than the output, itself a
+// mean over the rounded weights, shows, but 1e-5 and more of an lse.  To first order lse_i moves by scale (q_i - fp16(q_i)).(sum_j p_ij k_j), and the sum is what
+// the chunk kernel gives for V = K; what is left is of the square of the rounding.
+// Where both fp32 queries and statistics are asked for the chunks take twice the time for it (two sequences, 1668 new tokens under a window of 40, 24 / 4 heads of 256: 96 -> 148 us).  A warp: a head of a token of the chunk kernel's sequences, or several in turn.
+struct LseParams {
+    PrepareParams prepare;
+    const float* q;
+    const __half* mean_key;   // [total_tokens][query_heads][D]
+    float* lse;
+    uint32_t query_heads;
+    float scale;
+};
+template <int D>
+__global__ void __launch_bounds__(256) paged_lse_kernel(const __grid_constant__ LseParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const Paged& pool = p.prepare.pool;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t rows = static_cast<uint64_t>(pool.batch.total_tokens) * p.query_heads;
+    for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * 8 + threadIdx.x / 32; row < rows; row += static_cast<uint64_t>(gridDim.x) * 8) {
+        const uint32_t token = static_cast<uint32_t>(row / p.query_heads);
+        const Span span = span_of(pool, sequence_of(pool, token));
+        if (!p.prepare.mine(span) || token < span.first || token - span.first >= span.tokens) continue;
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < D; x += 128) {
+            const float4 q = *reinterpret_cast<const float4*>(p.q + row * D + x + lane * 4);
+            const uint2 raw = *reinterpret_cast<const uint2*>(p.mean_key + row * D + x + lane * 4);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+            const auto left = [](float v) { return v - __half2float(__float2half_rn(v)); };
+            sum += left(q.x) * a.x + left(q.y) * a.y + left(q.z) * b.x + left(q.w) * b.y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) p.lse[row] += p.scale * sum;   // where nothing is seen: minus infinity and a sum of zeros
+    }
+}
+
 // ---- the workspace of a call -----------------------------------------------------------------------------------------------------
 
 struct Room {
     uint64_t scratch_tiles;    // of all sequences together
     uint32_t max_items, max_parts;
     bool decode, chunks;       // which kernels the call may need
-    size_t decode_parts, items, groups, k, v, part_o, part_ml, bytes;   // offsets
+    size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, bytes;   // offsets
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
@@ -417,6 +459,7 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.v = take(plane);
     r.part_o = take(parts * kChunkRows * view.head_dim * sizeof(float));
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
+    r.mean_key = take(static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half));
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
     return r;
 }
@@ -479,6 +522,23 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const ChunkMergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
         B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, dim3(5 * sms), dim3(256), 0, s, mp)
                                               : launch_behind(paged_merge_kernel<256>, dim3(5 * sms), dim3(256), 0, s, mp));
+        if (lse != nullptr && q_dtype == B200KV_F32) {
+            ChunkLaunch keys = cl;
+            keys.v_scratch = cl.k_scratch;
+            keys.gate = nullptr;
+            keys.out = ws + room.mean_key;
+            keys.out_is_f16 = 1;
+            keys.lse = nullptr;
+            rc = launch_chunk(keys, s);
+            if (rc != B200KV_OK) return rc;
+            const ChunkMergeParams km{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, nullptr, keys.out, 1, nullptr, query_heads, view->kv_heads};
+            const LseParams lp{pp, static_cast<const float*>(q), reinterpret_cast<const __half*>(ws + room.mean_key), lse, query_heads, scale};
+            const uint32_t blocks_of_rows = static_cast<uint32_t>(std::min<uint64_t>((static_cast<uint64_t>(batch->total_tokens) * query_heads + 7) / 8, 8ull * sms));
+            B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, dim3(5 * sms), dim3(256), 0, s, km)
+                                                  : launch_behind(paged_merge_kernel<256>, dim3(5 * sms), dim3(256), 0, s, km));
+            B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_lse_kernel<128>, dim3(blocks_of_rows), dim3(256), 0, s, lp)
+                                                  : launch_behind(paged_lse_kernel<256>, dim3(blocks_of_rows), dim3(256), 0, s, lp));
+        }
     }
     if (room.decode) {
         PagedDecode dp{pool, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse, query_heads, window, sinks, 0, scale * 1.4426950408889634f};

@@ -116,7 +116,8 @@ extern "C" int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
     if (batch->total_tokens == 0 || batch->sequences == 0) return B200KV_OK;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    // four where every SM has sixteen warps with work all the same
+    // four where every SM has sixteen warps with work all the same: 48, 2000, 4700, 10000 and 40000 tokens of 8 heads of 128, q8_0, took 8.3, 11.2, 15.3, 21.5 and 62.3 us
+    // with one a warp, 13.2, 13.2, 15.3, 21.7 and 54.3 with four
     const uint32_t tokens = batch->total_tokens >= 4 * 16 * device_sms() / 2 ? 4 : 1, of_block = kLoadThreads / 32 * tokens;
     const LoadParams p{paged_of(*view, *batch), static_cast<__half*>(key), static_cast<__half*>(value), tokens};
     const dim3 grid((batch->total_tokens + of_block - 1) / of_block, key != nullptr && value != nullptr ? 2 : 1);

@@ -851,11 +851,15 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
 #pragma unroll
             for (int i = 0; i < kBN; i += 2) {
                 const float2 e = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, ref2));
-                const __half2 h = __floats2half2_rn(ex2_approx(e.x), ex2_approx(e.y));
+                const float w0 = ex2_approx(e.x), w1 = ex2_approx(e.y);
+                const __half2 h = __floats2half2_rn(w0, w1);
                 pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
-                // the sum uses the rounded values the MMA will multiply, so numerator and denominator stay consistent
-                const float2 hf = __half22float2(h);
-                sum = add_pair(sum, pack_pair(hf.x, hf.y));
+                if constexpr (PAGED) {   // the sum is also an output, the statistics: of the weights as they are (of rounded ones it is 4e-5 of its value off under a window of 19)
+                    sum = add_pair(sum, pack_pair(w0, w1));
+                } else {                 // the sum uses the rounded values the MMA will multiply, so numerator and denominator stay consistent
+                    const float2 hf = __half22float2(h);
+                    sum = add_pair(sum, pack_pair(hf.x, hf.y));
+                }
             }
             {
                 const float2 halves = unpack_pair(sum);

@@ -265,3 +265,35 @@ def test_calls_refuse_tensors_that_do_not_fit(cuda):
     with pytest.raises(ValueError, match="another device"):
         paged.launch_paged_load(elsewhere, batch, half(4, 2, 128), None)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("act", [np.float16, np.float32])
+@pytest.mark.parametrize("d,heads,hq,window,sinks", [(128, 2, 8, 3, 0), (128, 1, 4, 19, 0), (256, 2, 12, 40, 4), (256, 1, 1, 0, 0), (128, 2, 14, 0, 0)])
+def test_statistics_of_chunks_are_good_to_their_type(cuda, status, act, d, heads, hq, window, sinks):
+    """Over an fp16 cache nothing but products and sums of 32 bits stands between a chunk's lse and the formula: neither rounded queries nor rounded weights."""
+    rng = np.random.default_rng(d + hq + window)
+    lengths, tokens = [300, 64, 900, 1, 40], [70, 64, 130, 1, 2]
+    pool = po.Pool(rng, lengths, d=d, heads=heads, page=16, mode=0, qblock=d)
+    view = pool.upload()
+    batch, starts = po.batch_of(pool, tokens, pad_rows=3)
+    total, n = batch.total_tokens, sum(tokens)
+    q = (1.5 * rng.standard_normal((total, hq, d))).astype(act)
+    out, lse = torch.zeros(total, hq, d, dtype=torch.float16, device="cuda"), torch.full((total, hq), 5.0, device="cuda")
+    ws = paged.paged_workspace(view, batch, hq, window=window, sinks=sinks).fill_(255)
+    paged.launch_paged_attention(view, batch, to_dev(q), out, query_heads=hq, scale=d ** -0.5, window=window, sinks=sinks, lse=lse, workspace=ws)
+    _, want, _ = po.attention(pool, q, starts, d ** -0.5, window, sinks)
+    got = lse.cpu().numpy().astype(np.float64)
+    assert (got[n:] == 5.0).all() and int(status) == 0
+    # a score: d products in fp32 and its scale, 2^-20 of the largest sum of magnitudes; exponentials of 2 units of 2^-23 each, their sums of fewer than 1024 terms half a
+    # unit a step and on average half of that, 2^-17 of a sum at the most; the logarithm and its factor 2^-21 of the value.  fp32 queries: a score moves by e, at most
+    # 2^-11 of the sum of magnitudes; the first order is taken out but for the mean key's rounding and its fp16 weights (2^-9 of it), the second is e^2 / 2
+    most = max(np.abs(pool.rows(s, h, 0)).sum(-1).max() for s in range(5) for h in range(heads)) * np.abs(q.astype(np.float64)).max() * d ** -0.5
+    magnitude = max((np.abs(pool.rows(s, h, 0)) @ np.abs(q[starts[s]:starts[s + 1], h * (hq // heads):(h + 1) * (hq // heads)].reshape(-1, d).astype(np.float64)).T).max()
+                    for s in range(5) for h in range(heads)) * d ** -0.5
+    assert magnitude <= most
+    e = 2.0 ** -11 * magnitude if act == np.float32 else 0.0
+    limit = 2.0 ** -20 * magnitude + 2.0 ** -17 + 2.0 ** -21 * np.abs(want[:n]) + e * 2.0 ** -9 + e * e / 2
+    off = np.abs(got[:n] - want[:n])
+    assert (off <= limit).all(), (off.max(), limit.max())
+    # as a whole, in the 2-norm, to 1e-5 (roundings do not lie at their limits all at once)
+    assert np.linalg.norm(off) <= 1e-5 * np.linalg.norm(want[:n])
