@@ -456,10 +456,10 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.groups = take(parts * 4);
     const uint64_t plane = r.scratch_tiles * kChunkTile * view.kv_heads * view.head_dim * sizeof(__half);
     r.k = take(plane);
-    r.v = take(plane);
+    // the mean keys of the statistics lie over V, which the second pass of the chunk kernel does not read
+    r.v = r.mean_key = take(std::max(plane, static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half)));
     r.part_o = take(parts * kChunkRows * view.head_dim * sizeof(float));
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
-    r.mean_key = take(static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half));
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
     return r;
 }

@@ -297,3 +297,25 @@ def test_statistics_of_chunks_are_good_to_their_type(cuda, status, act, d, heads
     assert (off <= limit).all(), (off.max(), limit.max())
     # as a whole, in the 2-norm, to 1e-5 (roundings do not lie at their limits all at once)
     assert np.linalg.norm(off) <= 1e-5 * np.linalg.norm(want[:n])
+
+
+@pytest.mark.parametrize("chunk", [1, 20])
+def test_the_most_sequences(cuda, status, chunk):
+    rng = np.random.default_rng(chunk)
+    lengths = [int(n) for n in rng.integers(0, 4, 8192)]
+    lengths[4000] = lengths[8191] = 40
+    tokens = [min(n, 1) if s % 2 else 0 for s, n in enumerate(lengths)]
+    tokens[4000] = tokens[8191] = chunk
+    pool = po.Pool(rng, lengths, d=128, heads=1, page=16, mode=3, qblock=32)
+    run_attention(rng, pool, tokens, hq=2)
+    run_weights(rng, pool, tokens, hq=2)
+    view = pool.upload()
+    batch, _ = po.batch_of(pool, tokens)
+    kept, new_len = torch.zeros(8192, 1, 2, dtype=torch.int32, device="cuda"), torch.zeros(8192, dtype=torch.int32, device="cuda")
+    w = torch.rand(8192, 1, 40, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    paged.launch_paged_evict(view, batch, batch.tensors[0], w, keep=2, sinks=1, kept=kept, new_lengths=new_len)
+    host, found = w.cpu().numpy(), kept.cpu().numpy()
+    for s, n in enumerate(lengths):
+        want = po.evict(host[s, 0], n, 2, 1, 0)
+        assert np.array_equal(found[s, 0, :len(want)], want) and (found[s, 0, len(want):] == -1).all()
+    assert new_len.tolist() == [min(n, 2) for n in lengths] and int(status) == 0
