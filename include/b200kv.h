@@ -537,8 +537,8 @@ B200KV_API int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
  * Cache rows that any of a sequence's new tokens sees are finite, as b200kv_prefill_attn asks as well; those that none of them sees (past the length,
  * between the sinks and the window) may hold anything.  A sequence of up to 4 query rows (new tokens times query_heads / kv_heads; 8 where max_tokens allows no
  * more, or that quotient is above 4) is computed on the cache as it is stored, a longer one on a copy in fp16, where an int8 row's value of more than 65504 is
- * infinite (and where statistics of int8 rows are good to fp16 only); a batch of one sequence goes by max_tokens.  q, output and gate 16-byte aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no
- * consequence; one launch at a time uses it. */
+ * infinite and lse is good to 1e-4 of a score only (elsewhere to a few 1e-6 of itself); a batch of one sequence goes by max_tokens.  q, output and gate 16-byte
+ * aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no consequence; one launch at a time uses it. */
 B200KV_API size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window,
                        uint32_t sinks);
 B200KV_API int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* gate,

@@ -13,7 +13,8 @@
 //      O^T = V^T P        M = 128 dims (a thread each, per half of 256), K = positions
 //    int8 sides on kind::i8 -- the sums of a block of 32 dims are exact, so its scale multiplies the sum -- and fp16 sides on kind::f16.
 //  * Against int8 keys a query is a whole number in two int8 planes (16 bits; 8 rows) or three (24 bits; up to 4 rows: they fit the 16 columns all the
-//    same); against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
+//    same); of 16 bits a row's statistics are 3e-6 of their size off at 16 positions of 256 dims, 2e-5 at one, the output less than its own rounding (a third plane of eight
+//    rows would be 32 columns a block, more than TMEM has beside the sums).  Against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
 //    position's value scale, in two uint8 planes; for fp16 values two fp16 terms.  Sums of a tile are folded into fp32 registers.
 //  * A softmax thread has four query rows of a position; with five to eight rows a second group of 128 threads has the others.
 //  * Positions that no row sees weigh nothing and their values are cleared in shared memory where they are fp16 (0 x NaN is NaN), each by its own thread (by the warp that

@@ -84,6 +84,9 @@ __device__ __forceinline__ ChunkItem reload(const ChunkItem* from) {
     return item;
 }
 
+// Which of a tile's positions lie below n, a bit each.
+__device__ __forceinline__ uint64_t bits_below(uint32_t n, uint32_t pos0) { return n <= pos0 ? 0ull : n - pos0 >= kBN ? ~0ull : (1ull << (n - pos0)) - 1; }
+
 template <bool PAGED> struct KernelParams : Tc5Params {};
 template <> struct KernelParams<true> : Tc5Params {   // of the base: maps, q, gate, heads, scale and partials
     const ChunkItem* items;
@@ -804,8 +807,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // Only the tiles that straddle this row's causal length need the mask.
             if constexpr (PAGED) {
                 if (pos0 + kBN > len || pos0 < low) {   // 64 bits, one a position: below len, and from low on or among the sinks
-                    const auto below = [&](uint32_t n) -> uint64_t { return n <= pos0 ? 0ull : n - pos0 >= kBN ? ~0ull : (1ull << (n - pos0)) - 1; };
-                    const uint64_t seen = below(len) & (~below(low) | below(p.sinks));
+                    const uint64_t seen = bits_below(len, pos0) & (~bits_below(low, pos0) | bits_below(p.sinks, pos0));
 #pragma unroll
                     for (int i = 0; i < kBN; ++i) s[i] = (seen >> i) & 1 ? s[i] : -INFINITY;
                 }
