@@ -15,6 +15,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <utility>
 #include <vector>
 
@@ -152,6 +153,23 @@ public:
         if (!here(o)) return nullptr;
         if (THPVariable_Unpack(o).scalar_type() != type || static_cast<uint64_t>(n) < least) return static_cast<T*>(fail(PyExc_ValueError, text));
         return static_cast<T*>(p);
+    }
+    // The same of a given shape [at least `rows`][shape...], where a number of the shape is exact, or, as the last one with `width`, the least, and *width what it is.  (An
+    // account of more slots than the batch has sequences has the stride of its shape; its number of elements would say another.)
+    template <typename T>
+    T* shaped(at::ScalarType type, const char* text, uint64_t rows, std::initializer_list<uint64_t> shape, uint32_t* width = nullptr, bool optional = false) {
+        PyObject* o = ok_ ? args_[i_] : Py_None;
+        T* p = exactly<T>(type, text, 0, optional);
+        if (!ok_ || o == Py_None || rows == 0) return p;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        bool fits = static_cast<size_t>(t.dim()) == 1 + shape.size() && static_cast<uint64_t>(t.size(0)) >= rows;
+        for (size_t i = 1; fits && i <= shape.size(); ++i) {
+            const uint64_t want = shape.begin()[i - 1], n = static_cast<uint64_t>(t.size(i));
+            fits = width != nullptr && i == shape.size() ? n >= want && n <= 0xffffffffu : n == want;
+        }
+        if (!fits) return static_cast<T*>(fail(PyExc_ValueError, text));
+        if (width != nullptr) *width = static_cast<uint32_t>(t.size(t.dim() - 1));
+        return p;
     }
     // An activation tensor of fp16 or fp32 with at least `least` elements.
     void* activation(int* dtype, uint64_t least, const char* text) {
@@ -420,34 +438,30 @@ PyObject* py_paged_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const uint64_t rows = a.ok() ? static_cast<uint64_t>(batch->total_tokens) * heads : 0;
     const void* q = a.activation(&qd, rows * (a.ok() ? view->head_dim : 0), kSmall);
     const float* lse = a.exactly<const float>(at::kFloat, kSmall, rows);
-    float* weights = a.exactly<float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]",
-                                      a.ok() ? static_cast<uint64_t>(batch->sequences) * view->kv_heads * batch->max_length : 0);
-    const uint64_t stride = a.ok() && batch->sequences > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[5]).numel()) / (static_cast<uint64_t>(batch->sequences) * view->kv_heads) : 0;
+    uint32_t stride = 0;
+    float* weights = a.shaped<float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]", a.ok() ? batch->sequences : 0,
+                                     {a.ok() ? view->kv_heads : 0, a.ok() ? batch->max_length : 0}, &stride);
     const float scale = a.f32();
     const uint32_t window = a.u32(), sinks = a.u32(), observe = a.u32();
     void* s = a.stream();
-    if (a.ok() && stride > 0xffffffffu) a.fail(PyExc_ValueError, "weights: too many positions");
-    return call(a, [&] { return g_api.paged_weights(view, batch, q, qd, lse, weights, static_cast<uint32_t>(stride), heads, scale, window, sinks, observe, s); });
+    return call(a, [&] { return g_api.paged_weights(view, batch, q, qd, lse, weights, stride, heads, scale, window, sinks, observe, s); });
 }
 
 PyObject* py_paged_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Args a(args, n, 11);
     const auto* view = a.paged_view();
     const auto* batch = a.paged_batch();
-    const uint64_t sequences = a.ok() ? batch->sequences : 0, heads = a.ok() ? sequences * view->kv_heads : 0;
+    const uint64_t sequences = a.ok() ? batch->sequences : 0, heads = a.ok() ? view->kv_heads : 0;
     const uint32_t keep = a.u32(), sinks = a.u32(), recent = a.u32();
-    const int32_t* target = a.exactly<const int32_t>(at::kInt, "target: int32 [sequences][pages]", sequences);
-    const float* weights = a.exactly<const float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]", a.ok() ? heads * batch->max_length : 0);
-    int32_t* kept = a.exactly<int32_t>(at::kInt, "kept: int32 [sequences][kv_heads][keep]", heads * keep);
-    float* new_weights = a.exactly<float>(at::kFloat, "new_weights: fp32 [sequences][kv_heads][keep]", heads * keep, true);
+    uint32_t pages = 0, stride = 0;
+    const int32_t* target = a.shaped<const int32_t>(at::kInt, "target: int32 [sequences][pages]", sequences, {0}, &pages);
+    const float* weights = a.shaped<const float>(at::kFloat, "weights: fp32 [sequences][kv_heads][at least max_length]", sequences, {heads, a.ok() ? batch->max_length : 0}, &stride);
+    int32_t* kept = a.shaped<int32_t>(at::kInt, "kept: int32 [sequences][kv_heads][keep]", sequences, {heads, keep});
+    float* new_weights = a.shaped<float>(at::kFloat, "new_weights: fp32 [sequences][kv_heads][keep]", sequences, {heads, keep}, nullptr, true);
     int32_t* new_lengths = a.exactly<int32_t>(at::kInt, "new_lengths: int32 [sequences]", sequences);
     void* s = a.stream();
-    if (!a.ok()) return nullptr;
-    const uint64_t stride = heads > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[6]).numel()) / heads : 0;
-    const uint64_t pages = sequences > 0 ? static_cast<uint64_t>(THPVariable_Unpack(args[5]).numel()) / sequences : 0;
-    if (stride > 0xffffffffu || pages > 0xffffffffu) a.fail(PyExc_ValueError, "too many positions or pages");
     return call(a, [&] {
-        return g_api.paged_evict(view, batch, target, static_cast<uint32_t>(pages), weights, static_cast<uint32_t>(stride), keep, sinks, recent, kept, new_weights,
+        return g_api.paged_evict(view, batch, target, pages, weights, stride, keep, sinks, recent, kept, new_weights,
                                  new_lengths, s);
     });
 }

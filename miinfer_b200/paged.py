@@ -142,7 +142,7 @@ def launch_paged_attention(view: PagedView, batch: PagedBatch, q: torch.Tensor, 
 
 def launch_paged_weights(view: PagedView, batch: PagedBatch, q: torch.Tensor, lse: torch.Tensor, weights: torch.Tensor, *, query_heads: int,
                          scale: float, window: int = 0, sinks: int = 0, observe: int = 0, stream: Optional[torch.cuda.Stream] = None) -> None:
-    """Adds to `weights` (fp32 [sequences][kv_heads][max_length or more]) what the new tokens' attention gives each position, summed over
+    """Adds to `weights` (fp32 [sequences or more][kv_heads][max_length or more]) what the new tokens' attention gives each position, summed over
     tokens and heads; q, lse, scale, window and sinks of the attention call.  observe: only the last so many tokens of a sequence."""
     rc = native.paged_weights(view, batch, query_heads, q, lse, weights, scale, window, sinks, observe, stream)
     if rc:
@@ -154,7 +154,7 @@ def launch_paged_evict(view: PagedView, batch: PagedBatch, target_table: torch.T
                        stream: Optional[torch.cuda.Stream] = None) -> None:
     """Keeps the first `sinks`, the last `recent` and the heaviest other positions of every sequence and kv head, `keep` in all, moved together in the
     pages of target_table (int32 [sequences][pages]; the batch's own table: in place).  kept: int32 [sequences][kv_heads][keep],
-    new_weights: fp32 of that shape, new_lengths: int32 [sequences]."""
+    new_weights: fp32 of that shape, new_lengths: int32 [sequences].  Each may have rows for more sequences, which stay as they are."""
     rc = native.paged_evict(view, batch, keep, sinks, recent, target_table, weights, kept, new_weights, new_lengths, stream)
     if rc:
         check(rc, "b200kv_paged_evict")
