@@ -132,14 +132,16 @@ __device__ __forceinline__ float store_terms(uint8_t* q, int slab, int row, cons
     return exp2i(-up);
 }
 // One row as a whole number in PLANES int8 planes, the highest digit in row `row`, the next STRIDE rows on: 8 bits less one each.
+// The largest magnitude is found on the bits, which order as magnitudes do, with NaN above infinity: a NaN anywhere in a row, of which its digits know nothing, is
+// the row's factor and so its scores.
 template <int D, int PLANES, int STRIDE>
 __device__ __forceinline__ float store_planes(uint8_t* q, int slab, int row, const float (&x)[D / 32], int lane) {
     constexpr int E = D / 32;
     constexpr float kMost = PLANES == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
-    float amax = 0.0f;
+    uint32_t most = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    amax = warp_max(amax);
+    for (int e = 0; e < E; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+    const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
     const float inv = amax > 0.0f ? kMost / amax : 0.0f;
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
