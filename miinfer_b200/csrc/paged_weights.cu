@@ -446,8 +446,40 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive(bar(L::RAW_EMPTY + raw));
             const int base = c.span.base();
             const uint32_t groups = (sh.t1 - sh.t0 + group_tokens - 1) / group_tokens;
-            Pair sum[2] = {0, 0};
+            Pair sum[2] = {0, 0}, before_group[2] = {0, 0};
             const Pair factor2 = pack_pair(factor, factor);
+            // An fp32 query's element beyond fp16 (65504) has an infinite first term and a second one that takes infinity away again, so its row's scores are NaN.  Sums that a group
+            // leaves NaN are taken again, row by row, in fp32: K from TMEM, the query as it is.  (1 to 3 us a row, a call whose rows are all like that 45 to 85 times as long.  Found
+            // ahead of the products, by the warps that split the queries, such rows cost every call 4 to 12 %: those warps bound it.)
+            [[maybe_unused]] auto again = [&](uint32_t first, const float* stats, const int* places) {
+                const uint32_t rows = min(group_rows, (sh.t1 - first) * G);
+                float total = 0.0f;
+#pragma unroll 1
+                for (uint32_t x = 0; x < rows; ++x) {
+                    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + ((static_cast<size_t>(c.span.first) + first + x / G) * p.query_heads + c.head * G + x % G) * D);
+                    float s[4] = {};
+#pragma unroll 1
+                    for (int col = 0; col < D / 2; col += 8) {
+                        int hi[8], lo[8] = {};
+                        tmem_ld8(tmem_base + lane_addr + L::kColK + col, hi);
+                        if constexpr (KF == BLOCK) tmem_ld8(tmem_base + lane_addr + L::kColK + D / 2 + col, lo);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float4 four = q[(col + e) / 2];
+                            const float2 a = unpack2(hi[e]), b = unpack2(hi[e + 1]), a1 = unpack2(lo[e]), b1 = unpack2(lo[e + 1]);
+                            s[0] = fmaf(four.x, a.x + a1.x, s[0]);
+                            s[1] = fmaf(four.y, a.y + a1.y, s[1]);
+                            s[2] = fmaf(four.z, b.x + b1.x, s[2]);
+                            s[3] = fmaf(four.w, b.y + b1.y, s[3]);
+                        }
+                    }
+                    const int at = places[x];
+                    const bool seen = static_cast<int>(mine) <= at && (p.window == 0 || static_cast<long long>(mine) + p.window > at || mine < p.sinks);
+                    if (seen) total += ex2(fmaf((s[0] + s[1]) + (s[2] + s[3]), factor, stats[x]));
+                }
+                return total;
+            };
             for (uint32_t g = 0; g < groups; ++g, ++k) {
                 if ((k & 1) != static_cast<uint32_t>(wg)) continue;
                 const uint32_t sb = k % L::kSBufs, qb = k % L::kQBufs;
@@ -459,6 +491,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                 const uint32_t first = sh.t0 + g * group_tokens, last = first + group_tokens - 1;
                 const bool whole = last < sh.t1 && static_cast<int>(sh.pos0) + kTile - 1 <= base + static_cast<int>(first) &&
                                    (p.window == 0 || static_cast<long long>(sh.pos0) + p.window > static_cast<long long>(base) + last);   // all rows see all positions
+                if constexpr (Q32) { before_group[0] = sum[0]; before_group[1] = sum[1]; }
                 constexpr int kStep = 16;
 #pragma unroll
                 for (int col0 = 0; col0 < kGroup; col0 += kStep) {
@@ -496,6 +529,17 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                         };
                         if (p.window == 0) add_seen([&](int at) { return static_cast<int>(mine) <= at; });
                         else add_seen([&](int at) { return static_cast<int>(mine) <= at && (static_cast<long long>(mine) + p.window > at || mine < p.sinks); });
+                    }
+                }
+                if constexpr (Q32) {
+                    const float2 now = unpack_pair(add_pair(sum[0], sum[1])), then = unpack_pair(add_pair(before_group[0], before_group[1]));
+                    const bool mended = isnan(now.x + now.y) && !isnan(then.x + then.y);
+                    if (__any_sync(0xffffffffu, mended && !failed)) {
+                        const float group = again(first, stats, places);
+                        if (mended) {
+                            sum[0] = add_pair(before_group[0], pack_pair(group, 0.0f));
+                            sum[1] = before_group[1];
+                        }
                     }
                 }
                 __syncwarp();
