@@ -404,6 +404,18 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             const uint8_t* scales = smem + L::kOffScales + raw * U::kScales + t128 * U::kScale;
             const uint8_t* src = smem + raw * U::kData + t128 * 128;
             constexpr int kChunks = U::kRow / 32;                            // 16-byte chunks of half a row
+            float factor = p.scale_log2;
+            [[maybe_unused]] __half2 even = __float2half2_rn(1.0f);
+            if constexpr (KF == BLOCK) {   // a position's scales by a power of two, the largest to [2^7, 2^8), so that a product is in fp16's range whatever the scales are
+                uint32_t words[D / 64], most = 0;
+                if constexpr (D == 256) *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(scales);
+                else *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(scales);
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b) most = max(most, max(words[b] & 0x7fffu, (words[b] >> 16) & 0x7fffu));
+                const int up = min(22 - static_cast<int>(most >> 10), 15);   // 7 less the exponent; subnormal ones by 2^15
+                even = __half2half2(__ushort_as_half(static_cast<unsigned short>((up + 15) << 10)));
+                factor *= exp2i(-up);
+            }
 #pragma unroll
             for (int x = 0; x < kChunks; x += KF == F16 ? 2 : 1) {
                 const int chunk = wg * kChunks + x;
@@ -420,7 +432,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                     uint32_t hi[8];
                     [[maybe_unused]] uint32_t lo[8];
                     [[maybe_unused]] __half2 sc;
-                    if constexpr (KF == BLOCK) sc = __half2half2(reinterpret_cast<const __half*>(scales)[chunk >> 1]);
+                    if constexpr (KF == BLOCK) sc = __hmul2(__half2half2(reinterpret_cast<const __half*>(scales)[chunk >> 1]), even);   // exact, but for what is 2^-30 of the largest
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t pair = __byte_perm(w[e >> 1], 0x64646464u, e & 1 ? 0x4342 : 0x4140);
@@ -437,7 +449,6 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
                     if constexpr (KF == BLOCK) tmem_st8(col + D / 2, lo);
                 }
             }
-            float factor = p.scale_log2;
             if constexpr (KF == ROW) factor *= __half2float(*reinterpret_cast<const __half*>(scales));
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();

@@ -37,3 +37,18 @@ def test_weights_of_fp32_queries_of_any_size(cuda, status, tokens, observe, d, m
     q[0, 0, 3] = 1.0e5
     weigh(pool, q.astype(np.float32), tokens, 1.0e-5 * d ** -0.5, window=0 if group % 2 else 70, sinks=3, observe=observe)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("act", [np.float16, np.float32])
+@pytest.mark.parametrize("tokens,observe", [([1, 1, 1], 0), ([90, 1, 40], 0), ([90, 65, 40], 3)])
+@pytest.mark.parametrize("d,heads,group", [(128, 2, 4), (256, 1, 6), (256, 2, 1)])
+def test_weights_over_keys_of_any_size(cuda, status, act, tokens, observe, d, heads, group):
+    """Block scales of up to 6e4 (an int8 128 of them is 8e6), down to the least that fp16 holds, beside ordinary ones, in one row and in rows of their own."""
+    rng = np.random.default_rng(d + group)
+    pool = po.Pool(rng, [300, 129, 64], d=d, heads=heads, page=16, mode=3, qblock=32)
+    shape = pool.ks.shape
+    pool.ks = np.where(rng.random(shape) < 0.1, np.float16(6.0e4), np.where(rng.random(shape) < 0.1, np.float16(6.0e-8), pool.ks)).astype(np.float16)
+    pool.ks[::3] = (rng.choice([600.0, 3.0e-5], pool.ks[::3].shape[:3] + (1,)) * (1 + rng.random(pool.ks[::3].shape))).astype(np.float16)
+    total = sum(tokens) + 1
+    weigh(pool, rng.standard_normal((total, heads * group, d)).astype(act), tokens, 1.0e-7, window=0 if group > 1 else 70, sinks=3, observe=observe)
+    assert int(status) == 0
