@@ -9,12 +9,10 @@
 //  * K and V come as units of 128 rows through tensor maps over the whole pool, a box a page (pages of less than 128 positions: several), each into a ring
 //    of its own, the block scales beside them as bulk copies.  (One ring K0 V0 K1 V1 ... of an odd number of units would show an issuer, which reads one of
 //    the two, every second phase of a slot only, and a parity does not tell those apart.)  The bytes are operands as they land:
-//      S^T = K Q^T        M = 128 positions (a thread each), N = 16 columns
+//      S^T = K Q^T        M = 128 positions (a thread each), N = 16 or 32 columns
 //      O^T = V^T P        M = 128 dims (a thread each, per half of 256), K = positions
 //    int8 sides on kind::i8 -- the sums of a block of 32 dims are exact, so its scale multiplies the sum -- and fp16 sides on kind::f16.
-//  * Against int8 keys a query is a whole number in two int8 planes (16 bits; 8 rows) or three (24 bits; up to 4 rows: they fit the 16 columns all the
-//    same); of 16 bits a row's statistics are 3e-6 of their size off at 16 positions of 256 dims, 2e-5 at one, the output less than its own rounding (a third plane of eight
-//    rows would be 32 columns a block, more than TMEM has beside the sums).  Against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
+//  * Against int8 keys a query is a whole number in three int8 planes, 24 bits (two, 16 bits, where that does not show: launch_of).  Against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
 //    position's value scale, in two uint8 planes; for fp16 values two fp16 terms.  Sums of a tile are folded into fp32 registers.
 //  * A softmax thread has four query rows of a position; with five to eight rows a second group of 128 threads has the others.
 //  * Positions that no row sees weigh nothing and their values are cleared in shared memory where they are fp16 (0 x NaN is NaN), each by its own thread (by the warp that
@@ -32,7 +30,7 @@ namespace b200kv {
 
 namespace {
 
-template <int D, int KF, int VF, int RG>   // RG: groups of four query rows
+template <int D, int KF, int VF, int RG, int PLANES>   // RG: groups of four query rows; PLANES: of a query row, int8 planes or fp16 terms
 struct Layout {
     static constexpr int kTile = kDecodeTile;
     static constexpr int kHalves = D / 128;
@@ -44,13 +42,21 @@ struct Layout {
     // weights of a row group: rows of 32 bytes per position, one set per half of the dims where the halves' scales differ
     static constexpr int kPSets = VF == BLOCK ? kHalves : 1;
     static constexpr int kPBytes = kPSets * kTile * 32;
-    static constexpr int kPlanes = KF == F16 || RG == 2 ? 2 : 3;                          // of a query row: int8 planes, or fp16 terms
-    static_assert(kPlanes * RG * 4 <= 16, "the 16 columns of a score MMA");
-    static constexpr int kQBytes = 16 * D * (KF == F16 ? 2 : 1);
-    static constexpr int kSCols = KF == BLOCK ? D / 32 * 16 : 16;                         // TMEM columns of a score buffer
+    static_assert(PLANES == 2 || (PLANES == 3 && KF != F16));
+    static constexpr int kStride = PLANES == 3 ? RG * 4 : 8;                              // rows of the operand from a plane to the next
+    static constexpr int kQCols = PLANES * RG * 4 <= 16 ? 16 : 32;                        // columns of a score MMA
+    // Three planes of eight rows have 24 columns of sums, and the operand no more rows: what an MMA takes for the last eight is the next slab, or the scales behind the
+    // last one, and nobody looks at their sums.
+    static constexpr int kQRows = kQCols == 16 ? 16 : 24;
+    static constexpr int kQSlab = kQRows * 128, kQBytes = kQRows * D * (KF == F16 ? 2 : 1);
+    static constexpr int kSCols = KF == BLOCK ? D / 32 * kQCols : kQCols;                 // TMEM columns of a score buffer
     static constexpr int kOCols = RG * kHalves * 32;                                      // of a buffer of sums
-    static constexpr uint32_t kTmemCols = 2 * (kSCols + kOCols) <= 128 ? 128 : 2 * (kSCols + kOCols) <= 256 ? 256 : 512;
-    static constexpr uint32_t kColS = 0, kColO = 2 * kSCols;
+    // Three planes of eight rows of 256 dims against block scales leave room for one buffer of scores: the next tile's follow once these are in registers.
+    static constexpr int kSBufs = 2 * (kSCols + kOCols) <= 512 ? 2 : 1;
+    static constexpr int kCols = kSBufs * kSCols + 2 * kOCols;
+    static_assert(kCols <= 512);
+    static constexpr uint32_t kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+    static constexpr uint32_t kColS = 0, kColO = kSBufs * kSCols;
     static constexpr int kXchWords = 16;                                                  // 4 maxima of scores, up to 8 of value scales
     static constexpr int kMiscBytes = RG * 2 * 4 * kXchWords * 4 + RG * 64 + 2 * 8 * 4 + 12 * 16 + 24 * 8 + 80;
     static constexpr int kMostUnits = 6;
@@ -81,13 +87,13 @@ struct Layout {
     static constexpr int kOffMisc = kOffBar + kNumBars * 8;                               // tmem slot, fail flag, the piece
     static constexpr int kTotal = (kOffMisc + 48 + 15) / 16 * 16;
     static constexpr int kAlloc = kTotal + 1024;
-    static_assert(kTotal <= kBudget);
+    static_assert(kTotal <= kBudget && kOffQ + 2 * kQBytes + (kQCols - kQRows) * 128 <= kTotal);
 };
 
-template <int D, int KF, int VF, int RG>
-__global__ void __launch_bounds__(Layout<D, KF, VF, RG>::kThreads, Layout<D, KF, VF, RG>::kCtas)
+template <int D, int KF, int VF, int RG, int PLANES>
+__global__ void __launch_bounds__(Layout<D, KF, VF, RG, PLANES>::kThreads, Layout<D, KF, VF, RG, PLANES>::kCtas)
 paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using L = Layout<D, KF, VF, RG>;
+    using L = Layout<D, KF, VF, RG, PLANES>;
     constexpr int kHalves = L::kHalves;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -148,7 +154,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
         }
     } else if (warp == L::kQWarp) {
         // =============================== the query rows of a pair, as the operand of its score MMAs ===============================
-        // 16 rows of the operand: row 4 plane + r (three planes of four query rows) or 8 plane + r (two of eight).
+        // Rows of the operand: kStride plane + r.
         for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
             const uint32_t buf = k & 1;
             float x[RG * 4][D / 32];
@@ -158,8 +164,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
 #pragma unroll
             for (int r = 0; r < RG * 4; ++r) {
                 float unit;
-                if constexpr (KF == F16) unit = store_terms<D, 8>(q, 2048, r, x[r], lane);
-                else unit = store_planes<D, L::kPlanes, L::kPlanes == 3 ? 4 : 8>(q, 2048, r, x[r], lane);
+                if constexpr (KF == F16) unit = store_terms<D, L::kStride>(q, L::kQSlab, r, x[r], lane);
+                else unit = store_planes<D, PLANES, L::kStride>(q, L::kQSlab, r, x[r], lane);
                 if (lane == 0) reinterpret_cast<float*>(smem + L::kOffQmul)[buf * 8 + r] = unit * p.scale_log2;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read it through the async proxy
@@ -176,8 +182,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
             ok = wait_warp(bar(L::Q_FULL + (k & 1)), (k >> 1) & 1);
             const uint64_t qd = q_desc + (((k & 1) * L::kQBytes) >> 4);
             for (uint32_t j = 0; j < n && ok; ++j, ++i) {
-                const uint32_t buf = i & 1, slot = i % L::kKUnits;
-                ok = mbar_wait_both(bar(L::S_EMPTY + buf), ((i >> 1) & 1) ^ 1, bar(L::K_FULL + slot), (i / L::kKUnits) & 1);
+                const uint32_t buf = i % L::kSBufs, slot = i % L::kKUnits;
+                ok = mbar_wait_both(bar(L::S_EMPTY + buf), ((i / L::kSBufs) & 1) ^ 1, bar(L::K_FULL + slot), (i / L::kKUnits) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t kd = k_desc + ((slot * L::kKData) >> 4);
@@ -187,12 +193,12 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                         constexpr uint32_t idesc = idesc_f16(128, 16, 0, 0);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            umma_f16(d, kd + (((kk >> 2) * (kDecodeTile * 128) + (kk & 3) * 32) >> 4), qd + (((kk >> 2) * 2048 + (kk & 3) * 32) >> 4), idesc, kk > 0);
+                            umma_f16(d, kd + (((kk >> 2) * (kDecodeTile * 128) + (kk & 3) * 32) >> 4), qd + (((kk >> 2) * L::kQSlab + (kk & 3) * 32) >> 4), idesc, kk > 0);
                     } else {
-                        constexpr uint32_t idesc = idesc_i8(128, 16, 1, 1, 0, 0);
+                        constexpr uint32_t idesc = idesc_i8(128, L::kQCols, 1, 1, 0, 0);
 #pragma unroll
                         for (int b = 0; b < D / 32; ++b)   // 32 dims each: a block's sums in columns of their own, or all in the same
-                            umma_i8(d + (KF == BLOCK ? b * 16 : 0), kd + (((b >> 2) * (kDecodeTile * 128) + (b & 3) * 32) >> 4), qd + (((b >> 2) * 2048 + (b & 3) * 32) >> 4), idesc,
+                            umma_i8(d + (KF == BLOCK ? b * L::kQCols : 0), kd + (((b >> 2) * (kDecodeTile * 128) + (b & 3) * 32) >> 4), qd + (((b >> 2) * L::kQSlab + (b & 3) * 32) >> 4), idesc,
                                     KF == ROW && b > 0);
                     }
                     umma_commit(bar(L::S_FULL + buf));
@@ -294,16 +300,16 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                     }
             };
             auto step = [&](auto buf_c, uint32_t j) {
-                constexpr int buf = decltype(buf_c)::value;
+                constexpr int buf = decltype(buf_c)::value, sbuf = buf % L::kSBufs;
                 const uint32_t slot = i % L::kKUnits, vslot = i % L::kVUnits;
                 const uint32_t pos = c.t.position(c.tile + j) + t128;
-                if (!failed && !mbar_wait_both_lane(bar(L::K_FULL + slot), (i / L::kKUnits) & 1, bar(L::S_FULL + buf), (i >> 1) & 1)) failed = true;
+                if (!failed && !mbar_wait_both_lane(bar(L::K_FULL + slot), (i / L::kKUnits) & 1, bar(L::S_FULL + sbuf), (i / L::kSBufs) & 1)) failed = true;
                 __syncwarp();
                 tc_fence_after();
                 // ---- scores, in base-2 units ----
                 float s[4];
                 [[maybe_unused]] const uint8_t* kst = smem + L::kOffKScales + slot * L::kKScales;
-                const uint32_t s_at = tmem_base + lane_addr + L::kColS + buf * L::kSCols;
+                const uint32_t s_at = tmem_base + lane_addr + L::kColS + sbuf * L::kSCols;
                 if constexpr (KF == F16) {
                     int hi[4], lo[4];
                     tmem_ld4(s_at + 4 * g, hi);
@@ -313,11 +319,6 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                     for (int r = 0; r < 4; ++r) s[r] = terms(__int_as_float(hi[r]), __int_as_float(lo[r]));
                 } else {
                     constexpr int B = KF == BLOCK ? D / 32 : 1;
-                    int v[B][L::kPlanes][4];
-#pragma unroll
-                    for (int b = 0; b < B; ++b)
-#pragma unroll
-                        for (int d = 0; d < L::kPlanes; ++d) tmem_ld4(s_at + b * 16 + (L::kPlanes == 3 ? 4 * d : 8 * d + 4 * g), v[b][d]);
                     float ks[B];
                     if constexpr (KF == BLOCK) {
                         uint32_t raw[B / 2];
@@ -328,22 +329,30 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                     } else {
                         ks[0] = __half2float(*reinterpret_cast<const __half*>(kst + t128 * 2));
                     }
-                    tmem_ld_wait();
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float a = 0.0f;
+                    for (int r = 0; r < 4; ++r) s[r] = 0.0f;
+                    constexpr int kPart = RG == 2 && PLANES == 3 && B > 2 ? 2 : B;   // blocks' sums at a time (all 96 of a thread at once: 76.8 -> 78.8 us)
 #pragma unroll
-                        for (int b = 0; b < B; ++b) {
-                            float x;
-                            if constexpr (L::kPlanes == 3) x = fmaf(static_cast<float>(v[b][0][r]), 65536.0f, static_cast<float>(v[b][1][r] * 256 + v[b][2][r]));
-                            else x = static_cast<float>(v[b][0][r] * 256 + v[b][1][r]);
-                            a = fmaf(x, ks[b], a);
-                        }
-                        s[r] = a;
+                    for (int b0 = 0; b0 < B; b0 += kPart) {
+                        int v[kPart][PLANES][4];
+#pragma unroll
+                        for (int b = 0; b < kPart; ++b)
+#pragma unroll
+                            for (int d = 0; d < PLANES; ++d) tmem_ld4(s_at + (b0 + b) * L::kQCols + L::kStride * d + 4 * g, v[b][d]);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int b = 0; b < kPart; ++b) {
+                                float x;
+                                if constexpr (PLANES == 3) x = fmaf(static_cast<float>(v[b][0][r]), 65536.0f, static_cast<float>(v[b][1][r] * 256 + v[b][2][r]));
+                                else x = static_cast<float>(v[b][0][r] * 256 + v[b][1][r]);
+                                s[r] = fmaf(x, ks[b0 + b], s[r]);
+                            }
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(bar(L::S_EMPTY + buf));
+                mbar_arrive(bar(L::S_EMPTY + sbuf));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(L::K_EMPTY + slot));      // the scales are read
                 const uint32_t pos0 = pos - t128;
@@ -638,15 +647,26 @@ __global__ void __launch_bounds__(D) paged_decode_merge_kernel(const __grid_cons
     else static_cast<float*>(p.out)[at] = v;
 }
 
-template <int D, int KF, int VF, int RG>
-int launch_of(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
-    using L = Layout<D, KF, VF, RG>;
-    const auto kernel = paged_decode_kernel<D, KF, VF, RG>;
+template <int D, int KF, int VF, int RG, int PLANES>
+int launch_planes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+    using L = Layout<D, KF, VF, RG, PLANES>;
+    const auto kernel = paged_decode_kernel<D, KF, VF, RG, PLANES>;
     static std::atomic<uint64_t> done{0};
     B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, done));
     if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, p, kmap, vmap));
     else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap, vmap));
     return B200KV_OK;
+}
+// Three planes against int8 keys (a score to 2^-23 of its row's largest element), but for eight rows against block scales where the output alone is asked for, in fp16: two hold
+// 2^-16, which that does not show, and 96 sums of a tile in place of 64 are 8 to 13 % of the time at 256 dims (24 sequences of 4000, 24 / 4 heads, q8_0: 66.6 and 75 us; 4 % at 128, 2 %
+// and less against row scales).
+template <int D, int KF, int VF, int RG>
+int launch_of(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+    if constexpr (KF == F16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
+    if constexpr (KF == BLOCK && RG == 2) {
+        if (p.lse == nullptr && p.out_is_f16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
+    }
+    if constexpr (KF != F16) return launch_planes<D, KF, VF, RG, 3>(p, kmap, vmap, stream, behind);
 }
 template <int D, int RG>
 int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
