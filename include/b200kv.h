@@ -536,8 +536,10 @@ B200KV_API int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
  * the scaled scores, for b200kv_paged_weights.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8; scale > 0.
  * Cache rows that any of a sequence's new tokens sees are finite, as b200kv_prefill_attn asks as well; those that none of them sees (past the length,
  * between the sinks and the window) may hold anything.  A sequence of up to 4 query rows (new tokens times query_heads / kv_heads; 8 where max_tokens allows no
- * more, or that quotient is above 4) is computed on the cache as it is stored, a longer one on a copy in fp16, where an int8 row's value of more than 65504 is
- * infinite and lse is good to 1e-4 of a score only (elsewhere to a few 1e-6 of itself); a batch of one sequence goes by max_tokens.  q, output and gate 16-byte
+ * more, or that quotient is above 4) is computed on the cache as it is stored, with lse good to a few 1e-6 of itself.  A longer one is computed on a copy in fp16, with queries and
+ * weights rounded to fp16 as b200kv_prefill_attn does it: an int8 row's value or an fp32 query's element of more than 65504 is infinite there.  Its lse is as good over fp16 keys;
+ * over int8 keys each product of a score is off by up to 2^-11 of itself (twice that for fp32 queries), which moves lse by the weighted mean of what it moves the
+ * scores: a few 1e-4 where one position counts, less where many do.  A batch of one sequence goes by max_tokens.  q, output and gate 16-byte
  * aligned.  workspace: b200kv_paged_attn_workspace_bytes, 16-byte aligned, contents of no consequence; one launch at a time uses it. */
 B200KV_API size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window,
                        uint32_t sinks);

@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
 // The chunk kernel multiplies queries rounded to fp16, which moves the statistics of fp32 ones by up to a few 1e-4 of a score's spread: more than the output, itself a
 // mean over the rounded weights, shows, but 1e-5 and more of an lse.  To first order lse_i moves by scale (q_i - fp16(q_i)).(sum_j p_ij k_j), and the sum is what
 // the chunk kernel gives for V = K; what is left is of the square of the rounding.
-// Where both fp32 queries and statistics are asked for the chunks take twice the time for it (two sequences, 1668 new tokens under a window of 40, 24 / 4 heads of 256: 96 -> 148 us).  A warp: a head of a token of the chunk kernel's sequences, or several in turn.
+// Where both fp32 queries and statistics are asked for the chunks take twice the time for it (two sequences, 1668 new tokens under a window of 40, 24 / 4 heads of 256: 96 -> 148 us).
+// Over int8 keys they do not: the copy has rounded those, which costs as much again and is not put back.  A warp: a head of a token of the chunk kernel's sequences, or several in turn.
 struct LseParams {
     PrepareParams prepare;
     const float* q;
@@ -456,8 +457,8 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.groups = take(parts * 4);
     const uint64_t plane = r.scratch_tiles * kChunkTile * view.kv_heads * view.head_dim * sizeof(__half);
     r.k = take(plane);
-    // the mean keys of the statistics lie over V, which the second pass of the chunk kernel does not read
-    r.v = r.mean_key = take(std::max(plane, static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half)));
+    // the mean keys of the statistics (over fp16 keys) lie over V, which the second pass of the chunk kernel does not read
+    r.v = r.mean_key = take(is_k_q8(view.quant_mode) ? plane : std::max(plane, static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half)));
     r.part_o = take(parts * kChunkRows * view.head_dim * sizeof(float));
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
@@ -522,7 +523,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const ChunkMergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
         B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, dim3(5 * sms), dim3(256), 0, s, mp)
                                               : launch_behind(paged_merge_kernel<256>, dim3(5 * sms), dim3(256), 0, s, mp));
-        if (lse != nullptr && q_dtype == B200KV_F32) {
+        if (lse != nullptr && q_dtype == B200KV_F32 && !is_k_q8(view->quant_mode)) {
             ChunkLaunch keys = cl;
             keys.v_scratch = cl.k_scratch;
             keys.gate = nullptr;

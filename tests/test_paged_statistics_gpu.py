@@ -100,3 +100,16 @@ def test_of_chunks(cuda, status, act, d, heads, hq, mode, qblock, window, sinks)
         limit = own_arithmetic(pool, row, keys, want) + 2.0 ** -17 + 6 * U * moved + most ** 2 / 2
         assert abs(got[token, head] - want) <= limit, (token, head, got[token, head], want, limit)
     assert int(status) == 0 and bool((lse[-3:] == 5.0).all())
+
+
+@pytest.mark.parametrize("d,mode,qblock", [(128, 3, 32), (256, 1, 256), (256, 3, 32)])
+def test_of_chunks_with_fp32_queries_over_int8_keys_take_one_pass(cuda, d, mode, qblock):
+    """Over int8 keys, which the copy rounds, the statistics are those of the queries as the kernel multiplies them: a second pass would take out no more than the
+    smaller half of what the roundings cost."""
+    rng = np.random.default_rng(d + mode)
+    pool = po.Pool(rng, [300, 64], d=d, heads=2, page=16, mode=mode, qblock=qblock)
+    view = pool.upload()
+    batch, _ = po.batch_of(pool, [70, 64])
+    q = (1.5 * rng.standard_normal((134, 8, d))).astype(np.float32)
+    (_, lse), (_, rounded) = call(pool, view, batch, q, 8), call(pool, view, batch, q.astype(np.float16), 8)
+    assert torch.equal(lse, rounded)
