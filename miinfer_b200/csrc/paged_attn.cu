@@ -109,7 +109,7 @@ __device__ __forceinline__ Walk walk_of(const PrepareParams& p, const Span& span
 struct PlanScratch {
     Sums scan[kPrepareThreads / 32];
     uint32_t items[kCandidates], parts[kCandidates], longest, piece;
-    float work;
+    unsigned long long work;   // 128ths of a tile: whole numbers, whose sum knows no order
 };
 
 // The list of the chunk kernel's CTAs; one block.
@@ -123,7 +123,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     // ---- how far to split: candidate c has pieces of at most 3 longest / (c + 3) tiles.  The time is no less than a piece's, and about as many waves of average
     // pieces as there are: 152 pieces of one size on 148 SMs take twice as long as 148 (77 us for two chunks of 333 tokens over 5000).
     if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
-    if (tid == 0) { sh.longest = 0; sh.work = 0.0f; }
+    if (tid == 0) { sh.longest = 0; sh.work = 0; }
     __syncthreads();
     for (uint32_t s = tid; s < S; s += kPrepareThreads)
         if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
@@ -133,8 +133,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     for (uint32_t s = tid; s < S; s += kPrepareThreads) {
         const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
         if (n == 0) continue;
-        // (tokens of a chunk see on average half of it)
-        atomicAdd(&sh.work, static_cast<float>(n) * (static_cast<float>(tiles) - 0.5f * min(static_cast<float>(tiles), static_cast<float>(span_of(p.pool, s).tokens) / kChunkTile)));
+        atomicAdd(&sh.work, chunk_work(n, tiles, span_of(p.pool, s).tokens));
         for (uint32_t c = 0; c < kCandidates; ++c) {
             const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
             atomicAdd(&sh.items[c], n * pieces);
@@ -148,7 +147,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
             const float one = piece_of(tid) * p.costs.tile + p.costs.cta;
             const uint32_t n = sh.items[tid], full = n / p.sms, rest = n % p.sms;
             const float waves = full + (rest == 0 ? 0.0f : full == 0 ? 1.0f : p.costs.last_wave + (1.0f - p.costs.last_wave) * rest / p.sms);
-            us = max(one, waves * (sh.work / n * p.costs.tile + p.costs.cta)) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
+            us = max(one, waves * (static_cast<float>(sh.work) / (128.0f * n) * p.costs.tile + p.costs.cta)) + (sh.parts[tid] > 0 ? p.costs.merge + p.costs.part * sh.parts[tid] : 0.0f);
         }
         const float best = -warp_max_redux(-us);
         const uint32_t which = __ffs(__ballot_sync(0xffffffffu, us == best)) - 1;

@@ -47,6 +47,12 @@ __host__ __device__ inline ChunkTiles chunk_tiles(int base, uint32_t length, uin
     return t;
 }
 
+// Work of n row tiles of a sequence, in 128ths of a tile: tokens of a chunk see on average half of it.
+__host__ __device__ inline unsigned long long chunk_work(uint32_t n, uint32_t tiles, uint32_t tokens) {
+    const unsigned long long half = 64ull * tiles;
+    return n * (2 * half - (half < tokens ? half : tokens));
+}
+
 // The chunk kernel's launch.
 struct ChunkLaunch {
     const ChunkItem* items;
