@@ -438,6 +438,7 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     if (window > 0) each = std::min<uint64_t>(each, (static_cast<uint64_t>(sinks) + kChunkTile - 1) / kChunkTile + (static_cast<uint64_t>(window) + batch.max_tokens + kChunkTile - 1) / kChunkTile + 1);
     r.scratch_tiles = sequences * each;
     if (batch.total_length > 0) r.scratch_tiles = std::min(r.scratch_tiles, batch.total_length / kChunkTile + sequences);
+    r.scratch_tiles = std::max<uint64_t>(r.scratch_tiles, 1);   // lengths bounded by zero: the copy is a tile that nobody reads
     // every sequence's last row tile may be a partial one
     const uint64_t row_tiles = std::min<uint64_t>(batch.total_tokens * group / kChunkRows + sequences, sequences * ((batch.max_tokens * group + kChunkRows - 1) / kChunkRows));
     // (CTAs of the grid that turn out to have nothing to do cost a launch microseconds: row tiles are split where there are fewer of them than this)

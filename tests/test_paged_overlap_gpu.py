@@ -1,4 +1,4 @@
-"""Paged calls one behind the other under launch overlap, replayed from a graph, and again: the bits of the calls by themselves."""
+"""Paged calls one behind the other under launch overlap, replayed from a graph, and again: the bits of the calls by themselves; bounds at zero."""
 import numpy as np
 import pytest
 import torch
@@ -98,6 +98,20 @@ def test_a_step_with_its_eviction_replayed_from_a_graph(cuda, status, tokens, ov
         torch.cuda.synchronize()
         assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(alone, layer.found()))
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("hq,tokens", [(2, [1, 1]), (8, [1, 4]), (8, [20, 3]), (12, [9, 40])])
+@pytest.mark.parametrize("d,mode", [(128, 3), (256, 0)])
+def test_a_batch_whose_lengths_are_bounded_by_zero(cuda, status, hq, tokens, d, mode):
+    """Tokens of sequences that hold nothing see nothing, whatever kernel their number chooses."""
+    pool = po.Pool(np.random.default_rng(1), [0, 0], d=d, heads=2, page=16, mode=mode, qblock=d, capacity=16)
+    view = pool.upload()
+    batch, _ = po.batch_of(pool, tokens, max_length=0, total_length=0)
+    n = sum(tokens)
+    q, out, lse, w = torch.randn(n, hq, d, device="cuda"), torch.full((n, hq, d), 3.0, device="cuda"), torch.zeros(n, hq, device="cuda"), torch.full((2, 2, 5), 3.0, device="cuda")
+    paged.launch_paged_attention(view, batch, q, out, query_heads=hq, scale=0.1, lse=lse, workspace=paged.paged_workspace(view, batch, hq))
+    paged.launch_paged_weights(view, batch, q, lse, w, query_heads=hq, scale=0.1)
+    assert bool((out == 0).all()) and bool(torch.isneginf(lse).all()) and bool((w == 3.0).all()) and int(status) == 0
 
 
 def test_the_cut_of_a_large_batch_is_the_same_each_time(cuda, status):
