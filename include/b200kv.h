@@ -560,8 +560,8 @@ B200KV_API int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_
  * of the pages of target_table (DEVICE [sequences][target_max_pages], target_max_pages * page_size >= min(keep, max_length)); a sequence of at most `keep` positions
  * is copied as it is.  target_table == batch->page_table compacts in place; otherwise the target's pages and the sequences' must not overlap.
  * kept: DEVICE int32 [sequences][kv_heads][keep], the positions that stayed, -1 behind them.  new_weights (may be NULL): fp32 [sequences][kv_heads]
- * [keep], their weights, 0 behind them; must not overlap weights.  new_lengths: DEVICE int32 [sequences] = min(length, keep); not batch->lengths itself.
- * sinks + recent <= keep. */
+ * [keep], their weights, 0 behind them.  new_lengths: DEVICE int32 [sequences] = min(length, keep).  None of the three overlaps weights, one another or the
+ * arrays of the batch and the target.  sinks + recent <= keep. */
 B200KV_API int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const int32_t* target_table, uint32_t target_max_pages,
                        const float* weights, uint32_t weights_stride, uint32_t keep, uint32_t sinks, uint32_t recent, int32_t* kept,
                        float* new_weights, int32_t* new_lengths, void* stream);

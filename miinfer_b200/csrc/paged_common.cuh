@@ -20,6 +20,11 @@ struct Paged {
     uint32_t page_shift;       // log2 of the page size
     uint32_t* status;          // may be null
 };
+// Whether two arrays of so many bytes share any.
+inline bool share(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
 // A window that reaches over every length is none, and without one there are no sinks.
 void settle_window(const b200kv_paged_batch& batch, uint32_t* window, uint32_t* sinks);
 Paged paged_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch);

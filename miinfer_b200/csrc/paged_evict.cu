@@ -326,13 +326,18 @@ extern "C" int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_pa
     if (batch->sequences == 0) return B200KV_OK;
     const auto word = [](const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
     if (!word(target_table) || !word(weights) || !word(kept) || !word(new_lengths) || (new_weights != nullptr && !word(new_weights))) return B200KV_ERR_INVALID;
-    if (keep == 0 || static_cast<uint64_t>(sinks) + recent > keep || new_lengths == batch->lengths) return B200KV_ERR_INVALID;
+    if (keep == 0 || static_cast<uint64_t>(sinks) + recent > keep) return B200KV_ERR_INVALID;
     if (weights_stride < batch->max_length) return B200KV_ERR_INVALID;
     if (keep > 0x7fffffffu / 40 || static_cast<uint64_t>(target_max_pages) * view->page_size < std::min(keep, batch->max_length)) return B200KV_ERR_RANGE;
     if (view->kv_heads > 32767u) return B200KV_ERR_UNSUPPORTED;                                                                 // two grid rows a head
     const uint64_t heads = static_cast<uint64_t>(batch->sequences) * view->kv_heads;
-    const uintptr_t w0 = reinterpret_cast<uintptr_t>(weights), w1 = w0 + heads * weights_stride * 4, n0 = reinterpret_cast<uintptr_t>(new_weights);
-    if (new_weights != nullptr && n0 < w1 && w0 < n0 + heads * keep * 4) return B200KV_ERR_INVALID;
+    if (new_weights != nullptr && share(new_weights, heads * keep * 4, weights, heads * weights_stride * 4)) return B200KV_ERR_INVALID;
+    const uint64_t S = batch->sequences;   // what one CTA writes of these, another may not have read yet
+    const auto over_the_batch = [&](const void* out, uint64_t bytes) {
+        return share(out, bytes, batch->lengths, S * 4) || share(out, bytes, batch->query_starts, (S + 1) * 4) || share(out, bytes, batch->page_table, S * batch->max_pages * 4) ||
+               share(out, bytes, target_table, S * target_max_pages * 4);
+    };
+    if (over_the_batch(kept, heads * keep * 4) || over_the_batch(new_lengths, S * 4) || (new_weights != nullptr && over_the_batch(new_weights, heads * keep * 4))) return B200KV_ERR_INVALID;
     if (target_table == batch->page_table && target_max_pages != batch->max_pages) return B200KV_ERR_INVALID;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;

@@ -1,0 +1,19 @@
+"""Arrays of a paged call that lie over one another, scales of other shapes; no GPU needed."""
+import pytest
+from test_paged_cpu import DEVICE, INVALID, batch_of, evict, no_gpu, view_of
+
+
+@pytest.mark.parametrize("change", [
+    dict(new_lengths=12288 + 4), dict(new_lengths=12288 + 8), dict(new_lengths=12288 - 8),                     # the batch's three lengths, in part
+    dict(new_lengths=4096 + 4 * 29), dict(new_lengths=8192 + 4 * 3), dict(new_lengths=(1 << 14) - 8),          # its last page, its last start; the target's first page
+    dict(kept=12288), dict(kept=4096 - 4 * (3 * 2 * 64 - 1)), dict(kept=8192), dict(kept=(1 << 14) + 4 * 11), dict(new_weights=12288), dict(new_weights=(1 << 14) + 4 * 11),
+])
+def test_what_an_eviction_writes_lies_over_none_of_the_batch_s_arrays(change):
+    assert evict(view_of(), batch_of(), **change) == INVALID
+
+
+@no_gpu
+@pytest.mark.parametrize("change", [dict(new_lengths=12288 + 12), dict(new_lengths=12288 - 12), dict(new_lengths=4096 + 4 * 30), dict(new_lengths=8192 + 4 * 4),
+                                    dict(kept=(1 << 14) + 4 * 12), dict(new_weights=12288 - 4 * 3 * 2 * 64), dict(target=4096, pages=10)])
+def test_what_an_eviction_writes_may_lie_next_to_them(change):
+    assert evict(view_of(), batch_of(), **change) == DEVICE
