@@ -533,7 +533,7 @@ B200KV_API int b200kv_paged_load(const b200kv_paged_view* view, const b200kv_pag
  * [head_dim], q of q_dtype, gate fp32, output of output_dtype = attention * sigmoid(gate).  A token at cache position i
  * sees positions j <= i; with window > 0 only j > i - window and the first `sinks` ones.  (Positions are places in the cache: after an eviction the
  * window counts the positions that are left.)  lse (may be NULL): fp32 [total_tokens][query_heads], the natural logarithm of the sum of exponentials of
- * the scaled scores, for b200kv_paged_weights.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8; scale > 0.
+ * the scaled scores, for b200kv_paged_weights.  output and lse do not overlap q.  A token that sees nothing gets zeros and minus infinity.  query_heads / kv_heads up to 8; scale > 0.
  * Cache rows that any of a sequence's new tokens sees are finite, as b200kv_prefill_attn asks as well; those that none of them sees (past the length,
  * between the sinks and the window) may hold anything.  A sequence of up to 4 query rows (new tokens times query_heads / kv_heads; 8 where max_tokens allows no
  * more, or that quotient is above 4) is computed on the cache as it is stored, with lse good to a few 1e-6 of itself.  A longer one is computed on a copy in fp16, with queries and

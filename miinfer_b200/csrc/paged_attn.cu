@@ -493,6 +493,10 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     if (static_cast<uint64_t>(view->pages) * view->kv_heads * view->page_size > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
     if (batch->sequences == 0 || batch->total_tokens == 0 || batch->max_tokens == 0) return B200KV_OK;
     settle_window(*batch, &window, &sinks);
+    const uint32_t group = query_heads / view->kv_heads;
+    const bool again = lse != nullptr && q_dtype == B200KV_F32 && !is_k_q8(view->quant_mode) && !decode_takes_all(*batch, group);   // the queries are read once more when results are out
+    const uint64_t rows = static_cast<uint64_t>(batch->total_tokens) * query_heads, q_bytes = rows * view->head_dim * 4;
+    if (again && (share(q, q_bytes, output, output_dtype == B200KV_F32 ? q_bytes : q_bytes / 2) || share(q, q_bytes, lse, rows * 4))) return B200KV_ERR_INVALID;
     if (workspace == nullptr || workspace_bytes < b200kv_paged_attn_workspace_bytes(view, batch, query_heads, window, sinks)) return B200KV_ERR_WORKSPACE;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
@@ -500,7 +504,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     if (room.scratch_tiles * kChunkTile * view->kv_heads > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;
     uint8_t* ws = reinterpret_cast<uint8_t*>(up(reinterpret_cast<uintptr_t>(workspace), 1024));
     const Paged pool = paged_of(*view, *batch);
-    const uint32_t group = query_heads / view->kv_heads, sms = std::min(device_sms(), kMostSms);
+    const uint32_t sms = std::min(device_sms(), kMostSms);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
     if (room.chunks) {
@@ -523,7 +527,7 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const ChunkMergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
         B200KV_CUDA_TRY(view->head_dim == 128 ? launch_behind(paged_merge_kernel<128>, dim3(5 * sms), dim3(256), 0, s, mp)
                                               : launch_behind(paged_merge_kernel<256>, dim3(5 * sms), dim3(256), 0, s, mp));
-        if (lse != nullptr && q_dtype == B200KV_F32 && !is_k_q8(view->quant_mode)) {
+        if (again) {
             ChunkLaunch keys = cl;
             keys.v_scratch = cl.k_scratch;
             keys.gate = nullptr;

@@ -1,6 +1,7 @@
 """Arrays of a paged call that lie over one another, scales of other shapes; no GPU needed."""
 import pytest
-from test_paged_cpu import DEVICE, INVALID, batch_of, evict, no_gpu, view_of
+import torch
+from test_paged_cpu import DEVICE, INVALID, attend, batch_of, evict, no_gpu, view_of
 
 
 @pytest.mark.parametrize("change", [
@@ -17,3 +18,13 @@ def test_what_an_eviction_writes_lies_over_none_of_the_batch_s_arrays(change):
                                     dict(kept=(1 << 14) + 4 * 12), dict(new_weights=12288 - 4 * 3 * 2 * 64), dict(target=4096, pages=10)])
 def test_what_an_eviction_writes_may_lie_next_to_them(change):
     assert evict(view_of(), batch_of(), **change) == DEVICE
+
+
+def test_results_over_queries_that_are_read_again_are_refused():
+    """Statistics of fp32 queries over fp16 keys: the queries are read a second time when output and lse are written.  9 rows of 8 heads of 128."""
+    v, q, room = view_of(quant_mode=2, key_f16=4096), 1 << 22, 9 * 8 * 128 * 4
+    for out, lse in [(q, 1 << 26), (q + room - 16, 1 << 26), (q - room // 2 + 16, 1 << 26), (1 << 24, q), (1 << 24, q + room - 4), (1 << 24, q - 9 * 8 * 4 + 4)]:
+        assert attend(v, batch_of(), q=q, q_dtype=1, out=out, lse=lse) == INVALID
+    if not torch.cuda.is_available():
+        for out, lse in [(q + room, 1 << 26), (q - room // 2, 1 << 26), (1 << 24, q + room), (1 << 24, q - 9 * 8 * 4)]:
+            assert attend(v, batch_of(), q=q, q_dtype=1, out=out, lse=lse) == DEVICE
