@@ -41,7 +41,8 @@ class PagedView(_lib.PagedView):
                 raise ValueError("planes are [pages][kv_heads][page_size][head_dim] of the mode's types")
             tensors = [plane]
             if is_q8:
-                if scales is None or scales.dtype != torch.float16 or scales.shape[:3] != plane.shape[:3] or plane.shape[3] % scales.shape[3]:
+                if (scales is None or scales.dtype != torch.float16 or scales.dim() != 4 or scales.shape[:3] != plane.shape[:3] or scales.shape[3] == 0
+                        or plane.shape[3] % scales.shape[3]):
                     raise ValueError("scales are fp16 [pages][kv_heads][page_size][head_dim / qblock]")
                 blocks.add(plane.shape[3] // scales.shape[3])
                 tensors.append(scales)

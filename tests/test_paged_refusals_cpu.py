@@ -1,6 +1,8 @@
 """Arrays of a paged call that lie over one another, scales of other shapes; no GPU needed."""
 import pytest
 import torch
+
+from miinfer_b200 import kv, paged
 from test_paged_cpu import DEVICE, INVALID, attend, batch_of, evict, no_gpu, view_of
 
 
@@ -28,3 +30,12 @@ def test_results_over_queries_that_are_read_again_are_refused():
     if not torch.cuda.is_available():
         for out, lse in [(q + room, 1 << 26), (q - room // 2, 1 << 26), (1 << 24, q + room), (1 << 24, q - 9 * 8 * 4)]:
             assert attend(v, batch_of(), q=q, q_dtype=1, out=out, lse=lse) == DEVICE
+
+
+def test_scales_of_other_shapes_are_value_errors():
+    q8, q = torch.zeros(4, 2, 16, 128, dtype=torch.int8), kv.KvCacheQuantMode.kQ8Q8
+    good = torch.zeros(4, 2, 16, 4, dtype=torch.float16)
+    for bad in (torch.zeros(4, 2, 16, dtype=torch.float16), torch.zeros(4, 2, 16, 0, dtype=torch.float16), torch.zeros(4, 2, 16, 4, 1, dtype=torch.float16)):
+        for scales in ((bad, good), (good, bad)):
+            with pytest.raises(ValueError):
+                paged.PagedView.of(q8, scales[0], q8, scales[1], q)
