@@ -135,7 +135,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
 
     if (warp == L::kProducerWarp) {
         // =============================== copies: K and V units, a page's rows each lane ===============================
-        uint32_t i = 0, fixes = 0;
+        uint32_t i = 0, fixes = 0, begun_k = 0, begun_v = 0;
         for (; c.left > 0 && !failed; c.advance(p)) {
             const int32_t* pages = pages_of(p.pool, c.s);
             const uint32_t n = c.take(), length = c.span.length;
@@ -145,13 +145,20 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 const Boxes boxes = boxes_of(p.pool, page, c.head, pos0, length, lane);
                 if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), length, lane);
                 failed = i >= L::kKUnits && !wait_warp(bar(L::K_EMPTY + ks), ((i / L::kKUnits) & 1) ^ 1);
-                failed = failed || !bring_unit<D, KF>(smem, ks * L::kKData, L::kOffKScales + ks * L::kKScales, &kmap, p.pool.view.key_scales, boxes, bar(L::K_FULL + ks), bar(L::LANDED),
-                                                      &fixes, lane);
+                if (!failed) {
+                    ++begun_k;
+                    failed = !bring_unit<D, KF>(smem, ks * L::kKData, L::kOffKScales + ks * L::kKScales, &kmap, p.pool.view.key_scales, boxes, bar(L::K_FULL + ks), bar(L::LANDED), &fixes, lane);
+                }
                 failed = failed || (i >= L::kVUnits && !wait_warp(bar(L::V_EMPTY + vs), ((i / L::kVUnits) & 1) ^ 1));
-                failed = failed || !bring_unit<D, VF>(smem, L::kOffV + vs * L::kVData, L::kOffVScales + vs * L::kVScales, &vmap, p.pool.view.value_scales, boxes, bar(L::V_FULL + vs),
-                                                      bar(L::LANDED), &fixes, lane);
+                if (!failed) {
+                    ++begun_v;
+                    failed = !bring_unit<D, VF>(smem, L::kOffV + vs * L::kVData, L::kOffVScales + vs * L::kVScales, &vmap, p.pool.view.value_scales, boxes, bar(L::V_FULL + vs),
+                                                bar(L::LANDED), &fixes, lane);
+                }
             }
         }
+        last_phases(bar(L::K_FULL), L::kKUnits, begun_k);
+        last_phases(bar(L::V_FULL), L::kVUnits, begun_v);
     } else if (warp == L::kQWarp) {
         // =============================== the query rows of a pair, as the operand of its score MMAs ===============================
         // Rows of the operand: kStride plane + r.
@@ -208,10 +215,12 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 __syncwarp();
             }
         }
+        last_phases(bar(L::S_FULL), L::kSBufs, i);
     } else if (warp == L::kPvWarp) {
         // =============================== issuer of O^T = V^T P ===============================
         const uint64_t v_desc = umma_desc(sbase + L::kOffV, kDecodeTile * 128, 1024, 2);
         const uint64_t p_desc = umma_desc(sbase + L::kOffP, 32, 256, 6);
+        uint32_t begun = 0;
         bool ok = true;
         for (uint64_t i64 = 0; i64 < c.left && ok; ++i64) {
             const uint32_t i = static_cast<uint32_t>(i64), buf = i & 1, slot = i % L::kVUnits;
@@ -243,8 +252,10 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                     if (g + 1 == RG) umma_commit(bar(L::V_EMPTY + slot));
                 }
                 __syncwarp();
+                ++begun;
             }
         }
+        last_phases(bar(L::P_EMPTY), 2 * RG, begun);
     } else {
         // =============================== softmax: a thread has a position and four query rows ===============================
         const int g = warp >> 2, w4 = warp & 3, t128 = tid & 127;

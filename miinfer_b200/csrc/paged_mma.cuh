@@ -72,6 +72,11 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, int (&r)[8]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// What a warp has under way when it leaves its loop -- copies, or MMAs with their commits -- of a ring of `ring` barriers whose phases it has begun `begun` times in turn: waits, again
+// with a limit, for each barrier's last phase.  Whatever a wait that ran out has made the other warps leave out, the CTA keeps its shared memory and TMEM until then.
+__device__ __forceinline__ void last_phases(uint32_t bar0, uint32_t ring, uint32_t begun) {
+    for (uint32_t n = begun > ring ? begun - ring : 0; n < begun; ++n) wait_warp(bar0 + n % ring * 8, (n / ring) & 1);
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);

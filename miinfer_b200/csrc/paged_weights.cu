@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
     Cursor c(p, start);
 
     if (warp == L::kProducerWarp) {
-        uint32_t i = 0, fixes = 0;
+        uint32_t i = 0, fixes = 0, begun = 0;
         bool ok = true;
         for (; c.left > 0 && ok; c.advance(p)) {
             const int32_t* pages = pages_of(p.pool, c.s);
@@ -113,9 +113,12 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
                 const Boxes boxes = boxes_of(p.pool, page, c.head, c.t.position(c.tile + j), c.span.length, lane);
                 if (j + 1 < n) page = box_page(p.pool, pages, c.t.position(c.tile + j + 1), c.span.length, lane);
                 ok = i < L::kUnits || wait_warp(bar(L::EMPTY + slot), ((i / L::kUnits) & 1) ^ 1);
-                ok = ok && bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes, lane);
+                if (!ok) break;
+                ++begun;
+                ok = bring_unit<D, KF>(smem, slot * U::kData, L::kOffScales + slot * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::FULL + slot), bar(L::LANDED), &fixes, lane);
             }
         }
+        last_phases(bar(L::FULL), L::kUnits, begun);
     } else if (warp == L::kQWarp) {
         for (uint32_t k = 0; c.left > 0; c.advance(p), ++k) {
             const uint32_t buf = k & 1, tokens = p.observed(c.span), t0 = c.span.tokens - tokens;
@@ -175,6 +178,7 @@ __global__ void __launch_bounds__(256, FewLayout<D, KF, ROWS>::kCtas) few_kernel
                 __syncwarp();
             }
         }
+        last_phases(bar(L::S_FULL), 2, i);
     } else if (warp < 4) {
         // =============================== a thread a position ===============================
         const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
@@ -578,6 +582,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             ++i;
             return bring_unit<D, KF>(smem, raw * U::kData, L::kOffScales + raw * U::kScales, &kmap, p.pool.view.key_scales, boxes, bar(L::RAW_FULL + raw), bar(L::LANDED), &fixes, lane);
         });
+        last_phases(bar(L::RAW_FULL), L::kRaw, i);
     } else if (warp < L::kMmaWarp) {
         // =============================== the query rows, 64 at a time ===============================
         const uint32_t w = warp - kQWarp;
@@ -673,6 +678,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             }
             return true;
         });
+        if (!Q32 && w == 0) last_phases(bar(L::Q_FULL), L::kQBufs, k);
     } else {
         // =============================== issuer of S^T = K Q^T ===============================
         constexpr uint32_t idesc = idesc_f16(kTile, kGroup, 0, 0);
@@ -708,6 +714,7 @@ many_kernel(const __grid_constant__ WeightsParams p, const __grid_constant__ CUt
             }
             return true;
         });
+        last_phases(bar(L::S_FULL), L::kSBufs, k);
     }
     tc_fence_before();
     __syncthreads();
