@@ -668,13 +668,13 @@ int launch_planes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorM
     else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap, vmap));
     return B200KV_OK;
 }
-// Three planes against int8 keys (a score to 2^-23 of its row's largest element), but for eight rows against block scales where the output alone is asked for, in fp16: two hold
-// 2^-16, which that does not show, and 96 sums of a tile in place of 64 are 8 to 13 % of the time at 256 dims (24 sequences of 4000, 24 / 4 heads, q8_0: 66.6 and 75 us; 4 % at 128, 2 %
-// and less against row scales).
+// Three planes against int8 keys (a score to 2^-23 of its row's largest element), but for eight rows where the output alone is asked for, in fp16: two hold 2^-16, which that does not
+// show, and are up to 12 % faster (24 sequences of 4000, 24 / 4 heads of 256: q8_0 66.6 and 75 us, where a tile has 96 sums a thread in place of 64 and one buffer of them; one scale a row 59.4
+// and 61.4).
 template <int D, int KF, int VF, int RG>
 int launch_of(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
     if constexpr (KF == F16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
-    if constexpr (KF == BLOCK && RG == 2) {
+    if constexpr (KF != F16 && RG == 2) {
         if (p.lse == nullptr && p.out_is_f16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
     }
     if constexpr (KF != F16) return launch_planes<D, KF, VF, RG, 3>(p, kmap, vmap, stream, behind);
