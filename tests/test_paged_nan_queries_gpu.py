@@ -47,3 +47,24 @@ def test_a_nan_in_a_query_is_a_nan_in_its_row_and_in_no_other(cuda, status, act,
                     expected[s, head // group, :length - tokens[s] + t + 1] = True
     assert torch.equal(torch.isnan(w), expected) and torch.equal(w[~expected], w0[~expected])
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("act", [np.float16, np.float32])
+@pytest.mark.parametrize("d,mode,heads,hq,length", [(128, 0, 8, 64, 700), (256, 3, 8, 48, 500), (128, 3, 8, 64, 60)])
+def test_a_nan_in_a_chunk_whose_row_tiles_are_whole(cuda, status, act, d, mode, heads, hq, length):
+    """More row tiles than multiprocessors, or too few positions to divide: a block writes its rows and their statistics itself."""
+    rng = np.random.default_rng(d + length)
+    pool = po.Pool(rng, [length], d=d, heads=heads, page=64, mode=mode, qblock=d)
+    view = pool.upload()
+    batch, _ = po.batch_of(pool, [length])
+    clean = rng.standard_normal((length, hq, d)).astype(act)
+    q = clean.copy()
+    rows = [(0, 0), (length // 2, 3), (length - 1, hq - 1)]
+    for token, head in rows:
+        q[token, head, token % d] = np.nan
+    (out, lse), (out0, lse0) = attend(view, batch, q, hq, d ** -0.5), attend(view, batch, clean, hq, d ** -0.5)
+    bad = torch.zeros(length, hq, dtype=torch.bool, device="cuda")
+    for token, head in rows:
+        bad[token, head] = True
+    assert bool(torch.isnan(out[bad]).all()) and bool(torch.isnan(lse[bad]).all()), lse[bad]
+    assert torch.equal(out[~bad], out0[~bad]) and torch.equal(lse[~bad], lse0[~bad]) and int(status) == 0

@@ -76,6 +76,34 @@ def of_tokens(rng, pool, view, tokens, group, act, outlier, word):
     assert int(word) == 0 and bool((lse[-1] == 5.0).all())
 
 
+@pytest.mark.parametrize("group", [3, 5, 6, 8])
+@pytest.mark.parametrize("d,mode,qblock", [(128, 3, 32), (256, 3, 32), (256, 3, 256), (128, 1, 128), (256, 1, 32)])
+@pytest.mark.parametrize("act,outlier", [(np.float16, 1.0), (np.float16, 20.0), (np.float32, 20.0)])
+def test_the_output_alone_of_few_rows(cuda, status, group, d, mode, qblock, act, outlier):
+    """Where neither statistics nor an fp32 output are asked for, queries of five to eight rows may be whole numbers of 16 bits: off by at most half of amax / (127 * 2^8), 2^-16.9 of
+    amax with its own rounding, in every element; the weights move with the scores.  With statistics the output is that of 24 bits."""
+    rng = np.random.default_rng(100 * group + d + mode)
+    lengths = [1, 2, 17, 129, 300, 1030]
+    pool = po.Pool(rng, lengths, d=d, heads=2, page=16, mode=mode, qblock=qblock)
+    view = pool.upload()
+    tokens = [1, 1, 1, 1, 8 // group, 1]
+    batch, starts = po.batch_of(pool, tokens)
+    q = 1.5 * rng.standard_normal((batch.total_tokens, 2 * group, d))
+    q[:, :, 5] *= outlier
+    q = q.astype(act)
+    want, _, bound = po.attention(pool, q, starts, d ** -0.5)
+    more = np.zeros_like(bound)
+    for token, head, row, keys, p, _ in rows_of(pool, q, starts, 0, 0):
+        s = int(np.searchsorted(starts, token, side="right")) - 1
+        moved = np.abs(keys).sum(-1).max() * np.abs(row).max() * d ** -0.5 * 2.0 ** -16.9
+        more[token, head] = np.expm1(2 * moved) * (p @ np.abs(pool.rows(s, head // group, 1)[:len(keys)]))
+    out = torch.zeros(*q.shape, dtype=torch.float16, device="cuda")
+    paged.launch_paged_attention(view, batch, to_dev(q), out, query_heads=2 * group, scale=d ** -0.5, workspace=paged.paged_workspace(view, batch, 2 * group).fill_(255))
+    assert (np.abs(out.cpu().numpy().astype(np.float64) - want) <= bound + more).all()
+    out, _ = call(pool, view, batch, q, 2 * group)
+    assert (np.abs(out.cpu().numpy().astype(np.float64) - want) <= bound).all() and int(status) == 0
+
+
 @pytest.mark.parametrize("act", [np.float16, np.float32])
 @pytest.mark.parametrize("d,heads,hq,mode,qblock,window,sinks", [(128, 2, 8, 3, 32, 0, 0), (256, 1, 6, 3, 32, 0, 0), (256, 1, 6, 1, 256, 130, 4), (128, 2, 2, 3, 128, 19, 0), (128, 1, 7, 1, 32, 0, 0)])
 def test_of_chunks(cuda, status, act, d, heads, hq, mode, qblock, window, sinks):
