@@ -448,7 +448,7 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     size_t at = 256;                                     // the plan
     const auto take = [&](uint64_t bytes) { const size_t here = at; at += up(bytes, 1024); return here; };
     at = up(at, 1024);
-    r.decode_parts = take(r.decode ? decode_part_bytes(view, query_heads, sms) : 0);
+    r.decode_parts = take(r.decode ? decode_part_bytes(view, sms) : 0);
     if (!r.chunks) {
         r.bytes = at + 1024;
         return r;

@@ -692,11 +692,11 @@ int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMa
 
 }  // namespace
 
-uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t, uint32_t sms) {
+uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t sms) {
     return sms * (view.head_dim == 128 && view.quant_mode == B200KV_Q8_Q8 ? 2 : 1);
 }
-size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms) {
-    return decode_ctas(view, query_heads, sms) * (2ull * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2)) + sizeof(uint4));
+size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t sms) {
+    return decode_ctas(view, sms) * (2ull * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2)) + sizeof(uint4));
 }
 
 int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind) {
@@ -710,9 +710,8 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
         return B200KV_ERR_UNSUPPORTED;
     p.rows = decode_rows(b, group);
     const bool few = p.rows == 4;
-    const uint32_t sms = std::min(device_sms(), kMostSms), most = decode_ctas(v, p.query_heads, sms);
+    const uint32_t sms = std::min(device_sms(), kMostSms), most = decode_ctas(v, sms);
     p.ctas = few ? most : sms;
-    p.least_tiles = 1;
     p.part_o = static_cast<float*>(parts);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ull * most * kDecodeRows * v.head_dim);
     p.shared = reinterpret_cast<uint4*>(p.part_ml + 2ull * most * kDecodeRows);

@@ -21,7 +21,6 @@ struct PagedDecode {
     uint32_t rows;             // sequences of at most so many query rows are this launch's: 4 or 8
     float scale_log2;
     uint32_t ctas;             // of the launch: the tiles of all sequences are dealt to them in equal pieces
-    uint32_t least_tiles;      // fewest tiles of a piece
     float* part_o;             // [2 ctas][kDecodeRows][head_dim]: a CTA's piece begins and ends inside a kv head's tiles at most once each
     float2* part_ml;           // [2 ctas][kDecodeRows] {maximum in log2 units, sum}
     uint4* shared;             // [ctas]: the pair that begins in a CTA's piece and ends in another's: sequence, kv head, the other CTA, 1 (0: there is none)
@@ -38,8 +37,8 @@ inline bool decode_takes_all(const b200kv_paged_batch& b, uint32_t group) { retu
 // The rows of the launch: four where they are enough for all sequences, or, beside the chunk kernel, for a token.  (Four rows leave room for two CTAs an SM of int8
 // sides, 32 / 8 heads of 128: one token of 64 sequences of 4000 116 us with four, 153 with eight; beside a chunk of 40, of 39 129 and 145.  fp16 197 and 185, 170 and 168.)
 inline uint32_t decode_rows(const b200kv_paged_batch& b, uint32_t group) { return group <= 4 && (b.max_tokens * static_cast<uint64_t>(group) <= 4 || !decode_takes_all(b, group)) ? 4 : kDecodeRows; }
-uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);     // at most
-size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t query_heads, uint32_t sms);
+uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t sms);     // at most
+size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t sms);
 int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind);
 
 // A tensor map over a pool's plane as rows of head_dim: boxes of 128 bytes by `box_rows` rows, 128-byte swizzle.

@@ -27,7 +27,7 @@ struct ChunkItem {
 static_assert(sizeof(ChunkItem) == 64);
 
 struct ChunkPlan {
-    uint32_t items, groups, scratch_tiles, pad_;
+    uint32_t items, groups;
 };
 
 // Where a sequence's tiles lie in the cache.

@@ -1,7 +1,7 @@
 // The list of tiles that the streaming kernels over a paged cache deal out to their CTAs: all tiles of 128 positions of all (sequence, kv head) pairs, in equal
 // pieces.  Sequences and what they see are device memory, so every CTA finds its piece itself.
 //
-// A kernel's parameters P say what is in the list: P.pool, P.tiles_of(span) (a sequence's tiles, the same for each of its kv heads), P.ctas and P.least_tiles.
+// A kernel's parameters P say what is in the list: P.pool, P.tiles_of(span) (a sequence's tiles, the same for each of its kv heads) and P.ctas.
 #pragma once
 
 #include "paged_common.cuh"
@@ -41,7 +41,7 @@ __device__ __forceinline__ uint64_t tiles_before(const P& p, uint32_t s, int lan
 // CTAs that have a piece, and where piece c begins: the first all % pieces of them have a tile more.
 template <class P>
 __device__ __forceinline__ uint32_t pieces_of(const P& p, uint64_t all) {
-    return static_cast<uint32_t>(min(static_cast<uint64_t>(p.ctas), max(static_cast<uint64_t>(1), all / p.least_tiles)));
+    return static_cast<uint32_t>(min(static_cast<uint64_t>(p.ctas), max(static_cast<uint64_t>(1), all)));
 }
 __device__ __forceinline__ uint64_t piece_begin(uint64_t all, uint32_t c, uint32_t pieces) {
     const uint64_t each = all / pieces, more = all % pieces;

@@ -37,7 +37,7 @@ struct WeightsParams {
     float* weights;            // [sequences][kv_heads][stride]
     uint32_t stride, query_heads, window, sinks, observe;
     uint32_t from_rows, to_rows;   // this launch's sequences: from .. to observed query rows
-    uint32_t ctas, least_tiles;
+    uint32_t ctas;
     float scale_log2;
     __device__ __forceinline__ uint32_t observed(const Span& span) const { return observe > 0 ? min(observe, span.tokens) : span.tokens; }
     __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
@@ -740,7 +740,6 @@ int launch_few(WeightsParams p, cudaStream_t stream) {
     CUtensorMap kmap;
     if (!key_map(&kmap, p.pool.view)) return B200KV_ERR_UNSUPPORTED;
     p.ctas = std::min(device_sms(), kMostSms) * L::kCtas;
-    p.least_tiles = 1;
     B200KV_CUDA_TRY(launch_kernel(few_kernel<D, KF, ROWS>, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap));
     return B200KV_OK;
 }
@@ -754,7 +753,6 @@ int launch_many(WeightsParams p, bool behind, cudaStream_t stream) {
     CUtensorMap kmap, qmap{};
     if (!key_map(&kmap, p.pool.view) || (!Q32 && !encode_rows_map(&qmap, p.q, D, p.query_heads, p.pool.batch.total_tokens, G, kGroup / G))) return B200KV_ERR_UNSUPPORTED;
     p.ctas = std::min(device_sms(), kMostSms) * L::kCtas;
-    p.least_tiles = 1;
     if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, p, kmap, qmap));
     else B200KV_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, true, p, kmap, qmap));
     return B200KV_OK;
@@ -801,7 +799,7 @@ extern "C" int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_
     settle_window(*batch, &window, &sinks);
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    const WeightsParams p{paged_of(*view, *batch), q, q_dtype == B200KV_F16, lse, weights, weights_stride, query_heads, window, sinks, observe, 0, 0, 0, 0, scale * 1.4426950408889634f};
+    const WeightsParams p{paged_of(*view, *batch), q, q_dtype == B200KV_F16, lse, weights, weights_stride, query_heads, window, sinks, observe, 0, 0, 0, scale * 1.4426950408889634f};
     const uint64_t most_rows = static_cast<uint64_t>(observe > 0 ? std::min(observe, batch->max_tokens) : batch->max_tokens) * (query_heads / view->kv_heads);
     return view->head_dim == 128 ? launch_formats<128>(p, most_rows, batch->sequences, static_cast<cudaStream_t>(stream))
                                  : launch_formats<256>(p, most_rows, batch->sequences, static_cast<cudaStream_t>(stream));
