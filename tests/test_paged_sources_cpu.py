@@ -46,3 +46,15 @@ def test_a_block_ends_behind_what_it_has_under_way(name, kernel, rings):
 
 def test_every_kernel_with_tensor_memory_is_looked_at():
     assert {k for p in CSRC.glob("paged_*.cu") for k in kernels(p.name)} == {"paged_decode_kernel", "few_kernel", "many_kernel"}
+
+
+@pytest.mark.parametrize("name,kernel", [("paged_decode.cu", "paged_decode_kernel"), ("paged_weights.cu", "few_kernel"), ("paged_weights.cu", "many_kernel")])
+def test_loops_are_left_by_whole_warps(name, kernel):
+    """A wait that runs out for single lanes only marks them; what leaves a loop is the vote of a warp, or a comparison that is the same in all its lanes."""
+    body = kernels(name)[kernel]
+    body = body[:body.rindex("tcgen05.dealloc")]
+    for line in body.splitlines():
+        if re.search(r"\bmbar_wait(_both_lane)?\(", line):
+            assert re.search(r"failed = true;", line), line.strip()
+        for left in re.findall(r"(.*)\b(?:break|return false);", line):
+            assert re.search(r"!ok\b|!wait_warp\(|!mbar_wait_both\(|!free\(\)|row >= rows", left), line.strip()
