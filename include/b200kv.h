@@ -521,7 +521,7 @@ typedef struct b200kv_paged_batch {
 
 /* b200kv_append for a ragged batch: token t of sequence s goes to position lengths[s] - (its new tokens) + t.  key/value:
  * [total_tokens][kv_heads * head_dim] of `dtype`.  rope_positions (DEVICE int32 [total_tokens], may be NULL): the position each token is
- * rotated by where that is not its place in the cache, as after an eviction.  The same bits as b200kv_append for the same
+ * rotated by where that is not its place in the cache, as after an eviction (a negative one counts as 0).  The same bits as b200kv_append for the same
  * position. */
 B200KV_API int b200kv_paged_store(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* key, const void* value, int dtype,
                        const float* k_norm_weight, int rope_mode, float theta, float epsilon, const int32_t* rope_positions, void* stream);
@@ -550,7 +550,7 @@ B200KV_API int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_pag
 /* Adds to weights[s][kv_head][j] the weight that position j gets from sequence s's new tokens: sum of exp(score - lse) over them and over the query
  * heads of the kv head.  weights: fp32 [sequences][kv_heads][weights_stride], weights_stride >= max_length; entries at and past a
  * length are left alone.  q, lse, scale, window and sinks as in the b200kv_paged_attn call that produced lse.  observe > 0: only the last `observe`
- * new tokens of a sequence count. */
+ * new tokens of a sequence count.  q of any size, over rows of any scale; a row whose lse is NaN makes NaN of what it sees, and the account keeps that. */
 B200KV_API int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* lse,
                          float* weights, uint32_t weights_stride, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
                          uint32_t observe, void* stream);

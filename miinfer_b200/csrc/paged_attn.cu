@@ -12,7 +12,7 @@
 // a call: a chain of latencies.)  The chunk kernel follows, and the merge of what its CTAs left for shared row tiles, each launched while the one before
 // still runs.
 //
-// Measured, us, prepare / chunk kernel / merge: 512 new tokens over 8192, 24 / 4 heads of 256, q8_0: 131 in all (9 / 115 / 6); two chunks of 333 over up to 5000 beside
+// Measured, us, prepare / chunk kernel / merge: 512 new tokens over 8192, 24 / 4 heads of 256, q8_0: 131 to 135 in all (9 / 115 / 6); two chunks of 333 over up to 5000 beside
 // 14 single tokens, 32 / 8 heads of 128, q8_0: 132 (10 / 77 / 6, the tokens' kernel 35); 2048 over 6001 under a window of 1024, fp16: 82 (a CTA has 18 tiles of
 // 0.5 and 7 of set-up, Q and output).
 #include "decode_common.cuh"
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
 
 // The chunk kernel multiplies queries rounded to fp16, which moves the statistics of fp32 ones by up to a few 1e-4 of a score's spread: more than the output, itself a
 // mean over the rounded weights, shows, but 1e-5 and more of an lse.  To first order lse_i moves by scale (q_i - fp16(q_i)).(sum_j p_ij k_j), and the sum is what
-// the chunk kernel gives for V = K; what is left is of the square of the rounding.
+// the chunk kernel gives for V = K; what is left is of the square of the rounding.  (That mean key is an fp16 output: 2^-11 of a correction which is 2^-11 itself.)
 // Where both fp32 queries and statistics are asked for the chunks take twice the time for it (two sequences, 1668 new tokens under a window of 40, 24 / 4 heads of 256: 96 -> 148 us).
 // Over int8 keys they do not: the copy has rounded those, which costs as much again and is not put back.  A warp: a head of a token of the chunk kernel's sequences, or several in turn.
 struct LseParams {

@@ -12,13 +12,15 @@
 //      S^T = K Q^T        M = 128 positions (a thread each), N = 16 or 32 columns
 //      O^T = V^T P        M = 128 dims (a thread each, per half of 256), K = positions
 //    int8 sides on kind::i8 -- the sums of a block of 32 dims are exact, so its scale multiplies the sum -- and fp16 sides on kind::f16.
-//  * Against int8 keys a query is a whole number in three int8 planes, 24 bits (two, 16 bits, where that does not show: launch_of).  Against fp16 keys it is two fp16 terms.  Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the
-//    position's value scale, in two uint8 planes; for fp16 values two fp16 terms.  Sums of a tile are folded into fp32 registers.
+//  * Against int8 keys a query is a whole number in three int8 planes, 24 bits (two, 16 bits, where that does not show: launch_of).  Against fp16 keys it is two fp16 terms.
+//    Weights for int8 values are 16-bit fixed point relative to the tile's largest, times the position's value scale, in two uint8 planes (each is off by 2^-17 of the largest:
+//    1e-5 of an output, below fp16's rounding, and what fits the columns and two CTAs an SM); for fp16 values two fp16 terms.  Sums of a tile are folded into fp32
+//    registers.
 //  * A softmax thread has four query rows of a position; with five to eight rows a second group of 128 threads has the others.
 //  * Positions that no row sees weigh nothing and their values are cleared in shared memory where they are fp16 (0 x NaN is NaN), each by its own thread (by the warp that
 //    brings them, ahead of the next copies: 18 us a ragged tile), tiles that nobody sees
 //    (between the sinks and the window) are not in the list.
-// Measured, us: one token of 64 sequences of 512 to 16383 positions, 32 / 8 heads of 128, q8_0, pages of 64: 176 to 185 (5.9 TB/s; a tile a CTA 1.46, two CTAs an SM);
+// Measured, us: one token of 64 sequences of 512 to 16383 positions, 32 / 8 heads of 128, q8_0, pages of 64: 176 to 188 (5.7 TB/s; a tile a CTA 1.46, two CTAs an SM);
 // of 24 sequences under a window of 4096, 24 / 4 heads of 256, one scale a row, pages of 32: 53 (3.8 TB/s); of one sequence of 99: 10.2, of 74 of 100: 21, fp16 29.
 // Every wait is bounded: one that runs out poisons the CTA's results with NaN, sets a status bit, and the CTA ends in the normal way.
 #include "paged_decode.cuh"

@@ -52,3 +52,23 @@ def test_weights_over_keys_of_any_size(cuda, status, act, tokens, observe, d, he
     total = sum(tokens) + 1
     weigh(pool, rng.standard_normal((total, heads * group, d)).astype(act), tokens, 1.0e-7, window=0 if group > 1 else 70, sinks=3, observe=observe)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("d,mode,qblock,heads,group", [(128, 3, 32, 2, 4), (256, 3, 32, 1, 6), (128, 0, 128, 2, 7), (256, 1, 256, 1, 1), (256, 2, 32, 1, 3)])
+def test_attention_of_tokens_with_queries_and_scales_of_any_size(cuda, status, d, mode, qblock, heads, group):
+    """fp32 queries of 1e5 beside ones of 1 and 1e-6; scales of up to 6e4 beside ordinary ones.  The scores are of ordinary size by their scale."""
+    rng = np.random.default_rng(d + mode + group)
+    pool = po.Pool(rng, [300, 129, 64, 1], d=d, heads=heads, page=16, mode=mode, qblock=qblock)
+    for scales in (pool.ks, pool.vs):
+        if scales is not None:
+            scales[rng.random(scales.shape) < 0.05] = np.float16(6.0e4)
+    view = pool.upload()
+    batch, starts = po.batch_of(pool, [1, 1, 1, 1])
+    q = (rng.standard_normal((4, heads * group, d)) * rng.choice([1.0e5, 1.0e5, 1.0, 1.0e-6], (4, heads * group, 1))).astype(np.float32)
+    scale = 1.0e-5 * d ** -0.5 * (1.0 if pool.ks is None else 1.0e-6)
+    out, lse = torch.zeros(*q.shape, device="cuda"), torch.zeros(*q.shape[:2], device="cuda")
+    paged.launch_paged_attention(view, batch, to_dev(q), out, query_heads=heads * group, scale=scale, lse=lse, workspace=paged.paged_workspace(view, batch, heads * group))
+    want, want_lse, bound = po.attention(pool, q, starts, scale)
+    got = out.cpu().numpy().astype(np.float64)
+    assert (np.abs(got - want) <= bound).all(), np.abs(got - want).max()
+    assert np.allclose(lse.cpu().numpy(), want_lse, rtol=2.0 ** -18, atol=2.0 ** -17) and int(status) == 0
