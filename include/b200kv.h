@@ -71,7 +71,9 @@ typedef enum b200kv_status {
 #define B200KV_STATUS_PEER_TIMEOUT 4u   /* the cross-GPU merge never saw the partial of one of its peers */
 #define B200KV_STATUS_PIPE_TIMEOUT 8u   /* a tensor-core pipeline stage (MMA completion) never signalled */
 #define B200KV_STATUS_BAD_PAGE 16u      /* a page table named a page outside the pool (b200kv_paged_*; the page was not touched) */
-#define B200KV_STATUS_BAD_BOUND 32u     /* the sequences of a paged batch hold more than its host-side bounds say (b200kv_paged_batch) */
+#define B200KV_STATUS_BAD_BOUND 32u     /* the sequences of a paged batch hold more than its host-side bounds say (b200kv_paged_batch); an entry of a call that a table has no room for */
+#define B200KV_STATUS_BAD_SLOT 64u      /* an entry of a call named a sequence that there is not, that is not empty, or that an earlier entry named (b200kv_pages_*) */
+#define B200KV_STATUS_NO_PAGE 128u      /* a pool had too few free pages for an entry of a call (b200kv_pages_*) */
 
 /* KvCacheQuantMode, include/miinfer/prefill_v2/kv_cache.hpp:16-21 (same values). */
 typedef enum b200kv_quant_mode {
@@ -565,6 +567,89 @@ B200KV_API int b200kv_paged_weights(const b200kv_paged_view* view, const b200kv_
 B200KV_API int b200kv_paged_evict(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const int32_t* target_table, uint32_t target_max_pages,
                        const float* weights, uint32_t weights_stride, uint32_t keep, uint32_t sinks, uint32_t recent, int32_t* kept,
                        float* new_weights, int32_t* new_lengths, void* stream);
+
+/* ---- rotary positions of any of the usual forms, beside the store -------------------------------------------------------
+ *
+ * The angle of pair i of a head at position p is p f_i.  A frequency f_i comes as a 64-bit fraction of a turn, f_i / 2 pi modulo 1, so that p times it modulo 2^64 is the
+ * angle's, at any position. */
+typedef enum b200kv_rotary_layout {
+    B200KV_ROTARY_HALVES = 0,      /* pairs (i, i + dims / 2) */
+    B200KV_ROTARY_NEIGHBOURS = 1   /* pairs (2i, 2i + 1) */
+} b200kv_rotary_layout;
+/* How frequencies f_i = theta^(-2i / dims) are scaled for longer contexts. */
+typedef enum b200kv_rotary_kind {
+    B200KV_ROTARY_PLAIN = 0,
+    B200KV_ROTARY_LINEAR = 1,  /* f_i / factor (position interpolation) */
+    B200KV_ROTARY_BASE = 2,    /* theta * factor^(dims / (dims - 2)) in place of theta ("NTK-aware") */
+    B200KV_ROTARY_BANDS = 3,   /* f_i that turns fewer than `low` times in original_length positions: / factor; more than `high` times: as it is; between: w f_i + (1 - w) f_i / factor,
+                                  w = (times - low) / (high - low) */
+    B200KV_ROTARY_RAMP = 4     /* the same with w = 1 up to the pair that turns `high` times (rounded down), 0 from the one that turns `low` times on (rounded up), straight over i between;
+                                  magnitude 0.1 ln(factor) + 1 where factor > 1 (YaRN, Peng et al. 2023) */
+} b200kv_rotary_kind;
+typedef struct b200kv_rotary_scaling {
+    int kind;                /* b200kv_rotary_kind */
+    double factor;
+    double original_length;  /* BANDS, RAMP: positions the model was trained for */
+    double low, high;        /* BANDS, RAMP: 0 < low < high */
+} b200kv_rotary_scaling;
+/* turns[i] (HOST uint64 [dims / 2]) of the scaled frequencies (scaling may be NULL), and the factor for sines and cosines (may be NULL).  dims: a multiple of 16 up to 256;
+ * theta > 1.  Host only; the caller copies turns to the device. */
+B200KV_API int b200kv_rotary_turns(uint32_t dims, double theta, const b200kv_rotary_scaling* scaling, uint64_t* turns, float* magnitude);
+/* The same of frequencies of the caller's, in radians a position. */
+B200KV_API int b200kv_rotary_turns_of(const double* radians, uint32_t count, uint64_t* turns);
+
+typedef struct b200kv_rotary {
+    const uint64_t* turns;  /* DEVICE [dims / 2] */
+    uint32_t dims;          /* elements of a head that are rotated, the first ones: a multiple of 16 up to head_dim; 0: none */
+    uint32_t layout;        /* b200kv_rotary_layout */
+    float magnitude;        /* sines and cosines are multiplied by it */
+} b200kv_rotary;
+
+/* A layer's queries, keys and values of a ragged batch in one launch: K is normed (k_norm_weight, fp32 [head_dim], may be NULL), rotated, quantised and written into its pages
+ * as b200kv_paged_store does it, V quantised and written, and the queries, normed (q_norm_weight, may be NULL) and rotated, go to q_out, [total_tokens][query_heads][head_dim] of
+ * q_out_dtype.  q, key, value: rows of `dtype`, a token's head by head, the next token's `stride` elements on (columns of one matrix have its width as their stride).  gate
+ * (may be NULL): fp32 [total_tokens][query_heads][head_dim]; with it a head of q is a query and its gate, 2 head_dim elements, and gate gets the second ones.  key and
+ * value may both be NULL (queries only), or q and q_out (keys only).  A token's position is its place in the cache, or positions[t] (DEVICE int32 [total_tokens], may be NULL); a
+ * negative one counts as 0.  Rows of tokens that no sequence has are neither read nor written.  q, key, value, q_out and gate are 16-byte aligned, strides multiples of 16
+ * bytes.  q_out may be q, where its rows lie one behind the other in one type and there is no gate; what is written does not overlap what is read otherwise. */
+B200KV_API int b200kv_paged_rotary(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_rotary* rotary, const void* q, uint64_t q_stride, const void* key,
+                       uint64_t key_stride, const void* value, uint64_t value_stride, int dtype, const float* q_norm_weight, const float* k_norm_weight, float epsilon,
+                       const int32_t* positions, uint32_t query_heads, void* q_out, int q_out_dtype, float* gate, void* stream);
+
+/* ---- the book of a paged cache's pages ---------------------------------------------------------------------------------
+ *
+ * Which sequence holds which pages, and how many hold each, in device memory; one book serves the pools of all layers, which share its page numbers.  Its tables and
+ * lengths are those of a b200kv_paged_batch.  A page whose count is 0 is free.  Where a call needs pages it takes the lowest free ones, for its entries in order; an entry gets
+ * all that it needs or, as every later one that needs any, is left as it was (B200KV_STATUS_NO_PAGE).  Entries whose sequence is negative are left out; ones that a call
+ * cannot do are left out too, and set a status bit.  One call at a time changes a book or uses a workspace.  The calls can be captured. */
+typedef struct b200kv_page_book {
+    int32_t* refs;       /* DEVICE [pages], 16-byte aligned: who holds a page -- sequences, and whoever else adds to it; never negative */
+    int32_t* tables;     /* DEVICE [slots][max_pages]: entries past a sequence's pages are not looked at */
+    int32_t* lengths;    /* DEVICE [slots]: positions; 0 = an empty slot */
+    uint32_t pages;
+    uint32_t page_size;  /* 16, 32, 64, 128 or 256 */
+    uint32_t slots;      /* sequences there is room for, up to 8192 */
+    uint32_t max_pages;  /* of a sequence, up to 2^22 - 1 */
+} b200kv_page_book;
+
+B200KV_API size_t b200kv_pages_workspace_bytes(const b200kv_page_book* book);
+/* Room for add[e] (DEVICE int32 [count], 0 or more) further positions of sequence slots[e] (DEVICE int32 [count]): its length grows, fresh pages go into its table.  (Ahead of the
+ * store of a step, whose batch then reads the book's tables and lengths.)  A sequence is named once.  workspace: b200kv_pages_workspace_bytes, 16-byte aligned, contents of no
+ * consequence. */
+B200KV_API int b200kv_pages_grow(const b200kv_page_book* book, const int32_t* slots, const int32_t* add, uint32_t count, void* workspace, size_t workspace_bytes, void* stream);
+/* children[e], empty slots named once, go on from parents[e]: with all its positions, or the first at[e] (DEVICE int32 [count], at may be NULL).  Whole pages are shared, and their counts grow by
+ * one for each child; one that is not full is copied to a fresh page, in the pools of all layers.  So what a sequence still writes to is its own.  views: HOST [layers], up to
+ * 128 pools of one geometry with the book's pages.  All entries see the book as it was before the call. */
+B200KV_API int b200kv_pages_fork(const b200kv_page_book* book, const b200kv_paged_view* views, uint32_t layers, const int32_t* parents, const int32_t* children, const int32_t* at,
+                       uint32_t count, void* workspace, size_t workspace_bytes, void* stream);
+/* The sequences' slots become empty: length 0, their pages' counts less by one.  (A slot named twice is freed once, an empty one stays so.) */
+B200KV_API int b200kv_pages_free(const b200kv_page_book* book, const int32_t* slots, uint32_t count, void* stream);
+/* Moves the pages together: of n pages held, those at or above n go, in order, to the free ones below n, in the pools of all layers, with their counts, and the sequences' tables
+ * follow.  moved: DEVICE int32 [pages], where each page is now (-1: it was free), for whoever else keeps numbers of pages. */
+B200KV_API int b200kv_pages_compact(const b200kv_page_book* book, const b200kv_paged_view* views, uint32_t layers, int32_t* moved, void* workspace, size_t workspace_bytes, void* stream);
+/* Copies pages sources[i] of the pools `from` to pages targets[i] of the pools `to` (HOST [layers] each, one geometry; they may be the same pools), i < count (DEVICE int32 [count]).
+ * A negative target: nothing.  A target is named once, and no source is a target of the same pools. */
+B200KV_API int b200kv_pages_copy(const b200kv_paged_view* from, const b200kv_paged_view* to, uint32_t layers, const int32_t* sources, const int32_t* targets, uint32_t count, void* stream);
 
 /* ---- prefix snapshot / restore ---------------------------------------------
  * Raw compact layout of AttentionLayerKvCacheStorage::download_raw/upload_raw

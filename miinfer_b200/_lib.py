@@ -52,9 +52,34 @@ class PagedBatch(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    """b200kv_rotary: a table of rotary angles."""
+
+    device_index = -1      # likewise
+
+    _fields_ = [("turns", C.c_void_p), ("dims", C.c_uint32), ("layout", C.c_uint32), ("magnitude", C.c_float)]
+
+
+class RotaryScaling(C.Structure):
+    """b200kv_rotary_scaling."""
+
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("original_length", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class PageBook(C.Structure):
+    """b200kv_page_book: which sequence holds which pages."""
+
+    device_index = -1      # likewise
+
+    _fields_ = [
+        ("refs", C.c_void_p), ("tables", C.c_void_p), ("lengths", C.c_void_p),
+        ("pages", C.c_uint32), ("page_size", C.c_uint32), ("slots", C.c_uint32), ("max_pages", C.c_uint32),
+    ]
+
+
 u32, u64, sz, vp, fl, i32 = C.c_uint32, C.c_uint64, C.c_size_t, C.c_void_p, C.c_float, C.c_int
 VP = C.POINTER(View)
-PV, PB = C.POINTER(PagedView), C.POINTER(PagedBatch)
+PV, PB, PK = C.POINTER(PagedView), C.POINTER(PagedBatch), C.POINTER(PageBook)
 
 
 class PoolCounters(C.Structure):
@@ -126,6 +151,15 @@ SIGNATURES = {
     "b200kv_paged_attn": (i32, [PV, PB, vp, i32, vp, vp, i32, vp, u32, fl, u32, u32, vp, sz, vp]),
     "b200kv_paged_weights": (i32, [PV, PB, vp, i32, vp, vp, u32, u32, fl, u32, u32, u32, vp]),
     "b200kv_paged_evict": (i32, [PV, PB, vp, u32, vp, u32, u32, u32, u32, vp, vp, vp, vp]),
+    "b200kv_rotary_turns": (i32, [u32, C.c_double, C.POINTER(RotaryScaling), C.POINTER(u64), C.POINTER(fl)]),
+    "b200kv_rotary_turns_of": (i32, [C.POINTER(C.c_double), u32, C.POINTER(u64)]),
+    "b200kv_paged_rotary": (i32, [PV, PB, C.POINTER(Rotary), vp, u64, vp, u64, vp, u64, i32, vp, vp, fl, vp, u32, vp, i32, vp, vp]),
+    "b200kv_pages_workspace_bytes": (sz, [PK]),
+    "b200kv_pages_grow": (i32, [PK, vp, vp, u32, vp, sz, vp]),
+    "b200kv_pages_fork": (i32, [PK, PV, u32, vp, vp, vp, u32, vp, sz, vp]),
+    "b200kv_pages_free": (i32, [PK, vp, u32, vp]),
+    "b200kv_pages_compact": (i32, [PK, PV, u32, vp, vp, sz, vp]),
+    "b200kv_pages_copy": (i32, [PV, PV, u32, vp, vp, u32, vp]),
     "b200kv_snapshot_bytes": (sz, [VP, u64]),
     "b200kv_snapshot_save": (i32, [VP, u64, vp, vp]),
     "b200kv_snapshot_restore": (i32, [VP, u64, vp, vp]),
@@ -183,7 +217,7 @@ def load_native():
     spec = importlib.util.spec_from_file_location("_native", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.bind({"View": View, "PagedView": PagedView, "PagedBatch": PagedBatch, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
+    module.bind({"View": View, "PagedView": PagedView, "PagedBatch": PagedBatch, "Rotary": Rotary, "PageBook": PageBook, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
     return module
 
 

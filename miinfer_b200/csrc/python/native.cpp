@@ -35,12 +35,20 @@ struct Api {
     decltype(&b200kv_paged_attn) paged_attn;
     decltype(&b200kv_paged_weights) paged_weights;
     decltype(&b200kv_paged_evict) paged_evict;
+    decltype(&b200kv_paged_rotary) paged_rotary;
+    decltype(&b200kv_pages_grow) pages_grow;
+    decltype(&b200kv_pages_fork) pages_fork;
+    decltype(&b200kv_pages_free) pages_free;
+    decltype(&b200kv_pages_compact) pages_compact;
+    decltype(&b200kv_pages_copy) pages_copy;
     decltype(&b200kv_pool_capture) pool_capture;
     decltype(&b200kv_pool_restore) pool_restore;
 } g_api;
 PyObject* g_view_type;   // the ctypes structure of a cache view
 PyObject* g_paged_view_type;    // ... of a paged cache's view, and of a batch over it
 PyObject* g_paged_batch_type;
+PyObject* g_rotary_type;        // ... of a table of rotary angles
+PyObject* g_page_book_type;     // ... of the book of a paged cache's pages
 PyObject* g_device_index;       // the name of their attribute
 
 // One call's arguments, read left to right; the first failure sticks and leaves a Python exception set.
@@ -137,6 +145,42 @@ public:
     }
     const b200kv_paged_view* paged_view() { return structure<b200kv_paged_view>(g_paged_view_type, "a paged cache's view"); }
     const b200kv_paged_batch* paged_batch() { return structure<b200kv_paged_batch>(g_paged_batch_type, "a paged batch"); }
+    const b200kv_rotary* rotary() { return structure<b200kv_rotary>(g_rotary_type, "a table of rotary angles"); }
+    const b200kv_page_book* page_book() { return structure<b200kv_page_book>(g_page_book_type, "a page book"); }
+    // A list or tuple of paged views, one behind the other in `to`.
+    bool paged_views(std::vector<b200kv_paged_view>& to) {
+        if (!ok_) return false;
+        PyObject* list = args_[i_];
+        if (!PyList_Check(list) && !PyTuple_Check(list)) { fail(PyExc_TypeError, "expected a list of paged views"); return false; }
+        PyObject* const* const args = args_;
+        const Py_ssize_t at = i_ + 1;
+        for (Py_ssize_t k = 0; ok_ && k < PySequence_Fast_GET_SIZE(list); ++k) {
+            PyObject* item = PySequence_Fast_GET_ITEM(list, k);
+            args_ = &item;
+            i_ = 0;
+            if (const b200kv_paged_view* view = paged_view()) to.push_back(*view);
+            if (ok_) PyBuffer_Release(&buffers_[--held_]);   // copied
+        }
+        args_ = args;
+        i_ = at;
+        return ok_;
+    }
+    // Rows [at least `rows`][exactly `width`] of fp16 or fp32 whose elements lie one behind the other, or None; *stride: elements from a row to the next.
+    const void* strided(int* dtype, uint64_t rows, uint64_t width, uint64_t* stride, const char* text) {
+        if (!ok_) return nullptr;
+        PyObject* o = args_[i_++];
+        if (o == Py_None) return nullptr;
+        if (!THPVariable_Check(o)) return fail(PyExc_TypeError, "a torch tensor is required");
+        const at::Tensor& t = THPVariable_Unpack(o);
+        const auto type = t.scalar_type();
+        if (!t.is_cuda() || (type != at::kHalf && type != at::kFloat)) return fail(PyExc_ValueError, "expected a CUDA tensor of fp16 or fp32");
+        if (!here(o)) return nullptr;
+        if (t.dim() != 2 || static_cast<uint64_t>(t.size(0)) < rows || static_cast<uint64_t>(t.size(1)) != width || t.stride(1) != 1 || (t.size(0) > 1 && t.stride(0) < t.size(1)))
+            return fail(PyExc_ValueError, text);
+        *dtype = type == at::kHalf ? B200KV_F16 : B200KV_F32;
+        *stride = t.size(0) > 1 ? static_cast<uint64_t>(t.stride(0)) : width;
+        return t.data_ptr();
+    }
     // A tensor of one type and at least `least` elements, or None where that is allowed.
     template <typename T>
     T* exactly(at::ScalarType type, const char* text, uint64_t least, bool optional = false) {
@@ -233,7 +277,7 @@ private:
     Py_ssize_t i_ = 0;
     bool ok_ = true;
     int held_ = 0;
-    Py_buffer buffers_[2];
+    Py_buffer buffers_[4];
 };
 
 template <typename F>
@@ -466,6 +510,117 @@ PyObject* py_paged_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+PyObject* py_paged_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 14);
+    constexpr const char* kRows = "rows: [at least total_tokens][heads * head_dim, twice that for queries with gates], elements one behind the other";
+    int dtypes[3] = {-1, -1, -1}, od = B200KV_F16;
+    uint64_t strides[3] = {0, 0, 0};
+    const auto* view = a.paged_view();
+    const auto* batch = a.paged_batch();
+    const auto* rotary = a.rotary();
+    const uint32_t heads = a.u32();
+    const uint64_t tokens = a.ok() ? batch->total_tokens : 0, dim = a.ok() ? view->head_dim : 0, width = a.ok() ? view->kv_heads * dim : 0;
+    const void* key = a.strided(&dtypes[0], tokens, width, &strides[0], kRows);
+    const void* value = a.strided(&dtypes[1], tokens, width, &strides[1], kRows);
+    const void* q = a.strided(&dtypes[2], tokens, heads * dim * (a.ok() && args[7] != Py_None ? 2 : 1), &strides[2], kRows);
+    float* gate = a.exactly<float>(at::kFloat, kSmall, tokens * heads * dim, true);
+    void* out = nullptr;
+    if (a.ok() && args[8] != Py_None) out = a.activation(&od, tokens * heads * dim, kSmall);
+    else a.object();
+    const float* q_norm = a.exactly<const float>(at::kFloat, "a norm's weight: fp32 of head_dim elements", dim, true);
+    const float* k_norm = a.exactly<const float>(at::kFloat, "a norm's weight: fp32 of head_dim elements", dim, true);
+    const float epsilon = a.f32();
+    const int32_t* positions = a.exactly<const int32_t>(at::kInt, "positions: int32 of every token", tokens, true);
+    void* s = a.stream();
+    int dtype = -1;
+    for (const int d : dtypes) {
+        if (d < 0) continue;
+        if (a.ok() && dtype >= 0 && d != dtype) a.fail(PyExc_ValueError, "queries, keys and values must share a dtype");
+        dtype = d;
+    }
+    return call(a, [&] {
+        return g_api.paged_rotary(view, batch, rotary, q, strides[2], key, strides[0], value, strides[1], dtype, q_norm, k_norm, epsilon, positions, heads, out, od, gate, s);
+    });
+}
+
+// ---- the book of a paged cache's pages --------------------------------------------------------------------------
+
+constexpr const char* kEntries = "an int32 tensor of every entry";
+
+uint32_t entries(Args& a, PyObject* o) {   // of a call: the elements of its first array
+    if (!a.ok()) return 0;
+    if (!THPVariable_Check(o)) { a.fail(PyExc_TypeError, "a torch tensor is required"); return 0; }
+    const int64_t n = THPVariable_Unpack(o).numel();
+    if (n > 0x7fffffff) a.fail(PyExc_ValueError, "too many entries");
+    return a.ok() ? static_cast<uint32_t>(n) : 0;
+}
+void* workspace(Args& a, PyObject* o, size_t* bytes) {
+    void* ws = a.exactly<void>(at::kByte, "workspace: a uint8 tensor", 0, true);
+    if (a.ok() && ws != nullptr) *bytes = static_cast<size_t>(THPVariable_Unpack(o).numel());
+    return ws;
+}
+
+PyObject* py_pages_grow(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 5);
+    size_t bytes = 0;
+    const auto* book = a.page_book();
+    const uint32_t count = a.ok() ? entries(a, args[1]) : 0;
+    const int32_t* slots = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    const int32_t* add = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    void* ws = workspace(a, a.ok() ? args[3] : nullptr, &bytes);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.pages_grow(book, slots, add, count, ws, bytes, s); });
+}
+
+PyObject* py_pages_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 7);
+    size_t bytes = 0;
+    std::vector<b200kv_paged_view> views;
+    const auto* book = a.page_book();
+    a.paged_views(views);
+    const uint32_t count = a.ok() ? entries(a, args[2]) : 0;
+    const int32_t* parents = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    const int32_t* children = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    const int32_t* at = a.exactly<const int32_t>(at::kInt, kEntries, count, true);
+    void* ws = workspace(a, a.ok() ? args[5] : nullptr, &bytes);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.pages_fork(book, views.data(), static_cast<uint32_t>(views.size()), parents, children, at, count, ws, bytes, s); });
+}
+
+PyObject* py_pages_free(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 3);
+    const auto* book = a.page_book();
+    const uint32_t count = a.ok() ? entries(a, args[1]) : 0;
+    const int32_t* slots = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.pages_free(book, slots, count, s); });
+}
+
+PyObject* py_pages_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 5);
+    size_t bytes = 0;
+    std::vector<b200kv_paged_view> views;
+    const auto* book = a.page_book();
+    a.paged_views(views);
+    int32_t* moved = a.exactly<int32_t>(at::kInt, "moved: int32 of every page", a.ok() ? book->pages : 0);
+    void* ws = workspace(a, a.ok() ? args[3] : nullptr, &bytes);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.pages_compact(book, views.data(), static_cast<uint32_t>(views.size()), moved, ws, bytes, s); });
+}
+
+PyObject* py_pages_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n, 5);
+    std::vector<b200kv_paged_view> from, to;
+    a.paged_views(from);
+    a.paged_views(to);
+    if (a.ok() && from.size() != to.size()) a.fail(PyExc_ValueError, "as many views on both sides");
+    const uint32_t count = a.ok() ? entries(a, args[2]) : 0;
+    const int32_t* sources = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    const int32_t* targets = a.exactly<const int32_t>(at::kInt, kEntries, count);
+    void* s = a.stream();
+    return call(a, [&] { return g_api.pages_copy(from.data(), to.data(), static_cast<uint32_t>(from.size()), sources, targets, count, s); });
+}
+
 // ---- the snapshot pool: token ids and storage objects in, one library call ------------------------------------
 
 // Anything with a length that can be iterated over, as a list or tuple.
@@ -587,12 +742,13 @@ PyObject* py_pool(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return Py_BuildValue("iI", rc, CAPTURE ? static_cast<unsigned>(captured) : matched);
 }
 
-PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the structures "View", "PagedView" and "PagedBatch"
+PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the structures "View", "PagedView", "PagedBatch", "Rotary" and "PageBook"
     PyObject* view = PyDict_GetItemString(arg, "View");
     if (view == nullptr || !PyType_Check(view)) return PyErr_Format(PyExc_KeyError, "View");
     Py_INCREF(view);
     Py_XSETREF(g_view_type, view);
-    for (auto [name, slot] : {std::pair{"PagedView", &g_paged_view_type}, std::pair{"PagedBatch", &g_paged_batch_type}}) {
+    for (auto [name, slot] : {std::pair{"PagedView", &g_paged_view_type}, std::pair{"PagedBatch", &g_paged_batch_type}, std::pair{"Rotary", &g_rotary_type},
+                              std::pair{"PageBook", &g_page_book_type}}) {
         PyObject* type = PyDict_GetItemString(arg, name);
         if (type == nullptr || !PyType_Check(type)) return PyErr_Format(PyExc_KeyError, "%s", name);
         Py_INCREF(type);
@@ -610,6 +766,12 @@ PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the stru
         {"b200kv_paged_attn", reinterpret_cast<void**>(&g_api.paged_attn)},
         {"b200kv_paged_weights", reinterpret_cast<void**>(&g_api.paged_weights)},
         {"b200kv_paged_evict", reinterpret_cast<void**>(&g_api.paged_evict)},
+        {"b200kv_paged_rotary", reinterpret_cast<void**>(&g_api.paged_rotary)},
+        {"b200kv_pages_grow", reinterpret_cast<void**>(&g_api.pages_grow)},
+        {"b200kv_pages_fork", reinterpret_cast<void**>(&g_api.pages_fork)},
+        {"b200kv_pages_free", reinterpret_cast<void**>(&g_api.pages_free)},
+        {"b200kv_pages_compact", reinterpret_cast<void**>(&g_api.pages_compact)},
+        {"b200kv_pages_copy", reinterpret_cast<void**>(&g_api.pages_copy)},
         {"b200kv_pool_capture", reinterpret_cast<void**>(&g_api.pool_capture)},
         {"b200kv_pool_restore", reinterpret_cast<void**>(&g_api.pool_restore)},
     };
@@ -651,6 +813,12 @@ PyMethodDef g_methods[] = {{"bind", py_bind, METH_O, nullptr},
                            ENTRY("paged_attn", py_paged_attn),
                            ENTRY("paged_weights", py_paged_weights),
                            ENTRY("paged_evict", py_paged_evict),
+                           ENTRY("paged_rotary", py_paged_rotary),
+                           ENTRY("pages_grow", py_pages_grow),
+                           ENTRY("pages_fork", py_pages_fork),
+                           ENTRY("pages_free", py_pages_free),
+                           ENTRY("pages_compact", py_pages_compact),
+                           ENTRY("pages_copy", py_pages_copy),
                            ENTRY("pool_capture", py_pool<true>),
                            ENTRY("pool_restore", py_pool<false>),
                            {nullptr, nullptr, 0, nullptr}};

@@ -12,7 +12,8 @@ Argument errors raise B200KvError or ValueError.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+import enum
+from typing import Optional, Sequence
 
 import torch
 
@@ -21,9 +22,11 @@ from ._lib import check, lib, native
 from .kv import KvCacheQuantMode, RopeMode
 
 __all__ = ["PagedView", "PagedBatch", "PagedKvCache", "paged_workspace", "launch_paged_store", "launch_paged_load", "launch_paged_attention",
-           "launch_paged_weights", "launch_paged_evict", "STATUS_BAD_PAGE", "STATUS_BAD_BOUND"]
+           "launch_paged_weights", "launch_paged_evict", "RotaryLayout", "RotaryScaling", "RotaryTable", "launch_paged_rotary", "PageBook", "pages_workspace",
+           "launch_pages_grow", "launch_pages_fork", "launch_pages_free", "launch_pages_compact", "launch_pages_copy", "STATUS_BAD_PAGE", "STATUS_BAD_BOUND",
+           "STATUS_BAD_SLOT", "STATUS_NO_PAGE"]
 
-STATUS_BAD_PAGE, STATUS_BAD_BOUND = 16, 32      # bits of the word registered with kv.set_status_word
+STATUS_BAD_PAGE, STATUS_BAD_BOUND, STATUS_BAD_SLOT, STATUS_NO_PAGE = 16, 32, 64, 128      # bits of the word registered with kv.set_status_word
 
 
 class PagedView(_lib.PagedView):
@@ -159,3 +162,125 @@ def launch_paged_evict(view: PagedView, batch: PagedBatch, target_table: torch.T
     rc = native.paged_evict(view, batch, keep, sinks, recent, target_table, weights, kept, new_weights, new_lengths, stream)
     if rc:
         check(rc, "b200kv_paged_evict")
+
+
+class RotaryLayout(enum.IntEnum):
+    """b200kv_rotary_layout: pairs (i, i + dims / 2) or (2i, 2i + 1)."""
+
+    HALVES = 0
+    NEIGHBOURS = 1
+
+
+class RotaryScaling(enum.IntEnum):
+    """b200kv_rotary_kind: how the frequencies are scaled for longer contexts."""
+
+    NONE = 0
+    LINEAR = 1
+    BASE = 2
+    BANDS = 3
+    RAMP = 4
+
+
+class RotaryTable(_lib.Rotary):
+    """b200kv_rotary with its table on the device: the frequencies theta^(-2i / dims), scaled, or `frequencies` (radians a position, dims / 2 of them).
+
+    factor: of every scaling; original_length, low, high: of BANDS and RAMP.  magnitude: what sines and cosines are multiplied by (the default: the scaling's own)."""
+
+    def __init__(self, dims: int, *, theta: float = 1.0e6, layout: RotaryLayout = RotaryLayout.HALVES, scaling: RotaryScaling = RotaryScaling.NONE, factor: float = 1.0,
+                 original_length: float = 0.0, low: float = 1.0, high: float = 32.0, frequencies: Optional[Sequence[float]] = None, magnitude: Optional[float] = None,
+                 device: Optional[torch.device] = None):
+        if not 0 < int(dims) <= 256 or int(dims) % 16:
+            raise ValueError("dims: a multiple of 16 up to 256")
+        turns, of_scaling = (C.c_uint64 * (dims // 2))(), C.c_float(1.0)
+        if frequencies is not None:
+            if len(frequencies) != dims // 2 or RotaryScaling(scaling) != RotaryScaling.NONE:
+                raise ValueError("frequencies: one for every pair, as they are")
+            check(lib.b200kv_rotary_turns_of((C.c_double * len(frequencies))(*map(float, frequencies)), len(frequencies), turns), "b200kv_rotary_turns_of")
+        else:
+            how = _lib.RotaryScaling(int(RotaryScaling(scaling)), factor, original_length, low, high)
+            check(lib.b200kv_rotary_turns(dims, theta, C.byref(how), turns, C.byref(of_scaling)), "b200kv_rotary_turns")
+        self.table = torch.frombuffer(bytearray(bytes(turns)), dtype=torch.int64).to(device or torch.device("cuda", torch.cuda.current_device()))
+        super().__init__(self.table.data_ptr(), int(dims), int(RotaryLayout(layout)), of_scaling.value if magnitude is None else float(magnitude))
+        self.device_index = self.table.device.index
+
+
+def launch_paged_rotary(view: PagedView, batch: PagedBatch, rotary: RotaryTable, key: Optional[torch.Tensor], value: Optional[torch.Tensor], q: Optional[torch.Tensor] = None,
+                        q_out: Optional[torch.Tensor] = None, *, query_heads: int = 0, gate: Optional[torch.Tensor] = None, q_norm_weight: Optional[torch.Tensor] = None,
+                        k_norm_weight: Optional[torch.Tensor] = None, epsilon: float = 1.0e-6, positions: Optional[torch.Tensor] = None,
+                        stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Norms and rotates a batch's queries and keys, and writes keys and values into their pages.  q [total_tokens][query_heads * head_dim], key and value [total_tokens]
+    [kv_heads * head_dim]: fp16 or fp32, rows of any stride, such as columns of one matrix.  q_out: fp16 or fp32 [total_tokens][query_heads][head_dim], or q itself.  With gate (fp32
+    [total_tokens][query_heads][head_dim]) a head of q is a query and its gate, and gate gets the second.  key and value may be None, or q and q_out."""
+    if q is not None and query_heads <= 0:
+        raise ValueError("query_heads is required with q")
+    rc = native.paged_rotary(view, batch, rotary, query_heads, key, value, q, gate, q_out, q_norm_weight, k_norm_weight, epsilon, positions, stream)
+    if rc:
+        check(rc, "b200kv_paged_rotary")
+
+
+class PageBook(_lib.PageBook):
+    """b200kv_page_book over int32 CUDA tensors: refs [pages], tables [slots][max_pages], lengths [slots].  One book serves the pools of all layers; tables and lengths are what
+    a PagedBatch takes."""
+
+    def __init__(self, refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, *, page_size: int):
+        if refs.dim() != 1 or tables.dim() != 2 or lengths.dim() != 1 or tables.shape[0] != lengths.shape[0]:
+            raise ValueError("refs [pages], tables [slots][max_pages], lengths [slots]")
+        for t in (refs, tables, lengths):
+            if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.device != refs.device:
+                raise ValueError("expected contiguous int32 CUDA tensors of one device")
+        super().__init__(refs.data_ptr(), tables.data_ptr(), lengths.data_ptr(), refs.numel(), int(page_size), lengths.numel(), tables.shape[1])
+        self.tensors, self.device_index = (refs, tables, lengths), refs.device.index
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, slots: int, max_pages: int, device: Optional[torch.device] = None) -> "PageBook":
+        dev = device or torch.device("cuda", torch.cuda.current_device())
+        return cls(torch.zeros(pages, dtype=torch.int32, device=dev), torch.full((slots, max_pages), -1, dtype=torch.int32, device=dev),
+                   torch.zeros(slots, dtype=torch.int32, device=dev), page_size=page_size)
+
+    refs_tensor = property(lambda self: self.tensors[0])
+    tables_tensor = property(lambda self: self.tensors[1])
+    lengths_tensor = property(lambda self: self.tensors[2])
+
+
+def pages_workspace(book: PageBook, device=None) -> torch.Tensor:
+    """Scratch for launch_pages_* calls on this book."""
+    n = int(lib.b200kv_pages_workspace_bytes(C.byref(book)))
+    return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def launch_pages_grow(book: PageBook, slots: torch.Tensor, add: torch.Tensor, *, workspace: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Room for add[e] further positions of sequence slots[e] (int32 each): the lowest free pages, entry by entry."""
+    rc = native.pages_grow(book, slots, add, workspace, stream)
+    if rc:
+        check(rc, "b200kv_pages_grow")
+
+
+def launch_pages_fork(book: PageBook, views: Sequence[PagedView], parents: torch.Tensor, children: torch.Tensor, *, at: Optional[torch.Tensor] = None, workspace: torch.Tensor,
+                      stream: Optional[torch.cuda.Stream] = None) -> None:
+    """The empty slots children[e] go on from parents[e] (int32 each), with all its positions or the first at[e]: whole pages are shared, a last one that is not full is copied in
+    the pools of all layers (`views`)."""
+    rc = native.pages_fork(book, views, parents, children, at, workspace, stream)
+    if rc:
+        check(rc, "b200kv_pages_fork")
+
+
+def launch_pages_free(book: PageBook, slots: torch.Tensor, *, stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Sequences end: their slots (int32) become empty, their pages are given back."""
+    rc = native.pages_free(book, slots, stream)
+    if rc:
+        check(rc, "b200kv_pages_free")
+
+
+def launch_pages_compact(book: PageBook, views: Sequence[PagedView], moved: torch.Tensor, *, workspace: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Moves the pages that are held together at the front of the pools of all layers; moved (int32 [pages]): where each is now, -1 for one that was free."""
+    rc = native.pages_compact(book, views, moved, workspace, stream)
+    if rc:
+        check(rc, "b200kv_pages_compact")
+
+
+def launch_pages_copy(from_views: Sequence[PagedView], to_views: Sequence[PagedView], sources: torch.Tensor, targets: torch.Tensor, *,
+                      stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Copies pages sources[i] of one set of pools to pages targets[i] of another of the same geometry (int32 each; a negative target: nothing)."""
+    rc = native.pages_copy(from_views, to_views, sources, targets, stream)
+    if rc:
+        check(rc, "b200kv_pages_copy")
