@@ -549,6 +549,25 @@ B200KV_API int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_pag
                       void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same with scores and sights of other models.  With x = scale * q.k of a token at place i of its sequence and position j:
+ *   score = c - slopes[head] * |i - j|,  c = cap * tanh(x / cap) where cap > 0 (from 1e-6 to 1e6), x where it is 0;
+ * with ranges, token t sees j in [ranges[t][0], ranges[t][1]) in place of j <= i: a document that begins at position d is [d, i + 1) for its tokens, a prefix of n positions
+ * that sees itself in both directions [0, n), and [0, i + 1) behind it.  A window cuts a range as it cuts j <= i; the first `sinks` positions, which count with a window or with ranges, are
+ * seen by every token whose range does not end before them.  What lies past a sequence's length is never seen.  slopes: finite.  Cache rows from the lowest position that any of a
+ * sequence's new tokens sees up to the last one are finite, whether or not a range leaves them out in between, and so are the sinks; rows outside may hold anything.  Tiles of
+ * positions that nobody sees are neither read nor computed.  lse is that of the scores; over fp16 keys with fp32 queries and a cap a longer sequence's is as good as over int8 keys.  (It is not one for
+ * b200kv_paged_weights, which knows scores without a cap, a bias or ranges only.)  A scoring of nothing at all is b200kv_paged_attn. */
+typedef struct b200kv_paged_scoring {
+    float cap;
+    const float* slopes;    /* DEVICE [query_heads], may be NULL */
+    const int32_t* ranges;  /* DEVICE [total_tokens][2], 8-byte aligned, may be NULL */
+} b200kv_paged_scoring;
+B200KV_API size_t b200kv_paged_attn_scored_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring,
+                       uint32_t query_heads, uint32_t window, uint32_t sinks);
+B200KV_API int b200kv_paged_attn_scored(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring, const void* q, int q_dtype,
+                      const float* gate, void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* Adds to weights[s][kv_head][j] the weight that position j gets from sequence s's new tokens: sum of exp(score - lse) over them and over the query
  * heads of the kv head.  weights: fp32 [sequences][kv_heads][weights_stride], weights_stride >= max_length; entries at and past a
  * length are left alone.  q, lse, scale, window and sinks as in the b200kv_paged_attn call that produced lse.  observe > 0: only the last `observe`

@@ -52,6 +52,14 @@ class PagedBatch(C.Structure):
     ]
 
 
+class PagedScoring(C.Structure):
+    """b200kv_paged_scoring: what becomes of an attention call's scores, and who sees what."""
+
+    device_index = -1      # likewise
+
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("ranges", C.c_void_p)]
+
+
 class Rotary(C.Structure):
     """b200kv_rotary: a table of rotary angles."""
 
@@ -79,7 +87,7 @@ class PageBook(C.Structure):
 
 u32, u64, sz, vp, fl, i32 = C.c_uint32, C.c_uint64, C.c_size_t, C.c_void_p, C.c_float, C.c_int
 VP = C.POINTER(View)
-PV, PB, PK = C.POINTER(PagedView), C.POINTER(PagedBatch), C.POINTER(PageBook)
+PV, PB, PK, PS = C.POINTER(PagedView), C.POINTER(PagedBatch), C.POINTER(PageBook), C.POINTER(PagedScoring)
 
 
 class PoolCounters(C.Structure):
@@ -149,6 +157,8 @@ SIGNATURES = {
     "b200kv_paged_load": (i32, [PV, PB, vp, vp, vp]),
     "b200kv_paged_attn_workspace_bytes": (sz, [PV, PB, u32, u32, u32]),
     "b200kv_paged_attn": (i32, [PV, PB, vp, i32, vp, vp, i32, vp, u32, fl, u32, u32, vp, sz, vp]),
+    "b200kv_paged_attn_scored_workspace_bytes": (sz, [PV, PB, PS, u32, u32, u32]),
+    "b200kv_paged_attn_scored": (i32, [PV, PB, PS, vp, i32, vp, vp, i32, vp, u32, fl, u32, u32, vp, sz, vp]),
     "b200kv_paged_weights": (i32, [PV, PB, vp, i32, vp, vp, u32, u32, fl, u32, u32, u32, vp]),
     "b200kv_paged_evict": (i32, [PV, PB, vp, u32, vp, u32, u32, u32, u32, vp, vp, vp, vp]),
     "b200kv_rotary_turns": (i32, [u32, C.c_double, C.POINTER(RotaryScaling), C.POINTER(u64), C.POINTER(fl)]),
@@ -217,7 +227,7 @@ def load_native():
     spec = importlib.util.spec_from_file_location("_native", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.bind({"View": View, "PagedView": PagedView, "PagedBatch": PagedBatch, "Rotary": Rotary, "PageBook": PageBook, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
+    module.bind({"View": View, "PagedView": PagedView, "PagedBatch": PagedBatch, "PagedScoring": PagedScoring, "Rotary": Rotary, "PageBook": PageBook, **{name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}})
     return module
 
 

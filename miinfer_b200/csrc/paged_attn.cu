@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace b200kv {
 
@@ -43,9 +44,24 @@ struct PrepareParams {
     uint32_t few_rows;          // sequences of at most so many query rows are the other kernel's
     ChunkCosts costs;
     __half* out[2];             // the copy, K and V: [kv_head][scratch_tiles * kChunkTile][D]
+    // tokens with ranges of their own: {lowest position seen, one behind the last} of every row tile (chunk_slot) and of every sequence of the chunk kernel's; the sinks aside
+    const int32_t* ranges;
+    uint2* tile_bounds;
+    uint2* bounds;
     __device__ __forceinline__ bool mine(const Span& span) const { return span.tokens > 0 && static_cast<uint64_t>(span.tokens) * group > few_rows; }
     __device__ __forceinline__ uint32_t row_tiles(const Span& span) const { return (span.tokens * group + kChunkRows - 1) / kChunkRows; }
 };
+
+// Where a sequence's tiles lie.
+template <bool RANGED>
+__device__ __forceinline__ ChunkTiles tiles_of(const PrepareParams& p, const Span& span, uint32_t s) {
+    if constexpr (RANGED) {
+        const uint2 b = p.bounds[s];
+        return chunk_tiles_between(b.x, b.y, p.sinks);
+    } else {
+        return chunk_tiles(span.base(), span.length, p.window, p.sinks);
+    }
+}
 
 struct Sums { uint32_t a, b, c; };
 __device__ __forceinline__ Sums add(const Sums& x, const Sums& y) { return {x.a + y.a, x.b + y.b, x.c + y.c}; }
@@ -106,6 +122,15 @@ __device__ __forceinline__ Walk walk_of(const PrepareParams& p, const Span& span
     return w;
 }
 
+// The same from a row tile's bounds.
+__device__ __forceinline__ Walk walk_between(const PrepareParams& p, const uint2& b, const ChunkTiles& t) {
+    const uint32_t upto = (b.y + kChunkTile - 1) / kChunkTile, sink = (min(p.sinks, b.y) + kChunkTile - 1) / kChunkTile;
+    const uint32_t first = min(b.x / kChunkTile, upto), own0 = t.window0 / kChunkTile;   // (bounds of rows that see nothing: first == upto)
+    if (own0 == 0) return first <= sink ? Walk{upto, 0} : Walk{sink + upto - first, first - sink};
+    const uint32_t skip = max(first, own0) - own0;
+    return {t.sink_tiles + (upto > own0 + skip ? upto - own0 - skip : 0), skip};
+}
+
 struct PlanScratch {
     Sums scan[kPrepareThreads / 32];
     uint32_t items[kCandidates], parts[kCandidates], longest, piece;
@@ -113,6 +138,7 @@ struct PlanScratch {
 };
 
 // The list of the chunk kernel's CTAs; one block.
+template <bool RANGED>
 __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* tile_starts, const uint32_t* scratch_starts, PlanScratch& sh) {
     const uint32_t tid = threadIdx.x, S = p.pool.batch.sequences, H = p.pool.view.kv_heads, row_tiles = tile_starts[S];
     if (tid == 0) p.plan->items = p.plan->groups = 0;
@@ -125,19 +151,47 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0; }
     __syncthreads();
-    for (uint32_t s = tid; s < S; s += kPrepareThreads)
-        if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
+    const auto walk_in = [&](uint32_t i, uint32_t* sequence, ChunkTiles* tiles) {   // RANGED: of row tile i of all
+        const uint32_t s = last_from(tile_starts, S, i);
+        const Span span = span_of(p.pool, s);
+        *sequence = s;
+        *tiles = tiles_of<true>(p, span, s);
+        return walk_between(p, p.tile_bounds[chunk_slot(span.first, p.group, s, tile_starts[s + 1] - 1 - i)], *tiles);
+    };
+    if constexpr (RANGED) {   // row tiles differ by more than their place
+        for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
+            uint32_t s;
+            ChunkTiles t;
+            const uint32_t n = walk_in(i, &s, &t).tiles;
+            atomicMax(&sh.longest, n);
+            atomicAdd(&sh.work, 128ull * n * H);
+        }
+    } else {
+        for (uint32_t s = tid; s < S; s += kPrepareThreads)
+            if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
+    }
     __syncthreads();
     const uint32_t longest = sh.longest;
     const auto piece_of = [&](uint32_t c) { return max(3u, (3 * longest + c + 2) / (c + 3)); };
-    for (uint32_t s = tid; s < S; s += kPrepareThreads) {
-        const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
-        if (n == 0) continue;
-        atomicAdd(&sh.work, chunk_work(n, tiles, span_of(p.pool, s).tokens));
+    const auto count = [&](uint32_t n, uint32_t tiles) {
         for (uint32_t c = 0; c < kCandidates; ++c) {
             const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
             atomicAdd(&sh.items[c], n * pieces);
             if (pieces > 1) atomicAdd(&sh.parts[c], n * pieces);
+        }
+    };
+    if constexpr (RANGED) {
+        for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
+            uint32_t s;
+            ChunkTiles t;
+            count(H, walk_in(i, &s, &t).tiles);
+        }
+    } else {
+        for (uint32_t s = tid; s < S; s += kPrepareThreads) {
+            const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
+            if (n == 0) continue;
+            atomicAdd(&sh.work, chunk_work(n, tiles, span_of(p.pool, s).tokens));
+            count(n, tiles);
         }
     }
     __syncthreads();
@@ -167,15 +221,17 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         if (i < row_tiles) {
             const uint32_t s = last_from(tile_starts, S, i);
             const Span span = span_of(p.pool, s);
-            const ChunkTiles t = chunk_tiles(span.base(), span.length, p.window, p.sinks);
+            const ChunkTiles t = tiles_of<RANGED>(p, span, s);
             item.first = span.first;
             item.tokens = span.tokens;
             item.base = span.base();
+            item.length = span.length;
             item.row_tile = tile_starts[s + 1] - 1 - i;
-            walk = walk_of(p, span, t, item.row_tile);
+            if constexpr (RANGED) walk = walk_between(p, p.tile_bounds[chunk_slot(span.first, p.group, s, item.row_tile)], t);
+            else walk = walk_of(p, span, t, item.row_tile);
             if (scratch_starts[s] + t.tiles > p.scratch_tiles) walk.tiles = 0;   // no room for the copy
             item.scratch_row = scratch_starts[s] * kChunkTile;
-            const uint32_t sink = p.window > 0 ? (p.sinks + kChunkTile - 1) / kChunkTile : 0;
+            const uint32_t sink = RANGED || p.window > 0 ? (p.sinks + kChunkTile - 1) / kChunkTile : 0;
             item.sink_tiles = t.window0 == 0 ? min(sink, walk.tiles) : t.sink_tiles;
             item.window0 = t.window0 == 0 ? item.sink_tiles * kChunkTile : t.window0;
             item.skip = walk.skip;
@@ -209,7 +265,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
 }
 
 // A unit of the gather: a tile of 64 positions of one side of one kv head.
-template <int D>
+template <int D, bool RANGED>
 __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32_t* scratch_starts, uint32_t unit) {
     constexpr uint32_t CPR = D / 8, kEach = kChunkTile * CPR / kPrepareThreads;   // 16-byte pieces of a row of the copy; a thread's of a tile
     const Paged& pool = p.pool;
@@ -217,7 +273,9 @@ __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32
     const uint32_t side = unit & 1, head = (unit >> 1) % H, tile = (unit >> 1) / H;
     const uint32_t s = last_from(scratch_starts, pool.batch.sequences, tile);
     const Span span = span_of(pool, s);
-    const ChunkTiles t = chunk_tiles(span.base(), span.length, p.window, p.sinks);
+    const ChunkTiles t = tiles_of<RANGED>(p, span, s);
+    uint2 bounds = make_uint2(0, 0);
+    if constexpr (RANGED) bounds = p.bounds[s];
     const uint32_t u = tile - scratch_starts[s];
     const uint32_t pos0 = u < t.sink_tiles ? u * kChunkTile : t.window0 + (u - t.sink_tiles) * kChunkTile;
     const bool q8 = side == 0 ? is_k_q8(pool.view.quant_mode) : is_v_q8(pool.view.quant_mode);
@@ -233,7 +291,9 @@ __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32
         const uint32_t j = pos0 + threadIdx.x / CPR + i * (kPrepareThreads / CPR);
         v[i] = make_uint4(0, 0, 0, 0);
         scale[i] = __ushort_as_half(0);
-        const bool seen = j < span.length && (p.window == 0 || j < p.sinks || static_cast<int>(j + p.window) > span.base());   // by any of the tokens
+        bool seen;   // by any of the tokens
+        if constexpr (RANGED) seen = j < bounds.y && (j >= bounds.x || j < p.sinks);
+        else seen = j < span.length && (p.window == 0 || j < p.sinks || static_cast<int>(j + p.window) > span.base());
         const long long row = seen ? row_of(pool, s, head, j) : -1;
         if (row < 0) continue;   // zeros (a weight of 0 times what lies there would still be NaN where that is)
         const size_t at = static_cast<size_t>(row) * D + c * 8;
@@ -251,7 +311,39 @@ __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32
             q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
 }
 
-template <int D>
+// What the tokens of each row tile and of each sequence see, the sinks aside: a block a sequence, a warp a row tile at a time.
+constexpr int kBoundsThreads = 512;
+__global__ void __launch_bounds__(kBoundsThreads) paged_bounds_kernel(const __grid_constant__ PrepareParams p) {
+    __shared__ uint32_t lowest, end;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t s = blockIdx.x, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) { lowest = 0xffffffffu; end = 0; }
+    __syncthreads();
+    const Span span = span_of(p.pool, s);
+    if (!p.mine(span)) return;
+    const uint32_t rows = span.tokens * p.group, row_tiles = p.row_tiles(span);
+    for (uint32_t r = threadIdx.x / 32; r < row_tiles; r += kBoundsThreads / 32) {
+        const uint32_t t_last = min((r + 1) * kChunkRows - 1, rows - 1) / p.group;
+        uint32_t low = 0xffffffffu, upto = 0;
+        for (uint32_t t = r * kChunkRows / p.group + lane; t <= t_last; t += 32) {
+            const Sight sight = sight_of(p.ranges, span.first + t, span.base() + static_cast<int>(t), p.window, span.length);
+            if (!sight.empty()) low = min(low, sight.low);
+            upto = max(upto, sight.empty() ? min(sight.upto, p.sinks) : sight.upto);
+        }
+        low = __reduce_min_sync(0xffffffffu, low);
+        upto = __reduce_max_sync(0xffffffffu, upto);
+        if (lane == 0) {
+            p.tile_bounds[chunk_slot(span.first, p.group, s, r)] = make_uint2(low, upto);
+            atomicMin(&lowest, low);
+            atomicMax(&end, upto);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.bounds[s] = make_uint2(lowest, end);
+}
+
+template <int D, bool RANGED>
 __global__ void __launch_bounds__(kPrepareThreads) paged_prepare_kernel(const __grid_constant__ PrepareParams p) {
     extern __shared__ uint32_t starts[];   // row tiles, then tiles of the copy, before every sequence
     __shared__ PlanScratch sh;
@@ -268,7 +360,7 @@ __global__ void __launch_bounds__(kPrepareThreads) paged_prepare_kernel(const __
             const Span span = span_of(p.pool, s);
             if (p.mine(span)) {
                 v.a = p.row_tiles(span);
-                v.b = chunk_tiles(span.base(), span.length, p.window, p.sinks).tiles;
+                v.b = tiles_of<RANGED>(p, span, s).tiles;
             }
         }
         Sums total;
@@ -287,11 +379,11 @@ __global__ void __launch_bounds__(kPrepareThreads) paged_prepare_kernel(const __
     }
     __syncthreads();
     if (blockIdx.x == 0) {
-        lay_out(p, tile_starts, scratch_starts, sh);
+        lay_out<RANGED>(p, tile_starts, scratch_starts, sh);
         return;
     }
     const uint32_t units = scratch_starts[S] * p.pool.view.kv_heads * 2;
-    for (uint32_t unit = blockIdx.x - 1; unit < units; unit += gridDim.x - 1) gather_unit<D>(p, scratch_starts, unit);
+    for (uint32_t unit = blockIdx.x - 1; unit < units; unit += gridDim.x - 1) gather_unit<D, RANGED>(p, scratch_starts, unit);
 }
 
 struct ChunkMergeParams {
@@ -420,12 +512,12 @@ struct Room {
     uint64_t scratch_tiles;    // of all sequences together
     uint32_t max_items, max_parts;
     bool decode, chunks;       // which kernels the call may need
-    size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, bytes;   // offsets
+    size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, tile_bounds, bounds, bytes;   // offsets
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uint32_t query_heads, uint32_t window, uint32_t sinks, uint32_t sms) {
+Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uint32_t query_heads, uint32_t window, uint32_t sinks, bool ranged, uint32_t sms) {
     Room r{};
     const uint64_t group = query_heads / view.kv_heads;
     // A single sequence goes by its bound: the chunk kernel takes a token as well, and the other's launch is saved.
@@ -461,6 +553,10 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.v = r.mean_key = take(is_k_q8(view.quant_mode) ? plane : std::max(plane, static_cast<uint64_t>(batch.total_tokens) * query_heads * view.head_dim * sizeof(__half)));
     r.part_o = take(parts * kChunkRows * view.head_dim * sizeof(float));
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
+    if (ranged) {
+        r.tile_bounds = take((batch.total_tokens * group / kChunkRows + batch.sequences + 1) * sizeof(uint2));
+        r.bounds = take(static_cast<uint64_t>(batch.sequences) * sizeof(uint2));
+    }
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
     return r;
 }
@@ -471,17 +567,24 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
 
 using namespace b200kv;
 
-extern "C" {
+namespace {
 
-size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window, uint32_t sinks) {
-    if (view == nullptr || batch == nullptr || view->kv_heads == 0 || query_heads == 0 || query_heads % view->kv_heads != 0) return 0;
-    settle_window(*batch, &window, &sinks);
-    return room_of(*view, *batch, query_heads, window, sinks, kMostSms).bytes;
+// Without scoring (null) nothing but the window cuts what a token sees.
+void settle(const b200kv_paged_batch& batch, const b200kv_paged_scoring* scoring, uint32_t* window, uint32_t* sinks) {
+    const uint32_t most = std::min(*sinks, batch.max_length);
+    settle_window(batch, window, sinks);
+    if (scoring != nullptr && scoring->ranges != nullptr) *sinks = most;
 }
 
-int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* gate,
-                      void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
-                      void* workspace, size_t workspace_bytes, void* stream) {
+size_t workspace_of(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring, uint32_t query_heads, uint32_t window, uint32_t sinks) {
+    if (view == nullptr || batch == nullptr || view->kv_heads == 0 || query_heads == 0 || query_heads % view->kv_heads != 0) return 0;
+    settle(*batch, scoring, &window, &sinks);
+    return room_of(*view, *batch, query_heads, window, sinks, scoring != nullptr && scoring->ranges != nullptr, kMostSms).bytes;
+}
+
+int attend(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring, const void* q, int q_dtype, const float* gate,
+           void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+           void* workspace, size_t workspace_bytes, void* stream) {
     int rc = validate_paged(view, batch);
     if (rc != B200KV_OK) return rc;
     if (q == nullptr || output == nullptr || (q_dtype != B200KV_F16 && q_dtype != B200KV_F32) || (output_dtype != B200KV_F16 && output_dtype != B200KV_F32)) return B200KV_ERR_INVALID;
@@ -492,15 +595,21 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     if (query_heads / view->kv_heads > 8) return B200KV_ERR_UNSUPPORTED;
     if (static_cast<uint64_t>(view->pages) * view->kv_heads * view->page_size > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;   // coordinates are 32-bit
     if (batch->sequences == 0 || batch->total_tokens == 0 || batch->max_tokens == 0) return B200KV_OK;
-    settle_window(*batch, &window, &sinks);
+    settle(*batch, scoring, &window, &sinks);
+    const bool capped = scoring != nullptr && scoring->cap > 0.0f, ranged = scoring != nullptr && scoring->ranges != nullptr;
     const uint32_t group = query_heads / view->kv_heads;
-    const bool again = lse != nullptr && q_dtype == B200KV_F32 && !is_k_q8(view->quant_mode) && !decode_takes_all(*batch, group);   // the queries are read once more when results are out
+    if (scoring != nullptr) {   // read while results are written
+        const uint64_t out_bytes = static_cast<uint64_t>(batch->total_tokens) * query_heads * view->head_dim * (output_dtype == B200KV_F32 ? 4 : 2), lse_bytes = static_cast<uint64_t>(batch->total_tokens) * query_heads * 4;
+        for (const auto& [array, bytes] : {std::pair<const void*, uint64_t>{scoring->slopes, query_heads * 4ull}, std::pair<const void*, uint64_t>{scoring->ranges, batch->total_tokens * 8ull}})
+            if (array != nullptr && (share(array, bytes, output, out_bytes) || (lse != nullptr && share(array, bytes, lse, lse_bytes)))) return B200KV_ERR_INVALID;
+    }
+    const bool again = lse != nullptr && q_dtype == B200KV_F32 && !is_k_q8(view->quant_mode) && !capped && !decode_takes_all(*batch, group);   // the queries are read once more when results are out
     const uint64_t rows = static_cast<uint64_t>(batch->total_tokens) * query_heads, q_bytes = rows * view->head_dim * 4;
     if (again && (share(q, q_bytes, output, output_dtype == B200KV_F32 ? q_bytes : q_bytes / 2) || share(q, q_bytes, lse, rows * 4))) return B200KV_ERR_INVALID;
-    if (workspace == nullptr || workspace_bytes < b200kv_paged_attn_workspace_bytes(view, batch, query_heads, window, sinks)) return B200KV_ERR_WORKSPACE;
+    if (workspace == nullptr || workspace_bytes < workspace_of(view, batch, scoring, query_heads, window, sinks)) return B200KV_ERR_WORKSPACE;
     rc = ensure_device();
     if (rc != B200KV_OK) return rc;
-    const Room room = room_of(*view, *batch, query_heads, window, sinks, kMostSms);
+    const Room room = room_of(*view, *batch, query_heads, window, sinks, ranged, kMostSms);
     if (room.scratch_tiles * kChunkTile * view->kv_heads > 0x7fffffffull) return B200KV_ERR_UNSUPPORTED;
     uint8_t* ws = reinterpret_cast<uint8_t*>(up(reinterpret_cast<uintptr_t>(workspace), 1024));
     const Paged pool = paged_of(*view, *batch);
@@ -512,16 +621,24 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
         const PrepareParams pp{pool, reinterpret_cast<ChunkPlan*>(ws), reinterpret_cast<ChunkItem*>(ws + room.items), reinterpret_cast<uint32_t*>(ws + room.groups), room.max_items,
                                room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
                                view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.5f, 7.0f, 1.0f, 2.0f, 0.02f},
-                               {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}};
+                               {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}, ranged ? scoring->ranges : nullptr,
+                               reinterpret_cast<uint2*>(ws + room.tile_bounds), reinterpret_cast<uint2*>(ws + room.bounds)};
         const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
         const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;
-        static std::atomic<uint64_t> done[2];
-        const auto prepare = view->head_dim == 128 ? paged_prepare_kernel<128> : paged_prepare_kernel<256>;
-        if (smem > 32 * 1024) B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prepare), 2 * (kMostSequences + 1) * 4, done[view->head_dim == 256]));
-        B200KV_CUDA_TRY(launch_kernel(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, true, pp));
+        static std::atomic<uint64_t> done[4];
+        const auto prepare = ranged ? (view->head_dim == 128 ? paged_prepare_kernel<128, true> : paged_prepare_kernel<256, true>)
+                                    : (view->head_dim == 128 ? paged_prepare_kernel<128, false> : paged_prepare_kernel<256, false>);
+        if (smem > 32 * 1024) B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prepare), 2 * (kMostSequences + 1) * 4, done[(view->head_dim == 256) + 2 * ranged]));
+        if (ranged) {
+            B200KV_CUDA_TRY(launch_kernel(paged_bounds_kernel, dim3(batch->sequences), dim3(kBoundsThreads), 0, s, true, pp));
+            B200KV_CUDA_TRY(launch_behind(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, pp));
+        } else {
+            B200KV_CUDA_TRY(launch_kernel(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, true, pp));
+        }
         const ChunkLaunch cl{pp.items, pp.plan, room.max_items, pp.out[0], pp.out[1], static_cast<uint32_t>(room.scratch_tiles * kChunkTile), q, q_dtype == B200KV_F16, gate, output,
                              output_dtype == B200KV_F16, lse, query_heads, view->kv_heads, view->head_dim, window, sinks, scale * 1.4426950408889634f,
-                             reinterpret_cast<float*>(ws + room.part_o), reinterpret_cast<float2*>(ws + room.part_ml)};
+                             reinterpret_cast<float*>(ws + room.part_o), reinterpret_cast<float2*>(ws + room.part_ml), scoring != nullptr, capped ? scoring->cap : 0.0f, scale,
+                             scoring != nullptr ? scoring->slopes : nullptr, pp.ranges};
         rc = launch_chunk(cl, s);
         if (rc != B200KV_OK) return rc;
         const ChunkMergeParams mp{pp.plan, pp.items, pp.groups, cl.part_o, cl.part_ml, gate, output, cl.out_is_f16, lse, query_heads, view->kv_heads};
@@ -547,9 +664,46 @@ int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* b
     }
     if (room.decode) {
         PagedDecode dp{pool, q, q_dtype == B200KV_F16, gate, output, output_dtype == B200KV_F16, lse, query_heads, window, sinks, 0, scale * 1.4426950408889634f};
-        return launch_paged_decode(dp, ws + room.decode_parts, s, room.chunks);
+        if (scoring == nullptr) return launch_paged_decode(dp, ws + room.decode_parts, s, room.chunks);
+        PagedDecodeScored scored{};
+        static_cast<PagedDecode&>(scored) = dp;
+        scored.cap_log2 = capped ? scoring->cap * 1.4426950408889634f : 0.0f;
+        scored.cap_in = capped ? 1.0f / scored.cap_log2 : 0.0f;
+        scored.slopes = scoring->slopes;
+        scored.ranges = scoring->ranges;
+        return launch_paged_decode_scored(scored, ws + room.decode_parts, s, room.chunks);
     }
     return B200KV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200kv_paged_attn_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, uint32_t query_heads, uint32_t window, uint32_t sinks) {
+    return workspace_of(view, batch, nullptr, query_heads, window, sinks);
+}
+
+int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const void* q, int q_dtype, const float* gate,
+                      void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(view, batch, nullptr, q, q_dtype, gate, output, output_dtype, lse, query_heads, scale, window, sinks, workspace, workspace_bytes, stream);
+}
+
+size_t b200kv_paged_attn_scored_workspace_bytes(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring, uint32_t query_heads,
+                                                uint32_t window, uint32_t sinks) {
+    return scoring == nullptr ? 0 : workspace_of(view, batch, scoring, query_heads, window, sinks);
+}
+
+int b200kv_paged_attn_scored(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const b200kv_paged_scoring* scoring, const void* q, int q_dtype, const float* gate,
+                             void* output, int output_dtype, float* lse, uint32_t query_heads, float scale, uint32_t window, uint32_t sinks,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    if (scoring == nullptr || !std::isfinite(scoring->cap) || scoring->cap < 0.0f) return B200KV_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(scoring->slopes) & 3u) != 0 || (reinterpret_cast<uintptr_t>(scoring->ranges) & 7u) != 0) return B200KV_ERR_INVALID;
+    // a cap's quotients with the scale, and its product with log2 e, are ordinary numbers
+    if (scoring->cap > 0.0f && (scoring->cap < 1.0e-6f || scoring->cap > 1.0e6f)) return B200KV_ERR_UNSUPPORTED;
+    const bool nothing = scoring->cap == 0.0f && scoring->slopes == nullptr && scoring->ranges == nullptr;
+    return attend(view, batch, nothing ? nullptr : scoring, q, q_dtype, gate, output, output_dtype, lse, query_heads, scale, window, sinks, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

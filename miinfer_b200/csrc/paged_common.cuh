@@ -64,6 +64,41 @@ __device__ __forceinline__ uint32_t sequence_of(const Paged& p, uint32_t row) {
     return lo;
 }
 
+// What a new token sees: positions [low, upto), and the first sinks below upto.
+struct Sight {
+    uint32_t low, upto;
+    __device__ __forceinline__ bool empty() const { return low >= upto; }   // but for the sinks
+};
+// Of the token in row `row` of the activations, at place `place` of its sequence of `length` positions.  ranges (may be null): a token's own [low, upto) in place of [0, place + 1).
+__device__ __forceinline__ Sight sight_of(const int32_t* ranges, size_t row, int place, uint32_t window, uint32_t length) {
+    if (place < 0) return {0, 0};
+    int low = 0, upto = place + 1;
+    if (ranges != nullptr) {
+        const int2 r = reinterpret_cast<const int2*>(ranges)[row];
+        low = max(r.x, 0);
+        upto = max(r.y, 0);
+    }
+    if (window > 0) low = max(low, place + 1 - static_cast<int>(window));
+    return {static_cast<uint32_t>(low), min(static_cast<uint32_t>(upto), length)};
+}
+
+constexpr float kTanhSmall = 0.8f;
+// tanh of any x: 1 - 2 / (e^2x + 1), off by a few roundings of numbers near 1, and so by up to 3e-7.
+__device__ __forceinline__ float tanh_large(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.8853900817779268f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return fmaf(-2.0f, r, 1.0f);
+}
+// Of |x| <= kTanhSmall, by odd powers up to the eleventh: the polynomial with the smallest relative error, 5.8e-8 (Remez's exchange); 1e-7 in fp32.
+__device__ __forceinline__ float tanh_small(float x) {
+    const float k[6] = {0.99999994f, -0.333326757f, 0.13321048f, -0.0531143136f, 0.0190933011f, -0.00435529929f}, u = x * x;
+    float r = k[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) r = fmaf(r, u, k[i]);
+    return x * r;
+}
+
 // The first row of page number `page` for a kv head, or -1 for a page outside the pool.
 __device__ __forceinline__ long long page_row(const Paged& p, int page, uint32_t head) {
     if (static_cast<uint32_t>(page) >= p.view.pages) {

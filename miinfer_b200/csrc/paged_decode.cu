@@ -27,6 +27,7 @@
 #include "paged_unit.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200kv {
 
@@ -92,10 +93,12 @@ struct Layout {
     static_assert(kTotal <= kBudget && kOffQ + 2 * kQBytes + (kQCols - kQRows) * 128 <= kTotal);
 };
 
-template <int D, int KF, int VF, int RG, int PLANES>
+// P: PagedDecode, or PagedDecodeScored for scores that are changed or seen otherwise.
+template <int D, int KF, int VF, int RG, int PLANES, class P>
 __global__ void __launch_bounds__(Layout<D, KF, VF, RG, PLANES>::kThreads, Layout<D, KF, VF, RG, PLANES>::kCtas)
-paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using L = Layout<D, KF, VF, RG, PLANES>;
+    constexpr bool kScored = std::is_same_v<P, PagedDecodeScored>;
     constexpr int kHalves = L::kHalves;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -285,9 +288,32 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 upto[r] = static_cast<uint32_t>(max(at, 0));
                 low[r] = p.window > 0 && upto[r] > p.window ? upto[r] - p.window : 0;
             }
-            const uint32_t first_upto = static_cast<uint32_t>(max(c.span.base() + 1, 0));                             // what every row sees: [.., first_upto)
-            [[maybe_unused]] const uint32_t first_low = p.window > 0 && first_upto > p.window ? first_upto - p.window : 0;   // seen by nobody: below it, but for the sinks
-            const uint32_t last_low = p.window > 0 && c.span.length > p.window ? c.span.length - p.window : 0;        // from here on
+            uint32_t first_upto = static_cast<uint32_t>(max(c.span.base() + 1, 0));                             // what every row sees: [.., first_upto)
+            [[maybe_unused]] uint32_t first_low = p.window > 0 && first_upto > p.window ? first_upto - p.window : 0;   // seen by nobody: below it, but for the sinks
+            uint32_t last_low = p.window > 0 && c.span.length > p.window ? c.span.length - p.window : 0;        // from here on
+            [[maybe_unused]] uint32_t seen_end = c.span.length;                                                       // and seen by nobody from here on
+            [[maybe_unused]] float slope[4];             // of the rows, in log2 units, and their places
+            [[maybe_unused]] int place[4];
+            if constexpr (kScored) {
+                first_upto = first_low = 0xffffffffu;
+                last_low = seen_end = 0;
+                for (uint32_t t = 0; t < c.span.tokens; ++t) {
+                    const Sight s = p.sight(c.span, t);
+                    first_upto = min(first_upto, s.upto);
+                    last_low = max(last_low, s.low);
+                    if (!s.empty()) first_low = min(first_low, s.low);
+                    seen_end = max(seen_end, s.empty() ? min(s.upto, p.sinks) : s.upto);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t row = g * 4 + r, t = min(row, rows - 1) / G;
+                    const Sight s = p.sight(c.span, t);
+                    upto[r] = row < rows ? s.upto : 0;
+                    low[r] = s.low;
+                    place[r] = c.span.base() + static_cast<int>(t);
+                    slope[r] = p.slopes != nullptr ? p.slopes[c.head * G + min(row, rows - 1) % G] * 1.4426950408889634f : 0.0f;
+                }
+            }
             float acc[kHalves][4], m_run[4], l_run[4], pend[2][kHalves][4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -370,15 +396,31 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 if (lane == 0) mbar_arrive(bar(L::K_EMPTY + slot));      // the scales are read
                 const uint32_t pos0 = pos - t128;
                 bool any = true;
+                float qmul_now[4];
+                if constexpr (kScored) {   // what a score becomes, in base-2 units; the mask below leaves them as they are
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[r] *= qmul[r];
+                        if (p.cap_log2 > 0.0f) {
+                            const float x = s[r] * p.cap_in;
+                            s[r] = p.cap_log2 * (fabsf(x) <= kTanhSmall ? tanh_small(x) : tanh_large(x));
+                        }
+                        if (p.slopes != nullptr) s[r] = fmaf(-slope[r], fabsf(static_cast<float>(place[r] - static_cast<int>(pos))), s[r]);
+                        qmul_now[r] = 1.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) qmul_now[r] = qmul[r];
+                }
                 if (pos0 + kDecodeTile <= first_upto && pos0 >= last_low) {   // every row sees all of the tile
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[r] *= qmul[r];
+                    for (int r = 0; r < 4; ++r) s[r] *= qmul_now[r];
                 } else {
                     any = false;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool seen = pos < upto[r] && (pos >= low[r] || pos < p.sinks);
-                        s[r] = seen ? s[r] * qmul[r] : -INFINITY;
+                        s[r] = seen ? s[r] * qmul_now[r] : -INFINITY;
                         any |= seen;
                     }
                 }
@@ -386,7 +428,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecode p, const __grid_constant
                 wait(bar(L::V_FULL + vslot), (i / L::kVUnits) & 1);
                 __syncwarp();
                 if constexpr (VF == F16) {   // an fp16 value that none of the rows sees is cleared (int8 ones are finite whatever they are)
-                    if (g == 0 && (pos >= c.span.length || (pos < first_low && pos >= p.sinks))) {
+                    if (g == 0 && (pos >= seen_end || (pos < first_low && pos >= p.sinks))) {
                         uint8_t* row = smem + L::kOffV + vslot * L::kVData + t128 * 128;
 #pragma unroll 1
                         for (int x = 0; x < D / 64; ++x)
@@ -660,10 +702,10 @@ __global__ void __launch_bounds__(D) paged_decode_merge_kernel(const __grid_cons
     else static_cast<float*>(p.out)[at] = v;
 }
 
-template <int D, int KF, int VF, int RG, int PLANES>
-int launch_planes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+template <int D, int KF, int VF, int RG, int PLANES, class P>
+int launch_planes(const P& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
     using L = Layout<D, KF, VF, RG, PLANES>;
-    const auto kernel = paged_decode_kernel<D, KF, VF, RG, PLANES>;
+    const auto kernel = paged_decode_kernel<D, KF, VF, RG, PLANES, P>;
     static std::atomic<uint64_t> done{0};
     B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, done));
     if (behind) B200KV_CUDA_TRY(launch_behind(kernel, dim3(p.ctas), dim3(L::kThreads), L::kAlloc, stream, p, kmap, vmap));
@@ -673,16 +715,16 @@ int launch_planes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorM
 // Three planes against int8 keys (a score to 2^-23 of its row's largest element), but for eight rows where the output alone is asked for, in fp16: two hold 2^-16, which that does not
 // show, and are up to 12 % faster (24 sequences of 4000, 24 / 4 heads of 256: q8_0 66.6 and 75 us, where a tile has 96 sums a thread in place of 64 and one buffer of them; one scale a row 59.4
 // and 61.4).
-template <int D, int KF, int VF, int RG>
-int launch_of(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+template <int D, int KF, int VF, int RG, class P>
+int launch_of(const P& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
     if constexpr (KF == F16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
-    if constexpr (KF != F16 && RG == 2) {
+    if constexpr (KF != F16 && RG == 2 && std::is_same_v<P, PagedDecode>) {
         if (p.lse == nullptr && p.out_is_f16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);
     }
     if constexpr (KF != F16) return launch_planes<D, KF, VF, RG, 3>(p, kmap, vmap, stream, behind);
 }
-template <int D, int RG>
-int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
+template <int D, int RG, class P>
+int launch_modes(const P& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
     const bool blocks = p.pool.view.qblock != D;
     switch (p.pool.view.quant_mode) {
         case B200KV_F16_F16: return launch_of<D, F16, F16, RG>(p, kmap, vmap, stream, behind);
@@ -692,16 +734,9 @@ int launch_modes(const PagedDecode& p, const CUtensorMap& kmap, const CUtensorMa
     }
 }
 
-}  // namespace
-
-uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t sms) {
-    return sms * (view.head_dim == 128 && view.quant_mode == B200KV_Q8_Q8 ? 2 : 1);
-}
-size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t sms) {
-    return decode_ctas(view, sms) * (2ull * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2)) + sizeof(uint4));
-}
-
-int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind) {
+// A call's launch, and the merge behind it.
+template <class P>
+int launch_decode_of(P p, void* parts, cudaStream_t stream, bool behind) {
     const b200kv_paged_view& v = p.pool.view;
     const b200kv_paged_batch& b = p.pool.batch;
     const uint64_t rows = static_cast<uint64_t>(v.pages) * v.kv_heads * v.page_size;
@@ -724,9 +759,24 @@ int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool be
     if (b.max_length <= kDecodeTile) return B200KV_OK;
     const uint32_t most_rows = static_cast<uint32_t>(std::min<uint64_t>(p.rows, static_cast<uint64_t>(b.max_tokens) * group));
     const dim3 grid(most_rows, p.ctas);
-    B200KV_CUDA_TRY(v.head_dim == 128 ? launch_behind(paged_decode_merge_kernel<128>, grid, dim3(128), 0, stream, p)
-                                      : launch_behind(paged_decode_merge_kernel<256>, grid, dim3(256), 0, stream, p));
+    B200KV_CUDA_TRY(v.head_dim == 128 ? launch_behind(paged_decode_merge_kernel<128>, grid, dim3(128), 0, stream, static_cast<const PagedDecode&>(p))
+                                      : launch_behind(paged_decode_merge_kernel<256>, grid, dim3(256), 0, stream, static_cast<const PagedDecode&>(p)));
     return B200KV_OK;
 }
+
+}  // namespace
+
+#ifdef B200KV_PAGED_DECODE_SCORED
+int launch_paged_decode_scored(PagedDecodeScored p, void* parts, cudaStream_t stream, bool behind) { return launch_decode_of(p, parts, stream, behind); }
+#else
+uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t sms) {
+    return sms * (view.head_dim == 128 && view.quant_mode == B200KV_Q8_Q8 ? 2 : 1);
+}
+size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t sms) {
+    return decode_ctas(view, sms) * (2ull * kDecodeRows * (view.head_dim * sizeof(float) + sizeof(float2)) + sizeof(uint4));
+}
+
+int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind) { return launch_decode_of(p, parts, stream, behind); }
+#endif
 
 }  // namespace b200kv

@@ -32,6 +32,31 @@ struct PagedDecode {
     }
 };
 
+// The same with scores that are capped, biased by distance, or seen by ranges of the tokens' own (paged_decode_scored.cu).
+struct PagedDecodeScored : PagedDecode {
+    float cap_log2, cap_in;    // cap * log2 e and its reciprocal; 0: no cap
+    const float* slopes;       // [query_heads], may be null
+    const int32_t* ranges;     // [total_tokens][2], may be null
+    __device__ __forceinline__ Sight sight(const Span& span, uint32_t t) const {
+        return sight_of(ranges, static_cast<size_t>(span.first) + t, span.base() + static_cast<int>(t), window, span.length);
+    }
+    __device__ __forceinline__ Tiles tiles_of(const Span& span) const {
+        if (ranges == nullptr) return PagedDecode::tiles_of(span);
+        if (span.tokens == 0 || span.tokens > kDecodeRows || span.tokens * (query_heads / pool.view.kv_heads) > rows) return {0, 0, 0};
+        uint32_t lowest = 0xffffffffu, end = 0;
+        for (uint32_t t = 0; t < span.tokens; ++t) {
+            const Sight s = sight(span, t);
+            if (!s.empty()) lowest = min(lowest, s.low);
+            end = max(end, s.empty() ? min(s.upto, sinks) : s.upto);
+        }
+        const uint32_t all = (end + kDecodeTile - 1) / kDecodeTile, first = min(lowest / kDecodeTile, all), sink = (min(sinks, end) + kDecodeTile - 1) / kDecodeTile;
+        Tiles t{all, 0, 0};
+        if (first > sink) t = {sink + all - first, sink, first};
+        t.n = max(t.n, 1u);
+        return t;
+    }
+};
+
 // Whether the sequences of a batch can all be of this kernel, and whether any can be.
 inline bool decode_takes_all(const b200kv_paged_batch& b, uint32_t group) { return static_cast<uint64_t>(b.max_tokens) * group <= kDecodeRows; }
 // The rows of the launch: four where they are enough for all sequences, or, beside the chunk kernel, for a token.  (Four rows leave room for two CTAs an SM of int8
@@ -40,6 +65,7 @@ inline uint32_t decode_rows(const b200kv_paged_batch& b, uint32_t group) { retur
 uint32_t decode_ctas(const b200kv_paged_view& view, uint32_t sms);     // at most
 size_t decode_part_bytes(const b200kv_paged_view& view, uint32_t sms);
 int launch_paged_decode(PagedDecode p, void* parts, cudaStream_t stream, bool behind);
+int launch_paged_decode_scored(PagedDecodeScored p, void* parts, cudaStream_t stream, bool behind);
 
 // A tensor map over a pool's plane as rows of head_dim: boxes of 128 bytes by `box_rows` rows, 128-byte swizzle.
 bool encode_pool_map(CUtensorMap* map, const void* plane, bool f16, uint64_t rows, uint32_t head_dim, uint32_t box_rows);

@@ -22,7 +22,8 @@ struct ChunkItem {
     uint32_t tile0, tiles;     // its tiles, counted without those
     uint32_t part;             // where its unnormalised partial goes; kNoPart: it writes the output itself
     uint32_t parts;            // how many share the row tile (a partial's own number is part - the first one's)
-    uint32_t pad_[3];
+    uint32_t length;           // of the sequence
+    uint32_t pad_[2];
 };
 static_assert(sizeof(ChunkItem) == 64);
 
@@ -46,6 +47,19 @@ __host__ __device__ inline ChunkTiles chunk_tiles(int base, uint32_t length, uin
     t.tiles = sink + (t.tiles > first ? t.tiles - first : 0);
     return t;
 }
+
+// The same where tokens have ranges of their own: all that any of them sees lies in [lowest, end) or is among the sinks below end.
+__host__ __device__ inline ChunkTiles chunk_tiles_between(uint32_t lowest, uint32_t end, uint32_t sinks) {
+    ChunkTiles t{0, 0, (end + kChunkTile - 1) / kChunkTile};
+    const uint32_t first = lowest / kChunkTile, sink = ((sinks < end ? sinks : end) + kChunkTile - 1) / kChunkTile;
+    if (first <= sink) return t;
+    t.sink_tiles = sink;
+    t.window0 = first * kChunkTile;
+    t.tiles = sink + (t.tiles > first ? t.tiles - first : 0);
+    return t;
+}
+// The slot of row tile r of sequence s among those of all sequences: as many as there can be, and each its own where the starts ascend.
+__host__ __device__ inline size_t chunk_slot(uint32_t first, uint32_t group, uint32_t s, uint32_t r) { return static_cast<size_t>(static_cast<uint64_t>(first) * group / kChunkRows) + s + r; }
 
 // Work of n row tiles of a sequence, in 128ths of a tile: tokens of a chunk see on average half of it.
 __host__ __device__ inline unsigned long long chunk_work(uint32_t n, uint32_t tiles, uint32_t tokens) {
@@ -71,6 +85,10 @@ struct ChunkLaunch {
     float scale_log2;
     float* part_o;             // [part][kChunkRows][head_dim]
     float2* part_ml;           // [part][kChunkRows] {maximum in log2 units, sum}
+    bool scored;               // with what follows
+    float cap, scale;          // scores of at most cap; 0: any
+    const float* slopes;       // [query_heads], may be null
+    const int32_t* ranges;     // [total_tokens][2], may be null
 };
 int launch_chunk(const ChunkLaunch& c, cudaStream_t stream);
 

@@ -87,14 +87,27 @@ __device__ __forceinline__ ChunkItem reload(const ChunkItem* from) {
 // Which of a tile's positions lie below n, a bit each.
 __device__ __forceinline__ uint64_t bits_below(uint32_t n, uint32_t pos0) { return n <= pos0 ? 0ull : n - pos0 >= kBN ? ~0ull : (1ull << (n - pos0)) - 1; }
 
-template <bool PAGED> struct KernelParams : Tc5Params {};
-template <> struct KernelParams<true> : Tc5Params {   // of the base: maps, q, gate, heads, scale and partials
+// What scores become, in an instance of its own for each (SCORE; 0: nothing of this).
+enum Score : int {
+    kRanged = 1,   // tokens may have ranges of their own (all of the instances below)
+    kCapped = 2,   // cap * tanh(x / cap) in place of a scaled score x
+    kSloped = 4    // less slope * |i - j|
+};
+
+template <bool PAGED, bool SCORED = false> struct KernelParams : Tc5Params {};
+template <> struct KernelParams<true, false> : Tc5Params {   // of the base: maps, q, gate, heads, scale and partials
     const ChunkItem* items;
     const ChunkPlan* plan;
     void* typed_out;
     int out_is_f16;
     float* lse;                  // may be null
     uint32_t window, sinks;
+};
+template <> struct KernelParams<true, true> : KernelParams<true, false> {   // scale_log2: what the softmax multiplies what it is given by
+    float cap_in;                // scale / cap
+    float slope_scale;           // kSloped without a cap: scale * log2 e
+    const float* slopes;
+    const int32_t* ranges;       // may be null
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -198,6 +211,7 @@ __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
 }
 // Two fp32 values in one instruction, and the largest of three.
 __device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b) { Pair r; asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ Pair add_pair(Pair a, Pair b) { Pair r; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.ftz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 // A wait of a whole warp, which stays together: all lanes go on or none.
@@ -281,10 +295,40 @@ struct RowOffsets {
     }
 };
 
+// tanh(k s) of a tile's scores, in place.  Where no row of the warp has |k s| above kTanhSmall, by a polynomial, two values to an instruction: as many fp32 instructions as the rest of
+// the loop has, but none of the special function unit, which the exponentials keep busy.  Otherwise by two of its functions a value.
+__device__ __forceinline__ void cap_scores(float (&s)[kBN], float k) {
+    float m4[4] = {fabsf(s[0]), fabsf(s[1]), fabsf(s[2]), fabsf(s[3])};
+#pragma unroll
+    for (int i = 4; i + 8 <= kBN; i += 8)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], fabsf(s[i + c]), fabsf(s[i + 4 + c]));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fabsf(s[kBN - 4 + c]));
+    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k > kTanhSmall)) {   // (a row of NaN has no say)
+        const float c[6] = {0.99999994f, -0.333326757f, 0.13321048f, -0.0531143136f, 0.0190933011f, -0.00435529929f};
+        const Pair k2 = pack_pair(k, k);
+#pragma unroll
+        for (int i = 0; i < kBN; i += 2) {
+            const Pair x = mul_pair(pack_pair(s[i], s[i + 1]), k2), u = mul_pair(x, x);
+            Pair r = pack_pair(c[5], c[5]);
+#pragma unroll
+            for (int j = 4; j >= 0; --j) r = fma_pair(r, u, pack_pair(c[j], c[j]));
+            const float2 t = unpack_pair(mul_pair(x, r));
+            s[i] = t.x;
+            s[i + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kBN; ++i) s[i] = tanh_large(s[i] * k);
+    }
+}
+
 // STATE: the position comes from a device-side state (one row tile a CTA).  PAGED: everything does (ChunkItem).
-template <int D, int RT, bool STATE, bool PAGED = false>
-__global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel(const __grid_constant__ KernelParams<PAGED> p) {
+template <int D, int RT, bool STATE, bool PAGED = false, int SCORE = 0>
+__global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel(const __grid_constant__ KernelParams<PAGED, (SCORE > 0)> p) {
     static_assert(!PAGED || (RT == 1 && !STATE));
+    static_assert(PAGED || SCORE == 0);
     using L = Layout<D, RT>;
     constexpr int kThreads = L::kThreads;
     constexpr int kTmaWarp = L::kTmaWarp, kSWarp = L::kSWarp, kPvWarp = L::kPvWarp, kTmaVWarp = L::kTmaVWarp;
@@ -759,6 +803,17 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         }
         uint32_t low = 0;   // PAGED: the row sees positions [low, len) and those below p.sinks
         if constexpr (PAGED) low = p.window > 0 && len > p.window ? len - p.window : 0u;
+        [[maybe_unused]] int place = 0;        // SCORE: of the row's token in the cache
+        [[maybe_unused]] float slope = 0.0f;   // kSloped: in log2 units
+        if constexpr (SCORE != 0) {
+            if (gr < total_rows) {
+                place = item.base + static_cast<int>(gr / G);
+                const Sight sight = sight_of(p.ranges, static_cast<size_t>(item.first) + gr / G, place, p.window, item.length);
+                len = sight.upto;
+                low = sight.low;
+                if constexpr ((SCORE & kSloped) != 0) slope = p.slopes[kv_head * G + gr % G] * 1.4426950408889634f;
+            }
+        }
         volatile unsigned long long* ref = reinterpret_cast<volatile unsigned long long*>(smem + L::kOffRef) + rt * kBM + r;
         auto ref_after = [&](uint32_t seq, float* value) -> bool {   // the reference as tile seq-1 left it
             // Rolled up at 256: less code in the longer of the tile loops, whose warps wait for instructions (0.7 stalls an issue; 0.3 at 128, where it makes no
@@ -777,6 +832,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 m_known = m_new;
             }
         };
+        const float to_log2 = (SCORE & kSloped) != 0 ? 1.0f : p.scale_log2;   // biased scores are in log2 units already
         const int buf = rt * L::kGroups + grp;
         const uint32_t s_col = L::kColS + buf * kBN, o_col = L::kColO + rt * D;
         const int nt = L::kGroups == 4 ? (walked + grp + 1) / 2 : walked;
@@ -804,6 +860,24 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // Raw scores stay unscaled; the softmax scale is folded into the exponent: p = 2^(s*c - m*c).  The loop's instructions count: products and
             // sums go in pairs, maxima three values at a time.  32 / 8 heads of 128, 1024 tokens over 8192: 168.0 -> 163.7 us; 24 / 4 of 256, 512 over
             // 8192: 111.6 -> 110.3.
+            if constexpr ((SCORE & kCapped) != 0) cap_scores(s, p.cap_in);
+            if constexpr ((SCORE & kSloped) != 0) {
+                const float of_scores = (SCORE & kCapped) != 0 ? p.scale_log2 : p.slope_scale;
+                const int ahead = static_cast<int>(pos0) - place;   // of the tile's first position, from the token's
+                if (ahead + kBN <= 1) {                             // nothing behind the token: the distance falls from position to position
+                    const float first = slope * static_cast<float>(ahead);
+                    const Pair scale2 = pack_pair(of_scores, of_scores);
+#pragma unroll
+                    for (int i = 0; i < kBN; i += 2) {
+                        const float2 x = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, pack_pair(fmaf(static_cast<float>(i), slope, first), fmaf(static_cast<float>(i + 1), slope, first))));
+                        s[i] = x.x;
+                        s[i + 1] = x.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kBN; ++i) s[i] = fmaf(s[i], of_scores, -slope * fabsf(static_cast<float>(ahead + i)));
+                }
+            }
             // Only the tiles that straddle this row's causal length need the mask.
             if constexpr (PAGED) {
                 if (pos0 + kBN > len || pos0 < low) {   // 64 bits, one a position: below len, and from low on or among the sinks
@@ -822,7 +896,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], s[i + c], s[i + 4 + c]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], s[kBN - 4 + c]);
-            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;   // scale > 0: the maximum commutes with it
+            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * to_log2;   // scale > 0: the maximum commutes with it
             // the reference as the previous tile (another group's) left it; lazy rescale: keep it unless this tile's
             // maximum outgrew it by more than the threshold
             float m_prev = -INFINITY;
@@ -849,7 +923,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             const float neg_ref = (m_new == -INFINITY) ? 0.0f : -m_new;
             Pair sum = 0;
             uint32_t pk[kBN / 2];
-            const Pair scale2 = pack_pair(p.scale_log2, p.scale_log2), ref2 = pack_pair(neg_ref, neg_ref);
+            const Pair scale2 = pack_pair(to_log2, to_log2), ref2 = pack_pair(neg_ref, neg_ref);
 #pragma unroll
             for (int i = 0; i < kBN; i += 2) {
                 const float2 e = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, ref2));
@@ -1389,17 +1463,23 @@ int launch_prefill_tc5_prepare(const b200kv_view& view, uint32_t prepared_rows, 
 }
 
 // Chunks over a paged cache: the attention kernel alone, behind the call's other kernels.
-template <int D>
-static int launch_chunk_of(const KernelParams<true>& p, uint32_t max_items, cudaStream_t stream) {
+template <int D, int SCORE>
+static int launch_chunk_of(const KernelParams<true, (SCORE > 0)>& p, uint32_t max_items, cudaStream_t stream) {
     using L = Layout<D, 1>;
+    const auto kernel = prefill_tc5_kernel<D, 1, false, true, SCORE>;
     static std::atomic<uint64_t> done{0};
-    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prefill_tc5_kernel<D, 1, false, true>), L::kAlloc, done));
-    B200KV_CUDA_TRY(launch_behind(prefill_tc5_kernel<D, 1, false, true>, dim3(max_items), dim3(L::kThreads), L::kAlloc, stream, p));
+    B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, done));
+    B200KV_CUDA_TRY(launch_behind(kernel, dim3(max_items), dim3(L::kThreads), L::kAlloc, stream, p));
     return B200KV_OK;
+}
+template <int D>
+static int launch_scored(const KernelParams<true, true>& p, bool capped, uint32_t max_items, cudaStream_t stream) {
+    if (p.slopes == nullptr) return capped ? launch_chunk_of<D, kRanged | kCapped>(p, max_items, stream) : launch_chunk_of<D, kRanged>(p, max_items, stream);
+    return capped ? launch_chunk_of<D, kRanged | kCapped | kSloped>(p, max_items, stream) : launch_chunk_of<D, kRanged | kSloped>(p, max_items, stream);
 }
 int launch_chunk(const ChunkLaunch& c, cudaStream_t stream) {
     static_assert(kChunkRows == kBM && kChunkTile == kBN);
-    KernelParams<true> p{};
+    KernelParams<true, true> p{};
     if (!encode_f16_plane(&p.kmap, c.k_scratch, c.head_dim, c.scratch_rows, c.scratch_rows, c.kv_heads) ||
         !encode_f16_plane(&p.vmap, c.v_scratch, c.head_dim, c.scratch_rows, c.scratch_rows, c.kv_heads))
         return B200KV_ERR_UNSUPPORTED;
@@ -1420,7 +1500,16 @@ int launch_chunk(const ChunkLaunch& c, cudaStream_t stream) {
     p.lse = c.lse;
     p.window = c.window;
     p.sinks = c.sinks;
-    return c.head_dim == 256 ? launch_chunk_of<256>(p, c.max_items, stream) : launch_chunk_of<128>(p, c.max_items, stream);
+    if (!c.scored) return c.head_dim == 256 ? launch_chunk_of<256, 0>(p, c.max_items, stream) : launch_chunk_of<128, 0>(p, c.max_items, stream);
+    const bool capped = c.cap > 0.0f;
+    p.slopes = c.slopes;
+    p.ranges = c.ranges;
+    p.slope_scale = c.scale_log2;
+    if (capped) {
+        p.cap_in = c.scale / c.cap;
+        p.scale_log2 = c.cap * 1.4426950408889634f;
+    }
+    return c.head_dim == 256 ? launch_scored<256>(p, capped, c.max_items, stream) : launch_scored<128>(p, capped, c.max_items, stream);
 }
 
 }  // namespace b200kv

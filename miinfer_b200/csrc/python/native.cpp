@@ -33,6 +33,7 @@ struct Api {
     decltype(&b200kv_paged_store) paged_store;
     decltype(&b200kv_paged_load) paged_load;
     decltype(&b200kv_paged_attn) paged_attn;
+    decltype(&b200kv_paged_attn_scored) paged_attn_scored;
     decltype(&b200kv_paged_weights) paged_weights;
     decltype(&b200kv_paged_evict) paged_evict;
     decltype(&b200kv_paged_rotary) paged_rotary;
@@ -47,6 +48,7 @@ struct Api {
 PyObject* g_view_type;   // the ctypes structure of a cache view
 PyObject* g_paged_view_type;    // ... of a paged cache's view, and of a batch over it
 PyObject* g_paged_batch_type;
+PyObject* g_paged_scoring_type; // ... of what becomes of an attention call's scores
 PyObject* g_rotary_type;        // ... of a table of rotary angles
 PyObject* g_page_book_type;     // ... of the book of a paged cache's pages
 PyObject* g_device_index;       // the name of their attribute
@@ -145,6 +147,10 @@ public:
     }
     const b200kv_paged_view* paged_view() { return structure<b200kv_paged_view>(g_paged_view_type, "a paged cache's view"); }
     const b200kv_paged_batch* paged_batch() { return structure<b200kv_paged_batch>(g_paged_batch_type, "a paged batch"); }
+    const b200kv_paged_scoring* paged_scoring() {   // or None
+        if (ok_ && args_[i_] == Py_None) { ++i_; return nullptr; }
+        return structure<b200kv_paged_scoring>(g_paged_scoring_type, "a scoring");
+    }
     const b200kv_rotary* rotary() { return structure<b200kv_rotary>(g_rotary_type, "a table of rotary angles"); }
     const b200kv_page_book* page_book() { return structure<b200kv_page_book>(g_page_book_type, "a page book"); }
     // A list or tuple of paged views, one behind the other in `to`.
@@ -452,7 +458,7 @@ PyObject* py_paged_load(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* py_paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    Args a(args, n, 12);
+    Args a(args, n, 13);
     int qd = 0, od = 0;
     int64_t ws_bytes = 0;
     const auto* view = a.paged_view();
@@ -468,7 +474,10 @@ PyObject* py_paged_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* ws = a.exactly<void>(at::kByte, "workspace: a uint8 tensor", 0, true);
     if (a.ok() && ws != nullptr) ws_bytes = THPVariable_Unpack(args[10]).numel();
     void* s = a.stream();
+    const auto* scoring = a.paged_scoring();
     return call(a, [&] {
+        if (scoring != nullptr)
+            return g_api.paged_attn_scored(view, batch, scoring, q, qd, gate, out, od, lse, heads, scale, window, sinks, ws, static_cast<size_t>(ws_bytes), s);
         return g_api.paged_attn(view, batch, q, qd, gate, out, od, lse, heads, scale, window, sinks, ws, static_cast<size_t>(ws_bytes), s);
     });
 }
@@ -742,12 +751,12 @@ PyObject* py_pool(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return Py_BuildValue("iI", rc, CAPTURE ? static_cast<unsigned>(captured) : matched);
 }
 
-PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the structures "View", "PagedView", "PagedBatch", "Rotary" and "PageBook"
+PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the structures "View", "PagedView", "PagedBatch", "PagedScoring", "Rotary" and "PageBook"
     PyObject* view = PyDict_GetItemString(arg, "View");
     if (view == nullptr || !PyType_Check(view)) return PyErr_Format(PyExc_KeyError, "View");
     Py_INCREF(view);
     Py_XSETREF(g_view_type, view);
-    for (auto [name, slot] : {std::pair{"PagedView", &g_paged_view_type}, std::pair{"PagedBatch", &g_paged_batch_type}, std::pair{"Rotary", &g_rotary_type},
+    for (auto [name, slot] : {std::pair{"PagedView", &g_paged_view_type}, std::pair{"PagedBatch", &g_paged_batch_type}, std::pair{"PagedScoring", &g_paged_scoring_type}, std::pair{"Rotary", &g_rotary_type},
                               std::pair{"PageBook", &g_page_book_type}}) {
         PyObject* type = PyDict_GetItemString(arg, name);
         if (type == nullptr || !PyType_Check(type)) return PyErr_Format(PyExc_KeyError, "%s", name);
@@ -764,6 +773,7 @@ PyObject* py_bind(PyObject*, PyObject* arg) {   // {name: address}, and the stru
         {"b200kv_paged_store", reinterpret_cast<void**>(&g_api.paged_store)},
         {"b200kv_paged_load", reinterpret_cast<void**>(&g_api.paged_load)},
         {"b200kv_paged_attn", reinterpret_cast<void**>(&g_api.paged_attn)},
+        {"b200kv_paged_attn_scored", reinterpret_cast<void**>(&g_api.paged_attn_scored)},
         {"b200kv_paged_weights", reinterpret_cast<void**>(&g_api.paged_weights)},
         {"b200kv_paged_evict", reinterpret_cast<void**>(&g_api.paged_evict)},
         {"b200kv_paged_rotary", reinterpret_cast<void**>(&g_api.paged_rotary)},

@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import check, lib, native
 from .kv import KvCacheQuantMode, RopeMode
 
-__all__ = ["PagedView", "PagedBatch", "PagedKvCache", "paged_workspace", "launch_paged_store", "launch_paged_load", "launch_paged_attention",
+__all__ = ["PagedView", "PagedBatch", "PagedKvCache", "PagedScoring", "paged_workspace", "launch_paged_store", "launch_paged_load", "launch_paged_attention",
            "launch_paged_weights", "launch_paged_evict", "RotaryLayout", "RotaryScaling", "RotaryTable", "launch_paged_rotary", "PageBook", "pages_workspace",
            "launch_pages_grow", "launch_pages_fork", "launch_pages_free", "launch_pages_compact", "launch_pages_copy", "STATUS_BAD_PAGE", "STATUS_BAD_BOUND",
            "STATUS_BAD_SLOT", "STATUS_NO_PAGE"]
@@ -109,9 +109,35 @@ class PagedKvCache:
         return PagedView.of(self.key, self.key_scales, self.value, self.value_scales, self.quant_mode)
 
 
-def paged_workspace(view: PagedView, batch: PagedBatch, query_heads: int, *, window: int = 0, sinks: int = 0, device=None) -> torch.Tensor:
-    """Scratch for launch_paged_attention calls with this geometry and bounds no larger than the batch's."""
-    n = int(lib.b200kv_paged_attn_workspace_bytes(C.byref(view), C.byref(batch), query_heads, window, sinks))
+class PagedScoring(_lib.PagedScoring):
+    """b200kv_paged_scoring: scores cap * tanh(x / cap) in place of x = scale * q.k (cap 0: x), less slopes[head] * |i - j| (fp32 [query_heads]), and ranges (int32
+    [total_tokens][2]): token t sees positions ranges[t][0] <= j < ranges[t][1] in place of j <= its own, as documents that do not see one another ask for, or a prefix that
+    sees itself in both directions."""
+
+    def __init__(self, *, cap: float = 0.0, slopes: Optional[torch.Tensor] = None, ranges: Optional[torch.Tensor] = None):
+        for name, t, dtype, dims in (("slopes", slopes, torch.float32, 1), ("ranges", ranges, torch.int32, 2)):
+            if t is None:
+                continue
+            if t.dtype != dtype or t.dim() != dims or not t.is_cuda or not t.is_contiguous() or (dims == 2 and t.shape[1] != 2):
+                raise ValueError("slopes: fp32 [query_heads], ranges: int32 [total_tokens][2], contiguous CUDA tensors")
+        given = [t for t in (slopes, ranges) if t is not None]
+        if len({t.device for t in given}) > 1:
+            raise ValueError("slopes and ranges of two devices")
+        super().__init__(float(cap), None if slopes is None else slopes.data_ptr(), None if ranges is None else ranges.data_ptr())
+        self.heads, self.rows = None if slopes is None else slopes.shape[0], None if ranges is None else ranges.shape[0]
+        self.tensors, self.device_index = (slopes, ranges), given[0].device.index if given else -1
+
+    def check(self, query_heads: int, total_tokens: int) -> None:
+        if (self.heads is not None and self.heads < query_heads) or (self.rows is not None and self.rows < total_tokens):
+            raise ValueError("a slope for every query head and a range for every token")
+
+
+def paged_workspace(view: PagedView, batch: PagedBatch, query_heads: int, *, window: int = 0, sinks: int = 0, scoring: Optional[PagedScoring] = None, device=None) -> torch.Tensor:
+    """Scratch for launch_paged_attention calls with this geometry and bounds no larger than the batch's (and with ranges, if the scoring has some)."""
+    if scoring is None:
+        n = int(lib.b200kv_paged_attn_workspace_bytes(C.byref(view), C.byref(batch), query_heads, window, sinks))
+    else:
+        n = int(lib.b200kv_paged_attn_scored_workspace_bytes(C.byref(view), C.byref(batch), C.byref(scoring), query_heads, window, sinks))
     return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
 
 
@@ -135,11 +161,13 @@ def launch_paged_load(view: PagedView, batch: PagedBatch, key: Optional[torch.Te
 
 def launch_paged_attention(view: PagedView, batch: PagedBatch, q: torch.Tensor, output: torch.Tensor, *, query_heads: int, scale: float,
                            window: int = 0, sinks: int = 0, gate: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                           workspace: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> None:
+                           scoring: Optional[PagedScoring] = None, workspace: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> None:
     """Causal attention of every new token over its sequence's pages, times sigmoid(gate); with a window, over the last `window`
     positions and the first `sinks`.  q, output: fp16 or fp32 [total_tokens][query_heads][head_dim]; gate fp32; lse fp32
-    [total_tokens][query_heads].  workspace: `paged_workspace`."""
-    rc = native.paged_attn(view, batch, query_heads, q, gate, output, lse, scale, window, sinks, workspace, stream)
+    [total_tokens][query_heads].  scoring: scores that are capped or biased, tokens that see otherwise.  workspace: `paged_workspace`."""
+    if scoring is not None:
+        scoring.check(query_heads, batch.total_tokens)
+    rc = native.paged_attn(view, batch, query_heads, q, gate, output, lse, scale, window, sinks, workspace, stream, scoring)
     if rc:
         check(rc, "b200kv_paged_attn")
 
