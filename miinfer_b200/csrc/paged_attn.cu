@@ -44,7 +44,8 @@ struct PrepareParams {
     uint32_t few_rows;          // sequences of at most so many query rows are the other kernel's
     ChunkCosts costs;
     __half* out[2];             // the copy, K and V: [kv_head][scratch_tiles * kChunkTile][D]
-    // tokens with ranges of their own: {lowest position seen, one behind the last} of every row tile (chunk_slot) and of every sequence of the chunk kernel's; the sinks aside
+    // tokens with ranges of their own: of every row tile (chunk_slot) its walk {tiles, skip}, of every sequence of the chunk kernel's {lowest position seen, the sinks aside, one
+    // behind the last}
     const int32_t* ranges;
     uint2* tile_bounds;
     uint2* bounds;
@@ -151,21 +152,28 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0; }
     __syncthreads();
-    const auto walk_in = [&](uint32_t i, uint32_t* sequence, ChunkTiles* tiles) {   // RANGED: of row tile i of all
+    // RANGED: row tiles differ by more than their place.  A thread has the walks of up to four of them at hand, of further ones it looks them up again.
+    constexpr uint32_t kAtHand = 4;
+    [[maybe_unused]] uint32_t walks[kAtHand];
+    [[maybe_unused]] const auto walk_in = [&](uint32_t i) {
         const uint32_t s = last_from(tile_starts, S, i);
-        const Span span = span_of(p.pool, s);
-        *sequence = s;
-        *tiles = tiles_of<true>(p, span, s);
-        return walk_between(p, p.tile_bounds[chunk_slot(span.first, p.group, s, tile_starts[s + 1] - 1 - i)], *tiles);
+        return p.tile_bounds[chunk_slot(span_of(p.pool, s).first, p.group, s, tile_starts[s + 1] - 1 - i)].x;
     };
-    if constexpr (RANGED) {   // row tiles differ by more than their place
-        for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
-            uint32_t s;
-            ChunkTiles t;
-            const uint32_t n = walk_in(i, &s, &t).tiles;
-            atomicMax(&sh.longest, n);
-            atomicAdd(&sh.work, 128ull * n * H);
+    if constexpr (RANGED) {
+        uint32_t most = 0, sum = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtHand; ++k) {
+            walks[k] = tid + k * kPrepareThreads < row_tiles ? walk_in(tid + k * kPrepareThreads) : 0;
+            most = max(most, walks[k]);
+            sum += walks[k];
         }
+        for (uint32_t i = tid + kAtHand * kPrepareThreads; i < row_tiles; i += kPrepareThreads) {
+            const uint32_t n = walk_in(i);
+            most = max(most, n);
+            sum += n;
+        }
+        atomicMax(&sh.longest, most);
+        atomicAdd(&sh.work, 128ull * sum * H);
     } else {
         for (uint32_t s = tid; s < S; s += kPrepareThreads)
             if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
@@ -173,25 +181,36 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     __syncthreads();
     const uint32_t longest = sh.longest;
     const auto piece_of = [&](uint32_t c) { return max(3u, (3 * longest + c + 2) / (c + 3)); };
-    const auto count = [&](uint32_t n, uint32_t tiles) {
-        for (uint32_t c = 0; c < kCandidates; ++c) {
-            const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
-            atomicAdd(&sh.items[c], n * pieces);
-            if (pieces > 1) atomicAdd(&sh.parts[c], n * pieces);
-        }
-    };
     if constexpr (RANGED) {
-        for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
-            uint32_t s;
-            ChunkTiles t;
-            count(H, walk_in(i, &s, &t).tiles);
+        // a warp's row tiles are added up ahead of the one addition to what all share
+        for (uint32_t c = 0; c < kCandidates; ++c) {
+            uint32_t items = 0, parts = 0;
+            const auto count = [&](uint32_t tiles) {
+                const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
+                items += H * pieces;
+                if (pieces > 1) parts += H * pieces;
+            };
+#pragma unroll
+            for (uint32_t k = 0; k < kAtHand; ++k)
+                if (tid + k * kPrepareThreads < row_tiles) count(walks[k]);
+            for (uint32_t i = tid + kAtHand * kPrepareThreads; i < row_tiles; i += kPrepareThreads) count(walk_in(i));
+            items = __reduce_add_sync(0xffffffffu, items);
+            parts = __reduce_add_sync(0xffffffffu, parts);
+            if ((tid & 31) == 0) {
+                atomicAdd(&sh.items[c], items);
+                atomicAdd(&sh.parts[c], parts);
+            }
         }
     } else {
         for (uint32_t s = tid; s < S; s += kPrepareThreads) {
             const uint32_t tiles = scratch_starts[s + 1] - scratch_starts[s], n = (tile_starts[s + 1] - tile_starts[s]) * H;
             if (n == 0) continue;
             atomicAdd(&sh.work, chunk_work(n, tiles, span_of(p.pool, s).tokens));
-            count(n, tiles);
+            for (uint32_t c = 0; c < kCandidates; ++c) {
+                const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
+                atomicAdd(&sh.items[c], n * pieces);
+                if (pieces > 1) atomicAdd(&sh.parts[c], n * pieces);
+            }
         }
     }
     __syncthreads();
@@ -227,8 +246,12 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
             item.base = span.base();
             item.length = span.length;
             item.row_tile = tile_starts[s + 1] - 1 - i;
-            if constexpr (RANGED) walk = walk_between(p, p.tile_bounds[chunk_slot(span.first, p.group, s, item.row_tile)], t);
-            else walk = walk_of(p, span, t, item.row_tile);
+            if constexpr (RANGED) {
+                const uint2 w = p.tile_bounds[chunk_slot(span.first, p.group, s, item.row_tile)];
+                walk = {w.x, w.y};
+            } else {
+                walk = walk_of(p, span, t, item.row_tile);
+            }
             if (scratch_starts[s] + t.tiles > p.scratch_tiles) walk.tiles = 0;   // no room for the copy
             item.scratch_row = scratch_starts[s] * kChunkTile;
             const uint32_t sink = RANGED || p.window > 0 ? (p.sinks + kChunkTile - 1) / kChunkTile : 0;
@@ -311,8 +334,9 @@ __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32
             q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
 }
 
-// What the tokens of each row tile and of each sequence see, the sinks aside: a block a sequence, a warp a row tile at a time.
-constexpr int kBoundsThreads = 512;
+// What the tokens of each row tile and of each sequence see, and what each row tile walks of it: a block a sequence, a warp four row tiles at a time, whose loads are under way
+// together (one at a time: 12 us for 193 row tiles, a trip to L2 each).
+constexpr int kBoundsThreads = 1024, kBoundsTiles = 4;
 __global__ void __launch_bounds__(kBoundsThreads) paged_bounds_kernel(const __grid_constant__ PrepareParams p) {
     __shared__ uint32_t lowest, end;
     pdl_launch_dependents();
@@ -323,23 +347,46 @@ __global__ void __launch_bounds__(kBoundsThreads) paged_bounds_kernel(const __gr
     const Span span = span_of(p.pool, s);
     if (!p.mine(span)) return;
     const uint32_t rows = span.tokens * p.group, row_tiles = p.row_tiles(span);
-    for (uint32_t r = threadIdx.x / 32; r < row_tiles; r += kBoundsThreads / 32) {
-        const uint32_t t_last = min((r + 1) * kChunkRows - 1, rows - 1) / p.group;
-        uint32_t low = 0xffffffffu, upto = 0;
-        for (uint32_t t = r * kChunkRows / p.group + lane; t <= t_last; t += 32) {
-            const Sight sight = sight_of(p.ranges, span.first + t, span.base() + static_cast<int>(t), p.window, span.length);
-            if (!sight.empty()) low = min(low, sight.low);
-            upto = max(upto, sight.empty() ? min(sight.upto, p.sinks) : sight.upto);
+    uint2* const of_tiles = p.tile_bounds + chunk_slot(span.first, p.group, s, 0);
+    for (uint32_t r0 = threadIdx.x / 32 * kBoundsTiles; r0 < row_tiles; r0 += kBoundsThreads / 32 * kBoundsTiles) {
+        uint32_t low[kBoundsTiles], upto[kBoundsTiles];
+#pragma unroll
+        for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+            low[i] = 0xffffffffu;
+            upto[i] = 0;
         }
-        low = __reduce_min_sync(0xffffffffu, low);
-        upto = __reduce_max_sync(0xffffffffu, upto);
-        if (lane == 0) {
-            p.tile_bounds[chunk_slot(span.first, p.group, s, r)] = make_uint2(low, upto);
-            atomicMin(&lowest, low);
-            atomicMax(&end, upto);
+        for (uint32_t t0 = lane; t0 <= kChunkRows / p.group; t0 += 32) {   // of a row tile's tokens (one more than that, where heads of one lie in two)
+            Sight sight[kBoundsTiles];
+#pragma unroll
+            for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+                const uint32_t r = r0 + i, t = r * kChunkRows / p.group + t0;
+                sight[i] = {0, 0};
+                if (r < row_tiles && t <= min((r + 1) * kChunkRows - 1, rows - 1) / p.group)
+                    sight[i] = sight_of(p.ranges, static_cast<size_t>(span.first) + t, span.base() + static_cast<int>(t), p.window, span.length);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+                if (!sight[i].empty()) low[i] = min(low[i], sight[i].low);
+                upto[i] = max(upto[i], sight[i].empty() ? min(sight[i].upto, p.sinks) : sight[i].upto);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+            low[i] = __reduce_min_sync(0xffffffffu, low[i]);
+            upto[i] = __reduce_max_sync(0xffffffffu, upto[i]);
+            if (lane == 0 && r0 + i < row_tiles) {
+                of_tiles[r0 + i] = make_uint2(low[i], upto[i]);
+                atomicMin(&lowest, low[i]);
+                atomicMax(&end, upto[i]);
+            }
         }
     }
     __syncthreads();
+    const ChunkTiles t = chunk_tiles_between(lowest, end, p.sinks);
+    for (uint32_t r = threadIdx.x; r < row_tiles; r += kBoundsThreads) {
+        const Walk walk = walk_between(p, of_tiles[r], t);
+        of_tiles[r] = make_uint2(walk.tiles, walk.skip);
+    }
     if (threadIdx.x == 0) p.bounds[s] = make_uint2(lowest, end);
 }
 

@@ -294,7 +294,12 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
             [[maybe_unused]] uint32_t seen_end = c.span.length;                                                       // and seen by nobody from here on
             [[maybe_unused]] float slope[4];             // of the rows, in log2 units, and their places
             [[maybe_unused]] int place[4];
+            [[maybe_unused]] const bool capped = [&] { if constexpr (kScored) return p.cap_log2 > 0.0f; else return false; }();
             if constexpr (kScored) {
+                if (capped) {                            // scores over the cap
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) qmul[r] *= p.cap_in;
+                }
                 first_upto = first_low = 0xffffffffu;
                 last_low = seen_end = 0;
                 for (uint32_t t = 0; t < c.span.tokens; ++t) {
@@ -342,6 +347,13 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                 constexpr int buf = decltype(buf_c)::value, sbuf = buf % L::kSBufs;
                 const uint32_t slot = i % L::kKUnits, vslot = i % L::kVUnits;
                 const uint32_t pos = c.t.position(c.tile + j) + t128;
+                [[maybe_unused]] float bias[4] = {};     // while the scores are on their way
+                if constexpr (kScored) {
+                    if (p.slopes != nullptr) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) bias[r] = -slope[r] * fabsf(static_cast<float>(place[r] - static_cast<int>(pos)));
+                    }
+                }
                 if (!failed && !mbar_wait_both_lane(bar(L::K_FULL + slot), (i / L::kKUnits) & 1, bar(L::S_FULL + sbuf), (i / L::kSBufs) & 1)) failed = true;
                 __syncwarp();
                 tc_fence_after();
@@ -396,31 +408,35 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                 if (lane == 0) mbar_arrive(bar(L::K_EMPTY + slot));      // the scales are read
                 const uint32_t pos0 = pos - t128;
                 bool any = true;
-                float qmul_now[4];
-                if constexpr (kScored) {   // what a score becomes, in base-2 units; the mask below leaves them as they are
+                if constexpr (kScored) {   // what a score becomes, in base-2 units; the mask below leaves it as it is.  One vote a warp: four branches a thread were 13 % of a step's time
+                    if (capped) {
+                        bool large = false;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[r] *= qmul[r];
-                        if (p.cap_log2 > 0.0f) {
-                            const float x = s[r] * p.cap_in;
-                            s[r] = p.cap_log2 * (fabsf(x) <= kTanhSmall ? tanh_small(x) : tanh_large(x));
+                        for (int r = 0; r < 4; ++r) {
+                            s[r] *= qmul[r];
+                            large |= fabsf(s[r]) > kTanhSmall;
                         }
-                        if (p.slopes != nullptr) s[r] = fmaf(-slope[r], fabsf(static_cast<float>(place[r] - static_cast<int>(pos))), s[r]);
-                        qmul_now[r] = 1.0f;
-                    }
-                } else {
+                        if (__any_sync(0xffffffffu, large)) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) qmul_now[r] = qmul[r];
+                            for (int r = 0; r < 4; ++r) s[r] = fmaf(p.cap_log2, tanh_large(s[r]), bias[r]);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[r] = fmaf(p.cap_log2, tanh_small(s[r]), bias[r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[r] = fmaf(s[r], qmul[r], bias[r]);
+                    }
                 }
                 if (pos0 + kDecodeTile <= first_upto && pos0 >= last_low) {   // every row sees all of the tile
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[r] *= qmul_now[r];
+                    for (int r = 0; r < 4; ++r) s[r] = kScored ? s[r] : s[r] * qmul[r];
                 } else {
                     any = false;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool seen = pos < upto[r] && (pos >= low[r] || pos < p.sinks);
-                        s[r] = seen ? s[r] * qmul_now[r] : -INFINITY;
+                        s[r] = seen ? (kScored ? s[r] : s[r] * qmul[r]) : -INFINITY;
                         any |= seen;
                     }
                 }

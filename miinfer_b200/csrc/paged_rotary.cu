@@ -7,8 +7,7 @@
 // angle's fraction of a turn, exact but for the table's own rounding (p 2^-65 turns).  Its upper 32 bits less the nearest quarter are the argument of a Taylor polynomial (to x^9 / x^8
 // on |x| <= pi/4, 3e-8).
 //
-// A lane holds eight consecutive elements, D/8 lanes a row (two rows a warp at head_dim 128).  Halves that are not in the lane come by a shuffle of what was loaded, as it
-// lies.  A warp takes all rows of a token, or several share them where there are few tokens; the token's sines and cosines are worked out once a warp.
+// A lane holds eight consecutive elements, D/8 lanes a row (two rows a warp at head_dim 128).  Halves that are not in the lane come by shuffles.  A warp takes all rows of a token, or several share them where there are few tokens; the token's sines and cosines are worked out once a warp.
 // Bound by HBM for prompts, by latency for a decode step.
 #include "append_row.cuh"
 #include "paged_common.cuh"
@@ -22,6 +21,7 @@ namespace b200kv {
 namespace {
 
 constexpr int kRotaryWarps = 4;
+constexpr uint32_t kAhead = 2;   // steps
 
 struct RotaryParams {
     Paged pool;
@@ -74,16 +74,6 @@ __device__ __forceinline__ void widen(const Eight<IN_F16>& r, float (&x)[8]) {
             x[2 * i] = __uint_as_float(w[2 * i]); x[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
         }
     }
-}
-template <bool IN_F16>
-__device__ __forceinline__ Eight<IN_F16> shuffle_eight(const Eight<IN_F16>& r, int from) {
-    Eight<IN_F16> o;
-#pragma unroll
-    for (int i = 0; i < (IN_F16 ? 1 : 2); ++i) {
-        o.v[i].x = __shfl_sync(0xffffffffu, r.v[i].x, from); o.v[i].y = __shfl_sync(0xffffffffu, r.v[i].y, from);
-        o.v[i].z = __shfl_sync(0xffffffffu, r.v[i].z, from); o.v[i].w = __shfl_sync(0xffffffffu, r.v[i].w, from);
-    }
-    return o;
 }
 __device__ __forceinline__ uint4 eight_halves(const float (&x)[8]) {
     uint32_t w[4];
@@ -163,66 +153,64 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) paged_rotary_kernel(const _
         }
     }
 
-    // ---- its rows: queries, keys, values, gates, a step at a time, the next one's on their way
+    // ---- its rows: queries with their gates, keys, values, a step at a time; kAhead steps' loads are under way
     const uint32_t H = pool.view.kv_heads;
-    const uint32_t q_steps = p.q != nullptr ? (p.query_heads + kRows - 1) / kRows : 0, k_steps = p.key != nullptr ? (H + kRows - 1) / kRows : 0;
-    const uint32_t k0 = q_steps, v0 = k0 + k_steps, g0 = v0 + k_steps, steps = g0 + (p.gate != nullptr ? q_steps : 0);
-    const uint32_t q_width = p.gate != nullptr ? 2 * D : D;
-    enum { QUERY, KEY, VALUE, GATE };
+    const uint32_t k0 = p.q != nullptr ? (p.query_heads + kRows - 1) / kRows : 0, kv_steps = p.key != nullptr ? (H + kRows - 1) / kRows : 0, v0 = k0 + kv_steps, steps = v0 + kv_steps;
+    const bool gated = p.gate != nullptr;
+    enum { QUERY, KEY, VALUE };
     struct Step { int kind; uint32_t head; bool there; };
     const auto step_of = [&](uint32_t t) {
-        const int kind = t < k0 ? QUERY : t < v0 ? KEY : t < g0 ? VALUE : GATE;
-        const uint32_t head = (t - (kind == QUERY ? 0 : kind == KEY ? k0 : kind == VALUE ? v0 : g0)) * kRows + sub;
-        return Step{kind, head, head < (kind == KEY || kind == VALUE ? H : p.query_heads)};
+        const int kind = t < k0 ? QUERY : t < v0 ? KEY : VALUE;
+        const uint32_t head = (t - (kind == QUERY ? 0 : kind == KEY ? k0 : v0)) * kRows + sub;
+        return Step{kind, head, t < steps && head < (kind == QUERY ? p.query_heads : H)};
     };
-    const auto fetch = [&](uint32_t t) {
-        Eight<IN_F16> r{};
+    using Raw = Eight<IN_F16>;
+    Raw raw[kAhead], raw_gate[kAhead];
+    const auto fetch = [&](uint32_t t, Raw& r, Raw& g) {
         const Step at = step_of(t);
-        if (!at.there) return r;
-        if (at.kind == KEY) return load_eight<IN_F16>(p.key, token * p.key_stride + at.head * D + c * 8);
-        if (at.kind == VALUE) return load_eight<IN_F16>(p.value, token * p.value_stride + at.head * D + c * 8);
-        return load_eight<IN_F16>(p.q, token * p.q_stride + static_cast<uint64_t>(at.head) * q_width + (at.kind == GATE ? D : 0) + c * 8);
+        r = g = Raw{};
+        if (!at.there) return;
+        if (at.kind == QUERY) {
+            const size_t element = token * p.q_stride + static_cast<size_t>(at.head) * (gated ? 2 * D : D) + c * 8;
+            r = load_eight<IN_F16>(p.q, element);
+            if (gated) g = load_eight<IN_F16>(p.q, element + D);
+        } else {
+            r = at.kind == KEY ? load_eight<IN_F16>(p.key, token * p.key_stride + at.head * D + c * 8) : load_eight<IN_F16>(p.value, token * p.value_stride + at.head * D + c * 8);
+        }
     };
-    float w[8], w_other[8];
+    float w[8];
     int weighed = -1;                                    // whose norm's weights these are
-    Eight<IN_F16> raw = part < steps ? fetch(part) : Eight<IN_F16>{};
-    for (uint32_t t = part; t < steps; t += p.share) {
-        const Eight<IN_F16> now = raw;
-        if (t + p.share < steps) raw = fetch(t + p.share);
+    const auto take = [&](uint32_t t, const Raw& now, const Raw& now_gate) {
         const Step at = step_of(t);
         float x[8];
         widen<IN_F16>(now, x);
-        const size_t out = (static_cast<size_t>(token) * p.query_heads + at.head) * D + c * 8;
-        if (at.kind == GATE) {
-            if (at.there) store_floats(p.gate + out, x);
-            continue;
-        }
         if (at.kind == VALUE) {
             store_row<D>(pool.view, false, row0 + (static_cast<long long>(at.head) << pool.page_shift), x, c, at.there && row0 >= 0);
-            continue;
-        }
-        float y[8];
-        if (p.neighbours) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else {
-            widen<IN_F16>(shuffle_eight<IN_F16>(now, static_cast<int>(sub * kLanes + other)), y);
+            return;
         }
         const float* norm = at.kind == QUERY ? p.q_norm : p.k_norm;
         if (norm != nullptr) {
             if (weighed != at.kind) {
                 weighed = at.kind;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { w[i] = norm[c * 8 + i]; w_other[i] = norm[other * 8 + (p.neighbours ? i ^ 1 : i)]; }
+                for (int i = 0; i < 8; ++i) w[i] = norm[c * 8 + i];
             }
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float inv = __frsqrt_rn(__fdiv_rn(sum, static_cast<float>(D)) + p.epsilon);
+            const float inv = __frsqrt_rn(fmaf(sum, 1.0f / D, p.epsilon));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { x[i] = x[i] * inv * w[i]; y[i] = y[i] * inv * w_other[i]; }
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+        }
+        float y[8];
+        if (p.neighbours) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], static_cast<int>(sub * kLanes + other));
         }
         if (turns) {   // (an infinity in the rest of a head stays one)
 #pragma unroll
@@ -231,8 +219,26 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) paged_rotary_kernel(const _
         if (at.kind == KEY) {
             store_row<D>(pool.view, true, row0 + (static_cast<long long>(at.head) << pool.page_shift), x, c, at.there && row0 >= 0);
         } else if (at.there) {
+            const size_t out = (static_cast<size_t>(token) * p.query_heads + at.head) * D + c * 8;
             if (p.q_out_is_f16) *reinterpret_cast<uint4*>(static_cast<__half*>(p.q_out) + out) = eight_halves(x);
             else store_floats(static_cast<float*>(p.q_out) + out, x);
+            if (gated) {
+                float g[8];
+                widen<IN_F16>(now_gate, g);
+                store_floats(p.gate + out, g);
+            }
+        }
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) fetch(part + i * p.share, raw[i], raw_gate[i]);
+    for (uint32_t t0 = part; t0 < steps; t0 += kAhead * p.share) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t t = t0 + i * p.share;
+            if (t >= steps) break;
+            const Raw now = raw[i], now_gate = raw_gate[i];
+            fetch(t + kAhead * p.share, raw[i], raw_gate[i]);
+            take(t, now, now_gate);
         }
     }
 }
@@ -348,7 +354,7 @@ int b200kv_paged_rotary(const b200kv_paged_view* view, const b200kv_paged_batch*
                    value_stride, q_norm_weight, k_norm_weight, positions, q_out, q_out_dtype == B200KV_F16, gate, q != nullptr ? query_heads : 0, 1};
     // Warps to a token: one, or as many as there are steps where the tokens alone do not occupy the device.
     const uint32_t at_once = view->head_dim == 128 ? 2 : 1;
-    const uint64_t steps = (p.query_heads + at_once - 1) / at_once * (gate != nullptr ? 2 : 1) + (key != nullptr ? 2 * ((view->kv_heads + at_once - 1) / at_once) : 0);
+    const uint64_t steps = (p.query_heads + at_once - 1) / at_once + (key != nullptr ? 2 * ((view->kv_heads + at_once - 1) / at_once) : 0);
     p.share = static_cast<uint32_t>(std::min<uint64_t>(steps, std::max<uint64_t>(1, 32ull * device_sms() / tokens)));
     if (tokens * p.share > 0x7fffffffull) return B200KV_ERR_RANGE;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

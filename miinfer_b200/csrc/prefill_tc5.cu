@@ -104,8 +104,8 @@ template <> struct KernelParams<true, false> : Tc5Params {   // of the base: map
     uint32_t window, sinks;
 };
 template <> struct KernelParams<true, true> : KernelParams<true, false> {   // scale_log2: what the softmax multiplies what it is given by
-    float cap_in;                // scale / cap
-    float slope_scale;           // kSloped without a cap: scale * log2 e
+    // kCapped, of a score s = q.k: cap * tanh(cap_in s) in log2 units is s (cap_poly[0] + cap_poly[1] s^2 + ..) for |s| <= cap_small, cap_log2 * tanh(cap_in s) for any
+    float cap_in, cap_log2, cap_small, cap_poly[4];
     const float* slopes;
     const int32_t* ranges;       // may be null
 };
@@ -295,9 +295,16 @@ struct RowOffsets {
     }
 };
 
-// tanh(k s) of a tile's scores, in place.  Where no row of the warp has |k s| above kTanhSmall, by a polynomial, two values to an instruction: as many fp32 instructions as the rest of
-// the loop has, but none of the special function unit, which the exponentials keep busy.  Otherwise by two of its functions a value.
-__device__ __forceinline__ void cap_scores(float (&s)[kBN], float k) {
+// A score's capped form over the score itself, for two scores whose squares are given (KernelParams::cap_poly).
+template <class Params>
+__device__ __forceinline__ Pair cap_factor(const Params& p, Pair squares) {
+    Pair r = pack_pair(p.cap_poly[3], p.cap_poly[3]);
+#pragma unroll
+    for (int j = 2; j >= 0; --j) r = fma_pair(r, squares, pack_pair(p.cap_poly[j], p.cap_poly[j]));
+    return r;
+}
+// The largest magnitude of a tile's scores (NaN has no say).
+__device__ __forceinline__ float largest_of(const float (&s)[kBN]) {
     float m4[4] = {fabsf(s[0]), fabsf(s[1]), fabsf(s[2]), fabsf(s[3])};
 #pragma unroll
     for (int i = 4; i + 8 <= kBN; i += 8)
@@ -305,22 +312,22 @@ __device__ __forceinline__ void cap_scores(float (&s)[kBN], float k) {
         for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], fabsf(s[i + c]), fabsf(s[i + 4 + c]));
 #pragma unroll
     for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fabsf(s[kBN - 4 + c]));
-    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k > kTanhSmall)) {   // (a row of NaN has no say)
-        const float c[6] = {0.99999994f, -0.333326757f, 0.13321048f, -0.0531143136f, 0.0190933011f, -0.00435529929f};
-        const Pair k2 = pack_pair(k, k);
+    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+}
+// A tile's scores in log2 units, capped, in place.
+template <class Params>
+__device__ __forceinline__ void cap_scores(const Params& p, float (&s)[kBN], bool small) {
+    if (small) {
 #pragma unroll
         for (int i = 0; i < kBN; i += 2) {
-            const Pair x = mul_pair(pack_pair(s[i], s[i + 1]), k2), u = mul_pair(x, x);
-            Pair r = pack_pair(c[5], c[5]);
-#pragma unroll
-            for (int j = 4; j >= 0; --j) r = fma_pair(r, u, pack_pair(c[j], c[j]));
-            const float2 t = unpack_pair(mul_pair(x, r));
+            const Pair x = pack_pair(s[i], s[i + 1]);
+            const float2 t = unpack_pair(mul_pair(x, cap_factor(p, mul_pair(x, x))));
             s[i] = t.x;
             s[i + 1] = t.y;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kBN; ++i) s[i] = tanh_large(s[i] * k);
+        for (int i = 0; i < kBN; ++i) s[i] = tanh_large(s[i] * p.cap_in) * p.cap_log2;
     }
 }
 
@@ -832,7 +839,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 m_known = m_new;
             }
         };
-        const float to_log2 = (SCORE & kSloped) != 0 ? 1.0f : p.scale_log2;   // biased scores are in log2 units already
+        const float to_log2 = (SCORE & (kCapped | kSloped)) != 0 ? 1.0f : p.scale_log2;   // capped or biased scores are in log2 units already
         const int buf = rt * L::kGroups + grp;
         const uint32_t s_col = L::kColS + buf * kBN, o_col = L::kColO + rt * D;
         const int nt = L::kGroups == 4 ? (walked + grp + 1) / 2 : walked;
@@ -860,22 +867,28 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // Raw scores stay unscaled; the softmax scale is folded into the exponent: p = 2^(s*c - m*c).  The loop's instructions count: products and
             // sums go in pairs, maxima three values at a time.  32 / 8 heads of 128, 1024 tokens over 8192: 168.0 -> 163.7 us; 24 / 4 of 256, 512 over
             // 8192: 111.6 -> 110.3.
-            if constexpr ((SCORE & kCapped) != 0) cap_scores(s, p.cap_in);
+            // A cap.  cap * tanh(x / cap) grows with x, so the largest of the tile is that of the largest score; where no row of the warp has scores past half the cap or positions that it
+            // does not see, all the others become theirs within the exponent: a square and a polynomial of the third degree in it, two values to an instruction, and none of the
+            // special function unit, which the exponentials keep busy.  Otherwise they are capped in place, ahead of the mask.
+            [[maybe_unused]] bool within = false;
+            if constexpr ((SCORE & kCapped) != 0) {
+                const bool small = !__any_sync(0xffffffffu, largest_of(s) > p.cap_small);
+                if constexpr ((SCORE & kSloped) == 0) within = small && !__any_sync(0xffffffffu, pos0 + kBN > len || pos0 < low);
+                if (!within) cap_scores(p, s, small);
+            }
             if constexpr ((SCORE & kSloped) != 0) {
-                const float of_scores = (SCORE & kCapped) != 0 ? p.scale_log2 : p.slope_scale;
-                const int ahead = static_cast<int>(pos0) - place;   // of the tile's first position, from the token's
-                if (ahead + kBN <= 1) {                             // nothing behind the token: the distance falls from position to position
-                    const float first = slope * static_cast<float>(ahead);
-                    const Pair scale2 = pack_pair(of_scores, of_scores);
+                const float of_scores = (SCORE & kCapped) != 0 ? 1.0f : p.scale_log2, ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the first position, from the token's
+                if (ahead + kBN <= 1.0f) {   // nothing behind the token: the distance falls from position to position
+                    const Pair scale2 = pack_pair(of_scores, of_scores), slope2 = pack_pair(slope, slope), first2 = pack_pair(slope * ahead, slope * ahead);
 #pragma unroll
                     for (int i = 0; i < kBN; i += 2) {
-                        const float2 x = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, pack_pair(fmaf(static_cast<float>(i), slope, first), fmaf(static_cast<float>(i + 1), slope, first))));
+                        const float2 x = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, fma_pair(slope2, pack_pair(static_cast<float>(i), static_cast<float>(i + 1)), first2)));
                         s[i] = x.x;
                         s[i + 1] = x.y;
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kBN; ++i) s[i] = fmaf(s[i], of_scores, -slope * fabsf(static_cast<float>(ahead + i)));
+                    for (int i = 0; i < kBN; ++i) s[i] = fmaf(s[i], of_scores, -slope * fabsf(ahead + static_cast<float>(i)));
                 }
             }
             // Only the tiles that straddle this row's causal length need the mask.
@@ -896,7 +909,10 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], s[i + c], s[i + 4 + c]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], s[kBN - 4 + c]);
-            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * to_log2;   // scale > 0: the maximum commutes with it
+            float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * to_log2;   // scale > 0: the maximum commutes with it
+            if constexpr ((SCORE & kCapped) != 0) {
+                if (within) mt *= unpack_pair(cap_factor(p, pack_pair(mt * mt, 0.0f))).x;
+            }
             // the reference as the previous tile (another group's) left it; lazy rescale: keep it unless this tile's
             // maximum outgrew it by more than the threshold
             float m_prev = -INFINITY;
@@ -924,9 +940,8 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             Pair sum = 0;
             uint32_t pk[kBN / 2];
             const Pair scale2 = pack_pair(to_log2, to_log2), ref2 = pack_pair(neg_ref, neg_ref);
-#pragma unroll
-            for (int i = 0; i < kBN; i += 2) {
-                const float2 e = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, ref2));
+            const auto weigh = [&](int i, Pair exponents) {
+                const float2 e = unpack_pair(exponents);
                 const float w0 = ex2_approx(e.x), w1 = ex2_approx(e.y);
                 const __half2 h = __floats2half2_rn(w0, w1);
                 pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
@@ -936,6 +951,16 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                     const float2 hf = __half22float2(h);
                     sum = add_pair(sum, pack_pair(hf.x, hf.y));
                 }
+            };
+            if ((SCORE & kCapped) != 0 && within) {
+#pragma unroll
+                for (int i = 0; i < kBN; i += 2) {
+                    const Pair x = pack_pair(s[i], s[i + 1]);
+                    if constexpr ((SCORE & kCapped) != 0) weigh(i, fma_pair(x, cap_factor(p, mul_pair(x, x)), ref2));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kBN; i += 2) weigh(i, fma_pair(pack_pair(s[i], s[i + 1]), scale2, ref2));
             }
             {
                 const float2 halves = unpack_pair(sum);
@@ -1504,10 +1529,15 @@ int launch_chunk(const ChunkLaunch& c, cudaStream_t stream) {
     const bool capped = c.cap > 0.0f;
     p.slopes = c.slopes;
     p.ranges = c.ranges;
-    p.slope_scale = c.scale_log2;
     if (capped) {
         p.cap_in = c.scale / c.cap;
-        p.scale_log2 = c.cap * 1.4426950408889634f;
+        p.cap_log2 = c.cap * 1.4426950408889634f;
+        // tanh(x) / x for |x| <= 1/2 by powers of x^2: the polynomial of the third degree with the smallest relative error, 5.4e-7 (Remez's exchange), a tenth of a millionth of
+        // the cap and a thousandth of what the weights' rounding to fp16 is to a score.  Where its coefficients would leave fp32's range no score is small.
+        const double tanh_poly[4] = {0.9999994558, -0.3332631794, 0.131902966, -0.04440222613}, k = static_cast<double>(c.scale) / c.cap;
+        p.cap_small = k < 1.0e4 ? static_cast<float>(0.5 / k) : -1.0f;
+        double power = static_cast<double>(c.scale) * 1.4426950408889634;
+        for (int j = 0; j < 4; ++j, power *= k * k) p.cap_poly[j] = k < 1.0e4 ? static_cast<float>(tanh_poly[j] * power) : 0.0f;
     }
     return c.head_dim == 256 ? launch_scored<256>(p, capped, c.max_items, stream) : launch_scored<128>(p, capped, c.max_items, stream);
 }
