@@ -49,6 +49,7 @@ struct PrepareParams {
     const int32_t* ranges;
     uint2* tile_bounds;
     uint2* bounds;
+    uint2* walks;               // the same as tile_bounds, in the list's order
     __device__ __forceinline__ bool mine(const Span& span) const { return span.tokens > 0 && static_cast<uint64_t>(span.tokens) * group > few_rows; }
     __device__ __forceinline__ uint32_t row_tiles(const Span& span) const { return (span.tokens * group + kChunkRows - 1) / kChunkRows; }
 };
@@ -152,28 +153,23 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     if (tid < kCandidates) sh.items[tid] = sh.parts[tid] = 0;
     if (tid == 0) { sh.longest = 0; sh.work = 0; }
     __syncthreads();
-    // RANGED: row tiles differ by more than their place.  A thread has the walks of up to four of them at hand, of further ones it looks them up again.
-    constexpr uint32_t kAtHand = 4;
-    [[maybe_unused]] uint32_t walks[kAtHand];
-    [[maybe_unused]] const auto walk_in = [&](uint32_t i) {
-        const uint32_t s = last_from(tile_starts, S, i);
-        return p.tile_bounds[chunk_slot(span_of(p.pool, s).first, p.group, s, tile_starts[s + 1] - 1 - i)].x;
-    };
-    if constexpr (RANGED) {
-        uint32_t most = 0, sum = 0;
+    if constexpr (RANGED) {   // row tiles differ by more than their place
+        uint32_t most = 0;
+        unsigned long long sum = 0;
+        for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
+            const uint32_t s = last_from(tile_starts, S, i);
+            const uint2 walk = p.tile_bounds[chunk_slot(span_of(p.pool, s).first, p.group, s, tile_starts[s + 1] - 1 - i)];
+            p.walks[i] = walk;
+            most = max(most, walk.x);
+            sum += walk.x;
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
-        for (uint32_t k = 0; k < kAtHand; ++k) {
-            walks[k] = tid + k * kPrepareThreads < row_tiles ? walk_in(tid + k * kPrepareThreads) : 0;
-            most = max(most, walks[k]);
-            sum += walks[k];
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((tid & 31) == 0) {   // (an addition a thread to 64 bits that all share: 8 us)
+            atomicMax(&sh.longest, most);
+            atomicAdd(&sh.work, 128ull * sum * H);
         }
-        for (uint32_t i = tid + kAtHand * kPrepareThreads; i < row_tiles; i += kPrepareThreads) {
-            const uint32_t n = walk_in(i);
-            most = max(most, n);
-            sum += n;
-        }
-        atomicMax(&sh.longest, most);
-        atomicAdd(&sh.work, 128ull * sum * H);
     } else {
         for (uint32_t s = tid; s < S; s += kPrepareThreads)
             if (const uint32_t n = scratch_starts[s + 1] - scratch_starts[s]; n > 0) atomicMax(&sh.longest, n);
@@ -182,23 +178,36 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
     const uint32_t longest = sh.longest;
     const auto piece_of = [&](uint32_t c) { return max(3u, (3 * longest + c + 2) / (c + 3)); };
     if constexpr (RANGED) {
-        // a warp's row tiles are added up ahead of the one addition to what all share
-        for (uint32_t c = 0; c < kCandidates; ++c) {
-            uint32_t items = 0, parts = 0;
-            const auto count = [&](uint32_t tiles) {
-                const uint32_t pieces = c == 0 ? 1 : max(1u, (tiles + piece_of(c) - 1) / piece_of(c));
-                items += H * pieces;
-                if (pieces > 1) parts += H * pieces;
-            };
+        // A warp has every eighth candidate and goes over all row tiles; quotients by a reciprocal, put right.  (All candidates by all threads, added up a warp at a time: 16 us for 348 row
+        // tiles.)
+        constexpr uint32_t kWarps = kPrepareThreads / 32, kEach = (kCandidates + kWarps - 1) / kWarps;
+        const uint32_t warp = tid / 32;
+        uint32_t items[kEach] = {}, parts[kEach] = {}, size[kEach];
+        float over[kEach];
 #pragma unroll
-            for (uint32_t k = 0; k < kAtHand; ++k)
-                if (tid + k * kPrepareThreads < row_tiles) count(walks[k]);
-            for (uint32_t i = tid + kAtHand * kPrepareThreads; i < row_tiles; i += kPrepareThreads) count(walk_in(i));
-            items = __reduce_add_sync(0xffffffffu, items);
-            parts = __reduce_add_sync(0xffffffffu, parts);
-            if ((tid & 31) == 0) {
-                atomicAdd(&sh.items[c], items);
-                atomicAdd(&sh.parts[c], parts);
+        for (uint32_t k = 0; k < kEach; ++k) {
+            size[k] = warp + k * kWarps == 0 ? 0x7fffffffu : piece_of(warp + k * kWarps);
+            over[k] = 1.0f / static_cast<float>(size[k]);
+        }
+        for (uint32_t i = tid & 31; i < row_tiles; i += 32) {
+            const uint32_t tiles = p.walks[i].x;
+#pragma unroll
+            for (uint32_t k = 0; k < kEach; ++k) {
+                uint32_t pieces = static_cast<uint32_t>(static_cast<float>(tiles) * over[k]);   // of up to a dozen: off by one at most
+                if (static_cast<uint64_t>(pieces) * size[k] < tiles) ++pieces;
+                else if (pieces > 0 && static_cast<uint64_t>(pieces - 1) * size[k] >= tiles) --pieces;
+                pieces = max(pieces, 1u);
+                items[k] += H * pieces;
+                parts[k] += pieces > 1 ? H * pieces : 0;
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; ++k) {
+            items[k] = __reduce_add_sync(0xffffffffu, items[k]);
+            parts[k] = __reduce_add_sync(0xffffffffu, parts[k]);
+            if ((tid & 31) == 0 && warp + k * kWarps < kCandidates) {
+                sh.items[warp + k * kWarps] = items[k];
+                sh.parts[warp + k * kWarps] = parts[k];
             }
         }
     } else {
@@ -247,7 +256,7 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
             item.length = span.length;
             item.row_tile = tile_starts[s + 1] - 1 - i;
             if constexpr (RANGED) {
-                const uint2 w = p.tile_bounds[chunk_slot(span.first, p.group, s, item.row_tile)];
+                const uint2 w = p.walks[i];
                 walk = {w.x, w.y};
             } else {
                 walk = walk_of(p, span, t, item.row_tile);
@@ -269,8 +278,13 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
                 if (n > 1) p.groups[group++] = at;
                 for (uint32_t z = 0; z < n; ++z, ++at) {
                     item.kv_head = h;
-                    item.tile0 = static_cast<uint32_t>(static_cast<uint64_t>(walk.tiles) * z / n);
-                    item.tiles = static_cast<uint32_t>(static_cast<uint64_t>(walk.tiles) * (z + 1) / n) - item.tile0;
+                    if (RANGED && n == 1) {   // (64-bit divisions: as long as all the rest)
+                        item.tile0 = 0;
+                        item.tiles = walk.tiles;
+                    } else {
+                        item.tile0 = static_cast<uint32_t>(static_cast<uint64_t>(walk.tiles) * z / n);
+                        item.tiles = static_cast<uint32_t>(static_cast<uint64_t>(walk.tiles) * (z + 1) / n) - item.tile0;
+                    }
                     item.part = n > 1 ? part++ : kNoPart;
                     item.parts = n;
                     p.items[at] = item;
@@ -559,7 +573,7 @@ struct Room {
     uint64_t scratch_tiles;    // of all sequences together
     uint32_t max_items, max_parts;
     bool decode, chunks;       // which kernels the call may need
-    size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, tile_bounds, bounds, bytes;   // offsets
+    size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, tile_bounds, bounds, walks, bytes;   // offsets
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
@@ -602,6 +616,7 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
     if (ranged) {
         r.tile_bounds = take((batch.total_tokens * group / kChunkRows + batch.sequences + 1) * sizeof(uint2));
+        r.walks = take((batch.total_tokens * group / kChunkRows + batch.sequences + 1) * sizeof(uint2));
         r.bounds = take(static_cast<uint64_t>(batch.sequences) * sizeof(uint2));
     }
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
@@ -669,7 +684,7 @@ int attend(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const
                                room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
                                view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.5f, 7.0f, 1.0f, 2.0f, 0.02f},
                                {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}, ranged ? scoring->ranges : nullptr,
-                               reinterpret_cast<uint2*>(ws + room.tile_bounds), reinterpret_cast<uint2*>(ws + room.bounds)};
+                               reinterpret_cast<uint2*>(ws + room.tile_bounds), reinterpret_cast<uint2*>(ws + room.bounds), reinterpret_cast<uint2*>(ws + room.walks)};
         const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
         const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;
         static std::atomic<uint64_t> done[4];

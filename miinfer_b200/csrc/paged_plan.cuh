@@ -12,7 +12,7 @@ constexpr uint32_t kNoPart = 0xffffffffu;
 
 // What one CTA of the chunk kernel does: one row tile of one sequence and kv head, over some of its KV tiles.  A sequence's tiles are those of its
 // copy in the scratch: first the tiles of the sinks, if the window leaves a gap behind them, then those from position `window0` on.
-struct ChunkItem {
+struct alignas(16) ChunkItem {   // written and read 16 bytes at a time
     uint32_t first, tokens;    // the sequence's rows of the activations
     int32_t base;              // place in the cache of its first new token
     uint32_t row_tile, kv_head;

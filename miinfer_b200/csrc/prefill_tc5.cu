@@ -547,7 +547,16 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     bool failed = false;
     // The query rows of the CTA that takes this one's place, as far as the order of dispatch tells.  A warp.
     auto next_q = [&] {
-        if constexpr (PAGED) return;
+        if constexpr (PAGED && SCORE == 0) return;
+        if constexpr (PAGED && SCORE != 0) {   // short walks, as of documents, are half set-up
+            const uint32_t next = blockIdx.x + p.sms;
+            if (next >= p.plan->items) return;
+            const ChunkItem x = reload(p.items + next);
+            const uint32_t elem = p.q_is_f16 ? 2 : 4, r0 = x.row_tile * L::kRows, t_last = (min(r0 + L::kRows, x.tokens * G) - 1) / G;
+            for (uint32_t t = r0 / G + lane; t <= t_last; t += 32)
+                prefetch_l2(static_cast<const uint8_t*>(p.q) + ((static_cast<size_t>(x.first) + t) * p.query_heads + x.kv_head * G) * D * elem, G * D * elem);
+            return;
+        }
         const uint32_t next = blockIdx.x + p.sms;
         if (next < gridDim.x && next % p.kv_splits == 0)
             prefetch_q(((total_rows + L::kRows - 1) / L::kRows - 1 - next / p.kv_splits / p.kv_heads) * L::kRows, next / p.kv_splits % p.kv_heads);
@@ -621,6 +630,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             for (uint32_t t = row0 / G + lane; t <= t_last; t += 32)
                 prefetch_l2(p.gate + own_rows + (static_cast<size_t>(t) * p.query_heads + kv_head * G) * D, G * D * 4);
         }
+        if constexpr (SCORE != 0) next_q();
         bool ok = have_q;
         if (lane == 0)
             for (int j = 0; ok && j < whole_tiles; ++j) ok = load_v(j);
@@ -879,13 +889,24 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             if constexpr ((SCORE & kSloped) != 0) {
                 const float of_scores = (SCORE & kCapped) != 0 ? 1.0f : p.scale_log2, ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the first position, from the token's
                 if (ahead + kBN <= 1.0f) {   // nothing behind the token: the distance falls from position to position
-                    const Pair scale2 = pack_pair(of_scores, of_scores), slope2 = pack_pair(slope, slope), first2 = pack_pair(slope * ahead, slope * ahead);
+                    // four chains of sums of two values a step, eight roundings long (a product for each position's own: 64 more instructions, 280 us in place of ? for 1333 tokens over 6500)
+                    const Pair scale2 = pack_pair(of_scores, of_scores), step2 = pack_pair(2.0f * slope, 2.0f * slope);
+                    Pair bias[4];
 #pragma unroll
-                    for (int i = 0; i < kBN; i += 2) {
-                        const float2 x = unpack_pair(fma_pair(pack_pair(s[i], s[i + 1]), scale2, fma_pair(slope2, pack_pair(static_cast<float>(i), static_cast<float>(i + 1)), first2)));
-                        s[i] = x.x;
-                        s[i + 1] = x.y;
+                    for (int c = 0; c < 4; ++c) {
+                        const float first = slope * (ahead + static_cast<float>(16 * c));
+                        bias[c] = pack_pair(first, first + slope);
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int at = 16 * c + i;
+                            const float2 x = unpack_pair(fma_pair(pack_pair(s[at], s[at + 1]), scale2, bias[c]));
+                            s[at] = x.x;
+                            s[at + 1] = x.y;
+                            bias[c] = add_pair(bias[c], step2);
+                        }
                 } else {
 #pragma unroll
                     for (int i = 0; i < kBN; ++i) s[i] = fmaf(s[i], of_scores, -slope * fabsf(ahead + static_cast<float>(i)));
