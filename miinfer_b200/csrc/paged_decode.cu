@@ -327,8 +327,11 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) acc[h][r] = pend[0][h][r] = pend[1][h][r] = 0.0f;
             }
-            auto fold = [&](auto buf_c) {                // the sums of a tile into the accumulators of this thread's dims
-                constexpr int buf = decltype(buf_c)::value;
+            // The step is compiled once for each of the two buffers, which lie in registers -- but for scored instances, whose longer text would not stay in the instruction caches (1.6
+            // warps an issue without an instruction in place of 0.7, 48 sequences of up to 14000: 149 us and 126): theirs have the factors of the last two tiles move up instead.
+            const auto number = [](auto x) { if constexpr (std::is_same_v<decltype(x), int>) return x; else return decltype(x)::value; };
+            auto fold = [&](auto buf_c, int of) {        // the sums of a tile into the accumulators of this thread's dims
+                const int buf = number(buf_c);
                 int o[kHalves][8];
                 tc_fence_after();
 #pragma unroll
@@ -340,11 +343,11 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float v = VF == F16 ? terms(__int_as_float(o[h][r]), __int_as_float(o[h][4 + r])) : static_cast<float>(o[h][r] * 256 + o[h][4 + r]);
-                        acc[h][r] = fmaf(v, pend[buf][h][r], acc[h][r]);
+                        acc[h][r] = fmaf(v, pend[kScored ? of : buf][h][r], acc[h][r]);
                     }
             };
             auto step = [&](auto buf_c, uint32_t j) {
-                constexpr int buf = decltype(buf_c)::value, sbuf = buf % L::kSBufs;
+                const int buf = number(buf_c), sbuf = L::kSBufs == 2 ? buf : 0;
                 const uint32_t slot = i % L::kKUnits, vslot = i % L::kVUnits;
                 const uint32_t pos = c.t.position(c.tile + j) + t128;
                 [[maybe_unused]] float bias[4] = {};     // while the scores are on their way
@@ -408,7 +411,7 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                 if (lane == 0) mbar_arrive(bar(L::K_EMPTY + slot));      // the scales are read
                 const uint32_t pos0 = pos - t128;
                 bool any = true;
-                if constexpr (kScored) {   // what a score becomes, in base-2 units; the mask below leaves it as it is.  One vote a warp: four branches a thread were 13 % of a step's time
+                if constexpr (kScored) {   // what a score becomes, in base-2 units; the mask below leaves it as it is
                     if (capped) {
                         bool large = false;
 #pragma unroll
@@ -416,13 +419,15 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                             s[r] *= qmul[r];
                             large |= fabsf(s[r]) > kTanhSmall;
                         }
-                        if (__any_sync(0xffffffffu, large)) {
+                        if (__any_sync(0xffffffffu, large)) {   // (of values from one on; a value far below one has all its digits from the polynomial alone)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) s[r] = fmaf(p.cap_log2, tanh_large(s[r]), bias[r]);
+                            for (int r = 0; r < 4; ++r) s[r] = fabsf(s[r]) > kTanhSmall ? tanh_large(s[r]) : tanh_small(s[r]);
                         } else {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) s[r] = fmaf(p.cap_log2, tanh_small(s[r]), bias[r]);
+                            for (int r = 0; r < 4; ++r) s[r] = tanh_small(s[r]);
                         }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[r] = fmaf(p.cap_log2, s[r], bias[r]);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[r] = fmaf(s[r], qmul[r], bias[r]);
@@ -572,12 +577,19 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                 if (j >= 2) {
                     wait(bar(L::P_EMPTY + buf * RG + g), ((i >> 1) & 1) ^ 1);
                     __syncwarp();
-                    fold(buf_c);
+                    fold(buf_c, 0);
                 }
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) pend[buf][h][r] = scale_now[h][r];
+                    for (int r = 0; r < 4; ++r) {
+                        if constexpr (kScored) {
+                            pend[0][h][r] = pend[1][h][r];
+                            pend[1][h][r] = scale_now[h][r];
+                        } else {
+                            pend[buf][h][r] = scale_now[h][r];
+                        }
+                    }
                 const uint32_t pt = sbase + L::kOffP + (buf * RG + g) * L::kPBytes + t128 * 32;
 #pragma unroll
                 for (int x = 0; x < L::kPSets; ++x) {
@@ -592,7 +604,8 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
             using Buf0 = std::integral_constant<int, 0>;
             using Buf1 = std::integral_constant<int, 1>;
             for (uint32_t j = 0; j < n; ++j) {
-                if ((i & 1) == 0) step(Buf0{}, j);
+                if constexpr (kScored) step(static_cast<int>(i & 1), j);
+                else if ((i & 1) == 0) step(Buf0{}, j);
                 else step(Buf1{}, j);
             }
             // ---- the pair's end: row sums, the last two tiles' sums ----
@@ -603,8 +616,14 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
                 const uint32_t x = i - back;
                 wait(bar(L::P_EMPTY + (x & 1) * RG + g), (x >> 1) & 1);
                 __syncwarp();
-                if ((x & 1) == 0) fold(Buf0{});
-                else fold(Buf1{});
+                if constexpr (kScored) {
+                    if (back == 2) fold(static_cast<int>(x & 1), 0);
+                    else fold(static_cast<int>(x & 1), 1);
+                } else if ((x & 1) == 0) {
+                    fold(Buf0{}, 0);
+                } else {
+                    fold(Buf1{}, 1);
+                }
             }
             if (failed) *fail_flag = 1;
             group_sync();

@@ -411,10 +411,13 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     }
     [[maybe_unused]] int scratch_row = 0;
     if constexpr (PAGED) scratch_row = static_cast<int>(item.scratch_row);
-    // where the CTA's tile j lies: its row in what the maps cover, and its first position
+    // Where the CTA's tile j lies: its row in what the maps cover, and its first position.  With a bias by distance the last tile is the first one: it has the largest scores, and what
+    // comes behind it seldom moves a row's reference (the other way round that moved in nearly every tile of a steep slope, and O was rescaled: 265 us in place of 205 for 1333
+    // tokens over 6500).
+    auto tile_of = [&](int j) { return static_cast<uint32_t>(tile0 + ((SCORE & kSloped) != 0 ? ntiles - 1 - j : j)); };
     auto tile_row = [&](int j) -> int {
         if constexpr (PAGED) {
-            const uint32_t u = static_cast<uint32_t>(tile0 + j);
+            const uint32_t u = tile_of(j);
             return scratch_row + static_cast<int>(u) * kBN + (u < sink_tiles ? 0 : row_gap);
         } else {
             return (tile0 + j) * kBN;
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     };
     auto tile_position = [&](int j) -> uint32_t {
         if constexpr (PAGED) {
-            const uint32_t u = static_cast<uint32_t>(tile0 + j);
+            const uint32_t u = tile_of(j);
             return u * kBN + (u < sink_tiles ? 0 : position_gap);
         } else {
             return static_cast<uint32_t>(tile0 + j) * kBN;
@@ -887,29 +890,32 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 if (!within) cap_scores(p, s, small);
             }
             if constexpr ((SCORE & kSloped) != 0) {
-                const float of_scores = (SCORE & kCapped) != 0 ? 1.0f : p.scale_log2, ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the first position, from the token's
-                if (ahead + kBN <= 1.0f) {   // nothing behind the token: the distance falls from position to position
-                    // four chains of sums of two values a step, eight roundings long (a product for each position's own: 64 more instructions, 280 us in place of ? for 1333 tokens over 6500)
-                    const Pair scale2 = pack_pair(of_scores, of_scores), step2 = pack_pair(2.0f * slope, 2.0f * slope);
-                    Pair bias[4];
+                // Of the token's own distance |i - j| a row sees one branch in a tile, the one ahead of it or, in a range that reaches behind the token, the one behind it: four
+                // chains of sums of two values a step, eight roundings long.
+                const Pair of_scores = pack_pair((SCORE & kCapped) != 0 ? 1.0f : p.scale_log2, (SCORE & kCapped) != 0 ? 1.0f : p.scale_log2);
+                const float ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the tile's first position, from the token's
+                const bool mixed = ahead < 0.0f && ahead + kBN > 1.0f && len > static_cast<uint32_t>(place) + 1u;
+                const float of_step = ahead >= 0.0f ? -slope : slope;
+                const Pair step2 = pack_pair(2.0f * of_step, 2.0f * of_step);
+                Pair bias[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float first = of_step * (ahead + static_cast<float>(16 * c));
+                    bias[c] = pack_pair(first, first + of_step);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const float first = slope * (ahead + static_cast<float>(16 * c));
-                        bias[c] = pack_pair(first, first + slope);
+                        const int at = 16 * c + i;
+                        const float2 x = unpack_pair(fma_pair(pack_pair(s[at], s[at + 1]), of_scores, bias[c]));
+                        s[at] = x.x;
+                        s[at + 1] = x.y;
+                        bias[c] = add_pair(bias[c], step2);
                     }
+                if (__builtin_expect(__any_sync(0xffffffffu, mixed), 0)) {   // both: what lies behind the token is to be turned over
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int at = 16 * c + i;
-                            const float2 x = unpack_pair(fma_pair(pack_pair(s[at], s[at + 1]), scale2, bias[c]));
-                            s[at] = x.x;
-                            s[at + 1] = x.y;
-                            bias[c] = add_pair(bias[c], step2);
-                        }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kBN; ++i) s[i] = fmaf(s[i], of_scores, -slope * fabsf(ahead + static_cast<float>(i)));
+                    for (int i = 0; i < kBN; ++i) s[i] = fmaf(mixed ? -2.0f * slope : 0.0f, fmaxf(ahead + static_cast<float>(i), 0.0f), s[i]);
                 }
             }
             // Only the tiles that straddle this row's causal length need the mask.
