@@ -104,8 +104,9 @@ template <> struct KernelParams<true, false> : Tc5Params {   // of the base: map
     uint32_t window, sinks;
 };
 template <> struct KernelParams<true, true> : KernelParams<true, false> {   // scale_log2: what the softmax multiplies what it is given by
-    // kCapped, of a score s = q.k: cap * tanh(cap_in s) in log2 units is s (cap_poly[0] + cap_poly[1] s^2 + ..) for |s| <= cap_small, cap_log2 * tanh(cap_in s) for any
-    float cap_in, cap_log2, cap_small, cap_poly[4];
+    // kCapped, of a score s = q.k: cap * tanh(cap_in s) in log2 units is s (cap_short[0] + cap_short[1] s^2 + ..) for |s| <= cap_small / 2, the same with cap_long for |s| <= cap_small,
+    // and cap_log2 * tanh(cap_in s) for any
+    float cap_in, cap_log2, cap_small, cap_short[4], cap_long[6];
     const float* slopes;
     const int32_t* ranges;       // may be null
 };
@@ -295,12 +296,12 @@ struct RowOffsets {
     }
 };
 
-// A score's capped form over the score itself, for two scores whose squares are given (KernelParams::cap_poly).
-template <class Params>
-__device__ __forceinline__ Pair cap_factor(const Params& p, Pair squares) {
-    Pair r = pack_pair(p.cap_poly[3], p.cap_poly[3]);
+// A score's capped form over the score itself, for two scores whose squares are given: a polynomial in them.
+template <int N>
+__device__ __forceinline__ Pair cap_factor(const float (&c)[N], Pair squares) {
+    Pair r = pack_pair(c[N - 1], c[N - 1]);
 #pragma unroll
-    for (int j = 2; j >= 0; --j) r = fma_pair(r, squares, pack_pair(p.cap_poly[j], p.cap_poly[j]));
+    for (int j = N - 2; j >= 0; --j) r = fma_pair(r, squares, pack_pair(c[j], c[j]));
     return r;
 }
 // The largest magnitude of a tile's scores (NaN has no say).
@@ -321,7 +322,7 @@ __device__ __forceinline__ void cap_scores(const Params& p, float (&s)[kBN], boo
 #pragma unroll
         for (int i = 0; i < kBN; i += 2) {
             const Pair x = pack_pair(s[i], s[i + 1]);
-            const float2 t = unpack_pair(mul_pair(x, cap_factor(p, mul_pair(x, x))));
+            const float2 t = unpack_pair(mul_pair(x, cap_factor(p.cap_long, mul_pair(x, x))));
             s[i] = t.x;
             s[i + 1] = t.y;
         }
@@ -880,14 +881,16 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // Raw scores stay unscaled; the softmax scale is folded into the exponent: p = 2^(s*c - m*c).  The loop's instructions count: products and
             // sums go in pairs, maxima three values at a time.  32 / 8 heads of 128, 1024 tokens over 8192: 168.0 -> 163.7 us; 24 / 4 of 256, 512 over
             // 8192: 111.6 -> 110.3.
-            // A cap.  cap * tanh(x / cap) grows with x, so the largest of the tile is that of the largest score; where no row of the warp has scores past half the cap or positions that it
-            // does not see, all the others become theirs within the exponent: a square and a polynomial of the third degree in it, two values to an instruction, and none of the
-            // special function unit, which the exponentials keep busy.  Otherwise they are capped in place, ahead of the mask.
-            [[maybe_unused]] bool within = false;
+            // A cap.  cap * tanh(x / cap) grows with x, so the largest of the tile is that of the largest score; where no row of the warp has scores past the cap or positions that it
+            // does not see, all the others become theirs within the exponent: a square and a polynomial in it, two values to an instruction, and none of the special function unit,
+            // which the exponentials keep busy.  Otherwise they are capped in place, ahead of the mask.  Scores of up to half the cap have a polynomial of the third degree, larger ones of the fifth:
+            // 1333 tokens over 6500, 239 us and 254 to 264; by the special function unit, for scores past the cap, 367.
+            [[maybe_unused]] int within = 0;   // 1: of the short polynomial, 2: of the long one
             if constexpr ((SCORE & kCapped) != 0) {
-                const bool small = !__any_sync(0xffffffffu, largest_of(s) > p.cap_small);
-                if constexpr ((SCORE & kSloped) == 0) within = small && !__any_sync(0xffffffffu, pos0 + kBN > len || pos0 < low);
-                if (!within) cap_scores(p, s, small);
+                const float largest = largest_of(s);
+                const bool small = !__any_sync(0xffffffffu, largest > p.cap_small);
+                if ((SCORE & kSloped) == 0 && small && !__any_sync(0xffffffffu, pos0 + kBN > len || pos0 < low)) within = __any_sync(0xffffffffu, 2.0f * largest > p.cap_small) ? 2 : 1;
+                if (within == 0) cap_scores(p, s, small);
             }
             if constexpr ((SCORE & kSloped) != 0) {
                 // Of the token's own distance |i - j| a row sees one branch in a tile, the one ahead of it or, in a range that reaches behind the token, the one behind it: four
@@ -938,7 +941,9 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], s[kBN - 4 + c]);
             float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * to_log2;   // scale > 0: the maximum commutes with it
             if constexpr ((SCORE & kCapped) != 0) {
-                if (within) mt *= unpack_pair(cap_factor(p, pack_pair(mt * mt, 0.0f))).x;
+                const Pair square = pack_pair(mt * mt, 0.0f);
+                if (within == 1) mt *= unpack_pair(cap_factor(p.cap_short, square)).x;
+                else if (within == 2) mt *= unpack_pair(cap_factor(p.cap_long, square)).x;
             }
             // the reference as the previous tile (another group's) left it; lazy rescale: keep it unless this tile's
             // maximum outgrew it by more than the threshold
@@ -979,12 +984,17 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                     sum = add_pair(sum, pack_pair(hf.x, hf.y));
                 }
             };
-            if ((SCORE & kCapped) != 0 && within) {
+            [[maybe_unused]] const auto weigh_capped = [&](const auto& poly) {
 #pragma unroll
                 for (int i = 0; i < kBN; i += 2) {
                     const Pair x = pack_pair(s[i], s[i + 1]);
-                    if constexpr ((SCORE & kCapped) != 0) weigh(i, fma_pair(x, cap_factor(p, mul_pair(x, x)), ref2));
+                    weigh(i, fma_pair(x, cap_factor(poly, mul_pair(x, x)), ref2));
                 }
+            };
+            if ((SCORE & kCapped) != 0 && within == 1) {
+                if constexpr ((SCORE & kCapped) != 0) weigh_capped(p.cap_short);
+            } else if ((SCORE & kCapped) != 0 && within == 2) {
+                if constexpr ((SCORE & kCapped) != 0) weigh_capped(p.cap_long);
             } else {
 #pragma unroll
                 for (int i = 0; i < kBN; i += 2) weigh(i, fma_pair(pack_pair(s[i], s[i + 1]), scale2, ref2));
@@ -1559,12 +1569,18 @@ int launch_chunk(const ChunkLaunch& c, cudaStream_t stream) {
     if (capped) {
         p.cap_in = c.scale / c.cap;
         p.cap_log2 = c.cap * 1.4426950408889634f;
-        // tanh(x) / x for |x| <= 1/2 by powers of x^2: the polynomial of the third degree with the smallest relative error, 5.4e-7 (Remez's exchange), a tenth of a millionth of
-        // the cap and a thousandth of what the weights' rounding to fp16 is to a score.  Where its coefficients would leave fp32's range no score is small.
-        const double tanh_poly[4] = {0.9999994558, -0.3332631794, 0.131902966, -0.04440222613}, k = static_cast<double>(c.scale) / c.cap;
-        p.cap_small = k < 1.0e4 ? static_cast<float>(0.5 / k) : -1.0f;
+        // tanh(x) / x for |x| <= 1/2 and <= 1 by powers of x^2: the polynomials of their degree with the smallest relative error, 5.4e-7 and 5.9e-7 (Remez's exchange), a few ten-millionths
+        // of the cap and a thousandth of what the weights' rounding to fp16 is to a score.  Where the coefficients would leave fp32's range no score is small.
+        const double of_half[4] = {0.9999994558, -0.3332631794, 0.131902966, -0.04440222613};
+        const double of_one[6] = {0.9999994136, -0.3332904238, 0.1328143388, -0.051605674, 0.01674311506, -0.003067060326};
+        const double k = static_cast<double>(c.scale) / c.cap;
+        const bool fits = k < 1.0e3;
+        p.cap_small = fits ? static_cast<float>(1.0 / k) : -1.0f;
         double power = static_cast<double>(c.scale) * 1.4426950408889634;
-        for (int j = 0; j < 4; ++j, power *= k * k) p.cap_poly[j] = k < 1.0e4 ? static_cast<float>(tanh_poly[j] * power) : 0.0f;
+        for (int j = 0; j < 6; ++j, power *= k * k) {
+            p.cap_long[j] = fits ? static_cast<float>(of_one[j] * power) : 0.0f;
+            if (j < 4) p.cap_short[j] = fits ? static_cast<float>(of_half[j] * power) : 0.0f;
+        }
     }
     return c.head_dim == 256 ? launch_scored<256>(p, capped, c.max_items, stream) : launch_scored<128>(p, capped, c.max_items, stream);
 }
