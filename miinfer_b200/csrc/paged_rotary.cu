@@ -7,8 +7,12 @@
 // angle's fraction of a turn, exact but for the table's own rounding (p 2^-65 turns).  Its upper 32 bits less the nearest quarter are the argument of a Taylor polynomial (to x^9 / x^8
 // on |x| <= pi/4, 3e-8).
 //
-// A lane holds eight consecutive elements, D/8 lanes a row (two rows a warp at head_dim 128).  Halves that are not in the lane come by shuffles.  A warp takes all rows of a token, or several share them where there are few tokens; the token's sines and cosines are worked out once a warp.
-// Bound by HBM for prompts, by latency for a decode step.
+// A lane holds sixteen elements of a row, two runs of eight, so that the two halves of a pair are in one lane.  D/16 lanes are a row, a warp takes four rows of 128 or two of 256 at a time
+// and a token's rows one step after the other; several warps share a token where there are few.  The next steps' rows come by cp.async into places of the lane's own, 8 KB a warp under
+// way.  A token's sines and cosines are worked out once a warp, two or four of them a lane, and handed round.
+// Bound by HBM for prompts with gates, by latency and instruction issue (16 warps an SM) without them and for a decode step.  Three prompts, 6100 tokens in all, fp16 to one scale a row, norms,
+// halves, us: 24 / 4 heads of 256 with gates 79 (4.7 TB/s of 6.5; fp32 114, 5.8), 32 / 8 of 128 39 (3.4); 40 tokens 6.4.  With one run a lane, the other half by shuffles and the next step's
+// loads in registers: 98 (142), 62; two runs a lane, loads in registers: 86 (115), 50; runs 2 l and 2 l + 1 of neighbours, every second 16 bytes an instruction: 47, in place of 35.
 #include "append_row.cuh"
 #include "paged_common.cuh"
 
@@ -21,7 +25,6 @@ namespace b200kv {
 namespace {
 
 constexpr int kRotaryWarps = 4;
-constexpr uint32_t kAhead = 2;   // steps
 
 struct RotaryParams {
     Paged pool;
@@ -54,109 +57,169 @@ __device__ __forceinline__ void sincos_turns(uint64_t turns, float* s_out, float
     *c_out = (quarter + 1) & 2 ? -b : b;
 }
 
-template <bool IN_F16> struct Eight { uint4 v[IN_F16 ? 1 : 2]; };   // a lane's elements as they lie in memory
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair r; asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+// Eight elements as they lie in memory, and as pairs of fp32.
+template <bool IN_F16> struct Run { uint4 v[IN_F16 ? 1 : 2]; };
+// A lane's run on its way into its own places of shared memory, 32 pieces of 16 bytes of the warp one behind the other.
 template <bool IN_F16>
-__device__ __forceinline__ Eight<IN_F16> load_eight(const void* src, size_t element) {
-    Eight<IN_F16> r;
+__device__ __forceinline__ void bring_run(uint4* to, const void* src, size_t element) {
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + element * (IN_F16 ? 2 : 4));
 #pragma unroll
-    for (int i = 0; i < (IN_F16 ? 1 : 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + element * (IN_F16 ? 2 : 4))[i];
+    for (int i = 0; i < (IN_F16 ? 1 : 2); ++i) {
+        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to + 32 * i));
+        if constexpr (IN_F16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from + i) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from + i) : "memory");   // (half a sector each: the other half comes from L1)
+    }
+}
+template <bool IN_F16>
+__device__ __forceinline__ Run<IN_F16> brought_run(const uint4* at) {
+    Run<IN_F16> r;
+#pragma unroll
+    for (int i = 0; i < (IN_F16 ? 1 : 2); ++i) r.v[i] = at[32 * i];
     return r;
 }
 template <bool IN_F16>
-__device__ __forceinline__ void widen(const Eight<IN_F16>& r, float (&x)[8]) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
+__device__ __forceinline__ void widen(const Run<IN_F16>& r, Pair (&x)[4]) {
+    if constexpr (IN_F16) {
+        const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (IN_F16) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + i));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-        } else {
-            x[2 * i] = __uint_as_float(w[2 * i]); x[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[i] = pack_pair(f.x, f.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = pack_pair(__uint_as_float(r.v[i].x), __uint_as_float(r.v[i].y));
+            x[2 * i + 1] = pack_pair(__uint_as_float(r.v[i].z), __uint_as_float(r.v[i].w));
         }
     }
 }
-__device__ __forceinline__ uint4 eight_halves(const float (&x)[8]) {
+__device__ __forceinline__ uint4 as_halves(const Pair (&x)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        const float2 f = unpack_pair(x[i]);
+        const __half2 h = __floats2half2_rn(f.x, f.y);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void store_floats(float* to, const float (&x)[8]) {
-    reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store_floats(float* to, const Pair (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 a = unpack_pair(x[2 * i]), b = unpack_pair(x[2 * i + 1]);
+        reinterpret_cast<float4*>(to)[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
+}
+// Largest magnitude; a NaN counts as 0, as in quantize_row.
+__device__ __forceinline__ float amax_of(const Pair (&x)[4]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack_pair(x[i]);
+        asm("max.ftz.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
+    }
+    return m;
+}
+__device__ __forceinline__ uint2 quantize_eight(const Pair (&x)[4], float inv) {
+    const Pair inv2 = pack_pair(inv, inv);
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 a = unpack_pair(mul2(x[2 * i], inv2)), b = unpack_pair(mul2(x[2 * i + 1], inv2));
+        asm("{ .reg .b32 t; cvt.pack.sat.s8.s32.b32 t, %4, %3, 0; cvt.pack.sat.s8.s32.b32 %0, %2, %1, t; }"
+            : "=r"(w[i]) : "r"(__float2int_rn(a.x)), "r"(__float2int_rn(a.y)), "r"(__float2int_rn(b.x)), "r"(__float2int_rn(b.y)));
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-// A row into the cache: eight elements a lane, `lanes` of the row.  The bits are quantize_row's.
+// The rows of a step into the cache, runs ca and cb of each a lane.  The bits are quantize_row's.  The maxima of runs meet in `exchange`, [row of the step][run], a warp's own: sixteen
+// lanes have a block each, or the rows' first ones a row, and work out its scale and the reciprocal, the two divisions of a block once.
 template <int D>
-__device__ __forceinline__ void store_row(const b200kv_paged_view& view, bool is_k, long long row, const float (&x)[8], int c, bool there) {
+__device__ __forceinline__ void store_rows(const b200kv_paged_view& view, bool is_k, long long row, const Pair (&a)[4], const Pair (&b)[4], uint32_t ca, uint32_t cb, uint32_t sub, bool there,
+                                           float* exchange) {
+    constexpr uint32_t kRuns = D / 8, kRows = 512 / D;
     const bool q8 = is_k ? is_k_q8(view.quant_mode) : is_v_q8(view.quant_mode);
     if (!q8) {
-        if (there) *reinterpret_cast<uint4*>(static_cast<__half*>(is_k ? view.key_f16 : view.value_f16) + row * D + c * 8) = eight_halves(x);
+        __half* to = static_cast<__half*>(is_k ? view.key_f16 : view.value_f16) + row * D;
+        if (there) {
+            *reinterpret_cast<uint4*>(to + ca * 8) = as_halves(a);
+            *reinterpret_cast<uint4*>(to + cb * 8) = as_halves(b);
+        }
         return;
     }
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    const uint32_t lane = threadIdx.x & 31;
     const bool rows = view.qblock == D;
-    for (int o = 1; o < (rows ? D / 8 : 4); o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    exchange[sub * kRuns + ca] = amax_of(a);
+    exchange[sub * kRuns + cb] = amax_of(b);
+    __syncwarp();
+    float amax = 0.0f;
+    if (rows) {
+        const float4* of_row = reinterpret_cast<const float4*>(exchange + sub * kRuns);
+#pragma unroll
+        for (uint32_t i = 0; i < kRuns / 4; ++i) {
+            const float4 m = of_row[i];
+            amax = fmaxf(amax, fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)));
+        }
+    } else {
+        const float4 m = reinterpret_cast<const float4*>(exchange)[lane % (kRows * kRuns / 4)];   // block lane % 16: of row lane / (kRuns / 4)
+        amax = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+    }
     const float scale = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 1.0f;
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i / 4] |= static_cast<uint32_t>(quantize_s8(__fmul_rn(x[i], inv)) & 0xff) << (8 * (i % 4));
+    float inv_a = inv, inv_b = inv;
+    if (!rows) {
+        inv_a = __shfl_sync(0xffffffffu, inv, sub * (kRuns / 4) + ca / 4);
+        inv_b = __shfl_sync(0xffffffffu, inv, sub * (kRuns / 4) + cb / 4);
+    }
+    // whose scale a lane stores: its own block's, or its row's
+    const float scale_a = rows ? scale : __shfl_sync(0xffffffffu, scale, sub * (kRuns / 4) + ca / 4), scale_b = rows ? scale : __shfl_sync(0xffffffffu, scale, sub * (kRuns / 4) + cb / 4);
+    __syncwarp();   // the maxima are read
     if (!there) return;
-    *reinterpret_cast<uint2*>((is_k ? view.key_q8 : view.value_q8) + row * D + c * 8) = make_uint2(w[0], w[1]);
+    int8_t* to = (is_k ? view.key_q8 : view.value_q8) + row * D;
     __half* scales = static_cast<__half*>(is_k ? view.key_scales : view.value_scales);
-    if (rows ? c == 0 : (c & 3) == 0) scales[rows ? row : row * (D / 32) + c / 4] = __float2half_rn(scale);
+    *reinterpret_cast<uint2*>(to + ca * 8) = quantize_eight(a, inv_a);
+    *reinterpret_cast<uint2*>(to + cb * 8) = quantize_eight(b, inv_b);
+    if (rows) {
+        if (ca == 0) scales[row] = __float2half_rn(scale_a);
+    } else {
+        if (ca % 4 == 0) scales[row * (D / 32) + ca / 4] = __float2half_rn(scale_a);
+        if (cb % 4 == 0) scales[row * (D / 32) + cb / 4] = __float2half_rn(scale_b);
+    }
 }
 
 template <int D, bool IN_F16>
-__global__ void __launch_bounds__(kRotaryWarps * 32) paged_rotary_kernel(const __grid_constant__ RotaryParams p) {
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes;   // of a row; rows a warp takes at a time
+__global__ void __launch_bounds__(kRotaryWarps * 32, 4) paged_rotary_kernel(const __grid_constant__ RotaryParams p) {
+    constexpr uint32_t kLanes = D / 16, kRows = 32 / kLanes, kEach = 8 / kRows;   // lanes of a row, rows a step, angles a lane works out
+    constexpr uint32_t kPieces = IN_F16 ? 1 : 2, kAhead = IN_F16 ? 4 : 2;   // 16-byte pieces of a run; steps whose loads are under way
+    __shared__ __align__(16) float exchange[kRotaryWarps][kRows * D / 8];
+    __shared__ uint4 ring[kRotaryWarps][kAhead][4 * kPieces * 32];   // a lane's two runs, and the gate's
     pdl_wait();
     pdl_launch_dependents();                             // behind the wait: it writes cache rows
     const Paged& pool = p.pool;
-    const uint32_t lane = threadIdx.x & 31, c = lane % kLanes, sub = lane / kLanes;
+    const uint32_t lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
     const uint64_t me = static_cast<uint64_t>(blockIdx.x) * kRotaryWarps + threadIdx.x / 32;
     if (me >= static_cast<uint64_t>(pool.batch.total_tokens) * p.share) return;
     const uint32_t token = static_cast<uint32_t>(me / p.share), part = static_cast<uint32_t>(me % p.share);
 
-    // ---- where the token goes, and its angles
+    // ---- where the token goes
     const uint32_t s = sequence_of(pool, token);
     const Span span = span_of(pool, s);
     if (token < span.first || token - span.first >= span.tokens) return;
     const int place = span.base() + static_cast<int>(token - span.first);
     const long long row0 = place >= 0 && p.key != nullptr ? row_of(pool, s, 0, static_cast<uint32_t>(place)) : -1;   // for kv head 0
     const uint64_t position = static_cast<uint32_t>(max(p.positions != nullptr ? p.positions[token] : place, 0));
-    const bool turns = c * 8 < p.dims;
-    const uint32_t half = p.dims / 16;                   // chunks of a half
-    const uint32_t other = !turns || p.neighbours ? c : c < half ? c + half : c - half;   // the chunk of the elements' partners
-    float cs[8], sn[8];                                  // x' = x cs + partner sn
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { cs[i] = 1.0f; sn[i] = 0.0f; }
-    if (turns) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (p.neighbours && (i & 1)) {
-                cs[i] = cs[i - 1];
-                sn[i] = -sn[i - 1];
-                continue;
-            }
-            const uint32_t pair = p.neighbours ? c * 4 + i / 2 : (c < half ? c : c - half) * 8 + i;
-            float sine, cosine;
-            sincos_turns(position * p.turns[pair], &sine, &cosine);
-            cs[i] = cosine * p.magnitude;
-            sn[i] = (p.neighbours || c < half ? -sine : sine) * p.magnitude;
-        }
-    }
 
-    // ---- its rows: queries with their gates, keys, values, a step at a time; kAhead steps' loads are under way
-    const uint32_t H = pool.view.kv_heads;
+    // ---- its rows: queries with their gates, keys, values, a step at a time
+    const uint32_t H = pool.view.kv_heads, half = p.dims / 16;   // runs of a half
     const uint32_t k0 = p.q != nullptr ? (p.query_heads + kRows - 1) / kRows : 0, kv_steps = p.key != nullptr ? (H + kRows - 1) / kRows : 0, v0 = k0 + kv_steps, steps = v0 + kv_steps;
-    const bool gated = p.gate != nullptr;
+    const bool gated = p.gate != nullptr, in_halves = p.neighbours == 0 && l < half;
+    // Halves are run l and run l + half; behind the rotated part, and of neighbours, lanes next to each other have runs next to each other as well.
+    const uint32_t ca = p.neighbours ? l : in_halves ? l : l + half, cb = !p.neighbours && in_halves ? l + half : l + kLanes;
+    const bool turns_a = ca * 8 < p.dims, turns_b = cb * 8 < p.dims;
     enum { QUERY, KEY, VALUE };
     struct Step { int kind; uint32_t head; bool there; };
     const auto step_of = [&](uint32_t t) {
@@ -164,81 +227,126 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) paged_rotary_kernel(const _
         const uint32_t head = (t - (kind == QUERY ? 0 : kind == KEY ? k0 : v0)) * kRows + sub;
         return Step{kind, head, t < steps && head < (kind == QUERY ? p.query_heads : H)};
     };
-    using Raw = Eight<IN_F16>;
-    Raw raw[kAhead], raw_gate[kAhead];
-    const auto fetch = [&](uint32_t t, Raw& r, Raw& g) {
+    uint4* const mine = ring[threadIdx.x / 32][0] + lane;
+    constexpr uint32_t kRun = kPieces * 32, kStage = 4 * kRun;
+    const auto fetch = [&](uint32_t t, uint32_t stage) {   // (a lane waits for its own copies only, and reads no others')
         const Step at = step_of(t);
-        r = g = Raw{};
-        if (!at.there) return;
-        if (at.kind == QUERY) {
-            const size_t element = token * p.q_stride + static_cast<size_t>(at.head) * (gated ? 2 * D : D) + c * 8;
-            r = load_eight<IN_F16>(p.q, element);
-            if (gated) g = load_eight<IN_F16>(p.q, element + D);
-        } else {
-            r = at.kind == KEY ? load_eight<IN_F16>(p.key, token * p.key_stride + at.head * D + c * 8) : load_eight<IN_F16>(p.value, token * p.value_stride + at.head * D + c * 8);
+        if (at.there) {
+            const void* from = at.kind == QUERY ? p.q : at.kind == KEY ? p.key : p.value;
+            const size_t element = token * (at.kind == QUERY ? p.q_stride : at.kind == KEY ? p.key_stride : p.value_stride) + static_cast<size_t>(at.head) * (at.kind == QUERY && gated ? 2 * D : D);
+            uint4* to = mine + stage * kStage;
+            bring_run<IN_F16>(to, from, element + ca * 8);
+            bring_run<IN_F16>(to + kRun, from, element + cb * 8);
+            if (at.kind == QUERY && gated) {
+                bring_run<IN_F16>(to + 2 * kRun, from, element + D + ca * 8);
+                bring_run<IN_F16>(to + 3 * kRun, from, element + D + cb * 8);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float w[8];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) fetch(part + i * p.share, i);
+
+    // ---- its angles: eight a lane, of pair 8 l + i of halves, or of neighbours 4 ca + i and, from the fifth on, 4 cb + i - 4; a lane works out kEach of those that the lanes of its number share
+    float cs[8], sn[8];
+    {
+        float c[kEach], n[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = sub * kEach + i, pair = p.neighbours ? (at < 4 ? 4 * ca + at : 4 * cb + at - 4) : 8 * l + at;
+            c[i] = 1.0f;
+            n[i] = 0.0f;
+            if (2 * pair >= p.dims) continue;
+            sincos_turns(position * p.turns[pair], &n[i], &c[i]);
+            c[i] *= p.magnitude;
+            n[i] *= p.magnitude;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            cs[i] = __shfl_sync(0xffffffffu, c[i % kEach], i / kEach * kLanes + l);
+            sn[i] = __shfl_sync(0xffffffffu, n[i % kEach], i / kEach * kLanes + l);
+        }
+    }
+
+    Pair w[2][4];
     int weighed = -1;                                    // whose norm's weights these are
-    const auto take = [&](uint32_t t, const Raw& now, const Raw& now_gate) {
+    uint32_t stage = 0;
+    for (uint32_t t = part; t < steps; t += p.share, stage = stage + 1 == kAhead ? 0 : stage + 1) {
         const Step at = step_of(t);
-        float x[8];
-        widen<IN_F16>(now, x);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        const uint4* from = mine + stage * kStage;
+        Pair a[4], b[4];
+        widen<IN_F16>(brought_run<IN_F16>(from), a);
+        widen<IN_F16>(brought_run<IN_F16>(from + kRun), b);
+        const size_t out = (static_cast<size_t>(token) * p.query_heads + at.head) * D;
+        if (at.kind == QUERY && gated && at.there) {
+            Pair g[4];
+            widen<IN_F16>(brought_run<IN_F16>(from + 2 * kRun), g);
+            store_floats(p.gate + out + ca * 8, g);
+            widen<IN_F16>(brought_run<IN_F16>(from + 3 * kRun), g);
+            store_floats(p.gate + out + cb * 8, g);
+        }
+        fetch(t + kAhead * p.share, stage);
+        const long long row = row0 + (static_cast<long long>(at.head) << pool.page_shift);
         if (at.kind == VALUE) {
-            store_row<D>(pool.view, false, row0 + (static_cast<long long>(at.head) << pool.page_shift), x, c, at.there && row0 >= 0);
-            return;
+            store_rows<D>(pool.view, false, row, a, b, ca, cb, sub, at.there && row0 >= 0, exchange[threadIdx.x / 32]);
+            continue;
         }
         const float* norm = at.kind == QUERY ? p.q_norm : p.k_norm;
         if (norm != nullptr) {
             if (weighed != at.kind) {
                 weighed = at.kind;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = norm[c * 8 + i];
+                for (int i = 0; i < 4; ++i) {
+                    w[0][i] = pack_pair(norm[ca * 8 + 2 * i], norm[ca * 8 + 2 * i + 1]);
+                    w[1][i] = pack_pair(norm[cb * 8 + 2 * i], norm[cb * 8 + 2 * i + 1]);
+                }
             }
-            float sum = 0.0f;
+            Pair sums = mul2(a[0], a[0]), more = mul2(b[0], b[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+            for (int i = 1; i < 4; ++i) {
+                sums = fma2(a[i], a[i], sums);
+                more = fma2(b[i], b[i], more);
+            }
+            const float2 x = unpack_pair(sums), y = unpack_pair(more);
+            float sum = x.x + x.y + y.x + y.y;
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float inv = __frsqrt_rn(fmaf(sum, 1.0f / D, p.epsilon));
+            for (int o = 1; o < static_cast<int>(kLanes); o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = rsqrtf(fmaf(sum, 1.0f / D, p.epsilon));
+            const Pair inv2 = pack_pair(inv, inv);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+            for (int i = 0; i < 4; ++i) {
+                a[i] = mul2(mul2(a[i], inv2), w[0][i]);
+                b[i] = mul2(mul2(b[i], inv2), w[1][i]);
+            }
         }
-        float y[8];
         if (p.neighbours) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else {
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = unpack_pair(a[i]), y = unpack_pair(b[i]);   // (an infinity behind the rotated part stays one)
+                if (turns_a) a[i] = pack_pair(fmaf(x.x, cs[i], -x.y * sn[i]), fmaf(x.x, sn[i], x.y * cs[i]));
+                if (turns_b) b[i] = pack_pair(fmaf(y.x, cs[4 + i], -y.y * sn[4 + i]), fmaf(y.x, sn[4 + i], y.y * cs[4 + i]));
+            }
+        } else if (in_halves) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], static_cast<int>(sub * kLanes + other));
-        }
-        if (turns) {   // (an infinity in the rest of a head stays one)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i], y[i] * sn[i]);
-        }
-        if (at.kind == KEY) {
-            store_row<D>(pool.view, true, row0 + (static_cast<long long>(at.head) << pool.page_shift), x, c, at.there && row0 >= 0);
-        } else if (at.there) {
-            const size_t out = (static_cast<size_t>(token) * p.query_heads + at.head) * D + c * 8;
-            if (p.q_out_is_f16) *reinterpret_cast<uint4*>(static_cast<__half*>(p.q_out) + out) = eight_halves(x);
-            else store_floats(static_cast<float*>(p.q_out) + out, x);
-            if (gated) {
-                float g[8];
-                widen<IN_F16>(now_gate, g);
-                store_floats(p.gate + out, g);
+            for (int i = 0; i < 4; ++i) {
+                const Pair c = pack_pair(cs[2 * i], cs[2 * i + 1]), n = pack_pair(sn[2 * i], sn[2 * i + 1]), minus = pack_pair(-sn[2 * i], -sn[2 * i + 1]);
+                const Pair x = a[i], y = b[i];
+                a[i] = fma2(y, minus, mul2(x, c));
+                b[i] = fma2(x, n, mul2(y, c));
             }
         }
-    };
-#pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) fetch(part + i * p.share, raw[i], raw_gate[i]);
-    for (uint32_t t0 = part; t0 < steps; t0 += kAhead * p.share) {
-#pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t t = t0 + i * p.share;
-            if (t >= steps) break;
-            const Raw now = raw[i], now_gate = raw_gate[i];
-            fetch(t + kAhead * p.share, raw[i], raw_gate[i]);
-            take(t, now, now_gate);
+        if (at.kind == KEY) {
+            store_rows<D>(pool.view, true, row, a, b, ca, cb, sub, at.there && row0 >= 0, exchange[threadIdx.x / 32]);
+        } else if (at.there) {
+            if (p.q_out_is_f16) {
+                __half* to = static_cast<__half*>(p.q_out) + out;
+                *reinterpret_cast<uint4*>(to + ca * 8) = as_halves(a);
+                *reinterpret_cast<uint4*>(to + cb * 8) = as_halves(b);
+            } else {
+                store_floats(static_cast<float*>(p.q_out) + out + ca * 8, a);
+                store_floats(static_cast<float*>(p.q_out) + out + cb * 8, b);
+            }
         }
     }
 }
@@ -353,7 +461,7 @@ int b200kv_paged_rotary(const b200kv_paged_view* view, const b200kv_paged_batch*
     RotaryParams p{paged_of(*view, *batch), rotary->turns, rotary->dims, rotary->layout == B200KV_ROTARY_NEIGHBOURS, rotary->magnitude, epsilon, q, key, value, q_stride, key_stride,
                    value_stride, q_norm_weight, k_norm_weight, positions, q_out, q_out_dtype == B200KV_F16, gate, q != nullptr ? query_heads : 0, 1};
     // Warps to a token: one, or as many as there are steps where the tokens alone do not occupy the device.
-    const uint32_t at_once = view->head_dim == 128 ? 2 : 1;
+    const uint32_t at_once = view->head_dim == 128 ? 4 : 2;
     const uint64_t steps = (p.query_heads + at_once - 1) / at_once + (key != nullptr ? 2 * ((view->kv_heads + at_once - 1) / at_once) : 0);
     p.share = static_cast<uint32_t>(std::min<uint64_t>(steps, std::max<uint64_t>(1, 32ull * device_sms() / tokens)));
     if (tokens * p.share > 0x7fffffffull) return B200KV_ERR_RANGE;
