@@ -129,9 +129,8 @@ public:
     const T* structure(PyObject* type, const char* what) {
         if (!ok_) return nullptr;
         PyObject* o = args_[i_++];
-        const int is = PyObject_IsInstance(o, type);
-        if (is <= 0) {
-            if (is == 0) PyErr_Format(PyExc_TypeError, "expected %s, got %s", what, Py_TYPE(o)->tp_name);
+        if (!PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(type))) {   // (PyObject_IsInstance goes through the structures' metaclass: 0.1 us for each layer's view)
+            PyErr_Format(PyExc_TypeError, "expected %s, got %s", what, Py_TYPE(o)->tp_name);
             ok_ = false;
             return nullptr;
         }
