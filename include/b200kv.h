@@ -553,7 +553,7 @@ B200KV_API int b200kv_paged_attn(const b200kv_paged_view* view, const b200kv_pag
  *   score = c - slopes[head] * |i - j|,  c = cap * tanh(x / cap) where cap > 0 (from 1e-6 to 1e6), x where it is 0;
  * with ranges, token t sees j in [ranges[t][0], ranges[t][1]) in place of j <= i: a document that begins at position d is [d, i + 1) for its tokens, a prefix of n positions
  * that sees itself in both directions [0, n), and [0, i + 1) behind it.  A window cuts a range as it cuts j <= i; the first `sinks` positions, which count with a window or with ranges, are
- * seen by every token whose range does not end before them.  What lies past a sequence's length is never seen.  slopes: finite.  Cache rows from the lowest position that any of a
+ * seen by every token whose range does not end before them.  What lies past a sequence's length is never seen.  slopes: of magnitude up to 1e30.  Cache rows from the lowest position that any of a
  * sequence's new tokens sees up to the last one are finite, whether or not a range leaves them out in between, and so are the sinks; rows outside may hold anything.  Tiles of
  * positions that nobody sees are neither read nor computed.  lse is that of the scores; over fp16 keys with fp32 queries and a cap a longer sequence's is as good as over int8 keys.  (It is not one for
  * b200kv_paged_weights, which knows scores without a cap, a bias or ranges only.)  A scoring of nothing at all is b200kv_paged_attn. */

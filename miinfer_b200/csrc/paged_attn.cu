@@ -348,60 +348,63 @@ __device__ __forceinline__ void gather_unit(const PrepareParams& p, const uint32
             q8 ? dequant8(make_uint2(v[i].x, v[i].y), scale[i]) : v[i];
 }
 
-// What the tokens of each row tile and of each sequence see, and what each row tile walks of it: a block a sequence, a warp four row tiles at a time, whose loads are under way
+// What the tokens of each row tile and of each sequence see, and what each row tile walks of it: a block a sequence, or several in turn, a warp four row tiles at a time, whose loads are under way
 // together (one at a time: 12 us for 193 row tiles, a trip to L2 each).
 constexpr int kBoundsThreads = 1024, kBoundsTiles = 4;
 __global__ void __launch_bounds__(kBoundsThreads) paged_bounds_kernel(const __grid_constant__ PrepareParams p) {
     __shared__ uint32_t lowest, end;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t s = blockIdx.x, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) { lowest = 0xffffffffu; end = 0; }
-    __syncthreads();
-    const Span span = span_of(p.pool, s);
-    if (!p.mine(span)) return;
-    const uint32_t rows = span.tokens * p.group, row_tiles = p.row_tiles(span);
-    uint2* const of_tiles = p.tile_bounds + chunk_slot(span.first, p.group, s, 0);
-    for (uint32_t r0 = threadIdx.x / 32 * kBoundsTiles; r0 < row_tiles; r0 += kBoundsThreads / 32 * kBoundsTiles) {
-        uint32_t low[kBoundsTiles], upto[kBoundsTiles];
-#pragma unroll
-        for (uint32_t i = 0; i < kBoundsTiles; ++i) {
-            low[i] = 0xffffffffu;
-            upto[i] = 0;
-        }
-        for (uint32_t t0 = lane; t0 <= kChunkRows / p.group; t0 += 32) {   // of a row tile's tokens (one more than that, where heads of one lie in two)
-            Sight sight[kBoundsTiles];
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t s = blockIdx.x; s < p.pool.batch.sequences; s += gridDim.x) {
+        const Span span = span_of(p.pool, s);
+        if (!p.mine(span)) continue;   // the same for all threads
+        if (threadIdx.x == 0) { lowest = 0xffffffffu; end = 0; }
+        __syncthreads();
+        const uint32_t rows = span.tokens * p.group, row_tiles = p.row_tiles(span);
+        uint2* const of_tiles = p.tile_bounds + chunk_slot(span.first, p.group, s, 0);
+        for (uint32_t r0 = threadIdx.x / 32 * kBoundsTiles; r0 < row_tiles; r0 += kBoundsThreads / 32 * kBoundsTiles) {
+            uint32_t low[kBoundsTiles], upto[kBoundsTiles];
 #pragma unroll
             for (uint32_t i = 0; i < kBoundsTiles; ++i) {
-                const uint32_t r = r0 + i, t = r * kChunkRows / p.group + t0;
-                sight[i] = {0, 0};
-                if (r < row_tiles && t <= min((r + 1) * kChunkRows - 1, rows - 1) / p.group)
-                    sight[i] = sight_of(p.ranges, static_cast<size_t>(span.first) + t, span.base() + static_cast<int>(t), p.window, span.length);
+                low[i] = 0xffffffffu;
+                upto[i] = 0;
+            }
+            for (uint32_t t0 = lane; t0 <= kChunkRows / p.group; t0 += 32) {   // of a row tile's tokens (one more than that, where heads of one lie in two)
+                Sight sight[kBoundsTiles];
+#pragma unroll
+                for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+                    const uint32_t r = r0 + i, t = r * kChunkRows / p.group + t0;
+                    sight[i] = {0, 0};
+                    if (r < row_tiles && t <= min((r + 1) * kChunkRows - 1, rows - 1) / p.group)
+                        sight[i] = sight_of(p.ranges, static_cast<size_t>(span.first) + t, span.base() + static_cast<int>(t), p.window, span.length);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kBoundsTiles; ++i) {
+                    if (!sight[i].empty()) low[i] = min(low[i], sight[i].low);
+                    upto[i] = max(upto[i], sight[i].empty() ? min(sight[i].upto, p.sinks) : sight[i].upto);
+                }
             }
 #pragma unroll
             for (uint32_t i = 0; i < kBoundsTiles; ++i) {
-                if (!sight[i].empty()) low[i] = min(low[i], sight[i].low);
-                upto[i] = max(upto[i], sight[i].empty() ? min(sight[i].upto, p.sinks) : sight[i].upto);
+                low[i] = __reduce_min_sync(0xffffffffu, low[i]);
+                upto[i] = __reduce_max_sync(0xffffffffu, upto[i]);
+                if (lane == 0 && r0 + i < row_tiles) {
+                    of_tiles[r0 + i] = make_uint2(low[i], upto[i]);
+                    atomicMin(&lowest, low[i]);
+                    atomicMax(&end, upto[i]);
+                }
             }
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kBoundsTiles; ++i) {
-            low[i] = __reduce_min_sync(0xffffffffu, low[i]);
-            upto[i] = __reduce_max_sync(0xffffffffu, upto[i]);
-            if (lane == 0 && r0 + i < row_tiles) {
-                of_tiles[r0 + i] = make_uint2(low[i], upto[i]);
-                atomicMin(&lowest, low[i]);
-                atomicMax(&end, upto[i]);
-            }
+        __syncthreads();
+        const ChunkTiles t = chunk_tiles_between(lowest, end, p.sinks);
+        for (uint32_t r = threadIdx.x; r < row_tiles; r += kBoundsThreads) {
+            const Walk walk = walk_between(p, of_tiles[r], t);
+            of_tiles[r] = make_uint2(walk.tiles, walk.skip);
         }
+        if (threadIdx.x == 0) p.bounds[s] = make_uint2(lowest, end);
+        __syncthreads();   // the bounds are read
     }
-    __syncthreads();
-    const ChunkTiles t = chunk_tiles_between(lowest, end, p.sinks);
-    for (uint32_t r = threadIdx.x; r < row_tiles; r += kBoundsThreads) {
-        const Walk walk = walk_between(p, of_tiles[r], t);
-        of_tiles[r] = make_uint2(walk.tiles, walk.skip);
-    }
-    if (threadIdx.x == 0) p.bounds[s] = make_uint2(lowest, end);
 }
 
 template <int D, bool RANGED>
@@ -692,7 +695,7 @@ int attend(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const
                                     : (view->head_dim == 128 ? paged_prepare_kernel<128, false> : paged_prepare_kernel<256, false>);
         if (smem > 32 * 1024) B200KV_CUDA_TRY(opt_in_dynamic_smem(reinterpret_cast<const void*>(prepare), 2 * (kMostSequences + 1) * 4, done[(view->head_dim == 256) + 2 * ranged]));
         if (ranged) {
-            B200KV_CUDA_TRY(launch_kernel(paged_bounds_kernel, dim3(batch->sequences), dim3(kBoundsThreads), 0, s, true, pp));
+            B200KV_CUDA_TRY(launch_kernel(paged_bounds_kernel, dim3(std::min(batch->sequences, 2 * sms)), dim3(kBoundsThreads), 0, s, true, pp));
             B200KV_CUDA_TRY(launch_behind(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, pp));
         } else {
             B200KV_CUDA_TRY(launch_kernel(prepare, dim3(blocks), dim3(kPrepareThreads), smem, s, true, pp));

@@ -353,6 +353,44 @@ def test_a_stream_of_its_own_and_two_calls_at_once(cuda, status):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("d,mode", [(128, 0), (256, 3)])
+def test_many_sequences_with_ranges(cuda, status, d, mode):
+    """More sequences than the blocks that look at their ranges, most of a token and some of a chunk, empty ones among them."""
+    rng = np.random.default_rng(d)
+    lengths = [int(x) for x in rng.integers(1, 60, 700)]
+    tokens = [0 if i % 11 == 3 else 1 for i in range(700)]
+    for i in range(5, 700, 37):
+        lengths[i] = tokens[i] = int(rng.integers(9, 60))
+    pool = po.Pool(rng, lengths, d=d, heads=1, page=16, mode=mode, qblock=32)
+    run(rng, pool, tokens, hq=4, ranges=ranges_of(rng, "documents", tokens, lengths, 1), sinks=2, cap=20.0, word=status)
+    run(rng, pool, tokens, hq=4, ranges=ranges_of(rng, "any", tokens, lengths, 1), slopes=slopes_of(4), word=status)
+
+
+@pytest.mark.parametrize("scores", [dict(slopes=True), dict(kind="prefix"), dict(slopes=True, kind="documents")])
+@pytest.mark.parametrize("d", [128, 256])
+def test_statistics_of_fp32_queries_over_fp16_keys(cuda, status, scores, d):
+    """Without a cap they are as good as those of fp16 queries: what the queries' rounding to fp16 does to them is put back, up to its square and the rounding of the mean keys."""
+    rng = np.random.default_rng(d + len(scores))
+    pool = po.Pool(rng, [300, 70, 40], d=d, heads=2, page=32, mode=0, qblock=32)
+    view, tokens, hq = pool.upload(), [90, 9, 40], 8
+    batch, starts = po.batch_of(pool, tokens)
+    q = (1.5 * rng.standard_normal((batch.total_tokens, hq, d))).astype(np.float32)
+    slopes = slopes_of(hq) if "slopes" in scores else None
+    ranges = ranges_of(rng, scores["kind"], tokens, pool.lengths) if "kind" in scores else None
+    scoring = paged.PagedScoring(slopes=None if slopes is None else dev(slopes), ranges=None if ranges is None else dev(ranges))
+    out, lse = torch.zeros(q.shape, device="cuda"), torch.zeros(q.shape[:2], device="cuda")
+    paged.launch_paged_attention(view, batch, dev(q), out, query_heads=hq, scale=d ** -0.5, lse=lse, scoring=scoring, workspace=paged.paged_workspace(view, batch, hq, scoring=scoring))
+    exact = q.astype(np.float16).astype(np.float64)
+    want, want_lse, _, _ = so.attention(pool, q, starts, d ** -0.5, slopes=slopes, ranges=ranges)
+    _, _, _, limit = so.attention(pool, q.astype(np.float16), starts, d ** -0.5, slopes=slopes, ranges=ranges)      # of queries that need no rounding
+    left = np.abs(q - exact)
+    most = max(np.abs(pool.rows(s, h, 0)).max() for s in range(3) for h in range(2))
+    moved = left.sum(-1) * most * d ** -0.5                        # the most that the rounding moves a score by
+    # the square of it (the weights' own change times the scores'), and the mean key's rounding to fp16, with the weights' and the sum's: 2^-10 of what it corrects
+    assert (np.abs(lse.cpu().numpy() - want_lse) <= limit + 2 * moved ** 2 + moved * 2.0 ** -10).all()
+    assert int(status) == 0
+
+
 def test_tensors_that_are_refused(cuda):
     rng = np.random.default_rng(11)
     pool = po.Pool(rng, [30], d=128, heads=1, page=16, mode=0, qblock=128)
