@@ -50,6 +50,7 @@ struct PrepareParams {
     uint2* tile_bounds;
     uint2* bounds;
     uint2* walks;               // the same as tile_bounds, in the list's order
+    uint32_t max_walks;         // room of each of the two
     __device__ __forceinline__ bool mine(const Span& span) const { return span.tokens > 0 && static_cast<uint64_t>(span.tokens) * group > few_rows; }
     __device__ __forceinline__ uint32_t row_tiles(const Span& span) const { return (span.tokens * group + kChunkRows - 1) / kChunkRows; }
 };
@@ -144,7 +145,7 @@ template <bool RANGED>
 __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* tile_starts, const uint32_t* scratch_starts, PlanScratch& sh) {
     const uint32_t tid = threadIdx.x, S = p.pool.batch.sequences, H = p.pool.view.kv_heads, row_tiles = tile_starts[S];
     if (tid == 0) p.plan->items = p.plan->groups = 0;
-    if (static_cast<uint64_t>(row_tiles) * H > p.max_items) {   // starts that do not ascend: nothing of this is laid out
+    if (static_cast<uint64_t>(row_tiles) * H > p.max_items || (RANGED && row_tiles > p.max_walks)) {   // starts that do not ascend: nothing of this is laid out
         if (tid == 0) report(p.pool, B200KV_STATUS_BAD_BOUND);
         return;
     }
@@ -158,7 +159,11 @@ __device__ __forceinline__ void lay_out(const PrepareParams& p, const uint32_t* 
         unsigned long long sum = 0;
         for (uint32_t i = tid; i < row_tiles; i += kPrepareThreads) {
             const uint32_t s = last_from(tile_starts, S, i);
-            const uint2 walk = p.tile_bounds[chunk_slot(span_of(p.pool, s).first, p.group, s, tile_starts[s + 1] - 1 - i)];
+            const Span span = span_of(p.pool, s);
+            uint2 walk = p.tile_bounds[chunk_slot(span.first, p.group, s, tile_starts[s + 1] - 1 - i)];
+            const uint32_t tiles = tiles_of<true>(p, span, s).tiles;
+            walk.y = min(walk.y, tiles);           // (always so, but where starts do not ascend and two sequences have the same slot: nothing walks further than its copy)
+            walk.x = min(walk.x, tiles - walk.y);
             p.walks[i] = walk;
             most = max(most, walk.x);
             sum += walk.x;
@@ -574,6 +579,7 @@ __global__ void __launch_bounds__(256) paged_lse_kernel(const __grid_constant__ 
 
 struct Room {
     uint64_t scratch_tiles;    // of all sequences together
+    uint64_t max_walks;        // row tiles of all sequences together, with ranges
     uint32_t max_items, max_parts;
     bool decode, chunks;       // which kernels the call may need
     size_t decode_parts, items, groups, k, v, part_o, part_ml, mean_key, tile_bounds, bounds, walks, bytes;   // offsets
@@ -618,8 +624,9 @@ Room room_of(const b200kv_paged_view& view, const b200kv_paged_batch& batch, uin
     r.part_o = take(parts * kChunkRows * view.head_dim * sizeof(float));
     r.part_ml = take(parts * kChunkRows * sizeof(float2));
     if (ranged) {
-        r.tile_bounds = take((batch.total_tokens * group / kChunkRows + batch.sequences + 1) * sizeof(uint2));
-        r.walks = take((batch.total_tokens * group / kChunkRows + batch.sequences + 1) * sizeof(uint2));
+        r.max_walks = batch.total_tokens * group / kChunkRows + batch.sequences + 1;
+        r.tile_bounds = take(r.max_walks * sizeof(uint2));
+        r.walks = take(r.max_walks * sizeof(uint2));
         r.bounds = take(static_cast<uint64_t>(batch.sequences) * sizeof(uint2));
     }
     r.bytes = at + 1024;                                 // the base is brought to a multiple of 1024
@@ -687,7 +694,8 @@ int attend(const b200kv_paged_view* view, const b200kv_paged_batch* batch, const
                                room.max_parts, static_cast<uint32_t>(room.scratch_tiles), group, window, sinks, sms, few_rows,
                                view->head_dim == 256 ? ChunkCosts{0.62f, 12.4f, 0.5f, 0.0f, 0.024f} : ChunkCosts{0.5f, 7.0f, 1.0f, 2.0f, 0.02f},
                                {reinterpret_cast<__half*>(ws + room.k), reinterpret_cast<__half*>(ws + room.v)}, ranged ? scoring->ranges : nullptr,
-                               reinterpret_cast<uint2*>(ws + room.tile_bounds), reinterpret_cast<uint2*>(ws + room.bounds), reinterpret_cast<uint2*>(ws + room.walks)};
+                               reinterpret_cast<uint2*>(ws + room.tile_bounds), reinterpret_cast<uint2*>(ws + room.bounds), reinterpret_cast<uint2*>(ws + room.walks),
+                               static_cast<uint32_t>(room.max_walks)};
         const uint32_t blocks = 1 + static_cast<uint32_t>(std::min<uint64_t>(room.scratch_tiles * view->kv_heads * 2, 8ull * sms));
         const size_t smem = 2 * (static_cast<size_t>(batch->sequences) + 1) * 4;
         static std::atomic<uint64_t> done[4];

@@ -299,6 +299,25 @@ def test_bad_pages_bounds_and_padding(cuda, status):
         status.zero_()
 
 
+def test_starts_that_do_not_ascend_cost_results_only(cuda, status):
+    """Two sequences with the same rows: their row tiles share places in the workspace, and there may be more of them than it has room for.  The call ends, says so, and the next one is right."""
+    rng = np.random.default_rng(12)
+    pool = po.Pool(rng, [400] * 9, d=128, heads=1, page=16, mode=0, qblock=128)
+    view = pool.upload()
+    for hq in (1, 8):
+        batch, _ = po.batch_of(pool, [400] * 9, starts=[0] + [400, 0] * 4 + [400], total_tokens=400, max_tokens=400)
+        q = dev((1.5 * rng.standard_normal((400, hq, 128))).astype(np.float16))
+        ranges = dev(np.stack([rng.integers(0, 400, 400), np.full(400, 400)], 1).astype(np.int32))
+        scoring = paged.PagedScoring(ranges=ranges, cap=20.0)
+        ws = paged.paged_workspace(view, batch, hq, scoring=scoring)
+        guard = torch.full((ws.numel() + 4096,), 77, dtype=torch.uint8, device="cuda")
+        out = torch.zeros(q.shape, dtype=torch.float16, device="cuda")
+        paged.launch_paged_attention(view, batch, q, out, query_heads=hq, scale=0.09, workspace=guard[:ws.numel()], scoring=scoring)
+        assert int(status) & paged.STATUS_BAD_BOUND and bool((guard[ws.numel():] == 77).all())
+        status.zero_()
+        run(rng, pool, [40, 1, 0, 17, 400, 1, 1, 9, 64], hq=hq, ranges=ranges_of(rng, "documents", [40, 1, 0, 17, 400, 1, 1, 9, 64], pool.lengths, 1), cap=20.0, poison=False, word=status)
+
+
 def test_captured_replayed_and_two_graphs_over_one_workspace(cuda, status):
     """A step captured once replays with other ranges, slopes and lengths; two graphs that share a workspace, one after the other."""
     rng = np.random.default_rng(9)
