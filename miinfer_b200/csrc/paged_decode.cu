@@ -294,7 +294,7 @@ paged_decode_kernel(const __grid_constant__ P p, const __grid_constant__ CUtenso
             [[maybe_unused]] uint32_t seen_end = c.span.length;                                                       // and seen by nobody from here on
             [[maybe_unused]] float slope[4];             // of the rows, in log2 units, and their places
             [[maybe_unused]] int place[4];
-            [[maybe_unused]] const bool capped = [&] { if constexpr (kScored) return p.cap_log2 > 0.0f; else return false; }();
+            [[maybe_unused]] const bool capped = p.capped();
             if constexpr (kScored) {
                 if (capped) {                            // scores over the cap
 #pragma unroll

@@ -30,6 +30,7 @@ struct PagedDecode {
         t.n = max(t.n, 1u);    // one tile where there is no position: the rows that see nothing come out as zeros
         return t;
     }
+    __device__ __forceinline__ bool capped() const { return false; }
 };
 
 // The same with scores that are capped, biased by distance, or seen by ranges of the tokens' own (paged_decode_scored.cu).
@@ -37,6 +38,7 @@ struct PagedDecodeScored : PagedDecode {
     float cap_log2, cap_in;    // cap * log2 e and its reciprocal; 0: no cap
     const float* slopes;       // [query_heads], may be null
     const int32_t* ranges;     // [total_tokens][2], may be null
+    __device__ __forceinline__ bool capped() const { return cap_log2 > 0.0f; }
     __device__ __forceinline__ Sight sight(const Span& span, uint32_t t) const {
         return sight_of(ranges, static_cast<size_t>(span.first) + t, span.base() + static_cast<int>(t), window, span.length);
     }

@@ -593,6 +593,9 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         if (lane == 0) mbar_arrive(bar(V_FULL + st));
     };
 
+    // Scored instances of head_dim 256, whose walks are often short (documents), have the four warps of the other roles take a share of the output behind them: 64 of the 256 columns of
+    // the 32 rows whose TMEM they reach, the softmax groups 96 each.
+    constexpr bool kThird = SCORE != 0 && D == 256;
     if (D == 128 && warp == kTmaWarp) {
         // =============================== TMA producer, K and V tiles ===============================
         auto load_k = [&](int i) -> bool {
@@ -1039,7 +1042,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
         }
         // ---- epilogue: O / sum, gate, store; the columns are divided among a row's threads ----
         const bool partial = nsplit > 1, gated = !partial && p.gate != nullptr;
-        constexpr int kCols = D / L::kGroups;
+        constexpr int kCols = kThird ? 96 : D / L::kGroups;
         const int col0 = grp * kCols;
         if constexpr (PAGED) {
             item = reload(p.items + blockIdx.x);
@@ -1067,7 +1070,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             float* sums = reinterpret_cast<float*>(smem + L::kOffSum + rt * L::kSumStride);
             sums[grp * kBM + r] = failed ? __int_as_float(0x7fc00000) : l_sum;
             // the row tile's threads (a branch over two constant barriers duplicates what follows: 4 % slower with two row tiles)
-            if constexpr (RT == 1) asm volatile("bar.sync 2, %0;" ::"n"(L::kSoftmaxThreads) : "memory");
+            if constexpr (RT == 1) asm volatile("bar.sync 2, %0;" ::"n"(kThird ? L::kThreads : L::kSoftmaxThreads) : "memory");
             else asm volatile("bar.sync %0, 256;" ::"r"(2 + rt) : "memory");
             l_sum = sums[r] + sums[kBM + r];
             if constexpr (L::kGroups == 4) l_sum += sums[2 * kBM + r] + sums[3 * kBM + r];
@@ -1136,6 +1139,64 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                     if (i >= rows.valid) continue;
                     if (PAGED && !partial) store_out(out0 + rows.rel[i] + c0, v);
                     else *reinterpret_cast<float4*>(dst + (partial ? static_cast<uint32_t>(4 * i * D) : rows.rel[i]) + c0) = v;
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if constexpr (kThird) {
+        if (warp >= kTmaWarp) {
+            // =============================== the output's last columns ===============================
+            // As the softmax groups' epilogue.  A row that nobody sees has a sum of zero, and O finite where it was computed.
+            static_assert(L::kTmaWarp % 4 == 0 && L::kThreads == (L::kTmaWarp + 4) * 32);
+            constexpr int kCol0 = 192;
+            const bool partial = nsplit > 1, gated = !partial && p.gate != nullptr;
+            const RowOffsets<D> rows(warp_row0, turn_row, G, p.query_heads, total_rows);
+            const size_t out0 = own_rows + (static_cast<size_t>(warp_row0 / G) * p.query_heads + kv_head * G) * D + kCol0 + 4 * turn_chunk;
+            __syncwarp();
+            if (ntiles > 0 && !mbar_wait(bar(O_DONE), 0)) failed = true;
+            tc_fence_after();
+            asm volatile("bar.sync 2, %0;" ::"n"(L::kThreads) : "memory");
+            const float* sums = reinterpret_cast<const float*>(smem + L::kOffSum);
+            const int r = (warp & 3) * 32 + lane;
+            const float l_sum = sums[r] + sums[kBM + r];
+            const bool have_o = ntiles > 0 && !__any_sync(0xffffffffu, failed);
+            if (l_sum != l_sum) failed = true;
+            const float factor = failed ? __int_as_float(0x7fc00000) : partial ? 1.0f : l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
+            float* const dst = partial ? p.part_o + (part_row0 + (warp_row0 - row0) + turn_row) * D + kCol0 + 4 * turn_chunk : nullptr;
+            uint8_t* const turn = smem + L::kOffK + 8192 + (warp - kTmaWarp) * 4096;   // the K ring is free (its first bytes are the sums)
+#pragma unroll 1
+            for (int c0 = 0; c0 < D - kCol0; c0 += 32) {
+                float4 g[8];
+                if (gated) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < rows.valid) g[i] = *reinterpret_cast<const float4*>(p.gate + out0 + rows.rel[i] + c0);
+                }
+                float o[32];
+                if (have_o) {
+                    tmem_ld32(tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + L::kColO + kCol0 + c0, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<float4*>(turn + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                        make_float4(o[4 * c] * factor, o[4 * c + 1] * factor, o[4 * c + 2] * factor, o[4 * c + 3] * factor);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = 4 * i + turn_row;
+                    float4 v = *reinterpret_cast<const float4*>(turn + row * 128 + ((turn_chunk ^ (row & 7)) << 4));
+                    if (i >= rows.valid) continue;
+                    if (gated) {
+                        v.x *= 1.0f / (1.0f + __expf(-g[i].x)); v.y *= 1.0f / (1.0f + __expf(-g[i].y));
+                        v.z *= 1.0f / (1.0f + __expf(-g[i].z)); v.w *= 1.0f / (1.0f + __expf(-g[i].w));
+                    }
+                    if (partial) *reinterpret_cast<float4*>(dst + 4 * i * D + c0) = v;
+                    else store_out(out0 + rows.rel[i] + c0, v);
                 }
                 __syncwarp();
             }
