@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     };
 
     // Scored instances of head_dim 256, whose walks are often short (documents), have the four warps of the other roles take a share of the output behind them: 64 of the 256 columns of
-    // the 32 rows whose TMEM they reach, the softmax groups 96 each.
+    // the 32 rows whose TMEM they reach, the softmax groups 96 each (two prompts of documents of 4100 tokens: 207 -> 195 us).
     constexpr bool kThird = SCORE != 0 && D == 256;
     if (D == 128 && warp == kTmaWarp) {
         // =============================== TMA producer, K and V tiles ===============================
