@@ -331,6 +331,33 @@ __device__ __forceinline__ void cap_scores(const Params& p, float (&s)[kBN], boo
         for (int i = 0; i < kBN; ++i) s[i] = tanh_large(s[i] * p.cap_in) * p.cap_log2;
     }
 }
+// Two scores in log2 units, with their bias: of scores as they are, of scores that a polynomial caps, of capped ones.
+struct OfScores {
+    Pair scale;
+    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return fma_pair(x, scale, bias); }
+};
+template <int N>
+struct OfPolynomial {
+    const float (&c)[N];
+    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return fma_pair(x, cap_factor(c, mul_pair(x, x)), bias); }
+};
+struct OfCapped {
+    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return add_pair(x, bias); }
+};
+// A tile's scores with a bias that rises by the same step from score to score: four chains of it, each of two scores a step.
+template <class Score>
+__device__ __forceinline__ void add_bias(float (&s)[kBN], const Score& score, Pair (&bias)[4], Pair step2) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int at = 16 * c + i;
+            const float2 x = unpack_pair(score(pack_pair(s[at], s[at + 1]), bias[c]));
+            s[at] = x.x;
+            s[at + 1] = x.y;
+            bias[c] = add_pair(bias[c], step2);
+        }
+}
 
 // STATE: the position comes from a device-side state (one row tile a CTA).  PAGED: everything does (ChunkItem).
 template <int D, int RT, bool STATE, bool PAGED = false, int SCORE = 0>
@@ -888,17 +915,17 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
             // does not see, all the others become theirs within the exponent: a square and a polynomial in it, two values to an instruction, and none of the special function unit,
             // which the exponentials keep busy.  Otherwise they are capped in place, ahead of the mask.  Scores of up to half the cap have a polynomial of the third degree, larger ones of the fifth:
             // 1333 tokens over 6500, 239 us and 254 to 264; by the special function unit, for scores past the cap, 367.
-            [[maybe_unused]] int within = 0;   // 1: of the short polynomial, 2: of the long one
+            [[maybe_unused]] int degree = 0, within = 0;   // of the warp's scores: 1: the short polynomial's, 2: the long one's, 0: neither's; the same where all is done within the exponent
             if constexpr ((SCORE & kCapped) != 0) {
                 const float largest = largest_of(s);
-                const bool small = !__any_sync(0xffffffffu, largest > p.cap_small);
-                if ((SCORE & kSloped) == 0 && small && !__any_sync(0xffffffffu, pos0 + kBN > len || pos0 < low)) within = __any_sync(0xffffffffu, 2.0f * largest > p.cap_small) ? 2 : 1;
-                if (within == 0) cap_scores(p, s, small);
+                degree = __any_sync(0xffffffffu, largest > p.cap_small) ? 0 : __any_sync(0xffffffffu, 2.0f * largest > p.cap_small) ? 2 : 1;
+                if ((SCORE & kSloped) == 0 && !__any_sync(0xffffffffu, pos0 + kBN > len || pos0 < low)) within = degree;
+                if (within == 0 && ((SCORE & kSloped) == 0 || degree == 0)) cap_scores(p, s, degree > 0);
             }
             if constexpr ((SCORE & kSloped) != 0) {
                 // Of the token's own distance |i - j| a row sees one branch in a tile, the one ahead of it or, in a range that reaches behind the token, the one behind it: four
-                // chains of sums of two values a step, eight roundings long.
-                const Pair of_scores = pack_pair((SCORE & kCapped) != 0 ? 1.0f : p.scale_log2, (SCORE & kCapped) != 0 ? 1.0f : p.scale_log2);
+                // chains of sums of two values a step, eight roundings long.  A cap's polynomial ends in
+                // the sum: 1333 tokens over 6500, 264 us and 291; capped in place ahead of it, 295.
                 const float ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the tile's first position, from the token's
                 const bool mixed = ahead < 0.0f && ahead + kBN > 1.0f && len > static_cast<uint32_t>(place) + 1u;
                 const float of_step = ahead >= 0.0f ? -slope : slope;
@@ -909,16 +936,13 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                     const float first = of_step * (ahead + static_cast<float>(16 * c));
                     bias[c] = pack_pair(first, first + of_step);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; i += 2)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int at = 16 * c + i;
-                        const float2 x = unpack_pair(fma_pair(pack_pair(s[at], s[at + 1]), of_scores, bias[c]));
-                        s[at] = x.x;
-                        s[at + 1] = x.y;
-                        bias[c] = add_pair(bias[c], step2);
-                    }
+                if constexpr ((SCORE & kCapped) == 0) {
+                    add_bias(s, OfScores{pack_pair(p.scale_log2, p.scale_log2)}, bias, step2);
+                } else {
+                    if (degree == 1) add_bias(s, OfPolynomial<4>{p.cap_short}, bias, step2);
+                    else if (degree == 2) add_bias(s, OfPolynomial<6>{p.cap_long}, bias, step2);
+                    else add_bias(s, OfCapped{}, bias, step2);
+                }
                 if (__builtin_expect(__any_sync(0xffffffffu, mixed), 0)) {   // both: what lies behind the token is to be turned over
 #pragma unroll
                     for (int i = 0; i < kBN; ++i) s[i] = fmaf(mixed ? -2.0f * slope : 0.0f, fmaxf(ahead + static_cast<float>(i), 0.0f), s[i]);

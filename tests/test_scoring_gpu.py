@@ -231,6 +231,17 @@ def test_caps_far_from_the_scores(cuda, status, cap, tokens):
     assert float((got[0] - got[1]).abs().max()) <= 2.0 ** -10 * float(got[1].abs().max())
 
 
+@pytest.mark.parametrize("cap", [1.0, 6.0, 25.0, 400.0])
+@pytest.mark.parametrize("d,kind", [(128, None), (128, "documents"), (256, "prefix")])
+def test_caps_with_a_bias_over_tiles(cuda, status, cap, d, kind):
+    """Scores past the cap, up to it, up to half of it and far below, each with a bias by distance, in tiles that are seen whole and in part."""
+    rng = np.random.default_rng(23)
+    tokens = [150, 70, 1]
+    pool = po.Pool(rng, [400, 70, 333], d=d, heads=2, page=16, mode=0, qblock=d)
+    ranges = None if kind is None else ranges_of(rng, kind, tokens, pool.lengths, 1)
+    run(rng, pool, tokens, hq=8, ranges=ranges, cap=cap, slopes=slopes_of(8), q_std=2.0, word=status)
+
+
 def test_infinite_and_nan_queries_stay_in_their_rows(cuda, status):
     rng = np.random.default_rng(6)
     pool = po.Pool(rng, [90, 40], d=128, heads=2, page=16, mode=0, qblock=128)
