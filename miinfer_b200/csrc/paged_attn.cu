@@ -375,7 +375,8 @@ __global__ void __launch_bounds__(kBoundsThreads) paged_bounds_kernel(const __gr
                 low[i] = 0xffffffffu;
                 upto[i] = 0;
             }
-            for (uint32_t t0 = lane; t0 <= kChunkRows / p.group; t0 += 32) {   // of a row tile's tokens (one more than that, where heads of one lie in two)
+            // of a row tile's tokens: where the heads are no whole fraction of it, those of its first and of its last token may both lie in two (44 tokens in 128 rows of three heads)
+            for (uint32_t t0 = lane; t0 < (kChunkRows + 2 * (p.group - 1)) / p.group; t0 += 32) {
                 Sight sight[kBoundsTiles];
 #pragma unroll
                 for (uint32_t i = 0; i < kBoundsTiles; ++i) {
