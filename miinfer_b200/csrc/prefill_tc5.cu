@@ -331,31 +331,37 @@ __device__ __forceinline__ void cap_scores(const Params& p, float (&s)[kBN], boo
         for (int i = 0; i < kBN; ++i) s[i] = tanh_large(s[i] * p.cap_in) * p.cap_log2;
     }
 }
-// Two scores in log2 units, with their bias: of scores as they are, of scores that a polynomial caps, of capped ones.
+// Two scores in log2 units: of scores as they are, of scores that a polynomial caps, of capped ones.
 struct OfScores {
     Pair scale;
-    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return fma_pair(x, scale, bias); }
+    __device__ __forceinline__ Pair operator()(Pair x) const { return mul_pair(x, scale); }
 };
 template <int N>
 struct OfPolynomial {
     const float (&c)[N];
-    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return fma_pair(x, cap_factor(c, mul_pair(x, x)), bias); }
+    __device__ __forceinline__ Pair operator()(Pair x) const { return mul_pair(x, cap_factor(c, mul_pair(x, x))); }
 };
 struct OfCapped {
-    __device__ __forceinline__ Pair operator()(Pair x, Pair bias) const { return add_pair(x, bias); }
+    __device__ __forceinline__ Pair operator()(Pair x) const { return x; }
 };
-// A tile's scores with a bias that rises by the same step from score to score: four chains of it, each of two scores a step.
+// A tile's scores with a bias of `step` a position, for the first of them at distance `ahead`.  Distances are counted, whole numbers that fp32 holds, and the product with the step is
+// rounded with the sum: a bias is off by a fraction of itself, and by nothing at distance 0.  (Sums of steps in its place, an instruction fewer a pair, leave there a fraction of what they
+// began with: 1.4 of an lse under a slope of 1e6.)
 template <class Score>
-__device__ __forceinline__ void add_bias(float (&s)[kBN], const Score& score, Pair (&bias)[4], Pair step2) {
+__device__ __forceinline__ void add_bias(float (&s)[kBN], const Score& score, float ahead, float step) {
+    const Pair step2 = pack_pair(step, step), two = pack_pair(2.0f, 2.0f);
+    Pair distance[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) distance[c] = pack_pair(ahead + static_cast<float>(16 * c), ahead + static_cast<float>(16 * c + 1));
 #pragma unroll
     for (int i = 0; i < 16; i += 2)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int at = 16 * c + i;
-            const float2 x = unpack_pair(score(pack_pair(s[at], s[at + 1]), bias[c]));
+            const float2 x = unpack_pair(fma_pair(distance[c], step2, score(pack_pair(s[at], s[at + 1]))));
             s[at] = x.x;
             s[at + 1] = x.y;
-            bias[c] = add_pair(bias[c], step2);
+            distance[c] = add_pair(distance[c], two);
         }
 }
 
@@ -923,25 +929,18 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
                 if (within == 0 && ((SCORE & kSloped) == 0 || degree == 0)) cap_scores(p, s, degree > 0);
             }
             if constexpr ((SCORE & kSloped) != 0) {
-                // Of the token's own distance |i - j| a row sees one branch in a tile, the one ahead of it or, in a range that reaches behind the token, the one behind it: four
-                // chains of sums of two values a step, eight roundings long.  A cap's polynomial ends in
-                // the sum: 1333 tokens over 6500, 264 us and 291; capped in place ahead of it, 295.
+                // Of the token's own distance |i - j| a row sees one branch in a tile, the one ahead of it or, in a range that reaches behind the token, the one behind it.
+                // 1333 tokens over 6500, 32 / 8 heads of 128, L2 flushed, us: 189 without a bias, 210 with; with a cap as well 280 (scores up to half of it), 306, 388 (past it).  The products ahead
+                // of scores that end in the sum, in place of scores ahead of products that do: 212, 292, 314, 392 (and twice the spilled registers).
                 const float ahead = static_cast<float>(static_cast<int>(pos0) - place);   // of the tile's first position, from the token's
                 const bool mixed = ahead < 0.0f && ahead + kBN > 1.0f && len > static_cast<uint32_t>(place) + 1u;
-                const float of_step = ahead >= 0.0f ? -slope : slope;
-                const Pair step2 = pack_pair(2.0f * of_step, 2.0f * of_step);
-                Pair bias[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float first = of_step * (ahead + static_cast<float>(16 * c));
-                    bias[c] = pack_pair(first, first + of_step);
-                }
+                const float step = ahead >= 0.0f ? -slope : slope;
                 if constexpr ((SCORE & kCapped) == 0) {
-                    add_bias(s, OfScores{pack_pair(p.scale_log2, p.scale_log2)}, bias, step2);
+                    add_bias(s, OfScores{pack_pair(p.scale_log2, p.scale_log2)}, ahead, step);
                 } else {
-                    if (degree == 1) add_bias(s, OfPolynomial<4>{p.cap_short}, bias, step2);
-                    else if (degree == 2) add_bias(s, OfPolynomial<6>{p.cap_long}, bias, step2);
-                    else add_bias(s, OfCapped{}, bias, step2);
+                    if (degree == 1) add_bias(s, OfPolynomial<4>{p.cap_short}, ahead, step);
+                    else if (degree == 2) add_bias(s, OfPolynomial<6>{p.cap_long}, ahead, step);
+                    else add_bias(s, OfCapped{}, ahead, step);
                 }
                 if (__builtin_expect(__any_sync(0xffffffffu, mixed), 0)) {   // both: what lies behind the token is to be turned over
 #pragma unroll
