@@ -654,7 +654,7 @@ typedef struct b200kv_page_book {
 B200KV_API size_t b200kv_pages_workspace_bytes(const b200kv_page_book* book);
 /* Room for add[e] (DEVICE int32 [count], 0 or more) further positions of sequence slots[e] (DEVICE int32 [count]): its length grows, fresh pages go into its table.  (Ahead of the
  * store of a step, whose batch then reads the book's tables and lengths.)  A sequence is named once.  workspace: b200kv_pages_workspace_bytes, 16-byte aligned, contents of no
- * consequence. */
+ * consequence; it overlaps neither the book's arrays nor the call's (B200KV_ERR_INVALID). */
 B200KV_API int b200kv_pages_grow(const b200kv_page_book* book, const int32_t* slots, const int32_t* add, uint32_t count, void* workspace, size_t workspace_bytes, void* stream);
 /* children[e], empty slots named once, go on from parents[e]: with all its positions, or the first at[e] (DEVICE int32 [count], at may be NULL).  Whole pages are shared, and their counts grow by
  * one for each child; one that is not full is copied to a fresh page, in the pools of all layers.  So what a sequence still writes to is its own.  views: HOST [layers], up to

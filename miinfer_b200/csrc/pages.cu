@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 
 namespace b200kv {
 
@@ -548,9 +549,14 @@ Room room_of(const b200kv_page_book& b) {
     r.bytes = at;
     return r;
 }
-int check_workspace(const b200kv_page_book& book, const void* workspace, size_t bytes) {
+// A call's workspace, which lies over none of the book's arrays, nor over its entries' (of `count` words each; may be null).
+int check_workspace(const b200kv_page_book& book, const void* workspace, size_t bytes, std::initializer_list<const void*> entries = {}, uint64_t count = 0) {
     if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return B200KV_ERR_INVALID;
-    return workspace == nullptr || bytes < room_of(book).bytes ? B200KV_ERR_WORKSPACE : B200KV_OK;
+    const size_t room = room_of(book).bytes;
+    if (workspace == nullptr || bytes < room) return B200KV_ERR_WORKSPACE;
+    for (const void* array : entries)
+        if (array != nullptr && share(workspace, room, array, count * 4)) return B200KV_ERR_INVALID;
+    return over_book(book, workspace, room / 4) ? B200KV_ERR_INVALID : B200KV_OK;
 }
 
 int launch_take(const TakeParams& p, cudaStream_t stream) {
@@ -610,7 +616,7 @@ int b200kv_pages_grow(const b200kv_page_book* book, const int32_t* slots, const 
     if (rc != B200KV_OK) return rc;
     if (count == 0) return B200KV_OK;
     if (!words(slots) || !words(add) || count > kMostSequences || over_book(*book, slots, count) || over_book(*book, add, count)) return B200KV_ERR_INVALID;
-    rc = check_workspace(*book, workspace, workspace_bytes);
+    rc = check_workspace(*book, workspace, workspace_bytes, {slots, add}, count);
     if (rc == B200KV_OK) rc = ensure_device();
     if (rc != B200KV_OK) return rc;
     const Room room = room_of(*book);
@@ -627,7 +633,7 @@ int b200kv_pages_fork(const b200kv_page_book* book, const b200kv_paged_view* vie
     // an entry's result lies in a place of its own in the workspace, which has as many as there are slots
     if (!words(parents) || !words(children) || (at != nullptr && !words(at)) || count > book->slots) return B200KV_ERR_INVALID;
     if (over_book(*book, parents, count) || over_book(*book, children, count) || over_book(*book, at, count)) return B200KV_ERR_INVALID;
-    rc = check_workspace(*book, workspace, workspace_bytes);
+    rc = check_workspace(*book, workspace, workspace_bytes, {parents, children, at}, count);
     if (rc == B200KV_OK) rc = ensure_device();
     if (rc != B200KV_OK) return rc;
     const Room room = room_of(*book);
