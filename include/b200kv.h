@@ -640,7 +640,7 @@ B200KV_API int b200kv_paged_rotary(const b200kv_paged_view* view, const b200kv_p
  * Which sequence holds which pages, and how many hold each, in device memory; one book serves the pools of all layers, which share its page numbers.  Its tables and
  * lengths are those of a b200kv_paged_batch.  A page whose count is 0 is free.  Where a call needs pages it takes the lowest free ones, for its entries in order; an entry gets
  * all that it needs or, as every later one that needs any, is left as it was (B200KV_STATUS_NO_PAGE).  Entries whose sequence is negative are left out; ones that a call
- * cannot do are left out too, and set a status bit.  One call at a time changes a book or uses a workspace.  The calls can be captured. */
+ * cannot do are left out too, and set a status bit.  Growth takes up to 8192 entries, a fork as many as there are slots, those left out among them.  One call at a time changes a book or uses a workspace.  The calls can be captured. */
 typedef struct b200kv_page_book {
     int32_t* refs;       /* DEVICE [pages], 16-byte aligned: who holds a page -- sequences, and whoever else adds to it; never negative */
     int32_t* tables;     /* DEVICE [slots][max_pages]: entries past a sequence's pages are not looked at */

@@ -277,7 +277,7 @@ def pages_workspace(book: PageBook, device=None) -> torch.Tensor:
 
 
 def launch_pages_grow(book: PageBook, slots: torch.Tensor, add: torch.Tensor, *, workspace: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> None:
-    """Room for add[e] further positions of sequence slots[e] (int32 each): the lowest free pages, entry by entry."""
+    """Room for add[e] further positions of sequence slots[e] (int32 each, up to 8192 entries; a negative slot is left out): the lowest free pages, entry by entry."""
     rc = native.pages_grow(book, slots, add, workspace, stream)
     if rc:
         check(rc, "b200kv_pages_grow")
@@ -285,8 +285,8 @@ def launch_pages_grow(book: PageBook, slots: torch.Tensor, add: torch.Tensor, *,
 
 def launch_pages_fork(book: PageBook, views: Sequence[PagedView], parents: torch.Tensor, children: torch.Tensor, *, at: Optional[torch.Tensor] = None, workspace: torch.Tensor,
                       stream: Optional[torch.cuda.Stream] = None) -> None:
-    """The empty slots children[e] go on from parents[e] (int32 each), with all its positions or the first at[e]: whole pages are shared, a last one that is not full is copied in
-    the pools of all layers (`views`)."""
+    """The empty slots children[e] go on from parents[e] (int32 each, as many entries at most as there are slots; a negative child is left out), with all its positions or the first
+    at[e]: whole pages are shared, a last one that is not full is copied in the pools of all layers (`views`)."""
     rc = native.pages_fork(book, views, parents, children, at, workspace, stream)
     if rc:
         check(rc, "b200kv_pages_fork")
