@@ -32,6 +32,7 @@ constexpr uint32_t kCandidates = 31;       // sizes of a piece that the layout c
 constexpr int kPrepareThreads = 256;
 
 // Estimated costs of the chunk kernel, us, as the single-sequence launch's (pick_kv_splits): a tile, a CTA's set-up and output, a merge, a partial.
+// Of the plain instances; scored ones, whose tiles take up to a third longer (past a cap, twice as long), are split by the same.
 struct ChunkCosts { float tile, cta, last_wave, merge, part; };   // last_wave: of a wave, where it is not full
 
 struct PrepareParams {

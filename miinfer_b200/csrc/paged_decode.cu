@@ -749,7 +749,7 @@ int launch_planes(const P& p, const CUtensorMap& kmap, const CUtensorMap& vmap, 
 }
 // Three planes against int8 keys (a score to 2^-23 of its row's largest element), but for eight rows where the output alone is asked for, in fp16: two hold 2^-16, which that does not
 // show, and are up to 12 % faster (24 sequences of 4000, 24 / 4 heads of 256: q8_0 66.6 and 75 us, where a tile has 96 sums a thread in place of 64 and one buffer of them; one scale a row 59.4
-// and 61.4).
+// and 61.4).  Scored calls always take three: instances of two were not built or timed.
 template <int D, int KF, int VF, int RG, class P>
 int launch_of(const P& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream, bool behind) {
     if constexpr (KF == F16) return launch_planes<D, KF, VF, RG, 2>(p, kmap, vmap, stream, behind);

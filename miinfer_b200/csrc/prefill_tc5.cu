@@ -344,7 +344,7 @@ struct OfPolynomial {
 struct OfCapped {
     __device__ __forceinline__ Pair operator()(Pair x) const { return x; }
 };
-// A tile's scores with a bias of `step` a position, for the first of them at distance `ahead`.  Distances are counted, whole numbers that fp32 holds, and the product with the step is
+// A tile's scores with a bias of `step` a position, for the first of them at distance `ahead`.  Distances are counted, whole numbers that fp32 holds (up to 2^24; off by 2^-21 of themselves beyond), and the product with the step is
 // rounded with the sum: a bias is off by a fraction of itself, and by nothing at distance 0.  (Sums of steps in its place, an instruction fewer a pair, leave there a fraction of what they
 // began with: 1.4 of an lse under a slope of 1e6.)
 template <class Score>
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(Layout<D, RT>::kThreads, 1) prefill_tc5_kernel
     if constexpr (PAGED) scratch_row = static_cast<int>(item.scratch_row);
     // Where the CTA's tile j lies: its row in what the maps cover, and its first position.  With a bias by distance the last tile is the first one: it has the largest scores, and what
     // comes behind it seldom moves a row's reference (the other way round that moved in nearly every tile of a steep slope, and O was rescaled: 265 us in place of 205 for 1333
-    // tokens over 6500).
+    // tokens over 6500, of a bias that was summed up step by step).
     auto tile_of = [&](int j) { return static_cast<uint32_t>(tile0 + ((SCORE & kSloped) != 0 ? ntiles - 1 - j : j)); };
     auto tile_row = [&](int j) -> int {
         if constexpr (PAGED) {
